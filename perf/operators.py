@@ -1,0 +1,437 @@
+"""Measured cases of the training operators around a linear layer: dropout from a counter-based
+generator, the linear layer with bias, activation, dropout and residual, and the loss head that
+keeps no logits. Each case is one call (or a forward and its backward) as a training or decoding
+program makes it.
+
+`own` selects the framework's kernels; otherwise `run` computes the plain form in fp32.
+"""
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+_DEV = "cuda"
+_DT = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def _ops():
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "llm-cpp_b200", "python")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from llmgpu import ops
+    return ops
+
+
+# ------------------------------------------------------------------------------------ cases
+def _dropout(rows, cols, p, x, out, resid=False, pad=0, bwd=False, **kw):
+    return dict(op="dropout", rows=rows, cols=cols, p=p, x=x, out=out, resid=resid, pad=pad,
+                bwd=bwd, **kw)
+
+
+def _linear(M, K, N, act, p, out, resid=False, bias=True, w_mn=False, bwd=False, **kw):
+    return dict(op="linear", M=M, K=K, N=N, act=act, p=p, out=out, resid=resid, bias=bias,
+                w_mn=w_mn, bwd=bwd, **kw)
+
+
+def _head(rows, C, V, smoothing, ignored, bwd, w_mn=False, **kw):
+    return dict(op="head", rows=rows, C=C, V=V, smoothing=smoothing, ignored=ignored, bwd=bwd,
+                w_mn=w_mn, **kw)
+
+
+def listed():
+    return [
+        # embedding dropout of the tiny character model: 2 sequences of 128 tokens; the launch
+        # itself is most of it
+        _dropout(256, 128, 0.1, "bf16", "bf16", name="dropout_char"),
+        # a branch's bf16 output dropped and added to the fp32 residual stream, the largest batch
+        _dropout(16384, 4096, 0.1, "bf16", "f32", resid=True, name="dropout_resid_large"),
+        # the gradient of the stream through a mask, into the bf16 operand of the products below;
+        # ragged rows and columns, padded row strides
+        _dropout(8191, 1021, 0.25, "f32", "bf16", pad=3, bwd=True, name="dropout_bwd_ragged"),
+        # one new token through an FFN's first product while decoding
+        _linear(1, 1024, 4096, "gelu", 0.0, "bf16", name="linear_one_token"),
+        # an FFN's first product in training, 4 sequences of 2048 tokens, `pre` kept for backward
+        _linear(8192, 1024, 4096, "gelu", 0.0, "bf16", name="linear_up"),
+        # its second product: bias, dropout and the fp32 residual stream; weights [in, out], as
+        # the framework's parameters lie
+        _linear(8192, 4096, 1024, "none", 0.1, "f32", resid=True, w_mn=True,
+                name="linear_down_resid"),
+        # the backward of a first product
+        _linear(8192, 1024, 4096, "gelu", 0.0, "bf16", bwd=True, name="linear_up_bwd"),
+        # ragged rows and widths, backward through the mask and silu
+        _linear(1999, 765, 1021, "silu", 0.2, "f32", w_mn=True, bwd=True,
+                name="linear_ragged_bwd"),
+        # the tiny character model's head, a whole step's loss and gradients
+        _head(256, 128, 256, 0.0, 0.0, True, name="head_char"),
+        # evaluation: the loss of 8 x 1024 tokens over the GPT-2 vocabulary
+        _head(8192, 768, 50257, 0.0, 0.0, False, name="head_eval"),
+        # the same with its gradients: a training step's head
+        _head(8192, 768, 50257, 0.0, 0.0, True, name="head_train"),
+        # a wider model, untied head [C, V], smoothed labels, a padded batch (rows left out)
+        _head(4095, 1024, 32000, 0.1, 0.15, True, w_mn=True, name="head_padded"),
+    ]
+
+
+def _between(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(("dropout", "linear", "head"))
+    if op == "dropout":
+        rows, cols = _between(rng, 1, 16384), _between(rng, 1, 8192)
+        rows = max(1, min(rows, 16384 * 4096 // cols))
+        bwd = rng.random() < 0.4
+        return _dropout(rows, cols, rng.choice((0.05, 0.1, 0.25, 0.5, round(rng.random(), 3))),
+                        rng.choice(("bf16", "f32")), rng.choice(("bf16", "f32")),
+                        resid=not bwd and rng.random() < 0.5, pad=rng.choice((0, 0, 1, 8)),
+                        bwd=bwd)
+    if op == "linear":
+        M = rng.choice((rng.randint(1, 8), _between(rng, 1, 8192)))
+        K, N = _between(rng, 16, 4096), _between(rng, 16, 4096)
+        if rng.random() < 0.5:
+            K, N = -(-K // 64) * 64, -(-N // 64) * 64
+        return _linear(M, K, N, rng.choice(("none", "relu", "gelu", "silu")),
+                       rng.choice((0.0, 0.1, 0.25)), rng.choice(("bf16", "f32")),
+                       resid=rng.random() < 0.4, bias=rng.random() < 0.8,
+                       w_mn=rng.random() < 0.5, bwd=rng.random() < 0.5)
+    rows, C, V = _between(rng, 1, 8192), _between(rng, 64, 2048), _between(rng, 100, 50257)
+    rows = max(1, min(rows, 8192 * 768 * 50257 // (C * V)))
+    return _head(rows, C, V, rng.choice((0.0, 0.0, 0.1)), rng.choice((0.0, 0.2)),
+                 rng.random() < 0.6, w_mn=rng.random() < 0.3)
+
+
+def _matrix(g, rows, cols, dtype, multiple=8, scale=1.0, pad=0):
+    """Normal values in rows whose stride is a multiple of `multiple` elements, and pad more."""
+    ld = -(-cols // multiple) * multiple + pad
+    buf = torch.empty(rows, ld, dtype=dtype, device=_DEV)
+    buf.normal_(0.0, scale, generator=g)
+    return buf[:, :cols]
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=_DEV).manual_seed(seed)
+    s = dict(case=case)
+    # the generator's state as a program keeps it on the device: seed and offset
+    s["rng"] = torch.tensor([seed * 7919 + 12345, 1000003 * (seed % 4001)], dtype=torch.int64,
+                            device=_DEV)
+    if case["op"] == "dropout":
+        rows, cols, pad = case["rows"], case["cols"], case["pad"]
+        s["x"] = _matrix(g, rows, cols, _DT[case["x"]], 1, 1.0, pad)
+        s["resid"] = _matrix(g, rows, cols, _DT[case["out"]], 1, 2.0) if case["resid"] else None
+        return s
+    if case["op"] == "linear":
+        M, K, N, bf = case["M"], case["K"], case["N"], torch.bfloat16
+        s["x"] = _matrix(g, M, K, bf)
+        w = _matrix(g, K, N, bf, 8, 1.0 / math.sqrt(K)) if case["w_mn"] else \
+            _matrix(g, N, K, bf, 8, 1.0 / math.sqrt(K))
+        s["w"] = w
+        s["bias"] = torch.randn(N, generator=g, device=_DEV) * 0.3 if case["bias"] else None
+        if case["bwd"]:
+            s["dy"] = _matrix(g, M, N, _DT[case["out"]], 1, 0.01)
+            s["pre"] = None
+            if case["act"] != "none":  # what the forward kept
+                s["pre"] = _matrix(g, M, N, bf, 8)
+                z = s["x"].float() @ (w.float() if case["w_mn"] else w.float().t())
+                s["pre"].copy_(z if s["bias"] is None else z + s["bias"])
+        else:
+            s["resid"] = _matrix(g, M, N, _DT[case["out"]], 1, 2.0) if case["resid"] else None
+        return s
+    rows, C, V, bf = case["rows"], case["C"], case["V"], torch.bfloat16
+    # Zipf-like token ids, and hidden states that point some way towards their target's row, as
+    # a partly trained model's do
+    u = torch.rand(rows, generator=g, device=_DEV)
+    s["targets"] = (torch.exp(u * math.log(V)).long() - 1).clamp_(0, V - 1).to(torch.int32)
+    w = _matrix(g, C, V, bf, 8, 0.04) if case["w_mn"] else _matrix(g, V, C, bf, 8, 0.04)
+    s["w"] = w
+    x = _matrix(g, rows, C, bf)
+    t = s["targets"].long()
+    wt = (w[:, t].t() if case["w_mn"] else w[t]).float()
+    x.copy_(x.float() + 4.0 * wt / wt.norm(dim=1, keepdim=True))
+    s["x"] = x
+    if case["ignored"] > 0:
+        out = torch.rand(rows, generator=g, device=_DEV) < case["ignored"]
+        s["targets"] = torch.where(out, -1, s["targets"])
+    valid = (s["targets"] >= 0).sum().clamp(min=1)
+    # the gradient of the mean over the rows that count, times a loss scale
+    s["dloss"] = torch.full((rows,), 1024.0, device=_DEV) / valid
+    return s
+
+
+# -------------------------------------------------------------------------------- plain form
+def _keep(rng, rows, cols, p):
+    """Philox4x32-10 (Salmon et al., SC 2011), one call for 8 columns: keyed by the seed, counter
+    (column / 8, row, offset). Lane j of 16 bits decides column 8 i + j: kept when it is at
+    least round(p 65536). Returns the mask and the scale of what is kept."""
+    thr = int(round(p * 65536.0))
+    n8 = -(-cols // 8)
+    low = 0xFFFFFFFF
+    seed, offset = rng[0], rng[1]
+    k0, k1 = seed & low, (seed >> 32) & low
+    dev = rng.device
+    c0 = torch.arange(n8, dtype=torch.int64, device=dev).expand(rows, n8)
+    c1 = torch.arange(rows, dtype=torch.int64, device=dev)[:, None].expand(rows, n8)
+    c2 = (offset & low).expand(rows, n8)
+    c3 = ((offset >> 32) & low).expand(rows, n8)
+    for _ in range(10):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # wraps in 64 bits: the product's own bits
+        c0, c1, c2, c3 = ((b >> 32) & low) ^ c1 ^ k0, b & low, ((a >> 32) & low) ^ c3 ^ k1, a & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    words = torch.stack((c0 & 0xFFFF, c0 >> 16, c1 & 0xFFFF, c1 >> 16, c2 & 0xFFFF, c2 >> 16,
+                         c3 & 0xFFFF, c3 >> 16), -1)
+    keep = words.reshape(rows, 8 * n8)[:, :cols] >= thr
+    return keep, (65536.0 / (65536 - thr) if thr < 65536 else 0.0)
+
+
+def _act(z, act):
+    if act == "relu":
+        return torch.where(z > 0, z, torch.zeros_like(z))
+    if act == "gelu":
+        return 0.5 * z * (1 + torch.tanh(0.7978845608 * (z + 0.044715 * z * z * z)))
+    if act == "silu":
+        return z / (1 + torch.exp(-z))
+    return z
+
+
+def _act_grad(z, act):
+    if act == "relu":
+        return (z > 0).to(z.dtype)
+    if act == "gelu":
+        th = torch.tanh(0.7978845608 * (z + 0.044715 * z * z * z))
+        return 0.5 * (1 + th) + 0.5 * z * (1 - th * th) * 0.7978845608 * (1 + 0.134145 * z * z)
+    if act == "silu":
+        sg = 1 / (1 + torch.exp(-z))
+        return sg * (1 + z * (1 - sg))
+    return torch.ones_like(z)
+
+
+def _plain_dropout(s):
+    c = s["case"]
+    y = s["x"].float()
+    keep, scale = _keep(s["rng"], c["rows"], c["cols"], c["p"])
+    y = torch.where(keep, y * scale, torch.zeros_like(y))
+    if s["resid"] is not None:
+        y = y + s["resid"].float()
+    return {"y": y.to(_DT[c["out"]])}
+
+
+def _plain_linear(s):
+    c = s["case"]
+    w = s["w"].float() if c["w_mn"] else s["w"].float().t()
+    if c["bwd"]:
+        dz = s["dy"].float()
+        if c["p"] > 0:
+            keep, scale = _keep(s["rng"], c["M"], c["N"], c["p"])
+            dz = torch.where(keep, dz * scale, torch.zeros_like(dz))
+        if s["pre"] is not None:
+            dz = dz * _act_grad(s["pre"].float(), c["act"])
+        x = s["x"].float()
+        dw = x.t() @ dz if c["w_mn"] else dz.t() @ x
+        out = {"dx": (dz @ w.t()).bfloat16(), "dw": dw.bfloat16()}
+        if c["bias"]:
+            out["dbias"] = dz.sum(0)
+        return out
+    z = s["x"].float() @ w
+    if s["bias"] is not None:
+        z = z + s["bias"]
+    y = _act(z, c["act"])
+    if c["p"] > 0:
+        keep, scale = _keep(s["rng"], c["M"], c["N"], c["p"])
+        y = torch.where(keep, y * scale, torch.zeros_like(y))
+    if s["resid"] is not None:
+        y = y + s["resid"].float()
+    out = {"y": y.to(_DT[c["out"]])}
+    if c["act"] != "none":
+        out["pre"] = z.bfloat16()
+    return out
+
+
+def _plain_head(s):
+    c = s["case"]
+    V, sm = c["V"], c["smoothing"]
+    x = s["x"].float()
+    w = s["w"].float() if c["w_mn"] else s["w"].float().t()
+    z = x @ w
+    m = z.amax(1, keepdim=True)
+    lse = m + torch.log(torch.exp(z - m).sum(1, keepdim=True))
+    valid = s["targets"] >= 0
+    t = s["targets"].long().clamp(min=0)[:, None]
+    on, off = 1.0 - sm, sm / (V - 1)
+    zt = z.gather(1, t)
+    loss = on * (lse - zt)
+    if sm > 0:
+        loss = loss + off * ((V * lse - z.sum(1, keepdim=True)) - (lse - zt))
+    loss = torch.where(valid, loss[:, 0], torch.zeros_like(loss[:, 0]))
+    if not c["bwd"]:
+        return {"loss": loss}
+    g = torch.exp(z - lse) - off
+    g.scatter_add_(1, t, torch.full_like(zt, off - on))
+    g = torch.where(valid[:, None], g * s["dloss"][:, None], torch.zeros_like(g))
+    dw = x.t() @ g if c["w_mn"] else g.t() @ x
+    return {"loss": loss, "dx": (g @ w.t()).bfloat16(), "dw": dw.bfloat16()}
+
+
+# ---------------------------------------------------------------------------- the framework's
+def _own_dropout(s):
+    ops, c = _ops(), s["case"]
+    if c["bwd"]:
+        return {"y": ops.dropout_bwd(s["x"], c["p"], s["rng"], out_dtype=_DT[c["out"]])}
+    return {"y": ops.dropout_fwd(s["x"], c["p"], s["rng"], resid=s["resid"],
+                                 out_dtype=_DT[c["out"]])}
+
+
+def _own_linear(s):
+    ops, c = _ops(), s["case"]
+    if c["bwd"]:
+        dx, dw, db = ops.linear_bwd(s["dy"], s["x"], s["w"], pre=s["pre"], act=c["act"], p=c["p"],
+                                    rng=s["rng"], w_mn=c["w_mn"], need_dbias=c["bias"])
+        return {"dx": dx, "dw": dw, "dbias": db} if c["bias"] else {"dx": dx, "dw": dw}
+    y, pre = ops.linear_fwd(s["x"], s["w"], bias=s["bias"], act=c["act"], p=c["p"], rng=s["rng"],
+                            resid=s["resid"], w_mn=c["w_mn"], out_dtype=_DT[c["out"]],
+                            save_pre=c["act"] != "none")
+    return {"y": y, "pre": pre} if c["act"] != "none" else {"y": y}
+
+
+def _own_head(s):
+    ops, c = _ops(), s["case"]
+    loss, lse = ops.linear_cross_entropy_fwd(s["x"], s["w"], s["targets"],
+                                             smoothing=c["smoothing"], w_mn=c["w_mn"])
+    if not c["bwd"]:
+        return {"loss": loss}
+    dx, dw = ops.linear_cross_entropy_bwd(s["x"], s["w"], s["targets"], lse, s["dloss"],
+                                          smoothing=c["smoothing"], w_mn=c["w_mn"])
+    return {"loss": loss, "dx": dx, "dw": dw}
+
+
+def run(state):
+    op = state["case"]["op"]
+    if own:
+        return {"dropout": _own_dropout, "linear": _own_linear, "head": _own_head}[op](state)
+    return {"dropout": _plain_dropout, "linear": _plain_linear, "head": _plain_head}[op](state)
+
+
+def work(case):
+    c = case
+    size = {"bf16": 2, "f32": 4}
+    if c["op"] == "dropout":
+        n = c["rows"] * c["cols"]
+        per = size[c["x"]] + size[c["out"]] * (2 if c["resid"] else 1)
+        return {"bytes": n * per + 16, "flops": 2 * n}
+    if c["op"] == "linear":
+        M, K, N = c["M"], c["K"], c["N"]
+        o = size[c["out"]]
+        if c["bwd"]:
+            pre = 2 * M * N if c["act"] != "none" else 0
+            return {"bytes": o * M * N + pre + 2 * (2 * M * K + 2 * K * N) + 4 * N * c["bias"],
+                    "flops": 4 * M * N * K}
+        return {"bytes": 2 * (M * K + K * N) + o * M * N * (2 if c["resid"] else 1) +
+                (2 * M * N if c["act"] != "none" else 0) + 4 * N * c["bias"],
+                "flops": 2 * M * N * K}
+    R, C, V = c["rows"], c["C"], c["V"]
+    if c["bwd"]:  # logits, dx and dw: one product each
+        return {"bytes": 2 * (2 * R * C + 2 * C * V) + 12 * R, "flops": 6 * R * C * V}
+    return {"bytes": 2 * (R * C + C * V) + 8 * R, "flops": 2 * R * C * V}
+
+
+# ------------------------------------------------------------------------------- in 64 bits
+def _exact_keep(state, rows, cols, p):
+    """The same generator in numpy's unsigned integers."""
+    seed, offset = (int(v) & 0xFFFFFFFFFFFFFFFF for v in state["rng"].tolist())
+    u32, u64, mask = np.uint32, np.uint64, np.uint64(0xFFFFFFFF)
+    blocks = (cols + 7) // 8
+    ctr = [np.broadcast_to(np.arange(blocks, dtype=u64)[None, :], (rows, blocks)),
+           np.broadcast_to(np.arange(rows, dtype=u64)[:, None], (rows, blocks)),
+           np.full((1, 1), offset & 0xFFFFFFFF, dtype=u64), np.full((1, 1), offset >> 32, dtype=u64)]
+    key = [seed & 0xFFFFFFFF, seed >> 32]
+    for r in range(10):
+        pa = ctr[0] * u64(0xD2511F53)
+        pb = ctr[2] * u64(0xCD9E8D57)
+        ctr = [(pb >> u64(32)) ^ ctr[1] ^ u64(key[0]), pb & mask,
+               (pa >> u64(32)) ^ ctr[3] ^ u64(key[1]), pa & mask]
+        key = [(key[0] + 0x9E3779B9) % 2**32, (key[1] + 0xBB67AE85) % 2**32]
+    words = np.empty((rows, blocks, 4), dtype=u32)
+    for i in range(4):
+        words[:, :, i] = ctr[i]
+    lanes = words.view("<u2").reshape(rows, blocks * 8)[:, :cols]
+    limit = int(np.rint(np.float64(p) * 65536))
+    factor = 0.0 if limit == 65536 else 65536.0 / (65536.0 - limit)
+    return torch.from_numpy(lanes.astype(np.int32) >= limit).to(_DEV), factor
+
+
+def _exact_linear(c, s):
+    x, w = s["x"].double(), s["w"].double()
+    if not c["w_mn"]:
+        w = w.T
+    sig = torch.sigmoid
+    a = 2 * 0.7978845608
+    if c["p"] > 0:
+        keep, factor = _exact_keep(s, c["M"], c["N"], c["p"])
+    if c["bwd"]:
+        dz = s["dy"].double()
+        if c["p"] > 0:
+            dz = (dz * factor).masked_fill(~keep, 0)
+        if c["act"] != "none":
+            z = s["pre"].double()
+            if c["act"] == "relu":
+                dz = dz.masked_fill(z <= 0, 0)
+            elif c["act"] == "silu":
+                dz = dz * (sig(z) + z * sig(z) * sig(-z))
+            else:  # gelu(z) = z sigmoid(2u), u = k (z + 0.044715 z^3)
+                h = sig(a * (z + 0.044715 * z ** 3))
+                dz = dz * (h + z * h * (1 - h) * a * (1 + 3 * 0.044715 * z ** 2))
+        dw = torch.mm(dz.T, x)
+        out = {"dx": torch.mm(dz, w.T), "dw": dw.T.contiguous() if c["w_mn"] else dw}
+        if c["bias"]:
+            out["dbias"] = dz.sum(dim=0)
+        return out
+    z = torch.mm(x, w)
+    if c["bias"]:
+        z += s["bias"].double()
+    y = {"none": lambda: z, "relu": lambda: z.clamp(min=0), "silu": lambda: z * sig(z),
+         "gelu": lambda: z * sig(a * (z + 0.044715 * z ** 3))}[c["act"]]()
+    if c["p"] > 0:
+        y = (y * factor).masked_fill(~keep, 0)
+    if c["resid"]:
+        y = y + s["resid"].double()
+    return {"y": y} if c["act"] == "none" else {"y": y, "pre": z}
+
+
+def _exact_head(c, s):
+    x, w = s["x"].double(), s["w"].double()
+    if c["w_mn"]:
+        w = w.T
+    V, sm = c["V"], c["smoothing"]
+    dw = torch.zeros(V, c["C"], dtype=torch.float64, device=_DEV)
+    loss, dx = [], []
+    step = 2048  # rows at a time
+    for r in range(0, c["rows"], step):
+        xr, t, d = x[r:r + step], s["targets"][r:r + step].long(), s["dloss"][r:r + step].double()
+        logp = torch.log_softmax(torch.mm(xr, w.T), dim=1)
+        y = torch.full_like(logp, sm / (V - 1))
+        y.scatter_(1, t.clamp(min=0)[:, None], 1.0 - sm)
+        left = t < 0
+        loss.append((-(y * logp).sum(1)).masked_fill(left, 0))
+        if c["bwd"]:
+            g = ((logp.exp() - y) * d[:, None]).masked_fill(left[:, None], 0)
+            dx.append(torch.mm(g, w))
+            dw += torch.mm(g.T, xr)
+    out = {"loss": torch.cat(loss)}
+    if c["bwd"]:
+        out.update(dx=torch.cat(dx), dw=dw.T.contiguous() if c["w_mn"] else dw)
+    return out
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "linear":
+        return _exact_linear(case, s)
+    if case["op"] == "head":
+        return _exact_head(case, s)
+    keep, factor = _exact_keep(s, case["rows"], case["cols"], case["p"])
+    y = (s["x"].double() * factor).masked_fill(~keep, 0)
+    return {"y": y if s["resid"] is None else y + s["resid"].double()}
