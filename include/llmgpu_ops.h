@@ -142,6 +142,72 @@ int llmgpu_op_moe_route(const float* y, const float* mean, const float* rstd, co
 int llmgpu_op_moe_dispatch(const int* idx, int B, int T, int E, int k, int* grp, int* row_of,
                            int* tok_of, void* stream);
 
+/* Dropout from a counter-based generator: out = resid + (kept ? x * scale : 0) over [rows, cols],
+ * resid nullable. x and out are bf16 or f32 (x_f32, out_f32), resid has out's type; ld*: row
+ * strides in elements, any alignment; out may be x or resid itself. Calling it with the gradient
+ * in place of x (and no resid) is the backward: the mask is formed again, never stored.
+ *   Element (row, col) is dropped when its 16-bit lane is below round(p * 65536): lane col % 8 (low
+ *   half of word 0 first) of Philox4x32-10 keyed by the seed, at counter (col / 8, row, low and high
+ *   half of offset + site). scale = 65536 / (65536 - round(p * 65536)). p in [0, 1]: p = 1 drops
+ *   everything (out = resid or 0); a dropped element gives 0 whatever x holds.
+ *   rng: two uint64 in device memory, {seed, offset}, read when the kernel runs, so that the
+ *   replays of a captured step can advance the offset; `site` tells the dropouts of one step
+ *   apart. cols <= 2^30. */
+int llmgpu_op_dropout(const void* x, int x_f32, long long ldx, const void* resid, long long ldr,
+                      void* out, int out_f32, long long ldo, int rows, int cols, float p,
+                      const uint64_t* rng, uint64_t site, void* stream);
+/* Linear layer in one product: z = x w^T + bias, out = resid + drop(act(z)).
+ *   x [M, K] and w [N, K] (w_mn_major = 0) or [K, N] (1) are bf16, rows 16-byte aligned (base
+ *   address and ldx, ldw a multiple of 8 elements: otherwise a negative status); bias [N] f32,
+ *   nullable; act: 0 none, 1 relu, 2 gelu (tanh form), 3 silu; drop: llmgpu_op_dropout over the
+ *   [M, N] result with (p, rng, site), none when p = 0 (rng may then be NULL); resid (nullable) has
+ *   out's type, bf16 or f32 (out_f32), and may be out itself. pre (nullable, bf16): z, which the
+ *   backward needs when act is not none. out, resid and pre take any row stride. M = 0 is allowed.
+ *   err as in llmgpu_op_gemm. */
+int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long ldw, int w_mn_major,
+                         const float* bias, int act, float p, const uint64_t* rng, uint64_t site,
+                         const void* resid, long long ldr, void* pre, long long ld_pre, void* out,
+                         int out_f32, long long ldo, int M, int N, int K, int* err, void* stream);
+/* Its backward: dz = drop(dy) * act'(pre), rounded to bf16 for the products; dbias = column sums of
+ * dz before that rounding, dx = dz w, dw = dz^T x (in w's layout); the residual's gradient is dy
+ * itself. dx, dw, dbias are nullable; dx and dw are bf16 or f32. `accumulate` adds into dw (f32
+ * only) and dbias. M = 0 writes zero gradients. `work`: llmgpu_op_linear_bwd_work(M, N, K) bytes,
+ * 16-byte aligned. dy: bf16 or f32 (dy_f32), any row stride; x, w as in the forward; (p, rng,
+ * site) the forward's, with the values that rng held then. */
+long long llmgpu_op_linear_bwd_work(int M, int N, int K);
+int llmgpu_op_linear_bwd(const void* dy, int dy_f32, long long lddy, const void* x, long long ldx,
+                         const void* w, long long ldw, int w_mn_major, const void* pre,
+                         long long ld_pre, int act, float p, const uint64_t* rng, uint64_t site,
+                         void* dx, int dx_f32, long long lddx, void* dw, int dw_f32,
+                         long long lddw, float* dbias, int accumulate, int M, int N, int K,
+                         void* work, int* err, void* stream);
+/* Loss head without logits: softmax cross-entropy of x [rows, C] w^T against targets, w [V, C]
+ * (w_mn_major = 0) or [C, V] (1), both bf16 with 16-byte aligned rows. The logits are f32
+ * accumulators that are never written. row_loss = sum_v y_v (lse - z_v) with y = 1 - smoothing at the
+ * target and smoothing / (V - 1) elsewhere, whose gradient is the backward's below (and that of
+ * llmgpu_op_cross_entropy, which reports lse - z_target whatever the smoothing); lse [rows]: the
+ * rows' log-sum-exp, for the backward. A target outside [0, V) leaves its row out: loss 0. `work`:
+ * llmgpu_op_linear_ce_fwd_work(rows, V) bytes, 16-byte aligned. rows = 0 is allowed. */
+long long llmgpu_op_linear_ce_fwd_work(int rows, int V);
+int llmgpu_op_linear_ce_fwd(const void* x, long long ldx, const void* w, long long ldw,
+                            int w_mn_major, const int32_t* targets, int rows, int C, int V,
+                            float smoothing, float* row_loss, float* lse, void* work, int* err,
+                            void* stream);
+/* Gradients of sum_r scale * dloss[r] * row_loss[r] (dloss nullable: ones) by x (dx [rows, C]) and w
+ * (dw, in w's layout), both nullable, bf16 or f32; `accumulate` adds into an f32 dw. The logits
+ * are formed again in pieces of `piece` columns of the vocabulary (a multiple of 256; 0 lets the
+ * library choose), and the gradient by them, rounded to bf16, is held for one piece at a time.
+ * Rows left out get dx = 0 and add nothing to dw, whatever x holds there. An f32 dw or dx is as
+ * exact as that rounding. `work`: llmgpu_op_linear_ce_bwd_work(rows, C, V, piece) bytes, 16-byte
+ * aligned. */
+long long llmgpu_op_linear_ce_bwd_work(int rows, int C, int V, int piece);
+int llmgpu_op_linear_ce_bwd(const void* x, long long ldx, const void* w, long long ldw,
+                            int w_mn_major, const int32_t* targets, const float* lse,
+                            const float* dloss, float scale, int rows, int C, int V,
+                            float smoothing, void* dx, int dx_f32, long long lddx, void* dw,
+                            int dw_f32, long long lddw, int accumulate, int piece, void* work,
+                            int* err, void* stream);
+
 /* Number of SMs the library sizes persistent grids for (device 0 of the caller). */
 int llmgpu_op_num_sms(void);
 /* CTA pairs (clusters of two SMs) the 256x256-tile GEMM keeps resident at once. */

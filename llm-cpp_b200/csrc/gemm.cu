@@ -9,6 +9,7 @@
 // Every CTA loads its own operand tiles with plain TMA loads.
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <mutex>
@@ -17,6 +18,7 @@
 
 #include "common.cuh"
 #include "gemm.cuh"
+#include "philox.cuh"
 
 namespace llmgpu {
 
@@ -532,12 +534,312 @@ __device__ __forceinline__ void epilogue_tile(const GemmArgs& a, const CUtensorM
     }
 }
 
-template <int BN>
+// ---------------------------------------------------------------------------- epilogue families
+// The epilogues that take a GemmExt are compiled into kernels of their own: family 0 is every
+// epilogue above.
+enum GemmFamily : int { kFamBase = 0, kFamLinear = 1, kFamHeadStats = 2, kFamHeadGrad = 3 };
+struct NoExt {};
+template <int FAM>
+struct ExtOf {
+    using type = GemmExt;
+};
+template <>
+struct ExtOf<kFamBase> {
+    using type = NoExt;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + exp(-t)) from the special-function unit's 2^x and a correctly rounded reciprocal: a few
+// units in the last place, which an f32 output keeps. t far below 0: exp overflows to inf and
+// the result is 0.
+__device__ __forceinline__ float sigmoid_f32(float t) {
+    return __frcp_rn(1.0f + ex2_approx(-t * kLog2e));
+}
+__device__ __forceinline__ float act_apply(int act, float z) {
+    switch (act) {
+        case kActRelu:
+            return z > 0.0f ? z : (z == z ? 0.0f : z);
+        case kActGelu: {
+            // 0.5 z (1 + tanh u) = z sigmoid(2u)
+            const float u2 = 1.5957691216f * z * fmaf(0.044715f * z, z, 1.0f);
+            return z * sigmoid_f32(u2);
+        }
+        case kActSilu:
+            return z * sigmoid_f32(z);
+        default:
+            return z;
+    }
+}
+
+// resid + drop(act(acc + bias)). A lane holds 32 columns of its row; they are turned through the
+// warp's 8 KB of shared memory (32 rows of 33 floats) so that every access to the outputs and
+// to the residual is a row of 32 neighbouring columns, whatever their strides and alignment.
+template <int NCOLS>
+__device__ __forceinline__ void linear_epilogue_tile(const GemmArgs& a, const GemmExt& x,
+                                                     const DropKey& key, uint32_t tbase, int row0,
+                                                     int n0, int lane, EpiWarp& w, int c_begin,
+                                                     int c_end) {
+    if (row0 >= a.M) return;
+    const int row = row0 + lane;
+    const int nrows = min(32, a.M - row0);
+    float* tile = reinterpret_cast<float*>(w.stage);
+#pragma unroll 1
+    for (int c = c_begin; c < c_end; ++c) {
+        const int col0 = n0 + c * 32;
+        if (col0 >= a.N) break;
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tbase + (uint32_t)(c * 32), r);
+        const int col = col0 + lane;
+        const bool in = col < a.N;
+        const float b = (x.bias && in) ? x.bias[col] : 0.0f;
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + __shfl_sync(0xffffffffu, b, j);
+        if (a.aux) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = v[j];
+            __syncwarp();
+            __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.aux) + row0 * a.ld_aux + col;
+            if (in)
+                for (int i = 0; i < nrows; ++i)
+                    p[i * a.ld_aux] = __float2bfloat16_rn(tile[i * 33 + lane]);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = act_apply(x.act, v[j]);
+        if (x.rng) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t m =
+                    drop_keep8(key, (uint32_t)(col0 >> 3) + q, (uint32_t)row, x.drop_thr);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[8 * q + j] = ((m >> j) & 1u) ? v[8 * q + j] * x.drop_scale : 0.0f;
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = v[j];
+        __syncwarp();
+        if (in) {
+            if (x.out_f32) {
+                float* p = reinterpret_cast<float*>(a.out) + row0 * a.ldo + col;
+                const float* q = x.resid ? reinterpret_cast<const float*>(x.resid) + row0 * x.ldr + col
+                                         : nullptr;
+#pragma unroll 4
+                for (int i = 0; i < nrows; ++i) {
+                    float o = tile[i * 33 + lane];
+                    if (q) o += q[i * x.ldr];
+                    p[i * a.ldo] = o;
+                }
+            } else {
+                __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + row0 * a.ldo + col;
+                const __nv_bfloat16* q =
+                    x.resid ? reinterpret_cast<const __nv_bfloat16*>(x.resid) + row0 * x.ldr + col
+                            : nullptr;
+#pragma unroll 4
+                for (int i = 0; i < nrows; ++i) {
+                    float o = tile[i * 33 + lane];
+                    if (q) o += __bfloat162float(q[i * x.ldr]);
+                    p[i * a.ldo] = __float2bfloat16_rn(o);
+                }
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// out_f32 planes [split][M][ldo]: plane `split` (+)= the partial product of its k-range. One tile
+// owns an element of a plane in a launch, so the sums do not depend on the tiles' order.
+template <int NCOLS>
+__device__ __forceinline__ void plane_epilogue_tile(const GemmArgs& a, const CUtensorMap* tmO,
+                                                    uint32_t tbase, int row0, int n0, int split,
+                                                    int lane, EpiWarp& w, int c_begin, int c_end) {
+    if (row0 >= a.M) return;
+#pragma unroll 1
+    for (int c = c_begin; c < c_end; ++c) {
+        const int col0 = n0 + c * 32;
+        if (col0 >= a.N) break;
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tbase + (uint32_t)(c * 32), r);
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        uint8_t* box = w.stage + w.slot * kEpiSlotBytes;
+        if (lane == 0) bulk_wait_group_read<1>();
+        __syncwarp();
+        box_put_f32(box, lane, v);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            if (a.accumulate)
+                tma_reduce_add_3d(tmO, box, col0, row0, split);
+            else
+                tma_store_3d(tmO, box, col0, row0, split);
+            bulk_commit_group();
+        }
+        w.slot ^= 1;
+    }
+}
+
+// Softmax statistics of one lane's row over each 128 columns (a slot) of its share of the tile:
+// running maximum and sum of 2^((z - max) log2 e), merged over the slots by a later kernel. A
+// slot whose logits are all -inf keeps max = -inf and sum 0; NaN goes through the sum.
+template <int NCOLS>
+__device__ __forceinline__ void head_stats_tile(const GemmArgs& a, const GemmExt& x,
+                                                uint32_t tbase, int row0, int n0, int lane,
+                                                int c_begin, int c_end) {
+    static_assert(NCOLS % 128 == 0, "slots of 128 columns");
+    if (row0 >= a.M) return;
+    const int row = row0 + lane;
+    const int t = row < a.M ? x.targets[row] : -1;
+    const float ninf = __int_as_float(0xff800000);
+#pragma unroll 1
+    for (int c4 = c_begin; c4 < c_end; c4 += 4) {
+        if (n0 + c4 * 32 >= a.N) break;
+        float m = ninf, s = 0.0f, zs = 0.0f;
+#pragma unroll 1
+        for (int c = c4; c < c4 + 4; ++c) {
+            const int col0 = n0 + c * 32;
+            if (col0 >= a.N) break;
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(tbase + (uint32_t)(c * 32), r);
+            tmem_ld_wait();
+            const int nv = min(32, a.N - col0);
+            float mc = ninf;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                if (j >= nv) r[j] = 0xff800000u;
+                mc = fmaxf(mc, __uint_as_float(r[j]));
+            }
+            if (x.zsum) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) zs += j < nv ? __uint_as_float(r[j]) : 0.0f;
+            }
+            const int tj = t - (x.v0 + col0);
+            if (tj >= 0 && tj < nv) {
+                float z = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (j == tj) z = __uint_as_float(r[j]);
+                x.zt[row] = z;
+            }
+            __syncwarp();
+            if (mc > m) {
+                s = s == 0.0f ? 0.0f : s * ex2_approx((m - mc) * kLog2e);
+                m = mc;
+            }
+            const float ml = m == ninf ? 0.0f : m * kLog2e;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s += ex2_approx(fmaf(__uint_as_float(r[j]), kLog2e, -ml));
+        }
+        if (row < a.M) {
+            const long long at = (long long)((n0 + c4 * 32) >> 7) * a.M + row;
+            x.part[at] = make_float2(m, s);
+            if (x.zsum) x.zsum[at] = zs;
+        }
+        __syncwarp();
+    }
+}
+
+// coef * (softmax - y) of the recomputed logits, bf16, through 32 x 64 boxes (two chunks).
+template <int NCOLS>
+__device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt& x,
+                                               const CUtensorMap* tmO, uint32_t tbase, int row0,
+                                               int n0, int lane, EpiWarp& w, int c_begin,
+                                               int c_end) {
+    if (row0 >= a.M) return;
+    const int row = row0 + lane;
+    const int t = row < a.M ? x.targets[row] : -1;
+    const bool counts = t >= 0 && t < x.V;
+    const float coef = counts ? x.scale * (x.dloss ? x.dloss[row] : 1.0f) : 0.0f;
+    const float ll = counts ? x.lse[row] * kLog2e : 0.0f;
+#pragma unroll 1
+    for (int c = c_begin; c < c_end; c += 2) {
+        const int col0 = n0 + c * 32;
+        if (col0 >= a.N) break;
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(tbase + (uint32_t)(c * 32), r[0]);
+        tmem_ld_32x32b_x32(tbase + (uint32_t)((c + 1) * 32), r[1]);
+        tmem_ld_wait();
+        uint8_t* box = w.stage + w.slot * kEpiSlotBytes;
+        if (lane == 0) bulk_wait_group_read<1>();
+        __syncwarp();
+        const int tj = t - (x.v0 + col0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+                uint32_t o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float g[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 8 * ch + 2 * k + i;
+                        const float p =
+                            ex2_approx(fmaf(__uint_as_float(r[h][j]), kLog2e, -ll));
+                        const float y = (32 * h + j == tj) ? x.on : x.off;
+                        g[i] = counts ? coef * (p - y) : 0.0f;
+                    }
+                    o[k] = pack_bf16x2(g[0], g[1]);
+                }
+                *reinterpret_cast<uint4*>(box + box_off_f32(lane, 4 * h + ch)) =
+                    make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_3d(tmO, box, col0, row0, 0);
+            bulk_commit_group();
+        }
+        w.slot ^= 1;
+    }
+}
+
+// One accumulator tile of one warp, any family.
+template <int FAM, int NCOLS>
+__device__ __forceinline__ void family_tile(const GemmArgs& a,
+                                            const typename ExtOf<FAM>::type& x,
+                                            const DropKey& key, const CUtensorMap* tmO,
+                                            const CUtensorMap* tmX, uint32_t tbase, bool empty,
+                                            int row0, int n0, int split, int g, int lane,
+                                            EpiWarp& w, int c_begin, int c_end) {
+    if constexpr (FAM == kFamBase) {
+        epilogue_tile<NCOLS>(a, tmO, tmX, tbase, empty, row0, n0, split, g, lane, w, c_begin,
+                             c_end);
+    } else if constexpr (FAM == kFamLinear) {
+        if (a.epi == kEpiPlaneAdd)
+            plane_epilogue_tile<NCOLS>(a, tmO, tbase, row0, n0, split, lane, w, c_begin, c_end);
+        else
+            linear_epilogue_tile<NCOLS>(a, x, key, tbase, row0, n0, lane, w, c_begin, c_end);
+    } else if constexpr (FAM == kFamHeadStats) {
+        head_stats_tile<NCOLS>(a, x, tbase, row0, n0, lane, c_begin, c_end);
+    } else {
+        head_grad_tile<NCOLS>(a, x, tmO, tbase, row0, n0, lane, w, c_begin, c_end);
+    }
+}
+
+// The dropout key of an epilogue warp, read once.
+template <int FAM>
+__device__ __forceinline__ DropKey family_key(const typename ExtOf<FAM>::type& x) {
+    if constexpr (FAM == kFamLinear) {
+        if (x.rng) return drop_key(x.rng, x.site);
+    }
+    return DropKey{0u, 0u, 0u, 0u};
+}
+
+template <int BN, int FAM>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_bf16_tc_kernel(const __grid_constant__ CUtensorMap tmA,
                         const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmO,
-                        const __grid_constant__ CUtensorMap tmX, const GemmArgs args) {
+                        const __grid_constant__ CUtensorMap tmX, const GemmArgs args,
+                        const typename ExtOf<FAM>::type ext) {
     using Cfg = GemmCfg<BN>;
     constexpr int STAGES = Cfg::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -722,6 +1024,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         // ---------------- epilogue warpgroup
         const int q = warp - 4;
         EpiWarp ew{sEpi + q * 2 * kEpiSlotBytes, &epi_bar[2 * q], 0u, 0, 0u};
+        const DropKey key = family_key<FAM>(ext);
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int t = blockIdx.x; t < total; t += gridDim.x) {
@@ -730,7 +1033,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                            g, kb0, kb1))
                 continue;
             const int m0 = m_blk * BM, n0 = n_blk * BN;
-            epilogue_prefetch(args, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
+            if constexpr (FAM == kFamBase)
+                epilogue_prefetch(args, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
             if (!mbar_wait_bounded(&acc_full[acc], acc_phase, args.err, kDevTimeoutAcc)) {
                 epilogue_drain(args, lane, ew);
                 break;
@@ -738,8 +1042,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             tc_fence_after();
             const uint32_t tbase =
                 tmem_base + (uint32_t)(acc * BN) + ((uint32_t)(q * 32) << 16);
-            epilogue_tile<BN>(args, &tmO, &tmX, tbase, kb1 <= kb0, m0 + q * 32, n0, split, g,
-                              lane, ew);
+            family_tile<FAM, BN>(args, ext, key, &tmO, &tmX, tbase, kb1 <= kb0, m0 + q * 32, n0,
+                                 split, g, lane, ew, 0, BN / 32);
             tc_fence_before();
             mbar_arrive(&acc_empty[acc]);
             acc ^= 1;
@@ -806,7 +1110,7 @@ __device__ __forceinline__ uint32_t pair_stage_bytes(const GemmArgs& a, int am, 
 // (split-major tile order within a product). A pair whose SMs start late, held by another
 // kernel such as a collective, takes fewer units. queue[1] counts the pairs that have
 // finished claiming; the last one resets both counters for the next launch.
-template <int NG>
+template <int NG, int FAM = kFamBase>
 struct PairParams {
     CUtensorMap tmA[NG];
     CUtensorMap tmB[NG];
@@ -818,6 +1122,7 @@ struct PairParams {
     int* queue;
     int q_first;
     int q_total[2];
+    typename ExtOf<FAM>::type ext;
 };
 
 constexpr int kItemSlots = 4;
@@ -829,8 +1134,8 @@ constexpr int kItemConsumers = 2 + 2 * kPairEpiWarps;
 constexpr int kClaimAhead = 4;
 
 // Unit number idx of the run-time queue as (product << 24 | tile), -1 past the last one.
-template <int NG>
-__device__ __forceinline__ int pair_queue_unit(const PairParams<NG>& P, int idx) {
+template <int NG, int FAM>
+__device__ __forceinline__ int pair_queue_unit(const PairParams<NG, FAM>& P, int idx) {
     const int f = P.q_first, n0 = P.q_total[f];
     if (idx < n0) return (f << 24) | idx;
     idx -= n0;
@@ -903,7 +1208,8 @@ struct PairItems {
     const int* list;
     int n, i, next;
     int cid, nclusters, total;
-    __device__ __forceinline__ PairItems(const PairParams<NG>& P, int cid_, int ncl) {
+    template <int FAM>
+    __device__ __forceinline__ PairItems(const PairParams<NG, FAM>& P, int cid_, int ncl) {
         cid = cid_;
         nclusters = ncl;
         i = 0;
@@ -937,9 +1243,9 @@ struct PairItems {
     }
 };
 
-template <int NG>
+template <int NG, int FAM>
 __global__ void __launch_bounds__(kPairThreads, 1)
-    gemm_bf16_pair_kernel(const __grid_constant__ PairParams<NG> P) {
+    gemm_bf16_pair_kernel(const __grid_constant__ PairParams<NG, FAM> P) {
     using Cfg = PairCfg;
     constexpr int STAGES = Cfg::STAGES;
     constexpr int BN = Cfg::BN;
@@ -1162,6 +1468,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const int q = e & 3, half = e >> 2;
         const uint32_t acc_empty_leader = mapa_shared(smem_u32(&acc_empty[0]), 0);
         EpiWarp ew{sEpi + e * 2 * kEpiSlotBytes, &epi_bar[2 * e], 0u, 0, 0u};
+        const DropKey key = family_key<FAM>(P.ext);
         int acc = 0;
         uint32_t acc_phase = 0;
         int g, t;
@@ -1182,8 +1489,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tile_work(args, s_grp, t, sh.num_m, sh.num_n, sh.tiles_mn, sh.kblocks, m_blk, n_blk,
                       split, gi, kb0, kb1);
             const int m0 = m_blk * Cfg::BMP + 128 * (int)rank, n0 = n_blk * BN;
-            epilogue_prefetch(args, &P.tmX[g], m0 + q * 32, n0, lane, ew, half * (BN / 64),
-                              (half + 1) * (BN / 64));
+            if constexpr (FAM == kFamBase)
+                epilogue_prefetch(args, &P.tmX[g], m0 + q * 32, n0, lane, ew, half * (BN / 64),
+                                  (half + 1) * (BN / 64));
             if (!mbar_wait_bounded_cluster(&acc_full[acc], acc_phase, err, kDevTimeoutAcc)) {
                 epilogue_drain(args, lane, ew);
                 break;
@@ -1191,8 +1499,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const uint32_t tbase =
                 tmem_base + (uint32_t)(acc * BN) + ((uint32_t)(q * 32) << 16);
-            epilogue_tile<BN>(args, &P.tmO[g], &P.tmX[g], tbase, kb1 <= kb0, m0 + q * 32, n0,
-                              split, gi, lane, ew, half * (BN / 64), (half + 1) * (BN / 64));
+            family_tile<FAM, BN>(args, P.ext, key, &P.tmO[g], &P.tmX[g], tbase, kb1 <= kb0,
+                                 m0 + q * 32, n0, split, gi, lane, ew, half * (BN / 64),
+                                 (half + 1) * (BN / 64));
             tc_fence_before();
             if (leader)
                 mbar_arrive(&acc_empty[acc]);
@@ -1372,7 +1681,8 @@ int make_tmap_box(CUtensorMap* tm, const void* ptr, bool f32, uint64_t x, uint64
 // or base address cannot be described (the per-thread store path is used then).
 bool plan_tma_epilogue(GemmPlan* plan, const GemmArgs& a) {
     if (a.scalar_store) return false;
-    const bool f32 = (a.epi == kEpiStoreF32 || a.epi == kEpiResidF32 || a.epi == kEpiSplitPartial);
+    const bool f32 = (a.epi == kEpiStoreF32 || a.epi == kEpiResidF32 ||
+                      a.epi == kEpiSplitPartial || a.epi == kEpiPlaneAdd);
     const uint64_t elt = f32 ? 4 : 2;
     const uint64_t ys = (uint64_t)a.ldo * elt;
     uint64_t x = (uint64_t)a.N, z = 1, zs = ys * (uint64_t)a.M;
@@ -1389,6 +1699,8 @@ bool plan_tma_epilogue(GemmPlan* plan, const GemmArgs& a) {
         z = (uint64_t)a.splits;
         zs = (uint64_t)a.M * (uint64_t)a.N * 4;  // planes [split][M][N], ldo == N
         if (a.ldo != a.N) return false;
+    } else if (a.epi == kEpiPlaneAdd) {
+        z = (uint64_t)a.splits;  // planes [split][M][ldo]
     }
     zs = (zs + 15) & ~(uint64_t)15;  // a single plane: any aligned stride
     if (z > 1 && ((a.epi == kEpiStoreF32 && ((a.grp_mode == kGroupK ? a.out_grp_stride
@@ -1397,7 +1709,7 @@ bool plan_tma_epilogue(GemmPlan* plan, const GemmArgs& a) {
         return false;
     // plain bf16 outputs leave in 32 x 64 boxes (two chunks per store)
     if (make_tmap_box(&plan->tmO, a.out, f32, x, (uint64_t)a.M, z, ys, zs,
-                      a.epi == kEpiStoreBF16 || a.epi == kEpiDGeluBF16))
+                      a.epi == kEpiStoreBF16 || a.epi == kEpiDGeluBF16 || a.epi == kEpiHeadGrad))
         return false;
     if (a.epi == kEpiResidF32) {
         const uint64_t rs = (uint64_t)a.ldr * 4;
@@ -1427,33 +1739,44 @@ bool pdl_enabled() {
 
 namespace {
 
-template <int BN>
-int launch_bn(const GemmPlan& p, cudaStream_t stream) {
-    static bool attr_set = false;
-    if (!attr_set) {
-        if (cudaFuncSetAttribute(gemm_bf16_tc_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)GemmCfg<BN>::SMEM) != cudaSuccess)
-            return -10;
-        attr_set = true;
+// Raises a kernel's dynamic shared-memory limit, once per device (the attribute belongs to the
+// device's context).
+template <typename K>
+int set_smem_limit(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return -10;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+    if (bit && (done.load(std::memory_order_acquire) & bit)) return 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
+        cudaSuccess) {
+        cudaGetLastError();
+        return -10;
     }
-    return launch_kernel_pdl(gemm_bf16_tc_kernel<BN>, p.grid, kGemmThreads, GemmCfg<BN>::SMEM,
-                             stream, p.tmA, p.tmB, p.tmO, p.tmX, p.args);
+    done.fetch_or(bit, std::memory_order_release);
+    return 0;
 }
 
+template <int FAM>
+typename ExtOf<FAM>::type plan_ext(const GemmPlan& p) {
+    if constexpr (FAM == kFamBase)
+        return NoExt{};
+    else
+        return p.ext;
+}
+
+template <int BN, int FAM = kFamBase>
+int launch_bn(const GemmPlan& p, cudaStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    if (set_smem_limit(gemm_bf16_tc_kernel<BN, FAM>, GemmCfg<BN>::SMEM, done)) return -10;
+    return launch_kernel_pdl(gemm_bf16_tc_kernel<BN, FAM>, p.grid, kGemmThreads,
+                             GemmCfg<BN>::SMEM, stream, p.tmA, p.tmB, p.tmO, p.tmX, p.args,
+                             plan_ext<FAM>(p));
+}
+
+template <int NG, int FAM>
 int pair_set_attr() {
-    static int rc = -1;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        rc = (cudaFuncSetAttribute(gemm_bf16_pair_kernel<1>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)PairCfg::SMEM) == cudaSuccess &&
-              cudaFuncSetAttribute(gemm_bf16_pair_kernel<2>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)PairCfg::SMEM) == cudaSuccess)
-                 ? 0
-                 : -10;
-    });
-    return rc;
+    static std::atomic<uint64_t> done{0};
+    return set_smem_limit(gemm_bf16_pair_kernel<NG, FAM>, PairCfg::SMEM, done);
 }
 
 // Clusters of two that can be resident at once (one CTA per SM).
@@ -1462,7 +1785,7 @@ int pair_max_clusters(int num_sms) {
     static std::once_flag once;
     std::call_once(once, [num_sms] {
         n = num_sms / 2;
-        if (pair_set_attr()) return;
+        if (pair_set_attr<1, kFamBase>()) return;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * (num_sms / 2), 1, 1);
         cfg.blockDim = dim3(kPairThreads, 1, 1);
@@ -1475,7 +1798,7 @@ int pair_max_clusters(int num_sms) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int c = 0;
-        if (cudaOccupancyMaxActiveClusters(&c, gemm_bf16_pair_kernel<1>, &cfg) == cudaSuccess &&
+        if (cudaOccupancyMaxActiveClusters(&c, gemm_bf16_pair_kernel<1, kFamBase>, &cfg) == cudaSuccess &&
             c > 0)
             n = c < n ? c : n;
         cudaGetLastError();
@@ -1483,9 +1806,9 @@ int pair_max_clusters(int num_sms) {
     return n;
 }
 
-template <int NG>
-int launch_pair_params(const PairParams<NG>& P, int grid, cudaStream_t stream) {
-    if (pair_set_attr()) return -10;
+template <int NG, int FAM>
+int launch_pair_params(const PairParams<NG, FAM>& P, int grid, cudaStream_t stream) {
+    if (pair_set_attr<NG, FAM>()) return -10;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3(kPairThreads, 1, 1);
@@ -1500,12 +1823,13 @@ int launch_pair_params(const PairParams<NG>& P, int grid, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_bf16_pair_kernel<NG>, P);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_bf16_pair_kernel<NG, FAM>, P);
     return e == cudaSuccess ? 0 : -(1000 + (int)e);
 }
 
+template <int FAM = kFamBase>
 int launch_pair(const GemmPlan& p, cudaStream_t stream) {
-    PairParams<1> P;
+    PairParams<1, FAM> P;
     P.tmA[0] = p.tmA;
     P.tmB[0] = p.tmB;
     P.tmO[0] = p.tmO;
@@ -1516,16 +1840,21 @@ int launch_pair(const GemmPlan& p, cudaStream_t stream) {
     P.queue = nullptr;
     P.q_first = 0;
     P.q_total[0] = P.q_total[1] = 0;
-    return launch_pair_params<1>(P, p.grid, stream);
+    P.ext = plan_ext<FAM>(p);
+    return launch_pair_params(P, p.grid, stream);
 }
 
 }  // namespace
 
 int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major, const void* B,
                    long long ldb, int b_mn_major, int M, int N, int K, const GemmArgs& epi,
-                   int bn_hint, int num_sms) {
+                   int bn_hint, int num_sms, const GemmExt* ext) {
     if (M <= 0 || N <= 0 || K <= 0) return -1;
     GemmArgs a = epi;
+    if ((a.epi >= kEpiLinear) != (ext != nullptr)) return -45;
+    if (ext && a.grp_mode != kGroupNone) return -45;
+    const bool head = a.epi == kEpiHeadStats || a.epi == kEpiHeadGrad;
+    if (ext) plan->ext = *ext;
     a.M = M;
     a.N = N;
     a.K = K;
@@ -1547,7 +1876,8 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
     } else if (a.splits > kblocks) {
         return -5;
     }
-    if (a.splits > 1 && a.epi != kEpiSplitPartial && a.grp_mode != kGroupK) return -6;
+    if (a.splits > 1 && a.epi != kEpiSplitPartial && a.epi != kEpiPlaneAdd && a.grp_mode != kGroupK)
+        return -6;
     if (a.col_group <= 0) a.col_group = N;
     if (a.col_group != N && (a.col_group % 32) != 0) return -7;
     // alignment needed by the vectorised epilogue
@@ -1578,6 +1908,7 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
         const int cands[4] = {kGemmPairTile, 256, 128, 64};
         for (int i = pair_ok ? 0 : 1; i < 4; ++i) {
             const int c = cands[i];
+            if (head && c != kGemmPairTile && c != 128) continue;  // the tiles its kernels have
             double cost;
             if (c == kGemmPairTile) {
                 const long long tiles = (long long)((M + 255) / 256) * ((N + 255) / 256) * a.splits;
@@ -1597,7 +1928,15 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
     }
     plan->bn = bn;
     a.tma_epi = 0;
-    if (std::getenv("LLMGPU_GEMM_DIRECT_EPILOGUE") == nullptr) a.tma_epi = plan_tma_epilogue(plan, a) ? 1 : 0;
+    if (ext) {
+        if (head && bn != kGemmPairTile && bn != 128) return -46;
+        if (a.epi == kEpiHeadGrad || a.epi == kEpiPlaneAdd) {
+            a.tma_epi = plan_tma_epilogue(plan, a) ? 1 : 0;
+            if (!a.tma_epi) return -8;
+        }
+    } else if (std::getenv("LLMGPU_GEMM_DIRECT_EPILOGUE") == nullptr) {
+        a.tma_epi = plan_tma_epilogue(plan, a) ? 1 : 0;
+    }
     if (!a.tma_epi) plan->tmO = plan->tmX = CUtensorMap{};
     // the rotary epilogue runs on the bf16 TMA store path only
     if (a.rope && (a.epi != kEpiStoreBF16 || !a.tma_epi || a.rope_T <= 0 || a.rope_hd <= 0 ||
@@ -1759,7 +2098,7 @@ int gemm_run2(const GemmPlan2& plan, cudaStream_t stream, bool queue) {
     P.q_first = plan.q_first;
     P.q_total[0] = plan.q_total[0];
     P.q_total[1] = plan.q_total[1];
-    return launch_pair_params<2>(P, plan.grid, stream);
+    return launch_pair_params(P, plan.grid, stream);
 }
 
 void gemm_free_plan2(GemmPlan2* plan) {
@@ -1769,6 +2108,23 @@ void gemm_free_plan2(GemmPlan2* plan) {
 }
 
 int gemm_run(const GemmPlan& p, cudaStream_t stream) {
+    const bool pair = p.bn == kGemmPairTile;
+    switch (p.args.epi) {
+        case kEpiHeadStats:
+            return pair ? launch_pair<kFamHeadStats>(p, stream)
+                        : launch_bn<128, kFamHeadStats>(p, stream);
+        case kEpiHeadGrad:
+            return pair ? launch_pair<kFamHeadGrad>(p, stream)
+                        : launch_bn<128, kFamHeadGrad>(p, stream);
+        case kEpiLinear:
+        case kEpiPlaneAdd:
+            if (pair) return launch_pair<kFamLinear>(p, stream);
+            if (p.bn == 256) return launch_bn<256, kFamLinear>(p, stream);
+            return p.bn == 128 ? launch_bn<128, kFamLinear>(p, stream)
+                               : launch_bn<64, kFamLinear>(p, stream);
+        default:
+            break;
+    }
     switch (p.bn) {
         case 256:
             return launch_bn<256>(p, stream);

@@ -20,7 +20,43 @@ enum GemmEpilogue : int {
     kEpiResidF32 = 2,    // out_f32 = resid + acc
     kEpiGeluBF16 = 3,    // aux_bf16 = acc ; out_bf16 = gelu(acc)
     kEpiDGeluBF16 = 4,   // out_bf16 = acc * gelu'(aux_bf16)
-    kEpiSplitPartial = 5 // out_f32[split][M][N] = partial acc (reduced by gemm_splitk_reduce)
+    kEpiSplitPartial = 5, // out_f32[split][M][N] = partial acc (reduced by gemm_splitk_reduce)
+    // The epilogues below take a GemmExt and run in kernels of their own, so that the ones above
+    // keep their code.
+    kEpiLinear = 6,      // out = resid + drop(act(acc + bias)), bf16 or f32; aux = acc + bias
+    kEpiPlaneAdd = 7,    // out_f32[split][M][ldo] (+)= partial acc (planes kept apart)
+    kEpiHeadStats = 8,   // softmax statistics of the logits acc; no matrix is written
+    kEpiHeadGrad = 9     // out_bf16 = gradient of the loss by the logits acc
+};
+
+enum LinearAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
+
+// Arguments of the epilogues from kEpiLinear on.
+struct GemmExt {
+    // kEpiLinear
+    const float* bias;    // [N], nullable
+    int act;              // LinearAct
+    int out_f32;          // out and resid are f32, else bf16
+    const void* resid;    // nullable; row stride ldr elements
+    long long ldr;
+    const uint64_t* rng;  // device {seed, offset}; null: no dropout
+    uint64_t site;        // added to the offset
+    uint32_t drop_thr;
+    float drop_scale;
+    // kEpiHeadStats, kEpiHeadGrad: row m's target (left out unless in [0, V)), V = all columns
+    // of the vocabulary, this product's column 0 being column v0 of it
+    const int32_t* targets;
+    int v0, V;
+    // kEpiHeadStats: slot p of 128 columns writes (max, sum of exp(z - max)) to part[p * M + m],
+    // the sum of z to zsum[p * M + m] (nullable), and the target's logit to zt[m]
+    float2* part;
+    float* zsum;
+    float* zt;
+    // kEpiHeadGrad: out = coef * (exp(z - lse) - y), coef = scale * dloss[m] (dloss nullable: 1),
+    // y = on at the target and off elsewhere; 0 in rows left out
+    const float* lse;
+    const float* dloss;
+    float scale, on, off;
 };
 
 struct GemmArgs {
@@ -79,6 +115,7 @@ struct GemmPlan {
     CUtensorMap tmO;       // output boxes of 32x32 (3-D: column groups, splits or groups)
     CUtensorMap tmX;       // epilogue input / second output (residual or pre-activation)
     GemmArgs args;
+    GemmExt ext;           // epilogues from kEpiLinear on
     int bn;                // 64, 128, 256, or kGemmPairTile (256x256 on a CTA pair)
     int grid;
     size_t smem_bytes;
@@ -86,11 +123,12 @@ struct GemmPlan {
 
 // Builds a plan. A is [M,K] (K-major, lda >= K) or [K,M] (MN-major, lda >= M);
 // B is [N,K] (K-major) or [K,N] (MN-major). Returns 0 on success.
+// `ext` is needed by, and only by, the epilogues from kEpiLinear on (ungrouped products).
 // Grouped plans: kGroupRows takes M = row capacity of A/out and K a multiple of 64;
 // kGroupK takes M, N of one group's output and K = row capacity of A and B.
 int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major, const void* B,
                    long long ldb, int b_mn_major, int M, int N, int K, const GemmArgs& epi,
-                   int bn_hint, int num_sms);
+                   int bn_hint, int num_sms, const GemmExt* ext = nullptr);
 // Launches a plan on a stream.
 int gemm_run(const GemmPlan& plan, cudaStream_t stream);
 // CTA pairs of the pair-tile kernel that can be resident at once.

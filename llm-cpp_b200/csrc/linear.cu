@@ -1,0 +1,290 @@
+// Linear layer with bias, activation, dropout and residual applied where the product's tiles leave
+// tensor memory (gemm.cu, kEpiLinear), and its backward: one elementwise pass forms dz in bf16
+// and the bias gradient's partial sums, then two products give dx and dw.
+#include "linear.cuh"
+
+#include "common.cuh"
+#include "philox.cuh"
+
+namespace llmgpu {
+
+namespace {
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+long long ceil8(long long n) { return (n + 7) & ~7ll; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr int kDzCols = 256;  // columns of a block: 32 lanes of 8
+constexpr int kDzRows = 8;    // rows in flight, one per warp
+
+// Row groups of the elementwise backward: enough blocks to fill the device a few times over.
+int dz_groups(int M, int N) {
+    const int gx = (N + kDzCols - 1) / kDzCols;
+    int gy = (148 * 8 + gx - 1) / gx;
+    const int most = (M + kDzRows - 1) / kDzRows;
+    if (gy > most) gy = most;
+    return gy < 1 ? 1 : gy;
+}
+
+__device__ __forceinline__ float act_grad(int act, float z) {
+    switch (act) {
+        case kActRelu:
+            return z > 0.0f ? 1.0f : 0.0f;
+        case kActGelu: {
+            // gelu(z) = z h, h = sigmoid(2u): h + z h (1 - h) 2u'
+            const float z2 = z * z;
+            const float t = 1.5957691216f * z * fmaf(0.044715f, z2, 1.0f);
+            const float h = __frcp_rn(1.0f + ex2_approx(-t * 1.4426950408889634f));
+            return h + z * h * (1.0f - h) * 1.5957691216f * fmaf(0.134145f, z2, 1.0f);
+        }
+        case kActSilu: {
+            const float h = __frcp_rn(1.0f + ex2_approx(-z * 1.4426950408889634f));
+            return h * (1.0f + z * (1.0f - h));
+        }
+        default:
+            return 1.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        if (vec) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = bf16_lo(w[i]);
+                v[2 * i + 1] = bf16_hi(w[i]);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.0f;
+    } else {
+        if (vec) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0];
+            const float4 b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+    }
+}
+
+// dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable). `vec`:
+// rows of dy and pre start on 16 bytes.
+template <typename T>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long lddy,
+                                                        const bf16* __restrict__ pre,
+                                                        long long ld_pre, int act, DropArgs drop,
+                                                        bf16* __restrict__ dz, long long ldz,
+                                                        float* __restrict__ part, int M, int N,
+                                                        int vec) {
+    pdl_enter();
+    const int lane = threadIdx.x & 31, wr = threadIdx.x >> 5;
+    const int col = blockIdx.x * kDzCols + lane * 8;
+    const int n = min(8, N - col);
+    float sum[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+    if (n > 0) {
+        const bool v8 = vec && n == 8;
+        const DropKey key = drop.rng ? drop_key(drop.rng, drop.site) : DropKey{0u, 0u, 0u, 0u};
+        for (int row = blockIdx.y * kDzRows + wr; row < M; row += gridDim.y * kDzRows) {
+            float v[8], z[8];
+            load8(dy + row * lddy + col, n, v8, v);
+            if (act != kActNone) load8(pre + row * ld_pre + col, n, v8, z);
+            if (drop.rng) {
+                const uint32_t m = drop_keep8(key, (uint32_t)col >> 3, (uint32_t)row, drop.thr);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = ((m >> i) & 1u) ? v[i] * drop.scale : 0.0f;
+            }
+            if (act != kActNone) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= act_grad(act, z[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += v[i];
+            if (dz) {
+                // columns past N, up to the padded stride, are written as zeros
+                *reinterpret_cast<uint4*>(dz + row * ldz + col) =
+                    make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                               pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            }
+        }
+    }
+    if (!part) return;
+    __shared__ float red[kDzRows][kDzCols];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[wr][lane * 8 + i] = sum[i];
+    __syncthreads();
+    const int c = blockIdx.x * kDzCols + threadIdx.x;
+    if (c < N) {
+        float t = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kDzRows; ++r) t += red[r][threadIdx.x];
+        part[(long long)blockIdx.y * N + c] = t;
+    }
+}
+
+// dbias[c] (+)= sum over the row groups, in a fixed order.
+__global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict__ part, int groups,
+                                                         int N, float* __restrict__ dbias,
+                                                         int accumulate) {
+    pdl_enter();
+    __shared__ float red[32][33];
+    const int cc = threadIdx.x & 31, g0 = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + cc;
+    float t = 0.0f;
+    if (c < N)
+        for (int g = g0; g < groups; g += 32) t += part[(long long)g * N + c];
+    red[g0][cc] = t;
+    __syncthreads();
+    if (g0 == 0 && c < N) {
+        float u = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 32; ++g) u += red[g][cc];
+        dbias[c] = accumulate ? dbias[c] + u : u;
+    }
+}
+
+}  // namespace
+
+int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
+            int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
+            int* err, cudaStream_t s) {
+    if (accumulate && !out_f32) return -1;
+    GemmArgs g{};
+    g.out = out;
+    g.ldo = ldo;
+    g.splits = 1;
+    g.err = err;
+    GemmPlan plan;
+    int rc;
+    if (aligned16(out) && (ldo % (out_f32 ? 4 : 8)) == 0) {
+        g.epi = out_f32 ? kEpiStoreF32 : kEpiStoreBF16;
+        g.accumulate = accumulate;
+        rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, M, N, K, g, 0, num_sms);
+    } else {  // rows that no 16-byte store reaches
+        GemmExt x{};
+        g.epi = kEpiLinear;
+        x.out_f32 = out_f32;
+        x.resid = accumulate ? out : nullptr;
+        x.ldr = ldo;
+        rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, M, N, K, g, 0, num_sms, &x);
+    }
+    return rc ? rc : gemm_run(plan, s);
+}
+
+int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
+    if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.act < kActNone || a.act > kActSilu) return -1;
+    if (a.M == 0) return 0;
+    if (!a.x || !a.w || !a.out) return -1;
+    if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw)) return kBadOperand;
+    GemmArgs g{};
+    g.epi = kEpiLinear;
+    g.out = a.out;
+    g.ldo = a.ldo;
+    g.aux = a.pre;
+    g.ld_aux = a.ld_pre;
+    g.splits = 1;
+    g.err = a.err;
+    GemmExt x{};
+    x.bias = a.bias;
+    x.act = a.act;
+    x.out_f32 = a.out_f32;
+    x.resid = a.resid;
+    x.ldr = a.ldr;
+    if (a.drop.thr > 0) {
+        x.rng = a.drop.rng;
+        x.site = a.drop.site;
+        x.drop_thr = a.drop.thr;
+        x.drop_scale = a.drop.scale;
+    }
+    GemmPlan plan;
+    const int rc = gemm_make_plan(&plan, a.x, a.ldx, 0, a.w, a.ldw, a.w_mn_major, a.M, a.N, a.K, g,
+                                  0, num_sms, &x);
+    return rc ? rc : gemm_run(plan, s);
+}
+
+size_t linear_backward_work(int M, int N, int K) {
+    (void)K;
+    if (M <= 0 || N <= 0) return 0;
+    return align256((size_t)M * ceil8(N) * 2) + align256((size_t)dz_groups(M, N) * N * 4);
+}
+
+int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
+    if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.act < kActNone || a.act > kActSilu) return -1;
+    if (a.accumulate && a.dw && !a.dw_f32) return -1;
+    if (a.M == 0) {  // no rows: zero gradients, or nothing to add
+        if (a.accumulate) return 0;
+        const size_t es = a.dw_f32 ? 4 : 2;
+        const int rows = a.w_mn_major ? a.K : a.N, cols = a.w_mn_major ? a.N : a.K;
+        if (a.dw && cudaMemset2DAsync(a.dw, a.lddw * es, 0, cols * es, rows, s) != cudaSuccess)
+            return launch_status();
+        if (a.dbias && cudaMemsetAsync(a.dbias, 0, (size_t)a.N * 4, s) != cudaSuccess)
+            return launch_status();
+        return 0;
+    }
+    if (!a.dy || (a.act != kActNone && !a.pre)) return -1;
+    if ((a.dx && !a.w) || (a.dw && !a.x)) return -1;
+    if ((a.dx && !operand_ok(a.w, a.ldw)) || (a.dw && !operand_ok(a.x, a.ldx))) return kBadOperand;
+    const bool drops = a.drop.rng && a.drop.thr > 0;
+    const bool as_is = !a.dy_f32 && a.act == kActNone && !drops && aligned16(a.dy) &&
+                       (a.lddy & 7) == 0;  // dy is the products' operand itself
+    const bool need_dz = !as_is && (a.dx || a.dw);
+    const bf16* dz = reinterpret_cast<const bf16*>(a.dy);
+    long long ldz = a.lddy;
+    if (need_dz || a.dbias) {
+        if (!a.work || !aligned16(a.work)) return -1;
+        bf16* buf = reinterpret_cast<bf16*>(a.work);
+        float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.work) +
+                                               align256((size_t)a.M * ceil8(a.N) * 2));
+        const int groups = dz_groups(a.M, a.N);
+        DropArgs drop = a.drop;
+        if (!drops) drop.rng = nullptr;
+        const int per16 = a.dy_f32 ? 4 : 8;
+        const int vec = aligned16(a.dy) && (a.lddy % per16) == 0 &&
+                        (a.act == kActNone || (aligned16(a.pre) && (a.ld_pre & 7) == 0));
+        const dim3 grid((a.N + kDzCols - 1) / kDzCols, groups);
+        bf16* to = need_dz ? buf : nullptr;
+        float* sums = a.dbias ? part : nullptr;
+        int rc;
+        if (a.dy_f32)
+            rc = launch_kernel(linear_dz_kernel<float>, grid, 256, 0, s, (const float*)a.dy, a.lddy,
+                               a.pre, a.ld_pre, a.act, drop, to, ceil8(a.N), sums, a.M, a.N, vec);
+        else
+            rc = launch_kernel(linear_dz_kernel<bf16>, grid, 256, 0, s, (const bf16*)a.dy, a.lddy,
+                               a.pre, a.ld_pre, a.act, drop, to, ceil8(a.N), sums, a.M, a.N, vec);
+        if (rc) return rc;
+        if (a.dbias) {
+            rc = launch_kernel(linear_db_kernel, (a.N + 31) / 32, 1024, 0, s, part, groups, a.N,
+                               a.dbias, a.accumulate);
+            if (rc) return rc;
+        }
+        if (need_dz) {
+            dz = buf;
+            ldz = ceil8(a.N);
+        }
+    }
+    if (a.dx) {  // dz [M,N] times w
+        const int rc = product(dz, ldz, 0, a.w, a.ldw, a.w_mn_major ? 0 : 1, a.M, a.K, a.N, a.dx,
+                               a.dx_f32, a.lddx, 0, num_sms, a.err, s);
+        if (rc) return rc;
+    }
+    if (a.dw) {
+        const int rc =
+            a.w_mn_major
+                ? product(a.x, a.ldx, 1, dz, ldz, 1, a.K, a.N, a.M, a.dw, a.dw_f32, a.lddw,
+                          a.accumulate, num_sms, a.err, s)
+                : product(dz, ldz, 1, a.x, a.ldx, 1, a.N, a.K, a.M, a.dw, a.dw_f32, a.lddw,
+                          a.accumulate, num_sms, a.err, s);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+}  // namespace llmgpu

@@ -1,0 +1,109 @@
+// The linear layer with its epilogue (bias, activation, dropout, residual), its backward, and the
+// loss head that keeps no logits. All launchers are asynchronous on `s` and return 0 or a
+// negative status.
+#pragma once
+#include "gemm.cuh"
+#include "kernels.cuh"
+
+namespace llmgpu {
+
+// Status of an operand whose rows do not start on 16 bytes (the tensor maps need it).
+constexpr int kBadOperand = -3;
+inline bool operand_ok(const void* p, long long ld) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0;
+}
+
+// Dropout of a linear layer's output; thr 0 keeps everything.
+struct DropArgs {
+    const uint64_t* rng;  // device {seed, offset}; null: no dropout
+    uint64_t site;
+    uint32_t thr;
+    float scale;
+};
+
+// out[M,N] = resid + drop(act(x[M,K] w^T + bias)); w is [N,K], or [K,N] with w_mn_major. pre
+// (nullable, bf16) receives x w^T + bias. out and resid: f32 or bf16.
+struct LinearFwd {
+    const bf16* x;
+    long long ldx;
+    const bf16* w;
+    long long ldw;
+    int w_mn_major;
+    const float* bias;
+    int act;
+    DropArgs drop;
+    const void* resid;
+    long long ldr;
+    bf16* pre;
+    long long ld_pre;
+    void* out;
+    int out_f32;
+    long long ldo;
+    int M, N, K;
+    int* err;
+};
+int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s);
+
+// dz = drop'(dy) act'(pre) in bf16, dbias (+)= column sums of dz (before its rounding), dx = dz w,
+// dw (+)= dz^T x (laid out as w). dx, dw, dbias nullable.
+struct LinearBwd {
+    const void* dy;
+    int dy_f32;
+    long long lddy;
+    const bf16* x;
+    long long ldx;
+    const bf16* w;
+    long long ldw;
+    int w_mn_major;
+    const bf16* pre;
+    long long ld_pre;
+    int act;
+    DropArgs drop;
+    void* dx;
+    int dx_f32;
+    long long lddx;
+    void* dw;
+    int dw_f32;
+    long long lddw;
+    float* dbias;
+    int accumulate;  // into dw (f32 only) and dbias
+    int M, N, K;
+    void* work;  // linear_backward_work bytes, 256-byte aligned
+    int* err;
+};
+size_t linear_backward_work(int M, int N, int K);
+int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s);
+
+// Loss head on x [rows, C] and w [V, C] (or [C, V] with w_mn_major): row_loss = on (lse - z_t) +
+// off sum_{v != t} (lse - z_v), on = 1 - smoothing, off = smoothing / (V - 1) (the gradient of
+// cross_entropy_fwd_bwd, whose loss leaves the smoothing out); a row whose target is outside [0, V) is left out: loss 0.
+struct HeadArgs {
+    const bf16* x;
+    long long ldx;
+    const bf16* w;
+    long long ldw;
+    int w_mn_major;
+    const int32_t* targets;
+    int rows, C, V;
+    float smoothing;
+    void* work;
+    int* err;
+};
+size_t head_forward_work(int rows, int V);
+int head_forward(const HeadArgs& a, float* row_loss, float* lse, int num_sms, cudaStream_t s);
+// Gradients of sum_r scale * dloss[r] * row_loss[r] (dloss nullable: ones), in pieces of `piece`
+// columns of the vocabulary (0: chosen here). Rows left out contribute nothing, whatever x
+// holds there. dx, dw nullable; dw is laid out as w, and added to when `accumulate` (f32 only).
+int head_piece(int rows, int C, int V, int piece);
+size_t head_backward_work(int rows, int C, int V, int piece);
+int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float scale, void* dx,
+                  int dx_f32, long long lddx, void* dw, int dw_f32, long long lddw, int accumulate,
+                  int piece, int num_sms, cudaStream_t s);
+
+// D[M,N] (+)= A B^T on the tcgen05 kernels into bf16 or f32 `out`, any row stride (accumulate:
+// f32 only).
+int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
+            int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
+            int* err, cudaStream_t s);
+
+}  // namespace llmgpu

@@ -2,10 +2,13 @@
 // on caller-owned device buffers, used by the per-kernel parity tests.
 #include <cuda_runtime.h>
 
+#include "dropout.cuh"
 #include "gemm.cuh"
 #include "kernels.cuh"
+#include "linear.cuh"
 #include "llmgpu_ops.h"
 #include "moe.cuh"
+#include "philox.cuh"
 
 using namespace llmgpu;
 
@@ -198,4 +201,94 @@ extern "C" int llmgpu_op_moe_dispatch(const int* idx, int B, int T, int E, int k
                                       int* row_of, int* tok_of, void* stream) {
     MoeDims m{B, T, 8 /* C: unused by the dispatch */, E, k, moe_capacity(B * T, E, k)};
     return moe_dispatch(m, idx, grp, row_of, tok_of, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int llmgpu_op_dropout(const void* x, int x_f32, long long ldx, const void* resid,
+                                 long long ldr, void* out, int out_f32, long long ldo, int rows,
+                                 int cols, float p, const uint64_t* rng, uint64_t site,
+                                 void* stream) {
+    return dropout_apply(x, x_f32, ldx, resid, ldr, out, out_f32, ldo, rows, cols, p, rng, site,
+                         reinterpret_cast<cudaStream_t>(stream));
+}
+
+// Dropout arguments of a linear layer: p = 0 or no generator keeps everything.
+static bool linear_drop(float p, const uint64_t* rng, uint64_t site, DropArgs* d) {
+    *d = DropArgs{nullptr, site, 0u, 1.0f};
+    if (!drop_params(p, &d->thr, &d->scale) || (d->thr > 0 && !rng)) return false;
+    if (d->thr > 0) d->rng = rng;
+    return true;
+}
+
+extern "C" int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long ldw,
+                                    int w_mn_major, const float* bias, int act, float p,
+                                    const uint64_t* rng, uint64_t site, const void* resid,
+                                    long long ldr, void* pre, long long ld_pre, void* out,
+                                    int out_f32, long long ldo, int M, int N, int K, int* err,
+                                    void* stream) {
+    LinearFwd a{reinterpret_cast<const bf16*>(x), ldx, reinterpret_cast<const bf16*>(w), ldw,
+                w_mn_major != 0, bias, act, {}, resid, ldr, reinterpret_cast<bf16*>(pre), ld_pre,
+                out, out_f32 != 0, ldo, M, N, K, err};
+    if (!linear_drop(p, rng, site, &a.drop)) return -1;
+    if (M > 1 && (ldx < K || ldo < N || (resid && ldr < N) || (pre && ld_pre < N))) return -1;
+    if (ldw < (w_mn_major ? N : K) && (w_mn_major ? K : N) > 1) return -1;
+    return linear_forward(a, device_num_sms(), reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" long long llmgpu_op_linear_bwd_work(int M, int N, int K) {
+    return (long long)linear_backward_work(M, N, K);
+}
+
+extern "C" int llmgpu_op_linear_bwd(const void* dy, int dy_f32, long long lddy, const void* x,
+                                    long long ldx, const void* w, long long ldw, int w_mn_major,
+                                    const void* pre, long long ld_pre, int act, float p,
+                                    const uint64_t* rng, uint64_t site, void* dx, int dx_f32,
+                                    long long lddx, void* dw, int dw_f32, long long lddw,
+                                    float* dbias, int accumulate, int M, int N, int K, void* work,
+                                    int* err, void* stream) {
+    LinearBwd a{dy, dy_f32 != 0, lddy, reinterpret_cast<const bf16*>(x), ldx,
+                reinterpret_cast<const bf16*>(w), ldw, w_mn_major != 0,
+                reinterpret_cast<const bf16*>(pre), ld_pre, act, {}, dx, dx_f32 != 0, lddx, dw,
+                dw_f32 != 0, lddw, dbias, accumulate != 0, M, N, K, work, err};
+    if (!linear_drop(p, rng, site, &a.drop)) return -1;
+    const int wc = w_mn_major ? N : K, wr = w_mn_major ? K : N;  // columns and rows of w
+    if (M > 1 && (lddy < N || (dw && ldx < K) || (dx && lddx < K) ||
+                  (act != kActNone && ld_pre < N)))
+        return -1;
+    if (wr > 1 && ((dx && ldw < wc) || (dw && lddw < wc))) return -1;
+    return linear_backward(a, device_num_sms(), reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" long long llmgpu_op_linear_ce_fwd_work(int rows, int V) {
+    return (long long)head_forward_work(rows, V);
+}
+
+extern "C" int llmgpu_op_linear_ce_fwd(const void* x, long long ldx, const void* w, long long ldw,
+                                       int w_mn_major, const int32_t* targets, int rows, int C,
+                                       int V, float smoothing, float* row_loss, float* lse,
+                                       void* work, int* err, void* stream) {
+    if ((rows > 1 && ldx < C) || (ldw < (w_mn_major ? V : C) && (w_mn_major ? C : V) > 1)) return -1;
+    const HeadArgs a{reinterpret_cast<const bf16*>(x), ldx, reinterpret_cast<const bf16*>(w), ldw,
+                     w_mn_major != 0, targets, rows, C, V, smoothing, work, err};
+    return head_forward(a, row_loss, lse, device_num_sms(), reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" long long llmgpu_op_linear_ce_bwd_work(int rows, int C, int V, int piece) {
+    if (piece < 0 || piece % 256 != 0) return -1;
+    return (long long)head_backward_work(rows, C, V, piece);
+}
+
+extern "C" int llmgpu_op_linear_ce_bwd(const void* x, long long ldx, const void* w, long long ldw,
+                                       int w_mn_major, const int32_t* targets, const float* lse,
+                                       const float* dloss, float scale, int rows, int C, int V,
+                                       float smoothing, void* dx, int dx_f32, long long lddx,
+                                       void* dw, int dw_f32, long long lddw, int accumulate,
+                                       int piece, void* work, int* err, void* stream) {
+    const int wc = w_mn_major ? V : C, wr = w_mn_major ? C : V;
+    if (rows > 1 && (ldx < C || (dx && lddx < C))) return -1;
+    if (wr > 1 && (ldw < wc || (dw && lddw < wc))) return -1;
+    const HeadArgs a{reinterpret_cast<const bf16*>(x), ldx, reinterpret_cast<const bf16*>(w), ldw,
+                     w_mn_major != 0, targets, rows, C, V, smoothing, work, err};
+    return head_backward(a, lse, dloss, scale, dx, dx_f32 != 0, lddx, dw, dw_f32 != 0, lddw,
+                         accumulate != 0, piece, device_num_sms(),
+                         reinterpret_cast<cudaStream_t>(stream));
 }

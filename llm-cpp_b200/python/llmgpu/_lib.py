@@ -52,6 +52,29 @@ def _declare(lib):
     lib.llmgpu_op_moe_route.argtypes = [c_vp] * 5 + [c_int, c_vp] + [c_int] * 5 + [c_vp] * 5
     lib.llmgpu_op_moe_dispatch.argtypes = [c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp,
                                            c_vp]
+    c_u64 = ctypes.c_uint64
+    lib.llmgpu_op_dropout.argtypes = [c_vp, c_int, c_ll, c_vp, c_ll, c_vp, c_int, c_ll, c_int,
+                                      c_int, c_float, c_vp, c_u64, c_vp]
+    lib.llmgpu_op_linear_fwd.argtypes = [c_vp, c_ll, c_vp, c_ll, c_int, c_vp, c_int, c_float, c_vp,
+                                         c_u64, c_vp, c_ll, c_vp, c_ll, c_vp, c_int, c_ll, c_int,
+                                         c_int, c_int, c_vp, c_vp]
+    lib.llmgpu_op_linear_bwd.argtypes = [c_vp, c_int, c_ll, c_vp, c_ll, c_vp, c_ll, c_int, c_vp,
+                                         c_ll, c_int, c_float, c_vp, c_u64, c_vp, c_int, c_ll, c_vp,
+                                         c_int, c_ll, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp,
+                                         c_vp]
+    lib.llmgpu_op_linear_ce_fwd.argtypes = [c_vp, c_ll, c_vp, c_ll, c_int, c_vp, c_int, c_int,
+                                            c_int, c_float, c_vp, c_vp, c_vp, c_vp, c_vp]
+    lib.llmgpu_op_linear_ce_bwd.argtypes = [c_vp, c_ll, c_vp, c_ll, c_int, c_vp, c_vp, c_vp,
+                                            c_float, c_int, c_int, c_int, c_float, c_vp, c_int,
+                                            c_ll, c_vp, c_int, c_ll, c_int, c_int, c_vp, c_vp,
+                                            c_vp]
+    for n, k in (("llmgpu_op_linear_bwd_work", 3), ("llmgpu_op_linear_ce_fwd_work", 2),
+                 ("llmgpu_op_linear_ce_bwd_work", 4)):
+        getattr(lib, n).argtypes = [c_int] * k
+        getattr(lib, n).restype = c_ll
+    for n in ("llmgpu_op_dropout", "llmgpu_op_linear_fwd", "llmgpu_op_linear_bwd",
+              "llmgpu_op_linear_ce_fwd", "llmgpu_op_linear_ce_bwd"):
+        getattr(lib, n).restype = c_int
     for n in ("llmgpu_op_embed", "llmgpu_op_norm_fwd", "llmgpu_op_norm_bwd",
               "llmgpu_op_cross_entropy", "llmgpu_op_attention_fwd", "llmgpu_op_attention_bwd",
               "llmgpu_op_attention_fwd_ws",

@@ -230,3 +230,259 @@ def moe_dispatch(idx, B, T, E):
     _sync_check(lib.llmgpu_op_moe_dispatch(_ptr(idx), B, T, E, k, _ptr(grp), _ptr(row_of),
                                            _ptr(tok_of), _stream()), "moe_dispatch")
     return grp, row_of, tok_of
+
+
+# ---- dropout, the linear layer and the loss head -------------------------------------------------
+# These run asynchronously on the current stream of their tensors' device, like any torch operation,
+# and allocate what they return (and their workspace) from torch's allocator, so they can be captured
+# into a graph. Matrices are 2-D with neighbouring columns and any row stride; the matrices they
+# return start their rows on 16 bytes (the row stride is rounded up to 8 elements), so that one
+# operator's result can be another's operand.
+ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+_err_words = {}
+
+
+def _err_word(device):
+    """The device's error word of these operators (made outside a capture, once per device)."""
+    w = _err_words.get(device.index)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None  # the first call on this device is being captured: waits stay bounded
+        w = _err_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()  # any later stream may use it
+    return w
+
+
+def check_device(device="cuda"):
+    """Waits for the device and raises if a wait inside one of these operators' kernels gave up;
+    the word is cleared."""
+    device = torch.device(device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    torch.cuda.synchronize(index)
+    w = _err_words.get(index)
+    if w is not None:
+        code = int(w.item())
+        if code:
+            w.zero_()
+            raise KernelError(f"device error code {code}")
+
+
+def _want(ok, what):
+    if not ok:
+        raise KernelError(what)
+
+
+def _matrix(t, name, dtypes, rows, cols, device, operand=False):
+    """Checks a 2-D matrix argument and returns its row stride in elements."""
+    _want(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a CUDA tensor is needed")
+    _want(t.device == device, f"{name}: on {t.device}, not on {device}")
+    _want(t.dtype in dtypes, f"{name}: {t.dtype} is not one of {[str(d) for d in dtypes]}")
+    _want(tuple(t.shape) == (rows, cols), f"{name}: shape {tuple(t.shape)}, not {(rows, cols)}")
+    _want(cols <= 1 or t.stride(1) == 1, f"{name}: neighbouring columns are needed")
+    if rows <= 1:
+        ld = (cols + 7) // 8 * 8
+    else:
+        ld = t.stride(0)
+        _want(ld >= cols, f"{name}: rows overlap (stride {ld} of {cols} columns)")
+    if operand and t.numel():
+        _want(t.data_ptr() % 16 == 0 and ld % 8 == 0,
+              f"{name}: rows have to start on 16 bytes (address {t.data_ptr():#x}, stride {ld})")
+    return ld
+
+
+def _vector(t, name, dtype, n, device):
+    _want(isinstance(t, torch.Tensor) and t.is_cuda and t.device == device and t.dtype == dtype
+          and tuple(t.shape) == (n,) and t.is_contiguous(),
+          f"{name}: a contiguous {dtype} tensor of {n} on {device} is needed")
+
+
+def _rows(rows, cols, dtype, device):
+    return torch.empty(rows, (cols + 7) // 8 * 8, dtype=dtype, device=device)[:, :cols]
+
+
+def _drop(p, rng, device):
+    _want(0.0 <= p <= 1.0, f"p = {p} is not in [0, 1]")
+    if p > 0.0:
+        _want(rng is not None, "dropout needs rng, an int64 tensor (seed, offset) on the device")
+    if rng is not None:
+        _vector(rng, "rng", torch.int64, 2, device)
+
+
+_FLOATS = (torch.float32, torch.bfloat16)
+_BF16 = (torch.bfloat16,)
+
+
+def dropout_fwd(x, p, rng, site=0, resid=None, out=None, out_dtype=None):
+    """resid + (kept ? x / (1 - p) : 0) over a 2-D x (f32 or bf16), in `out_dtype` (x's if not
+    given). `rng`: int64 device tensor (seed, offset); `site` tells the dropouts of a step apart.
+    The mask depends on (seed, offset + site, row, column) alone and p counts in steps of
+    1 / 65536; see llmgpu_op_dropout. `out` may be x or resid."""
+    _want(isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2, "x: a 2-D CUDA tensor is needed")
+    rows, cols = x.shape
+    dev = x.device
+    ldx = _matrix(x, "x", _FLOATS, rows, cols, dev)
+    _drop(p, rng, dev)
+    _want(rng is not None, "dropout needs rng, an int64 tensor (seed, offset) on the device")
+    if out is None:
+        out = _rows(rows, cols, out_dtype or x.dtype, dev)
+    _want(out_dtype is None or out.dtype == out_dtype, f"out: {out.dtype} is not {out_dtype}")
+    ldo = _matrix(out, "out", _FLOATS, rows, cols, dev)
+    ldr = 0
+    if resid is not None:
+        ldr = _matrix(resid, "resid", (out.dtype,), rows, cols, dev)
+    with torch.cuda.device(dev):
+        _check(load().llmgpu_op_dropout(
+            _ptr(x), int(x.dtype == torch.float32), ldx, _ptr(resid), ldr, _ptr(out),
+            int(out.dtype == torch.float32), ldo, rows, cols, p, _ptr(rng), site, _stream()),
+            "llmgpu_op_dropout")
+    return out
+
+
+def dropout_bwd(dy, p, rng, site=0, out=None, out_dtype=None):
+    """The gradient by x of dropout_fwd with the same (p, rng, site); the residual's is dy itself."""
+    return dropout_fwd(dy, p, rng, site, out=out, out_dtype=out_dtype)
+
+
+def _linear_shapes(x, w, w_mn):
+    for t, n in ((x, "x"), (w, "w")):
+        _want(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2,
+              f"{n}: a 2-D CUDA tensor is needed")
+    M, K = x.shape
+    N = w.shape[1] if w_mn else w.shape[0]
+    _want(N > 0 and K > 0, f"an empty product: x {tuple(x.shape)}, w {tuple(w.shape)}")
+    ldx = _matrix(x, "x", _BF16, M, K, x.device, operand=True)
+    ldw = _matrix(w, "w", _BF16, K if w_mn else N, N if w_mn else K, x.device, operand=True)
+    return M, K, N, ldx, ldw
+
+
+def linear_fwd(x, w, bias=None, act="none", p=0.0, rng=None, site=0, resid=None, w_mn=False,
+               out=None, out_dtype=torch.bfloat16, save_pre=False):
+    """resid + drop(act(x w^T + bias)) in one product. x [M, K] and w [N, K] (or [K, N] with
+    `w_mn`) are bf16 with rows on 16 bytes, bias [N] f32, act one of ACT, (p, rng, site) as in
+    dropout_fwd, resid of the result's type. Returns (y, pre): pre = x w^T + bias in bf16 when
+    `save_pre` (linear_bwd needs it unless act is "none"), else None."""
+    M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
+    dev = x.device
+    _want(act in ACT, f"act: {act!r} is not one of {sorted(ACT)}")
+    _drop(p, rng, dev)
+    if bias is not None:
+        _vector(bias, "bias", torch.float32, N, dev)
+    if out is None:
+        out = _rows(M, N, out_dtype, dev)
+    ldo = _matrix(out, "out", _FLOATS, M, N, dev)
+    ldr = ldp = 0
+    if resid is not None:
+        ldr = _matrix(resid, "resid", (out.dtype,), M, N, dev)
+    pre = None
+    if save_pre:
+        pre = _rows(M, N, torch.bfloat16, dev)
+        ldp = _matrix(pre, "pre", _BF16, M, N, dev)
+    with torch.cuda.device(dev):
+        _check(load().llmgpu_op_linear_fwd(
+            _ptr(x), ldx, _ptr(w), ldw, int(w_mn), _ptr(bias), ACT[act], p, _ptr(rng), site,
+            _ptr(resid), ldr, _ptr(pre), ldp, _ptr(out), int(out.dtype == torch.float32), ldo, M, N,
+            K, _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_fwd")
+    return out, pre
+
+
+def linear_bwd(dy, x, w, pre=None, act="none", p=0.0, rng=None, site=0, w_mn=False,
+               dx_dtype=torch.bfloat16, dw=None, dbias=None, accumulate=False, need_dx=True,
+               need_dw=True, need_dbias=True):
+    """Gradients (dx, dw, dbias) of linear_fwd for the gradient dy [M, N] (f32 or bf16) of its
+    result, with the forward's x, w, pre, act and (p, rng, site); the residual's gradient is dy. dw
+    has w's layout, bf16 unless given; `accumulate` adds into the given dw (f32) and dbias. What
+    is not needed is None."""
+    M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
+    dev = x.device
+    _want(act in ACT, f"act: {act!r} is not one of {sorted(ACT)}")
+    _drop(p, rng, dev)
+    lddy = _matrix(dy, "dy", _FLOATS, M, N, dev)
+    ldp = 0
+    if act != "none":
+        _want(pre is not None, f"act {act!r}: the backward needs pre")
+        ldp = _matrix(pre, "pre", _BF16, M, N, dev)
+    dx = _rows(M, K, dx_dtype, dev) if need_dx else None
+    lddx = _matrix(dx, "dx", _FLOATS, M, K, dev) if need_dx else 0
+    wr, wc = (K, N) if w_mn else (N, K)
+    if not need_dw:
+        dw = None
+    elif dw is None:
+        _want(not accumulate, "accumulate: dw has to be given")
+        dw = _rows(wr, wc, torch.bfloat16, dev)
+    lddw = _matrix(dw, "dw", _FLOATS, wr, wc, dev) if need_dw else 0
+    _want(not (accumulate and need_dw) or dw.dtype == torch.float32, "accumulate: dw has to be f32")
+    if not need_dbias:
+        dbias = None
+    elif dbias is None:
+        _want(not accumulate, "accumulate: dbias has to be given")
+        dbias = torch.empty(N, dtype=torch.float32, device=dev)
+    if need_dbias:
+        _vector(dbias, "dbias", torch.float32, N, dev)
+    lib = load()
+    work = torch.empty(int(lib.llmgpu_op_linear_bwd_work(M, N, K)), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib.llmgpu_op_linear_bwd(
+            _ptr(dy), int(dy.dtype == torch.float32), lddy, _ptr(x), ldx, _ptr(w), ldw, int(w_mn),
+            _ptr(pre), ldp, ACT[act], p, _ptr(rng), site, _ptr(dx),
+            int(dx_dtype == torch.float32), lddx, _ptr(dw),
+            int(need_dw and dw.dtype == torch.float32), lddw, _ptr(dbias), int(accumulate), M, N,
+            K, _ptr(work), _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_bwd")
+    return dx, dw, dbias
+
+
+def linear_cross_entropy_fwd(x, w, targets, smoothing=0.0, w_mn=False):
+    """Softmax cross-entropy of the logits x w^T without forming them in memory: (row_loss, lse),
+    f32 [rows]. x [rows, C] and w [V, C] (or [C, V] with `w_mn`) are bf16 with rows on 16 bytes,
+    targets int32 [rows]; a target outside [0, V) leaves its row out (loss 0). `smoothing` s:
+    targets of 1 - s and s / (V - 1) elsewhere, in the loss as in the gradient."""
+    rows, C, V, ldx, ldw = _linear_shapes(x, w, w_mn)
+    dev = x.device
+    _want(0.0 <= smoothing < 1.0, f"smoothing = {smoothing} is not in [0, 1)")
+    _vector(targets, "targets", torch.int32, rows, dev)
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    lse = torch.empty(rows, dtype=torch.float32, device=dev)
+    lib = load()
+    work = torch.empty(int(lib.llmgpu_op_linear_ce_fwd_work(rows, V)), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib.llmgpu_op_linear_ce_fwd(
+            _ptr(x), ldx, _ptr(w), ldw, int(w_mn), _ptr(targets), rows, C, V, smoothing, _ptr(loss),
+            _ptr(lse), _ptr(work), _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_ce_fwd")
+    return loss, lse
+
+
+def linear_cross_entropy_bwd(x, w, targets, lse, dloss=None, scale=1.0, smoothing=0.0, w_mn=False,
+                             dx_dtype=torch.bfloat16, dw=None, accumulate=False, piece=0,
+                             need_dx=True, need_dw=True):
+    """Gradients (dx, dw) of sum(scale * dloss * row_loss) (dloss f32 [rows], ones if None), with
+    the forward's arguments and its lse. The logits are formed again in pieces of `piece` columns of
+    the vocabulary (a multiple of 256; 0: chosen by the library), which bounds the workspace. dw
+    has w's layout, bf16 unless given; `accumulate` adds into the given f32 dw."""
+    rows, C, V, ldx, ldw = _linear_shapes(x, w, w_mn)
+    dev = x.device
+    _want(0.0 <= smoothing < 1.0, f"smoothing = {smoothing} is not in [0, 1)")
+    _want(piece >= 0 and piece % 256 == 0, f"piece = {piece} is not a multiple of 256")
+    _vector(targets, "targets", torch.int32, rows, dev)
+    _vector(lse, "lse", torch.float32, rows, dev)
+    if dloss is not None:
+        _vector(dloss, "dloss", torch.float32, rows, dev)
+    dx = _rows(rows, C, dx_dtype, dev) if need_dx else None
+    lddx = _matrix(dx, "dx", _FLOATS, rows, C, dev) if need_dx else 0
+    wr, wc = (C, V) if w_mn else (V, C)
+    if not need_dw:
+        dw = None
+    elif dw is None:
+        _want(not accumulate, "accumulate: dw has to be given")
+        dw = _rows(wr, wc, torch.bfloat16, dev)
+    lddw = _matrix(dw, "dw", _FLOATS, wr, wc, dev) if need_dw else 0
+    _want(not (accumulate and need_dw) or dw.dtype == torch.float32, "accumulate: dw has to be f32")
+    lib = load()
+    work = torch.empty(int(lib.llmgpu_op_linear_ce_bwd_work(rows, C, V, piece)), dtype=torch.uint8,
+                       device=dev)
+    with torch.cuda.device(dev):
+        _check(lib.llmgpu_op_linear_ce_bwd(
+            _ptr(x), ldx, _ptr(w), ldw, int(w_mn), _ptr(targets), _ptr(lse), _ptr(dloss), scale,
+            rows, C, V, smoothing, _ptr(dx), int(dx_dtype == torch.float32), lddx, _ptr(dw),
+            int(need_dw and dw.dtype == torch.float32), lddw, int(accumulate), piece, _ptr(work),
+            _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_ce_bwd")
+    return dx, dw

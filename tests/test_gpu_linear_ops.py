@@ -1,0 +1,659 @@
+"""Dropout, the linear layer with its epilogue and the loss head without logits on the GPU, against
+plain 64-bit forms (tests/linear_ops_ref.py). Tolerances count roundings: H16 and H32 are half a
+step of bf16 and f32 relative to the value; a product of length K accumulated in f32 is off by at
+most about K steps of the sum of its terms' magnitudes (ACC per term, two half steps: the tensor
+cores may truncate)."""
+import math
+
+import pytest
+
+import linear_ops_ref as ref
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+BF, F32 = torch.bfloat16, torch.float32
+H16, H32 = 2.0 ** -8, 2.0 ** -24
+ACC = 2.0 ** -23
+# 2-norm of a gradient's error over its own: the roundings of the products' bf16 operand and of the
+# bf16 result, each at most H16 with a root mean square of at most H16 / sqrt(3)
+NORM16 = math.sqrt(2.0 / 3.0) * H16 * 1.1
+
+
+def _mat(g, rows, cols, dtype, dev, scale=1.0, offset=0, pad=0, fill=float("nan")):
+    """A [rows, cols] view with `fill` everywhere around it: behind each row, before and after."""
+    ld = -(-(cols + pad) // 8) * 8 if offset % 8 == 0 and pad % 8 == 0 else cols + pad
+    buf = torch.full((offset + rows * ld + 64,), fill, dtype=dtype, device=dev)
+    v = buf[offset:offset + rows * ld].view(rows, ld)[:, :cols] if rows else \
+        torch.empty(0, cols, dtype=dtype, device=dev)
+    v.copy_((torch.randn(rows, cols, generator=g) * scale).to(dtype))
+    return v, buf
+
+
+def _guard(rows, cols, dtype, dev, ld, offset=0):
+    """An output view in a buffer of sentinels, and a check that nothing else was written."""
+    buf = torch.full((offset + rows * ld + 64,), 7.0, dtype=dtype, device=dev)
+    view = buf[offset:offset + rows * ld].view(rows, ld)[:, :cols]
+
+    def check():
+        b = buf.clone()
+        b[offset:offset + rows * ld].view(rows, ld)[:, :cols] = 7.0
+        assert bool((b == 7.0).all()), "written outside the output"
+    return view, check
+
+
+def _rng(dev, seed=0x1234567890ABCDEF, offset=0xFFFFFFF0):
+    return torch.tensor([seed, offset], dtype=torch.int64, device=dev)
+
+
+def _close(got, want, tol, what=""):
+    got, want = got.double().cpu(), want.double().cpu()
+    assert bool(torch.isfinite(got).all()), what + ": not finite"
+    bad = (got - want).abs() > tol.double().cpu() + 1e-30
+    assert not bool(bad.any()), (what, int(bad.sum()), float((got - want).abs().max()))
+
+
+def _norm_close(got, want, tol, what=""):
+    n = float(want.double().norm())
+    e = float((got.double().cpu() - want.double().cpu()).norm())
+    assert e <= tol * n + 1e-30, (what, e / max(n, 1e-30), tol)
+
+
+# ------------------------------------------------------------------------------------ dropout
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 8), (3, 7), (2, 256), (257, 300), (5, 4099),
+                                       (64, 1024)])
+@pytest.mark.parametrize("xt", [BF, F32])
+@pytest.mark.parametrize("ot", [BF, F32])
+@pytest.mark.parametrize("p,resid,offset,pad", [(0.1, False, 0, 0), (0.5, True, 0, 8),
+                                                (0.25, True, 3, 5), (0.0, True, 0, 0),
+                                                (1.0, True, 0, 0)])
+def test_dropout(cuda, rows, cols, xt, ot, p, resid, offset, pad):
+    from llmgpu import ops
+    g = torch.Generator().manual_seed(rows * 7 + cols)
+    x, _ = _mat(g, rows, cols, xt, cuda, 1.0, offset, pad)
+    r, _ = _mat(g, rows, cols, ot, cuda, 2.0, offset, pad) if resid else (None, None)
+    rng = _rng(cuda)
+    ld = cols + 11 if offset else -(-cols // 8) * 8
+    out, check = _guard(rows, cols, ot, cuda, ld, offset)
+    ops.dropout_fwd(x, p, rng, site=37, resid=r, out=out)
+    keep, scale = ref.keep_mask(0x1234567890ABCDEF, 0xFFFFFFF0 + 37, rows, cols, p)
+    want = torch.where(keep, x.double().cpu() * scale, 0.0)
+    mag = want.abs()
+    if resid:
+        want = want + r.double().cpu()
+        mag = mag + r.double().cpu().abs()
+    # the scale, the product and the sum round in f32, the result in its type
+    tol = 3 * H32 * mag * (1 + H16) + (H16 if ot == BF else 0.0) * want.abs()
+    _close(out, want, tol, "dropout")
+    check()
+    again = ops.dropout_fwd(x, p, rng, site=37, resid=r, out_dtype=ot)
+    assert torch.equal(again, out)  # the same map wherever it is written
+
+
+def test_dropout_dropped_elements_give_zero_whatever_they_hold(cuda):
+    from llmgpu import ops
+    rng = _rng(cuda, 3, 4)
+    keep, _ = ref.keep_mask(3, 4, 64, 96, 0.5)
+    keep = keep.to(cuda)
+    for bad in (float("nan"), float("inf"), torch.finfo(F32).min):
+        for pad in (0, 1):  # both memory paths
+            x = torch.ones(64, 96 + pad, device=cuda)[:, :96]
+            x[~keep] = bad
+            y = ops.dropout_fwd(x, 0.5, rng)
+            assert torch.equal(y, torch.where(keep, 2.0, 0.0))
+
+
+def test_dropout_in_place_and_backward_mask(cuda):
+    """out may be x or resid; the backward's mask is the forward's, in any type and layout."""
+    from llmgpu import ops
+    g = torch.Generator().manual_seed(2)
+    rng = _rng(cuda, 9, 1 << 40)
+    x, _ = _mat(g, 130, 1021, F32, cuda)
+    r, _ = _mat(g, 130, 1021, F32, cuda, 1.0, 3, 5)
+    want = ops.dropout_fwd(x, 0.3, rng, site=2, resid=r)
+    a = x.clone()
+    ops.dropout_fwd(a, 0.3, rng, site=2, resid=r, out=a)
+    b = r.clone()
+    ops.dropout_fwd(x, 0.3, rng, site=2, resid=b, out=b)
+    assert torch.equal(a, want) and torch.equal(b, want)
+    ones = torch.ones(130, 1021, dtype=BF, device=cuda)
+    dx = ops.dropout_bwd(ones, 0.3, rng, site=2, out_dtype=F32)
+    y = ops.dropout_fwd(torch.ones(130, 1021, device=cuda), 0.3, rng, site=2)
+    assert torch.equal(dx, y)
+    assert not torch.equal(y, ops.dropout_fwd(torch.ones(130, 1021, device=cuda), 0.3, rng, site=3))
+
+
+def test_dropout_offsets_past_32_bits(cuda):
+    """Rows whose element offsets pass 2^31 and 2^32 bytes and elements."""
+    from llmgpu import ops
+    rows, ld, cols = 90, 50_000_000, 24
+    buf = torch.zeros(rows * ld, dtype=BF, device=cuda)
+    x = buf.view(rows, ld)[:, :cols]
+    x.fill_(1.0)
+    y = ops.dropout_fwd(x, 0.5, _rng(cuda, 1, 2))
+    keep, _ = ref.keep_mask(1, 2, rows, cols, 0.5)
+    assert torch.equal(y.cpu() > 0, keep)
+    ops.dropout_fwd(x, 0.5, _rng(cuda, 1, 2), out=x)
+    assert torch.equal(x.cpu() > 0, keep)
+
+
+def test_dropout_empty(cuda):
+    from llmgpu import ops
+    assert ops.dropout_fwd(torch.empty(0, 8, device=cuda), 0.5, _rng(cuda)).shape == (0, 8)
+    assert ops.dropout_fwd(torch.empty(8, 0, device=cuda), 0.5, _rng(cuda)).shape == (8, 0)
+
+
+# ------------------------------------------------------------------------------------- linear
+def _linear_case(dev, M, K, N, act, p, out, resid, bias, w_mn, seed, pad=0):
+    g = torch.Generator().manual_seed(seed)
+    x, _ = _mat(g, M, K, BF, dev, 1.0, 0, pad)
+    w, _ = _mat(g, K if w_mn else N, N if w_mn else K, BF, dev, 1.5 / math.sqrt(K), 8, pad)
+    b = (torch.randn(N, generator=g) * 0.5).to(dev) if bias else None
+    r = _mat(g, M, N, out, dev, 2.0, 1, 2)[0] if resid else None
+    return g, x, w, b, r
+
+
+def _linear_want(x, w, b, r, act, p, w_mn, rng, site):
+    wd = w.double().cpu() if w_mn else w.double().cpu().t()
+    xd = x.double().cpu()
+    z = xd @ wd
+    ez = (x.shape[1] + 4) * ACC * (xd.abs() @ wd.abs())
+    if b is not None:
+        z = z + b.double().cpu()
+        ez = ez + H32 * (z.abs() + b.double().cpu().abs())
+    y = ref.act(z, act)
+    # an activation's slope is at most 1.13; its sigmoid is off by a few steps times its argument
+    e = 1.13 * ez + (8 + 2 * ref.sigmoid_arg(z, act).abs()) * 2 * H32 * y.abs()
+    if p > 0:
+        keep, scale = ref.keep_mask(int(rng[0]), int(rng[1]) + site, *z.shape, p)
+        y, e = torch.where(keep, y * scale, 0.0), torch.where(keep, e * scale, 0.0)
+        e = e + 2 * H32 * y.abs()
+    if r is not None:
+        y = y + r.double().cpu()
+        e = e + H32 * (y.abs() + r.double().cpu().abs())
+    return z, ez, y, e
+
+
+SHAPES = [(1, 8, 1), (1, 768, 2304), (2, 40, 7), (3, 16, 300), (7, 1024, 257), (8, 264, 64),
+          (9, 72, 33), (64, 128, 512), (127, 200, 129), (130, 768, 96), (300, 765, 1021),
+          (513, 64, 640)]
+
+
+@pytest.mark.parametrize("M,K,N", SHAPES)
+@pytest.mark.parametrize("act,p,out,resid,bias,w_mn", [
+    ("none", 0.0, BF, False, True, False), ("gelu", 0.0, BF, False, True, True),
+    ("none", 0.1, F32, True, True, True), ("relu", 0.25, BF, True, False, False),
+    ("silu", 0.0, F32, False, False, False), ("gelu", 0.5, F32, True, True, False)])
+def test_linear_fwd(cuda, M, K, N, act, p, out, resid, bias, w_mn):
+    from llmgpu import ops
+    _, x, w, b, r = _linear_case(cuda, M, K, N, act, p, out, resid, bias, w_mn, M + K + N, 8)
+    rng, site = _rng(cuda, 77, 5), 3
+    z, ez, want, e = _linear_want(x, w, b, r, act, p, w_mn, rng, site)
+    y, pre = ops.linear_fwd(x, w, b, act, p, rng, site, r, w_mn, out_dtype=out, save_pre=True)
+    tol = e + (H16 if out == BF else 0.0) * (want.abs() + e)
+    _close(y, want, tol, "y")
+    _close(pre, z, ez + H16 * (z.abs() + ez), "pre")
+    # into rows of any stride and alignment, nothing around them touched
+    for ld, off in ((-(-N // 8) * 8 + 8, 0), (N + 3, 5)):
+        o, check = _guard(M, N, out, cuda, ld, off)
+        ops.linear_fwd(x, w, b, act, p, rng, site, r, w_mn, out=o)
+        _close(o, want, tol, "y into a view")
+        check()
+    if resid:  # the residual updated in place
+        o = r.clone()
+        ops.linear_fwd(x, w, b, act, p, rng, site, o, w_mn, out=o)
+        _close(o, want, tol, "y over its residual")
+    ops.check_device(cuda)
+
+
+def _linear_bwd_want(dy, x, w, pre, act, p, w_mn, rng, site):
+    dz = dy.double().cpu()
+    if p > 0:
+        keep, scale = ref.keep_mask(int(rng[0]), int(rng[1]) + site, *dz.shape, p)
+        dz = torch.where(keep, dz * scale, 0.0)
+    e = 4 * H32 * dz.abs()
+    if act != "none":
+        zd = pre.double().cpu()
+        gr = ref.act_grad(zd, act)
+        # h + z h (1 - h) c: each sigmoid off by a few steps times its argument
+        h = torch.sigmoid(ref.sigmoid_arg(zd, act))
+        mag = h * (1 + zd.abs() * (1.6 * (1 + 0.14 * zd ** 2) if act == "gelu" else 1.0))
+        eg = (16 + 4 * ref.sigmoid_arg(zd, act).abs()) * 2 * H32 * mag if act != "relu" else 0.0
+        e = dz.abs() * eg + e * gr.abs()
+        dz = dz * gr
+    xd = x.double().cpu()
+    wd = w.double().cpu().t() if w_mn else w.double().cpu()  # [N, K]
+    dx, dw = dz @ wd, dz.t() @ xd
+    ex = (H16 * dz.abs() + e) @ wd.abs() + (dz.shape[1] + 4) * ACC * (dz.abs() @ wd.abs())
+    ew = (H16 * dz.abs() + e).t() @ xd.abs() + (dz.shape[0] + 4) * ACC * (dz.abs().t() @ xd.abs())
+    if w_mn:
+        dw, ew = dw.t(), ew.t()
+    db = dz.sum(0)
+    eb = e.sum(0) + (dz.shape[0] + 4) * H32 * dz.abs().sum(0)
+    return dx, ex, dw, ew, db, eb
+
+
+@pytest.mark.parametrize("M,K,N", SHAPES)
+@pytest.mark.parametrize("act,p,dyt,w_mn", [("none", 0.0, BF, False), ("none", 0.0, F32, True),
+                                            ("none", 0.2, BF, True), ("gelu", 0.0, BF, False),
+                                            ("silu", 0.1, F32, True), ("relu", 0.5, BF, False)])
+def test_linear_bwd(cuda, M, K, N, act, p, dyt, w_mn):
+    from llmgpu import ops
+    g, x, w, _, _ = _linear_case(cuda, M, K, N, act, p, dyt, False, False, w_mn, M + K + N, 8)
+    rng, site = _rng(cuda, 5, 99), 8
+    dy = _mat(g, M, N, dyt, cuda, 0.1, 0 if N % 2 else 1, 8 if N % 2 else 3)[0]
+    pre = _mat(g, M, N, BF, cuda, 2.0)[0] if act != "none" else None
+    dx, ex, dw, ew, db, eb = _linear_bwd_want(dy, x, w, pre, act, p, w_mn, rng, site)
+    gx, gw, gb = ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn)
+    _close(gx, dx, ex + H16 * (dx.abs() + ex), "dx")
+    _close(gw, dw, ew + H16 * (dw.abs() + ew), "dw")
+    _close(gb, db, eb, "dbias")
+    if M * N >= 4096:
+        _norm_close(gx, dx, NORM16, "dx")
+        _norm_close(gw, dw, NORM16, "dw")
+    # f32 gradients, added to what is there; rows of any stride
+    wr, wc = (K, N) if w_mn else (N, K)
+    aw, check = _guard(wr, wc, F32, cuda, wc + 3, 1)
+    aw.fill_(0.5)
+    ab = torch.full((N,), 2.0, device=cuda)
+    gx32, _, _ = ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn, dx_dtype=F32, dw=aw, dbias=ab,
+                                accumulate=True)
+    _close(gx32, dx, ex, "f32 dx")
+    _close(aw, dw + 0.5, ew + H32 * (dw.abs() + 0.5 + ew), "accumulated dw")
+    _close(ab, db + 2.0, eb + H32 * (db.abs() + 2.0 + eb), "accumulated dbias")
+    check()
+    # each gradient alone
+    assert torch.equal(ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn, need_dw=False,
+                                      need_dbias=False)[0], gx)
+    assert torch.equal(ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn, need_dx=False,
+                                      need_dbias=False)[1], gw)
+    assert torch.equal(ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn, need_dx=False,
+                                      need_dw=False)[2], gb)
+    ops.check_device(cuda)
+
+
+def test_linear_no_rows(cuda):
+    from llmgpu import ops
+    x, w = torch.empty(0, 16, dtype=BF, device=cuda), torch.ones(24, 16, dtype=BF, device=cuda)
+    y, _ = ops.linear_fwd(x, w)
+    assert y.shape == (0, 24)
+    dx, dw, db = ops.linear_bwd(y, x, w)
+    assert dx.shape == (0, 16) and not dw.any() and not db.any()
+    one = torch.ones(24, 16, device=cuda)
+    ops.linear_bwd(y, x, w, dw=one, dbias=torch.ones(24, device=cuda), accumulate=True)
+    assert bool((one == 1).all())
+
+
+def test_linear_activations_at_the_ends(cuda):
+    """Pre-activations of the type's largest values, infinities and NaN: relu, gelu and silu go
+    to 0 on the left and to z on the right; their gradients at +-1e4 are 0 and 1."""
+    from llmgpu import ops
+    z = torch.tensor([-3e38, -1e20, -100.0, -0.0, 0.0, 100.0, 1e20, 3e38], device=cuda)
+    x = torch.zeros(4, 8, dtype=BF, device=cuda)
+    w = torch.zeros(8, 8, dtype=BF, device=cuda)
+    for act in ("relu", "gelu", "silu"):
+        y, _ = ops.linear_fwd(x, w, z, act, out_dtype=F32)
+        assert torch.equal(y[0, 5:], z[5:]) and bool((y[0, :5].abs() <= 1e-30).all()), (act, y[0])
+        pre = torch.tensor([-1e4, -100.0, 100.0, 1e4] * 2, device=cuda).to(BF).repeat(4, 1)
+        dy = torch.ones(4, 8, device=cuda)
+        _, _, db = ops.linear_bwd(dy, x, w, pre, act, need_dx=False, need_dw=False)
+        assert torch.equal(db, torch.tensor([0.0, 0.0, 4.0, 4.0] * 2, device=cuda)), (act, db)
+        nan, _ = ops.linear_fwd(x, w, torch.full((8,), float("nan"), device=cuda), act)
+        assert bool(nan.isnan().all())
+
+
+# --------------------------------------------------------------------------------------- head
+def _head_case(dev, rows, C, V, w_mn, ignored, seed, sharp=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x, _ = _mat(g, rows, C, BF, dev, 1.0, 0, 8)
+    w, _ = _mat(g, C if w_mn else V, V if w_mn else C, BF, dev, sharp / math.sqrt(C), 8, 8)
+    t = torch.randint(0, V, (rows,), generator=g, dtype=torch.int32)
+    if ignored:
+        t[torch.rand(rows, generator=g) < 0.3] = -1
+        t[rows // 2] = V  # past the vocabulary: left out too
+    d = torch.rand(rows, generator=g) + 0.5
+    return x, w, t.to(dev), d.to(dev)
+
+
+def _head_want(x, w, t, d, scale, smoothing, w_mn):
+    xd, wd = x.double().cpu(), w.double().cpu()
+    if w_mn:
+        wd = wd.t()
+    loss, lse, z, y, valid = ref.head(xd, wd, t.cpu(), smoothing)
+    V, C = wd.shape
+    ez = (C + 4) * ACC * (xd.abs() @ wd.abs().t())
+    el = ez.amax(1) + (4 * H32) * (1 + lse.abs()) + 16 * H32
+    # smoothing adds V terms of size smoothing / (V - 1): lse - z, each off by ez + el, summed in f32
+    eloss = 2 * el + ez.amax(1) + 4 * H32 * loss.abs() + \
+        smoothing * 4 * H32 * (lse.abs() + z.abs().amax(1)) * (1 + math.log2(V))
+    coef = torch.where(valid, d.double().cpu() * scale, 0.0)[:, None]
+    p = (z - lse[:, None]).exp()
+    gr = coef * (p - y)
+    eg = coef.abs() * (p * (ez + el[:, None] + (z - lse[:, None]).abs() * 4 * H32 + 8 * H32) +
+                       4 * H32 * (p + y)) + H16 * gr.abs()
+    dx, dw = gr @ wd, gr.t() @ xd
+    ex = eg @ wd.abs() + (V + 4) * ACC * (gr.abs() @ wd.abs())
+    ew = eg.t() @ xd.abs() + (xd.shape[0] + 4) * ACC * (gr.abs().t() @ xd.abs())
+    if w_mn:
+        dw, ew = dw.t(), ew.t()
+    return loss, eloss, lse, el, dx, ex, dw, ew
+
+
+HEADS = [(1, 64, 1, 0), (1, 768, 5003, 0), (5, 8, 100, 256), (33, 72, 257, 256), (256, 128, 256, 0),
+         (130, 200, 1000, 512), (300, 765, 3001, 1024), (513, 264, 2048, 2048), (64, 64, 20011, 0)]
+
+
+@pytest.mark.parametrize("rows,C,V,piece", HEADS)
+@pytest.mark.parametrize("smoothing,w_mn,ignored", [(0.0, False, False), (0.1, True, True),
+                                                    (0.0, True, False), (0.2, False, True)])
+def test_loss_head(cuda, rows, C, V, piece, smoothing, w_mn, ignored):
+    from llmgpu import ops
+    x, w, t, d = _head_case(cuda, rows, C, V, w_mn, ignored, rows + C + V)
+    loss, eloss, lse, el, dx, ex, dw, ew = _head_want(x, w, t, d, 0.5, smoothing, w_mn)
+    gl, gs = ops.linear_cross_entropy_fwd(x, w, t, smoothing, w_mn)
+    _close(gl, loss, eloss, "loss")
+    _close(gs, lse, el, "lse")
+    gx, gw = ops.linear_cross_entropy_bwd(x, w, t, gs, d, 0.5, smoothing, w_mn, piece=piece)
+    _close(gx, dx, ex + H16 * (dx.abs() + ex), "dx")
+    _close(gw, dw, ew + H16 * (dw.abs() + ew), "dw")
+    left = (t < 0) | (t >= V)
+    assert not bool(gl[left].any()) and not bool(gx[left].any())
+    if rows * V >= 4096:
+        _norm_close(gx, dx, NORM16, "dx")
+        _norm_close(gw, dw, NORM16, "dw")
+    wr, wc = (C, V) if w_mn else (V, C)
+    aw, check = _guard(wr, wc, F32, cuda, wc + 3, 1)
+    aw.fill_(0.25)
+    gx32, _ = ops.linear_cross_entropy_bwd(x, w, t, gs, d, 0.5, smoothing, w_mn, dx_dtype=F32, dw=aw,
+                                           accumulate=True, piece=piece)
+    _close(gx32, dx, ex, "f32 dx")
+    _close(aw, dw + 0.25, ew + H32 * (dw.abs() + 0.25 + ew), "accumulated dw")
+    check()
+    assert torch.equal(ops.linear_cross_entropy_bwd(x, w, t, gs, d, 0.5, smoothing, w_mn, piece=piece,
+                                                    need_dw=False)[0], gx)
+    assert torch.equal(ops.linear_cross_entropy_bwd(x, w, t, gs, d, 0.5, smoothing, w_mn, piece=piece,
+                                                    need_dx=False)[1], gw)
+    ops.check_device(cuda)
+
+
+def test_loss_head_rows_left_out_may_hold_anything(cuda):
+    """A padded batch whose padding rows hold NaN and infinities: they reach nothing."""
+    from llmgpu import ops
+    x, w, t, d = _head_case(cuda, 70, 64, 700, False, True, 1)
+    left = (t < 0) | (t >= 700)
+    clean = [ops.linear_cross_entropy_fwd(x, w, t)]
+    clean.append(ops.linear_cross_entropy_bwd(x, w, t, clean[0][1], d))
+    for bad in (float("nan"), float("inf"), torch.finfo(BF).min):
+        y = x.clone()
+        y[left] = bad
+        dd = d.clone()
+        dd[left] = float("nan")
+        loss, lse = ops.linear_cross_entropy_fwd(y, w, t)
+        dx, dw = ops.linear_cross_entropy_bwd(y, w, t, lse, dd)
+        assert torch.equal(loss, clean[0][0])
+        assert torch.equal(dx, clean[1][0]) and torch.equal(dw, clean[1][1])
+    none = torch.full_like(t, -1)  # every row left out
+    loss, lse = ops.linear_cross_entropy_fwd(x, w, none)
+    dx, dw = ops.linear_cross_entropy_bwd(x, w, none, lse, d)
+    assert not loss.any() and not dx.any() and not dw.any()
+
+
+def test_loss_head_extreme_logits(cuda):
+    """Logits of -inf (a vocabulary entry ruled out) and rows of very large logits."""
+    from llmgpu import ops
+    C, V = 64, 300
+    x = torch.zeros(40, C, dtype=BF, device=cuda)
+    x[:, 0] = 1.0
+    x[1::2, 0] = 1000.0
+    g = torch.Generator().manual_seed(0)
+    w = torch.zeros(V, C, dtype=BF)
+    w[:, 0] = torch.randn(V, generator=g).to(BF)
+    w[130:260, 0] = torch.finfo(BF).min  # -inf from the second row on, the lowest value in the first
+    t = torch.randint(0, 130, (40,), generator=g, dtype=torch.int32).to(cuda)
+    w = w.to(cuda)
+    z = (x.float() @ w.float().t()).double()
+    loss, lse = ops.linear_cross_entropy_fwd(x, w, t)
+    want = torch.logsumexp(z, 1)
+    _close(lse, want, 8 * H32 * (1 + want.abs()), "lse")
+    wl = want - z.gather(1, t.long()[:, None])[:, 0]
+    _close(loss, wl, 16 * H32 * (1 + want.abs()), "loss")
+    dx, _ = ops.linear_cross_entropy_bwd(x, w[:130].contiguous(), t,
+                                         ops.linear_cross_entropy_fwd(x, w[:130].contiguous(), t)[1])
+    assert bool(torch.isfinite(dx.float()).all())
+
+
+def test_loss_head_no_rows(cuda):
+    from llmgpu import ops
+    x, w = torch.empty(0, 16, dtype=BF, device=cuda), torch.ones(40, 16, dtype=BF, device=cuda)
+    t = torch.empty(0, dtype=torch.int32, device=cuda)
+    loss, lse = ops.linear_cross_entropy_fwd(x, w, t)
+    dx, dw = ops.linear_cross_entropy_bwd(x, w, t, lse)
+    assert loss.shape == (0,) and dx.shape == (0, 16) and not dw.any()
+
+
+def test_loss_head_agrees_with_cross_entropy_over_logits(cuda):
+    """The framework's loss over logits in memory, on the same (bf16-rounded) logits: an identity
+    weight makes the head's logits the rows of x themselves. The gradients agree with smoothed
+    labels too; the loss over logits leaves the smoothing out of what it reports."""
+    from llmgpu import ops
+    g = torch.Generator().manual_seed(4)
+    V = 512
+    x = (torch.randn(96, V, generator=g) * 2).to(BF).to(cuda)
+    w = torch.eye(V, dtype=BF, device=cuda)
+    t = torch.randint(0, V, (96,), generator=g, dtype=torch.int32).to(cuda)
+    logits = x.clone()
+    want = ops.cross_entropy(logits, V, t, 0.5, 0.1)
+    loss, lse = ops.linear_cross_entropy_fwd(x, w, t)
+    assert float((loss - want).abs().max()) < 2e-5  # f32 sums of 512 terms on both sides
+    dx, _ = ops.linear_cross_entropy_bwd(x, w, t, lse, None, 0.5, 0.1)
+    # both round the same gradient to bf16 (dx = G I exactly); a difference in the last f32 bits
+    # can cross a rounding border: one step
+    assert float((dx.float() - logits.float()).abs().max()) <= 2 * H16 * float(logits.float().abs().max())
+
+
+# -------------------------------------------------------------------------- gradients by difference
+def test_gradients_against_differences(cuda):
+    """Central differences of the operators' own forward along directions that bf16 holds exactly:
+    inputs are multiples of 1/16 below 4, the step is 1/16, so x +- h d are exact. The cubic
+    term of a difference is at most h^2 / 6 times the third derivative along d."""
+    from llmgpu import ops
+    g = torch.Generator().manual_seed(12)
+    rows, C, V, h = 24, 32, 96, 1.0 / 16
+
+    def grid(*shape):
+        return (torch.randint(-16, 17, shape, generator=g) / 16).to(BF).to(cuda)
+    x, w = grid(rows, C), grid(V, C)
+    t = torch.randint(0, V, (rows,), generator=g, dtype=torch.int32).to(cuda)
+
+    def loss(a, b):
+        return ops.linear_cross_entropy_fwd(a, b, t, 0.1)[0].double().sum().item()
+    _, lse = ops.linear_cross_entropy_fwd(x, w, t, 0.1)
+    dx, dw = ops.linear_cross_entropy_bwd(x, w, t, lse, None, 1.0, 0.1)
+    for grad, at in ((dx, 0), (dw, 1)):
+        for _ in range(4):
+            # one coordinate per row of x (rows do not interact) or a single entry of w
+            d = torch.zeros_like(x if at == 0 else w)
+            if at == 0:
+                d[torch.arange(rows), torch.randint(0, C, (rows,), generator=g)] = 1.0
+            else:
+                d[int(torch.randint(0, V, (1,), generator=g)), int(torch.randint(0, C, (1,), generator=g))] = 1.0
+            hi = (x + h * d, w) if at == 0 else (x, w + h * d)
+            lo = (x - h * d, w) if at == 0 else (x, w - h * d)
+            got = (loss(*hi) - loss(*lo)) / (2 * h)
+            want = float((grad.double() * d.double()).sum())
+            # |third derivative| of a log-sum-exp along a unit coordinate: at most 2 max |c|^3 per
+            # row, |c| <= 1 (its coefficients are entries of x or w, at most 1)
+            tol = rows * (2 * h * h / 6) + 2 * H16 * float((grad.double() * d.double()).abs().sum()) + \
+                rows * 64 * H32 / h
+            assert abs(got - want) <= tol, (at, got, want, tol)
+    # the linear layer: silu, dropout, bias; the sum of its f32 outputs weighted by dy
+    xl, wl = grid(rows, C), grid(48, C)
+    b = torch.zeros(48, device=cuda)
+    rng = _rng(cuda, 6, 7)
+    dy = torch.randn(rows, 48, generator=g).to(cuda)
+
+    def total(a, m, c):
+        y, _ = ops.linear_fwd(a, m, c, "silu", 0.25, rng, 1, out_dtype=F32)
+        return (y.double() * dy.double()).sum().item()
+    _, pre = ops.linear_fwd(xl, wl, b, "silu", 0.25, rng, 1, save_pre=True)
+    gx, gw, gb = ops.linear_bwd(dy, xl, wl, pre, "silu", 0.25, rng, 1)
+    for grad, at in ((gx, 0), (gw, 1), (gb, 2)):
+        for k in range(4):
+            args_hi, args_lo = [xl, wl, b], [xl, wl, b]
+            d = torch.zeros_like(args_hi[at])
+            d.view(-1)[int(torch.randint(0, d.numel(), (1,), generator=g))] = 1.0
+            args_hi[at], args_lo[at] = args_hi[at] + h * d, args_lo[at] - h * d
+            got = (total(*args_hi) - total(*args_lo)) / (2 * h)
+            want = float((grad.double() * d.double()).sum())
+            # silu''' is below 0.6; pre is rounded to bf16 (|z| below 16: off by 16 H16, silu'' below
+            # 0.5); dz and the gradient are rounded to bf16
+            reach = float(dy.double().abs().sum()) / 0.75 / (1 if at == 0 else 48) * 4
+            tol = reach * (0.6 * h * h / 6 + 8 * H16 + 2 * H16 + 64 * H32 / h)
+            assert abs(got - want) <= tol, (at, got, want, tol)
+
+
+# ----------------------------------------------------------------------------- used together
+def _block(ops, s, rng):
+    """Embedding dropout, a feed-forward block with its residual, the head's loss, and the way back:
+    the losses and every gradient."""
+    x0 = ops.dropout_fwd(s["x"], 0.1, rng, site=0)
+    a, pre = ops.linear_fwd(x0, s["w1"], s["b1"], "gelu", save_pre=True)
+    y, _ = ops.linear_fwd(a, s["w2"], s["b2"], "none", 0.1, rng, 1, resid=x0, w_mn=True)
+    loss, lse = ops.linear_cross_entropy_fwd(y, s["wv"], s["t"])
+    dy, dwv = ops.linear_cross_entropy_bwd(y, s["wv"], s["t"], lse, s["d"])
+    da, dw2, db2 = ops.linear_bwd(dy, a, s["w2"], None, "none", 0.1, rng, 1, w_mn=True)
+    dx0, dw1, db1 = ops.linear_bwd(da, x0, s["w1"], pre, "gelu")
+    dx = ops.dropout_bwd(dx0 + dy, 0.1, rng, site=0)
+    return dict(loss=loss, dwv=dwv, dw2=dw2, db2=db2, dw1=dw1, db1=db1, dx=dx)
+
+
+def _block_state(cuda, seed, rows=200, C=96, F=256, V=517):
+    g = torch.Generator().manual_seed(seed)
+
+    def m(r, c, scale):
+        return _mat(g, r, c, BF, cuda, scale)[0]
+    return dict(x=m(rows, C, 1.0), w1=m(F, C, 0.1), w2=m(F, C, 0.06), wv=m(V, C, 0.2),
+                b1=(torch.randn(F, generator=g) * 0.1).to(cuda),
+                b2=(torch.randn(C, generator=g) * 0.1).to(cuda),
+                t=torch.randint(-1, V, (rows,), generator=g, dtype=torch.int32).to(cuda),
+                d=torch.full((rows,), 1.0 / rows, device=cuda))
+
+
+def _block_want(s, rng):
+    """The same in 64 bits by autograd."""
+    v = {k: s[k].double().cpu().requires_grad_(True) for k in ("x", "w1", "w2", "wv", "b1", "b2")}
+    rows, C = s["x"].shape
+    seed, off = (int(q) for q in rng.tolist())
+    k0, sc = ref.keep_mask(seed, off, rows, C, 0.1)
+    k1, _ = ref.keep_mask(seed, off + 1, rows, C, 0.1)
+    x0 = torch.where(k0, v["x"] * sc, 0.0)
+    a = ref.act(x0 @ v["w1"].t() + v["b1"], "gelu")
+    y = x0 + torch.where(k1, (a @ v["w2"] + v["b2"]) * sc, 0.0)
+    loss = ref.head(y, v["wv"], s["t"].cpu(), 0.0)[0]
+    (loss * s["d"].double().cpu()).sum().backward()
+    return dict(loss=loss.detach(), dwv=v["wv"].grad, dw2=v["w2"].grad, db2=v["b2"].grad,
+                dw1=v["w1"].grad, db1=v["b1"].grad, dx=v["x"].grad)
+
+
+def test_block_forward_and_backward(cuda):
+    """Every value passes at most 8 roundings to bf16 on its way (x0, pre, a, y, the gradients by
+    logits, dy, dz twice), each with a root mean square of at most H16 / sqrt(3)."""
+    from llmgpu import ops
+    s, rng = _block_state(cuda, 3), _rng(cuda, 21, 4)
+    got, want = _block(ops, s, rng), _block_want(s, rng)
+    for k in want:
+        _norm_close(got[k], want[k], 8 * H16 / math.sqrt(3), k)
+    ops.check_device(cuda)
+
+
+def test_block_is_repeatable_and_captures(cuda):
+    """Same bits on every run and in a captured graph; a replay reads the generator's new offset;
+    two graphs and eager calls on two streams do not disturb one another."""
+    from llmgpu import ops
+    s, s2 = _block_state(cuda, 3), _block_state(cuda, 4, rows=333, C=64, F=128, V=1000)
+    rng, rng2 = _rng(cuda, 21, 4), _rng(cuda, 5, 6)
+    first = _block(ops, s, rng)
+    for k, v in _block(ops, s, rng).items():
+        assert torch.equal(v, first[k]), k
+    other = _block(ops, s2, rng2)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        o1 = _block(ops, s, rng)
+    with torch.cuda.graph(g2):
+        o2 = _block(ops, s2, rng2)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(a):
+            g1.replay()
+        with torch.cuda.stream(b):
+            g2.replay()
+    e = _block(ops, s, rng)
+    torch.cuda.synchronize()
+    for k in first:
+        assert torch.equal(o1[k], first[k]) and torch.equal(e[k], first[k]), k
+        assert torch.equal(o2[k], other[k]), k
+    rng[1] += 1000
+    g1.replay()
+    torch.cuda.synchronize()
+    moved = _block(ops, s, rng)
+    assert all(torch.equal(o1[k], moved[k]) for k in moved)
+    assert not torch.equal(moved["dx"], first["dx"])
+    ops.check_device(cuda)
+
+
+def test_two_calls_at_once(cuda):
+    """The same operators at once on two streams, each with its own workspace."""
+    from llmgpu import ops
+    s = [_block_state(cuda, 10 + i, rows=700, C=128, F=512, V=3000) for i in range(2)]
+    rng = _rng(cuda, 1, 1)
+    want = [_block(ops, q, rng) for q in s]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i] = _block(ops, s[i], rng)
+    torch.cuda.synchronize()
+    for i in range(2):
+        for k in want[i]:
+            assert torch.equal(got[i][k], want[i][k]), (i, k)
+
+
+# ------------------------------------------------------------------------------------ refusals
+def test_wrapper_refusals(cuda):
+    from llmgpu import ops
+    x, w = torch.zeros(6, 16, dtype=BF, device=cuda), torch.zeros(24, 16, dtype=BF, device=cuda)
+    rng = _rng(cuda)
+    t = torch.zeros(6, dtype=torch.int32, device=cuda)
+    odd = torch.zeros(6, 17, dtype=BF, device=cuda)
+    bad = [lambda: ops.dropout_fwd(x, 1.5, rng), lambda: ops.dropout_fwd(x, 0.5, None),
+           lambda: ops.dropout_fwd(x, 0.5, rng.to(torch.int32)),
+           lambda: ops.dropout_fwd(x.half(), 0.5, rng), lambda: ops.dropout_fwd(x.t(), 0.5, rng),
+           lambda: ops.dropout_fwd(x, 0.5, rng, resid=w),
+           lambda: ops.dropout_fwd(x, 0.5, rng, resid=x.float()),
+           lambda: ops.dropout_fwd(x[0], 0.5, rng),
+           lambda: ops.dropout_fwd(x, 0.5, rng, out=x.new_zeros(1, 16).expand(6, 16)),
+           lambda: ops.linear_fwd(x, w, act="tanh"), lambda: ops.linear_fwd(x.float(), w),
+           lambda: ops.linear_fwd(x, w, w_mn=True), lambda: ops.linear_fwd(odd[:, 1:], w),
+           lambda: ops.linear_fwd(odd[:, :16], w), lambda: ops.linear_fwd(x, w, p=0.5),
+           lambda: ops.linear_fwd(x, w, bias=torch.zeros(16, device=cuda)),
+           lambda: ops.linear_fwd(x, w, resid=torch.zeros(6, 24, device=cuda)),
+           lambda: ops.linear_fwd(x, w, out=torch.zeros(6, 23, dtype=BF, device=cuda)),
+           lambda: ops.linear_bwd(torch.zeros(6, 24, device=cuda), x, w, act="gelu"),
+           lambda: ops.linear_bwd(torch.zeros(6, 23, device=cuda), x, w),
+           lambda: ops.linear_bwd(torch.zeros(6, 24, device=cuda), x, w, accumulate=True),
+           lambda: ops.linear_bwd(torch.zeros(6, 24, device=cuda), x, w, accumulate=True,
+                                  dw=torch.zeros_like(w), dbias=torch.zeros(24, device=cuda)),
+           lambda: ops.linear_cross_entropy_fwd(x, w, t.long()),
+           lambda: ops.linear_cross_entropy_fwd(x, w, t, 1.0),
+           lambda: ops.linear_cross_entropy_fwd(x, w, t[:5]),
+           lambda: ops.linear_cross_entropy_bwd(x, w, t, torch.zeros(6, device=cuda), piece=100),
+           lambda: ops.linear_cross_entropy_bwd(x, w, t, torch.zeros(5, device=cuda)),
+           lambda: ops.linear_cross_entropy_bwd(x, w, t, torch.zeros(6, device=cuda),
+                                                dw=torch.zeros_like(w), accumulate=True)]
+    for i, f in enumerate(bad):
+        with pytest.raises(ops.KernelError):
+            f()
+            pytest.fail(f"call {i} was not refused")

@@ -1,0 +1,142 @@
+"""CPU checks of dropout, the linear layer and the loss head: the generator against its published
+known answers, and the refusals that no kernel has to see (the C ABI's and the wrappers')."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import linear_ops_ref as ref
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("ctr,key,want", [
+    ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((ref.LOW,) * 4, (ref.LOW,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_generator_known_answers(ctr, key, want):
+    """The known-answer vectors published with the generator."""
+    assert tuple(int(v) for v in ref.philox(ctr, key)) == want
+
+
+def test_mask_frequency():
+    """Kept share within 5 standard deviations of the quantised probability."""
+    n = 512 * 1024
+    for p in (0.1, 0.5):
+        keep, scale = ref.keep_mask(5, 11, 512, 1024, p)
+        q = 1 / scale
+        assert abs(keep.double().mean().item() - q) < 5 * np.sqrt(q * (1 - q) / n)
+
+
+def _lib():
+    from llmgpu import load
+    return load()
+
+
+P = 0x1000  # a made-up device address: every call below is refused before it is used
+REFUSED = (-1, -3)  # the checks' own codes; a launch or a tensor map that failed has others
+
+
+@pytest.mark.parametrize("bad", [dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(rows=-1),
+                                 dict(cols=(1 << 30) + 1), dict(x=None), dict(out=None),
+                                 dict(rng=None), dict(ldx=7), dict(ldo=7), dict(resid=P, ldr=7)])
+def test_dropout_refusals(bad):
+    a = dict(x=P, ldx=8, resid=None, ldr=0, out=P, ldo=8, rows=4, cols=8, p=0.5, rng=P)
+    a.update(bad)
+    assert _lib().llmgpu_op_dropout(a["x"], 0, a["ldx"], a["resid"], a["ldr"], a["out"], 0, a["ldo"],
+                                    a["rows"], a["cols"], a["p"], a["rng"], 0, None) in REFUSED
+
+
+def test_empty_calls_do_nothing():
+    lib = _lib()
+    assert lib.llmgpu_op_dropout(None, 0, 8, None, 0, None, 0, 8, 0, 8, 0.5, None, 0, None) == 0
+    assert lib.llmgpu_op_linear_fwd(None, 8, P, 8, 0, None, 0, 0.0, None, 0, None, 0, None, 0, None,
+                                    0, 8, 0, 8, 8, None, None) == 0
+    assert lib.llmgpu_op_linear_ce_fwd(None, 8, P, 8, 0, None, 0, 8, 8, 0.0, None, None, None, None,
+                                       None) == 0
+    assert lib.llmgpu_op_linear_bwd_work(0, 8, 8) == 0
+    assert lib.llmgpu_op_linear_ce_fwd_work(0, 8) == 0
+    assert lib.llmgpu_op_linear_ce_bwd_work(0, 8, 8, 0) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(act=4), dict(act=-1), dict(K=0), dict(N=0), dict(M=-1),
+                                 dict(p=2.0), dict(p=0.5), dict(x=None), dict(w=None),
+                                 dict(out=None), dict(ldx=8), dict(ldw=8), dict(ldo=8),
+                                 dict(resid=P, ldr=8), dict(pre=P, ld_pre=8), dict(x=P + 2),
+                                 dict(ldx=17), dict(w=P + 8), dict(w_mn=1, ldw=8)])
+def test_linear_fwd_refusals(bad):
+    a = dict(x=P, ldx=16, w=P, ldw=16, w_mn=0, act=0, p=0.0, resid=None, ldr=0, pre=None, ld_pre=0,
+             out=P, ldo=16, M=4, N=16, K=16)
+    a.update(bad)
+    rc = _lib().llmgpu_op_linear_fwd(a["x"], a["ldx"], a["w"], a["ldw"], a["w_mn"], None, a["act"],
+                                     a["p"], None, 0, a["resid"], a["ldr"], a["pre"], a["ld_pre"],
+                                     a["out"], 0, a["ldo"], a["M"], a["N"], a["K"], None, None)
+    assert rc in REFUSED
+
+
+@pytest.mark.parametrize("bad", [dict(act=5), dict(act=1, pre=None), dict(p=0.5), dict(dy=None),
+                                 dict(work=None), dict(work=P + 8), dict(lddy=8), dict(ldx=8),
+                                 dict(lddx=8), dict(lddw=8), dict(acc=1), dict(N=0), dict(K=-1)])
+def test_linear_bwd_refusals(bad):
+    a = dict(dy=P, lddy=16, ldx=16, pre=None, act=0, p=0.0, lddx=16, lddw=16, acc=0, M=4, N=16, K=16,
+             work=P)
+    a.update(bad)
+    rc = _lib().llmgpu_op_linear_bwd(a["dy"], 1, a["lddy"], P, a["ldx"], P, 16, 0, a["pre"], 16,
+                                     a["act"], a["p"], None, 0, P, 0, a["lddx"], P, 0, a["lddw"], P,
+                                     a["acc"], a["M"], a["N"], a["K"], a["work"], None, None)
+    assert rc in REFUSED
+
+
+@pytest.mark.parametrize("bad", [dict(smoothing=1.0), dict(smoothing=-0.1), dict(V=0), dict(C=0),
+                                 dict(V=(1 << 30) + 1), dict(targets=None), dict(work=None),
+                                 dict(lse=None), dict(ldx=8), dict(ldw=8), dict(x=P + 2),
+                                 dict(rows=-1)])
+def test_loss_head_refusals(bad):
+    a = dict(x=P, ldx=16, ldw=16, targets=P, rows=4, C=16, V=32, smoothing=0.0, lse=P, work=P)
+    a.update(bad)
+    lib = _lib()
+    assert lib.llmgpu_op_linear_ce_fwd(a["x"], a["ldx"], P, a["ldw"], 0, a["targets"], a["rows"],
+                                       a["C"], a["V"], a["smoothing"], P, a["lse"], a["work"], None,
+                                       None) in REFUSED
+    assert lib.llmgpu_op_linear_ce_bwd(a["x"], a["ldx"], P, a["ldw"], 0, a["targets"], a["lse"], None,
+                                       1.0, a["rows"], a["C"], a["V"], a["smoothing"], P, 0, 16, P, 0,
+                                       16, 0, 0, a["work"], None, None) in REFUSED
+
+
+@pytest.mark.parametrize("bad", [dict(piece=100), dict(piece=-256), dict(acc=1), dict(lddx=8),
+                                 dict(lddw=8)])
+def test_loss_head_bwd_refusals(bad):
+    a = dict(piece=0, acc=0, lddx=16, lddw=16)
+    a.update(bad)
+    lib = _lib()
+    assert lib.llmgpu_op_linear_ce_bwd(P, 16, P, 16, 0, P, P, None, 1.0, 4, 16, 32, 0.0, P, 0,
+                                       a["lddx"], P, 0, a["lddw"], a["acc"], a["piece"], P, None,
+                                       None) in REFUSED
+    if "piece" in bad:
+        assert lib.llmgpu_op_linear_ce_bwd_work(4, 16, 32, bad["piece"]) < 0
+
+
+def test_workspace_covers_any_piece():
+    """The workspace grows with the piece and never past the whole vocabulary's."""
+    f = _lib().llmgpu_op_linear_ce_bwd_work
+    sizes = [f(100, 64, 5000, p) for p in (256, 512, 2048, 4096, 8192, 1 << 20)]
+    assert sizes == sorted(sizes) and sizes[-1] == sizes[-2] and sizes[0] > 0
+    assert f(100, 64, 5000, 0) <= sizes[-1]
+
+
+def test_wrappers_refuse_cpu_tensors():
+    from llmgpu import ops
+    x, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    rng = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.dropout_fwd(x, 0.5, rng)
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.linear_fwd(x, w)
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.linear_bwd(x, x, w)
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.linear_cross_entropy_fwd(x, w, torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.linear_cross_entropy_bwd(x, w, torch.zeros(4, dtype=torch.int32), torch.zeros(4))
