@@ -62,10 +62,117 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const TI* x, long
     }
 }
 
+// Eight neighbouring elements, 16 bytes at a time.
+__device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = bf16_lo(w[i]);
+        v[2 * i + 1] = bf16_hi(w[i]);
+    }
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0];
+    const float4 b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void store8(bf16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                   pack_bf16x2(v[6], v[7]));
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Rows on 16 bytes: a thread takes 8 columns (one call of the generator) at a time, kDropUnroll of
+// them with all loads in flight before the generator's arithmetic. The positions of a thread lie
+// gridDim * 256 groups of 8 apart; (dr, dc) is that distance in rows and groups, so the loop
+// divides nothing.
+constexpr int kDropUnroll = 4;
+template <typename TI, typename TO, bool RES>
+__global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(
+    const TI* x, long long ldx, const TO* resid, long long ldr, TO* out, long long ldo,
+    uint32_t rows, int cols, uint32_t n8, uint32_t dr, uint32_t dc, uint32_t thr, float scale,
+    const uint64_t* rng, uint64_t site) {
+    pdl_enter();
+    const DropKey key = drop_key(rng, site);
+    const uint32_t first = blockIdx.x * kDropThreads + threadIdx.x;
+    uint32_t row = first / n8, c8 = first - row * n8;
+    while (row < rows) {
+        float v[kDropUnroll][8], r[kDropUnroll][8];
+        uint32_t ur[kDropUnroll], uc[kDropUnroll];
+#pragma unroll
+        for (int u = 0; u < kDropUnroll; ++u) {
+            ur[u] = row;
+            uc[u] = c8;
+            const int c = (int)(c8 * 8);
+            if (row < rows) {
+                if (c + 8 <= cols) {
+                    load8(x + row * ldx + c, v[u]);
+                    if (RES) load8(resid + row * ldr + c, r[u]);
+                } else {
+                    for (int j = 0; j < 8; ++j) {
+                        v[u][j] = c + j < cols ? to_f32(x[row * ldx + c + j]) : 0.0f;
+                        if (RES) r[u][j] = c + j < cols ? to_f32(resid[row * ldr + c + j]) : 0.0f;
+                    }
+                }
+            }
+            row += dr;
+            c8 += dc;
+            if (c8 >= n8) {
+                c8 -= n8;
+                ++row;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kDropUnroll; ++u) {
+            if (ur[u] >= rows) break;
+            const uint32_t m = drop_keep8(key, uc[u], ur[u], thr);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[u][j] = ((m >> j) & 1u) ? v[u][j] * scale : 0.0f;
+                if (RES) v[u][j] += r[u][j];
+            }
+            const int c = (int)(uc[u] * 8);
+            if (c + 8 <= cols) {
+                store8(out + ur[u] * ldo + c, v[u]);
+            } else {
+                for (int j = 0; j < 8; ++j)
+                    if (c + j < cols) out[ur[u] * ldo + c + j] = from_f32<TO>(v[u][j]);
+            }
+        }
+    }
+}
+
+template <typename T>
+bool rows_on_16(const T* p, long long ld) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
+}
+
 template <typename TI, typename TO>
 int launch_dropout(const void* x, long long ldx, const void* resid, long long ldr, void* out,
                    long long ldo, int rows, int cols, uint32_t thr, float scale,
                    const uint64_t* rng, uint64_t site, cudaStream_t s) {
+    if (rows_on_16((const TI*)x, ldx) && rows_on_16((const TO*)out, ldo) &&
+        (!resid || rows_on_16((const TO*)resid, ldr))) {
+        const uint32_t n8 = (uint32_t)(cols + 7) / 8;
+        const long long items = (long long)rows * n8;
+        long long blocks = (items + kDropThreads - 1) / kDropThreads;
+        if (blocks > 148 * 8) blocks = 148 * 8;
+        const uint32_t step = (uint32_t)blocks * kDropThreads;
+        return resid ? launch_kernel(dropout_vec_kernel<TI, TO, true>, (int)blocks, kDropThreads, 0, s,
+                                     (const TI*)x, ldx, (const TO*)resid, ldr, (TO*)out, ldo,
+                                     (uint32_t)rows, cols, n8, step / n8, step % n8, thr, scale, rng,
+                                     site)
+                     : launch_kernel(dropout_vec_kernel<TI, TO, false>, (int)blocks, kDropThreads, 0, s,
+                                     (const TI*)x, ldx, (const TO*)resid, ldr, (TO*)out, ldo,
+                                     (uint32_t)rows, cols, n8, step / n8, step % n8, thr, scale, rng,
+                                     site);
+    }
     const long long warps = (long long)rows * ((cols + 255) / 256);
     long long blocks = (warps + kDropThreads / 32 - 1) / (kDropThreads / 32);
     if (blocks > 148 * 8) blocks = 148 * 8;

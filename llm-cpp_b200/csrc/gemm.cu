@@ -31,6 +31,7 @@ constexpr int kGemmThreads = 256;
 // quarter, each draining half of a tile's columns)
 constexpr int kPairThreads = 384;
 constexpr int kPairEpiWarps = 8;
+constexpr int kChainBlocks = 8;  // k-blocks of an accumulator chain (512 products), see chain_sum
 constexpr int kGroupM = 16;  // tile raster: groups of 16 m-blocks share B tiles in L2
 
 template <int BN>
@@ -550,11 +551,10 @@ struct ExtOf<kFamBase> {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// 1 / (1 + exp(-t)) from the special-function unit's 2^x and a correctly rounded reciprocal: a few
-// units in the last place, which an f32 output keeps. t far below 0: exp overflows to inf and
-// the result is 0.
+// 1 / (1 + exp(-t)) from the special-function unit's 2^x and reciprocal: a few units in the last
+// place, which an f32 output keeps. t far below 0: exp overflows to inf and the result is 0.
 __device__ __forceinline__ float sigmoid_f32(float t) {
-    return __frcp_rn(1.0f + ex2_approx(-t * kLog2e));
+    return rcp_approx(1.0f + ex2_approx(-t * kLog2e));
 }
 __device__ __forceinline__ float act_apply(int act, float z) {
     switch (act) {
@@ -572,33 +572,82 @@ __device__ __forceinline__ float act_apply(int act, float z) {
     }
 }
 
-// resid + drop(act(acc + bias)). A lane holds 32 columns of its row; they are turned through the
-// warp's 8 KB of shared memory (32 rows of 33 floats) so that every access to the outputs and
-// to the residual is a row of 32 neighbouring columns, whatever their strides and alignment.
-template <int NCOLS>
-__device__ __forceinline__ void linear_epilogue_tile(const GemmArgs& a, const GemmExt& x,
-                                                     const DropKey& key, uint32_t tbase, int row0,
-                                                     int n0, int lane, EpiWarp& w, int c_begin,
-                                                     int c_end) {
+// One lane's 32 accumulator columns [col0, col0 + 32) plus the bias.
+__device__ __forceinline__ void linear_bias(const GemmArgs& a, const GemmExt& x, int col0, int lane,
+                                            const uint32_t (&r)[32], float (&v)[32]) {
+    if (!x.bias) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+    } else if (col0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(x.bias) & 15) == 0) {
+        const float4* b4 = reinterpret_cast<const float4*>(x.bias + col0);  // same for all lanes
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float4 b = b4[q];
+            v[4 * q] = __uint_as_float(r[4 * q]) + b.x;
+            v[4 * q + 1] = __uint_as_float(r[4 * q + 1]) + b.y;
+            v[4 * q + 2] = __uint_as_float(r[4 * q + 2]) + b.z;
+            v[4 * q + 3] = __uint_as_float(r[4 * q + 3]) + b.w;
+        }
+    } else {
+        const float b = col0 + lane < a.N ? x.bias[col0 + lane] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + __shfl_sync(0xffffffffu, b, j);
+    }
+}
+// act, then dropout, of those columns.
+__device__ __forceinline__ void linear_act_drop(const GemmExt& x, const DropKey& key, int col0,
+                                                int row, float (&v)[32]) {
+    // the switch stands outside the loops: one branch for 32 columns
+    switch (x.act) {
+        case kActRelu:
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_apply(kActRelu, v[j]);
+            break;
+        case kActGelu:
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_apply(kActGelu, v[j]);
+            break;
+        case kActSilu:
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_apply(kActSilu, v[j]);
+            break;
+        default:
+            break;
+    }
+    if (x.rng) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t m =
+                drop_keep8(key, (uint32_t)(col0 >> 3) + q, (uint32_t)row, x.drop_thr);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[8 * q + j] = ((m >> j) & 1u) ? v[8 * q + j] * x.drop_scale : 0.0f;
+        }
+    }
+}
+
+// Outputs (and a residual) of any stride and alignment, and the rare pairs of them that the boxes
+// below do not cover: a lane's 32 columns are turned through the warp's 8 KB of shared memory (32
+// rows of 33 floats), so that every access to global memory is 32 neighbouring columns of a row.
+__device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const GemmExt& x,
+                                                   const DropKey& key, uint32_t tbase, int row0,
+                                                   int n0, int lane, EpiWarp& w, int c_begin,
+                                                   int c_end) {
     if (row0 >= a.M) return;
-    const int row = row0 + lane;
     const int nrows = min(32, a.M - row0);
     float* tile = reinterpret_cast<float*>(w.stage);
 #pragma unroll 1
     for (int c = c_begin; c < c_end; ++c) {
         const int col0 = n0 + c * 32;
         if (col0 >= a.N) break;
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tbase + (uint32_t)(c * 32), r);
         const int col = col0 + lane;
         const bool in = col < a.N;
-        const float b = (x.bias && in) ? x.bias[col] : 0.0f;
-        tmem_ld_wait();
+        uint32_t r[32];
         float v[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + __shfl_sync(0xffffffffu, b, j);
+        tmem_ld_32x32b_x32(tbase + (uint32_t)(c * 32), r);
+        tmem_ld_wait();
+        linear_bias(a, x, col0, lane, r, v);
         if (a.aux) {
-            __syncwarp();
 #pragma unroll
             for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = v[j];
             __syncwarp();
@@ -606,49 +655,208 @@ __device__ __forceinline__ void linear_epilogue_tile(const GemmArgs& a, const Ge
             if (in)
                 for (int i = 0; i < nrows; ++i)
                     p[i * a.ld_aux] = __float2bfloat16_rn(tile[i * 33 + lane]);
+            __syncwarp();
         }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = act_apply(x.act, v[j]);
-        if (x.rng) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t m =
-                    drop_keep8(key, (uint32_t)(col0 >> 3) + q, (uint32_t)row, x.drop_thr);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    v[8 * q + j] = ((m >> j) & 1u) ? v[8 * q + j] * x.drop_scale : 0.0f;
-            }
-        }
-        __syncwarp();
+        linear_act_drop(x, key, col0, row0 + lane, v);
 #pragma unroll
         for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = v[j];
         __syncwarp();
-        if (in) {
-            if (x.out_f32) {
-                float* p = reinterpret_cast<float*>(a.out) + row0 * a.ldo + col;
-                const float* q = x.resid ? reinterpret_cast<const float*>(x.resid) + row0 * x.ldr + col
-                                         : nullptr;
+        if (in && x.out_f32) {
+            float* p = reinterpret_cast<float*>(a.out) + row0 * a.ldo + col;
+            const float* q = reinterpret_cast<const float*>(x.resid) + row0 * x.ldr + col;
 #pragma unroll 4
-                for (int i = 0; i < nrows; ++i) {
-                    float o = tile[i * 33 + lane];
-                    if (q) o += q[i * x.ldr];
-                    p[i * a.ldo] = o;
-                }
-            } else {
-                __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + row0 * a.ldo + col;
-                const __nv_bfloat16* q =
-                    x.resid ? reinterpret_cast<const __nv_bfloat16*>(x.resid) + row0 * x.ldr + col
-                            : nullptr;
+            for (int i = 0; i < nrows; ++i) {
+                float o = tile[i * 33 + lane];
+                if (x.resid) o += q[i * x.ldr];
+                p[i * a.ldo] = o;
+            }
+        } else if (in) {
+            __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + row0 * a.ldo + col;
+            const __nv_bfloat16* q =
+                reinterpret_cast<const __nv_bfloat16*>(x.resid) + row0 * x.ldr + col;
 #pragma unroll 4
-                for (int i = 0; i < nrows; ++i) {
-                    float o = tile[i * 33 + lane];
-                    if (q) o += __bfloat162float(q[i * x.ldr]);
-                    p[i * a.ldo] = __float2bfloat16_rn(o);
-                }
+            for (int i = 0; i < nrows; ++i) {
+                float o = tile[i * 33 + lane];
+                if (x.resid) o += __bfloat162float(q[i * x.ldr]);
+                p[i * a.ldo] = __float2bfloat16_rn(o);
             }
         }
         __syncwarp();
     }
+}
+
+// End of the chunks that leave in boxes of u chunks. A bulk store clips at 16 bytes, not at the
+// element: a last box whose columns end inside 16 bytes would write over what lies behind the
+// row, so those columns are turned.
+__device__ __forceinline__ int linear_box_end(const GemmArgs& a, const GemmExt& x, int row0, int n0,
+                                              int c_begin, int c_end, int u) {
+    const int ce = epi_chunk_end(a, row0, n0, c_begin, c_end);
+    if ((a.N & (x.out_f32 ? 3 : 7)) == 0 || n0 + ce * 32 < a.N) return ce;
+    const int whole = (a.N - n0 - c_begin * 32) / (32 * u) * u;  // chunks of whole boxes
+    return min(ce, c_begin + max(whole, 0));
+}
+
+// The residual's first two units of a tile, loaded before the accumulator is ready (see
+// epilogue_prefetch): f32 units are 32 columns, bf16 units 64, 4 KB each.
+__device__ __forceinline__ void linear_prefetch(const GemmArgs& a, const GemmExt& x,
+                                                const CUtensorMap* tmX, int row0, int n0, int lane,
+                                                EpiWarp& w, int c_begin, int c_end) {
+    if (!a.tma_epi || !x.resid) return;
+    const int u = x.out_f32 ? 1 : 2;
+    const int ce = linear_box_end(a, x, row0, n0, c_begin, c_end, u);
+    if (lane == 0 && ce > c_begin) {
+        bulk_wait_group_read<0>();
+        epi_load_unit(tmX, w, w.slot, n0 + c_begin * 32, row0);
+        if (c_begin + u < ce) epi_load_unit(tmX, w, w.slot ^ 1, n0 + (c_begin + u) * 32, row0);
+    }
+    __syncwarp();
+}
+
+// resid + drop(act(acc + bias)) through swizzled boxes and bulk stores: f32 outputs 32 columns at a
+// time, bf16 outputs 64 (with `pre` beside them, 32 of each). A residual arrives by bulk loads
+// in the box that it is combined in, one unit ahead.
+__device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt& x,
+                                                const DropKey& key, const CUtensorMap* tmO,
+                                                const CUtensorMap* tmX, uint32_t tbase, int row0,
+                                                int n0, int lane, EpiWarp& w, int c_begin,
+                                                int c_end) {
+    const int u = (x.out_f32 || a.aux) ? 1 : 2;
+    const int ce = linear_box_end(a, x, row0, n0, c_begin, c_end, u);
+    const bool res = x.resid != nullptr;
+#pragma unroll 1
+    for (int c = c_begin; c < ce; c += u) {
+        if (res) {
+            // the next unit's residual goes into the box the previous unit stored from
+            if (c > c_begin && c + u < ce && lane == 0) {
+                bulk_wait_group_read<0>();
+                epi_load_unit(tmX, w, w.slot ^ 1, n0 + (c + u) * 32, row0);
+            }
+        } else if (lane == 0) {
+            bulk_wait_group_read<1>();  // this box's previous store has read it
+        }
+        __syncwarp();
+        uint8_t* box = w.stage + w.slot * kEpiSlotBytes;
+        if (res) {
+            mbar_wait_bounded(&w.bar[w.slot], (w.phase >> w.slot) & 1u, a.err, kDevTimeoutFull);
+            w.phase ^= 1u << w.slot;
+            w.pend &= ~(1u << w.slot);
+        }
+#pragma unroll 1
+        for (int h = 0; h < u; ++h) {
+            const int col0 = n0 + (c + h) * 32;
+            uint32_t r[32];
+            float v[32];
+            tmem_ld_32x32b_x32(tbase + (uint32_t)((c + h) * 32), r);
+            tmem_ld_wait();
+            linear_bias(a, x, col0, lane, r, v);
+            if (a.aux) box_put_bf16(box, lane, v);
+            linear_act_drop(x, key, col0, row0 + lane, v);
+            if (a.aux) {
+                box_put_bf16(box + 2048, lane, v);
+            } else if (x.out_f32) {
+#pragma unroll
+                for (int ch = 0; ch < 8; ++ch) {
+                    float4* p = reinterpret_cast<float4*>(box + box_off_f32(lane, ch));
+                    float4 q = make_float4(v[4 * ch], v[4 * ch + 1], v[4 * ch + 2], v[4 * ch + 3]);
+                    if (res) {
+                        const float4 o = *p;
+                        q.x += o.x;
+                        q.y += o.y;
+                        q.z += o.z;
+                        q.w += o.w;
+                    }
+                    *p = q;
+                }
+            } else {
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint4* p = reinterpret_cast<uint4*>(box + box_off_f32(lane, 4 * h + ch));
+                    if (res) {
+                        const uint4 o = *p;
+                        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            v[8 * ch + 2 * k] += bf16_lo(ow[k]);
+                            v[8 * ch + 2 * k + 1] += bf16_hi(ow[k]);
+                        }
+                    }
+                    *p = make_uint4(pack_bf16x2(v[8 * ch], v[8 * ch + 1]),
+                                    pack_bf16x2(v[8 * ch + 2], v[8 * ch + 3]),
+                                    pack_bf16x2(v[8 * ch + 4], v[8 * ch + 5]),
+                                    pack_bf16x2(v[8 * ch + 6], v[8 * ch + 7]));
+                }
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            if (a.aux) {
+                tma_store_3d(tmX, box, n0 + c * 32, row0, 0);
+                tma_store_3d(tmO, box + 2048, n0 + c * 32, row0, 0);
+            } else {
+                tma_store_3d(tmO, box, n0 + c * 32, row0, 0);
+            }
+            bulk_commit_group();
+        }
+        w.slot ^= 1;
+    }
+    if (ce < c_end && n0 + ce * 32 < a.N && row0 < a.M) {
+        if (lane == 0) bulk_wait_group_read<0>();  // the boxes are about to be reused
+        __syncwarp();
+        linear_turned_tile(a, x, key, tbase, row0, n0, lane, w, ce, c_end);
+        fence_proxy_async_smem();
+    }
+}
+
+// Accumulator chains. The tensor cores truncate as they accumulate, so a sum of K products is off
+// by an amount that grows with K (2e-6 of the result at K = 4096, measured), which an f32 output
+// shows. With `chain` the MMA role starts a new accumulator every `chain` k-blocks; the epilogue
+// adds the finished ones up in registers, rounding to nearest, and writes the sum back over the last
+// one, from where the tile's epilogue goes on as for a single chain. COLS: a warp's columns.
+template <int COLS, typename Wait, typename Free>
+__device__ __forceinline__ bool chain_sum(int chains, uint32_t tmem0, int acc_cols, int& acc,
+                                          uint32_t& acc_phase, Wait wait, Free free_acc) {
+    float s[COLS];
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) s[j] = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < chains; ++i) {
+        if (!wait(acc, acc_phase)) return false;
+        tc_fence_after();
+        const uint32_t t = tmem0 + (uint32_t)(acc * acc_cols);
+#pragma unroll
+        for (int q = 0; q < COLS / 16; ++q) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(t + 16 * q, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[16 * q + j] += __uint_as_float(r[j]);
+        }
+        if (i + 1 < chains) {
+            tc_fence_before();
+            free_acc(acc);
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1u;
+        }
+    }
+    const uint32_t t = tmem0 + (uint32_t)(acc * acc_cols);
+#pragma unroll
+    for (int q = 0; q < COLS / 16; ++q) {
+        uint32_t r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(s[16 * q + j]);
+        tmem_st_32x32b_x16(t + 16 * q, r);
+    }
+    tmem_st_wait();
+    return true;
+}
+// k-blocks of a chain of a tile whose k-blocks are [kb0, kb1).
+template <int FAM>
+__device__ __forceinline__ int chain_blocks(const typename ExtOf<FAM>::type& x, int kb0, int kb1) {
+    if constexpr (FAM == kFamLinear) {
+        if (x.chain > 0) return x.chain;
+    }
+    return kb1 - kb0;
 }
 
 // out_f32 planes [split][M][ldo]: plane `split` (+)= the partial product of its k-range. One tile
@@ -815,8 +1023,10 @@ __device__ __forceinline__ void family_tile(const GemmArgs& a,
     } else if constexpr (FAM == kFamLinear) {
         if (a.epi == kEpiPlaneAdd)
             plane_epilogue_tile<NCOLS>(a, tmO, tbase, row0, n0, split, lane, w, c_begin, c_end);
+        else if (a.tma_epi)
+            linear_box_tile(a, x, key, tmO, tmX, tbase, row0, n0, lane, w, c_begin, c_end);
         else
-            linear_epilogue_tile<NCOLS>(a, x, key, tbase, row0, n0, lane, w, c_begin, c_end);
+            linear_turned_tile(a, x, key, tbase, row0, n0, lane, w, c_begin, c_end);
     } else if constexpr (FAM == kFamHeadStats) {
         head_stats_tile<NCOLS>(a, x, tbase, row0, n0, lane, c_begin, c_end);
     } else {
@@ -980,44 +1190,51 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if (!tile_work(args, s_grp, t, num_m, num_n, tiles_mn, kblocks, m_blk, n_blk,
                                split, g, kb0, kb1))
                     continue;
-                if (!mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1u, args.err,
-                                       kDevTimeoutAccFree)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait_bounded(&full[stage], phase, args.err, kDevTimeoutFull)) {
+                // one accumulator for the tile, or one for each chain of it
+                const int ck = chain_blocks<FAM>(ext, kb0, kb1);
+                int kc = kb0;
+                do {
+                    const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
+                    if (!mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1u, args.err,
+                                           kDevTimeoutAccFree)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(sA + stage * Cfg::A_BYTES);
-                    const uint32_t b_addr = smem_u32(sB + stage * Cfg::B_BYTES);
+                    const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+                    for (int kb = kc; kb < kend; ++kb) {
+                        if (!mbar_wait_bounded(&full[stage], phase, args.err, kDevTimeoutFull)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a_addr = smem_u32(sA + stage * Cfg::A_BYTES);
+                        const uint32_t b_addr = smem_u32(sB + stage * Cfg::B_BYTES);
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; ++kk) {
-                        const uint64_t ad =
-                            args.a_mn_major ? make_sw128_desc(a_addr + kk * 2048, 8192, 1024)
-                                            : make_sw128_desc(a_addr + kk * 32, 16, 1024);
-                        const uint64_t bd =
-                            args.b_mn_major ? make_sw128_desc(b_addr + kk * 2048, 8192, 1024)
-                                            : make_sw128_desc(b_addr + kk * 32, 16, 1024);
-                        umma_bf16(d, ad, bd, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+                        for (int kk = 0; kk < BK / 16; ++kk) {
+                            const uint64_t ad =
+                                args.a_mn_major ? make_sw128_desc(a_addr + kk * 2048, 8192, 1024)
+                                                : make_sw128_desc(a_addr + kk * 32, 16, 1024);
+                            const uint64_t bd =
+                                args.b_mn_major ? make_sw128_desc(b_addr + kk * 2048, 8192, 1024)
+                                                : make_sw128_desc(b_addr + kk * 32, 16, 1024);
+                            umma_bf16(d, ad, bd, idesc, (kb > kc || kk > 0) ? 1u : 0u);
+                        }
+                        umma_commit(&empty[stage]);
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
-                    umma_commit(&empty[stage]);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                }
-                if (!ok) break;
-                if (kb1 > kb0)
-                    umma_commit(&acc_full[acc]);
-                else
-                    mbar_arrive(&acc_full[acc]);  // empty group: the epilogue writes zeros
-                acc ^= 1;
-                if (acc == 0) acc_phase ^= 1u;
+                    if (!ok) break;
+                    if (kb1 > kb0)
+                        umma_commit(&acc_full[acc]);
+                    else
+                        mbar_arrive(&acc_full[acc]);  // empty group: the epilogue writes zeros
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1u;
+                    kc = kend;
+                } while (FAM == kFamLinear && kc < kb1);
             }
         }
     } else if (warp >= 4) {
@@ -1035,7 +1252,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const int m0 = m_blk * BM, n0 = n_blk * BN;
             if constexpr (FAM == kFamBase)
                 epilogue_prefetch(args, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
-            if (!mbar_wait_bounded(&acc_full[acc], acc_phase, args.err, kDevTimeoutAcc)) {
+            auto wait_acc = [&](int i, uint32_t ph) {
+                return mbar_wait_bounded(&acc_full[i], ph, args.err, kDevTimeoutAcc);
+            };
+            bool ready;
+            if constexpr (FAM == kFamLinear && BN <= 128) {
+                linear_prefetch(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
+                const int ck = chain_blocks<FAM>(ext, kb0, kb1);
+                const int chains = (kb1 - kb0 + ck - 1) / ck;
+                ready = chains > 1
+                            ? chain_sum<BN>(chains, tmem_base + ((uint32_t)(q * 32) << 16), BN, acc,
+                                            acc_phase, wait_acc,
+                                            [&](int i) { mbar_arrive(&acc_empty[i]); })
+                            : wait_acc(acc, acc_phase);
+            } else {
+                if constexpr (FAM == kFamLinear)
+                    linear_prefetch(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
+                ready = wait_acc(acc, acc_phase);
+            }
+            if (!ready) {
                 epilogue_drain(args, lane, ew);
                 break;
             }
@@ -1419,46 +1654,52 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 int m_blk, n_blk, split, gi, kb0, kb1;
                 tile_work(args, s_grp, t, sh.num_m, sh.num_n, sh.tiles_mn, sh.kblocks, m_blk,
                           n_blk, split, gi, kb0, kb1);
-                if (!mbar_wait_bounded_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
-                                               kDevTimeoutAccFree)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait_bounded_cluster(&full[stage], phase, err, kDevTimeoutFull)) {
+                const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
+                int kc = kb0;
+                do {
+                    const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
+                    if (!mbar_wait_bounded_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
+                                                   kDevTimeoutAccFree)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(sA + stage * Cfg::A_BYTES);
-                    const uint32_t b_addr = smem_u32(sB + stage * Cfg::B_BYTES);
+                    const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+                    for (int kb = kc; kb < kend; ++kb) {
+                        if (!mbar_wait_bounded_cluster(&full[stage], phase, err, kDevTimeoutFull)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a_addr = smem_u32(sA + stage * Cfg::A_BYTES);
+                        const uint32_t b_addr = smem_u32(sB + stage * Cfg::B_BYTES);
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; ++kk) {
-                        const uint64_t ad =
-                            args.a_mn_major ? make_sw128_desc(a_addr + kk * 2048, 8192, 1024)
-                                            : make_sw128_desc(a_addr + kk * 32, 16, 1024);
-                        const uint64_t bd =
-                            args.b_mn_major ? make_sw128_desc(b_addr + kk * 2048, 8192, 1024)
-                                            : make_sw128_desc(b_addr + kk * 32, 16, 1024);
-                        umma_bf16_pair(d, ad, bd, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+                        for (int kk = 0; kk < BK / 16; ++kk) {
+                            const uint64_t ad =
+                                args.a_mn_major ? make_sw128_desc(a_addr + kk * 2048, 8192, 1024)
+                                                : make_sw128_desc(a_addr + kk * 32, 16, 1024);
+                            const uint64_t bd =
+                                args.b_mn_major ? make_sw128_desc(b_addr + kk * 2048, 8192, 1024)
+                                                : make_sw128_desc(b_addr + kk * 32, 16, 1024);
+                            umma_bf16_pair(d, ad, bd, idesc, (kb > kc || kk > 0) ? 1u : 0u);
+                        }
+                        umma_commit_pair(&empty[stage], 0x3);
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
-                    umma_commit_pair(&empty[stage], 0x3);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
+                    if (!ok) break;
+                    if (kb1 > kb0) {
+                        umma_commit_pair(&acc_full[acc], 0x3);
+                    } else {  // empty group: both epilogues write zeros
+                        mbar_arrive(&acc_full[acc]);
+                        mbar_arrive_cluster(acc_full_peer + 8u * (uint32_t)acc);
                     }
-                }
-                if (!ok) break;
-                if (kb1 > kb0) {
-                    umma_commit_pair(&acc_full[acc], 0x3);
-                } else {  // empty group: both epilogues write zeros
-                    mbar_arrive(&acc_full[acc]);
-                    mbar_arrive_cluster(acc_full_peer + 8u * (uint32_t)acc);
-                }
-                acc ^= 1;
-                if (acc == 0) acc_phase ^= 1u;
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1u;
+                    kc = kend;
+                } while (FAM == kFamLinear && kc < kb1);
             }
         }
     } else if (warp >= 4) {
@@ -1492,7 +1733,31 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             if constexpr (FAM == kFamBase)
                 epilogue_prefetch(args, &P.tmX[g], m0 + q * 32, n0, lane, ew, half * (BN / 64),
                                   (half + 1) * (BN / 64));
-            if (!mbar_wait_bounded_cluster(&acc_full[acc], acc_phase, err, kDevTimeoutAcc)) {
+            auto wait_acc = [&](int i, uint32_t ph) {
+                return mbar_wait_bounded_cluster(&acc_full[i], ph, err, kDevTimeoutAcc);
+            };
+            bool ready;
+            if constexpr (FAM == kFamLinear) {
+                linear_prefetch(args, P.ext, &P.tmX[g], m0 + q * 32, n0, lane, ew,
+                                half * (BN / 64), (half + 1) * (BN / 64));
+                const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
+                const int chains = (kb1 - kb0 + ck - 1) / ck;
+                auto free_acc = [&](int i) {
+                    if (leader)
+                        mbar_arrive(&acc_empty[i]);
+                    else
+                        mbar_arrive_cluster(acc_empty_leader + 8u * (uint32_t)i);
+                };
+                ready = chains > 1
+                            ? chain_sum<BN / 2>(chains,
+                                                tmem_base + ((uint32_t)(q * 32) << 16) +
+                                                    (uint32_t)(half * (BN / 2)),
+                                                BN, acc, acc_phase, wait_acc, free_acc)
+                            : wait_acc(acc, acc_phase);
+            } else {
+                ready = wait_acc(acc, acc_phase);
+            }
+            if (!ready) {
                 epilogue_drain(args, lane, ew);
                 break;
             }
@@ -1727,6 +1992,31 @@ bool plan_tma_epilogue(GemmPlan* plan, const GemmArgs& a) {
     return true;
 }
 
+// Tensor maps of the linear epilogue's boxes; false where a stride or address does not allow
+// them, or for the pairs of outputs that one box does not hold (those take linear_turned_tile).
+bool plan_linear_boxes(GemmPlan* plan, const GemmArgs& a, const GemmExt& x) {
+    if ((x.resid || x.out_f32) && a.aux) return false;
+    auto plane = [&](uint64_t ld_bytes) { return (ld_bytes * (uint64_t)a.M + 15) & ~(uint64_t)15; };
+    const uint64_t es = x.out_f32 ? 4 : 2;
+    const uint64_t os = (uint64_t)a.ldo * es;
+    const bool wide = !x.out_f32 && !a.aux;
+    if (make_tmap_box(&plan->tmO, a.out, x.out_f32 != 0, (uint64_t)a.N, (uint64_t)a.M, 1, os,
+                      plane(os), wide))
+        return false;
+    plan->tmX = plan->tmO;
+    if (x.resid) {
+        const uint64_t rs = (uint64_t)x.ldr * es;
+        if (make_tmap_box(&plan->tmX, x.resid, x.out_f32 != 0, (uint64_t)a.N, (uint64_t)a.M, 1, rs,
+                          plane(rs), wide))
+            return false;
+    } else if (a.aux) {
+        const uint64_t xs = (uint64_t)a.ld_aux * 2;
+        if (make_tmap_box(&plan->tmX, a.aux, false, (uint64_t)a.N, (uint64_t)a.M, 1, xs, plane(xs)))
+            return false;
+    }
+    return true;
+}
+
 }  // namespace
 
 bool pdl_enabled() {
@@ -1897,9 +2187,12 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
         if (reinterpret_cast<uintptr_t>(a.out) & 15) return -8;
     }
     const int num_m = (M + BM - 1) / BM;
+    // f32 results of long sums: see chain_sum
+    const bool chained = a.epi == kEpiLinear && ext->out_f32 && kblocks > kChainBlocks;
     const bool pair_ok = a.grp_mode != kGroupRows;  // a pair tile spans 256 rows of one group
     int bn = bn_hint;
     if (bn == kGemmPairTile && !pair_ok) return -44;
+    if (bn == 256 && chained) return -46;
     if (bn != 64 && bn != 128 && bn != 256 && bn != kGemmPairTile) {
         // pick the tile with the smallest estimated makespan; a CTA pair streams a third
         // less operand data per MMA than one CTA with a 128x256 tile, and runs about
@@ -1909,6 +2202,7 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
         for (int i = pair_ok ? 0 : 1; i < 4; ++i) {
             const int c = cands[i];
             if (head && c != kGemmPairTile && c != 128) continue;  // the tiles its kernels have
+            if (chained && c == 256) continue;  // 256 sums a thread do not fit in registers
             double cost;
             if (c == kGemmPairTile) {
                 const long long tiles = (long long)((M + 255) / 256) * ((N + 255) / 256) * a.splits;
@@ -1930,6 +2224,10 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
     a.tma_epi = 0;
     if (ext) {
         if (head && bn != kGemmPairTile && bn != 128) return -46;
+        if (a.epi == kEpiLinear) {
+            a.tma_epi = plan_linear_boxes(plan, a, *ext) ? 1 : 0;
+            plan->ext.chain = chained ? kChainBlocks : 0;
+        }
         if (a.epi == kEpiHeadGrad || a.epi == kEpiPlaneAdd) {
             a.tma_epi = plan_tma_epilogue(plan, a) ? 1 : 0;
             if (!a.tma_epi) return -8;

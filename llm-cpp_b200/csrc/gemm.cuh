@@ -43,6 +43,7 @@ struct GemmExt {
     uint64_t site;        // added to the offset
     uint32_t drop_thr;
     float drop_scale;
+    int chain;            // set by the planner: k-blocks of one accumulator chain, 0: all of them
     // kEpiHeadStats, kEpiHeadGrad: row m's target (left out unless in [0, V)), V = all columns
     // of the vocabulary, this product's column 0 being column v0 of it
     const int32_t* targets;

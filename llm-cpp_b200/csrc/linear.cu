@@ -34,11 +34,11 @@ __device__ __forceinline__ float act_grad(int act, float z) {
             // gelu(z) = z h, h = sigmoid(2u): h + z h (1 - h) 2u'
             const float z2 = z * z;
             const float t = 1.5957691216f * z * fmaf(0.044715f, z2, 1.0f);
-            const float h = __frcp_rn(1.0f + ex2_approx(-t * 1.4426950408889634f));
+            const float h = rcp_approx(1.0f + ex2_approx(-t * 1.4426950408889634f));
             return h + z * h * (1.0f - h) * 1.5957691216f * fmaf(0.134145f, z2, 1.0f);
         }
         case kActSilu: {
-            const float h = __frcp_rn(1.0f + ex2_approx(-z * 1.4426950408889634f));
+            const float h = rcp_approx(1.0f + ex2_approx(-z * 1.4426950408889634f));
             return h * (1.0f + z * (1.0f - h));
         }
         default:
@@ -164,11 +164,12 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
     g.err = err;
     GemmPlan plan;
     int rc;
-    if (aligned16(out) && (ldo % (out_f32 ? 4 : 8)) == 0) {
+    const int per16 = out_f32 ? 4 : 8;
+    if (aligned16(out) && (ldo % per16) == 0 && (N % per16) == 0) {
         g.epi = out_f32 ? kEpiStoreF32 : kEpiStoreBF16;
         g.accumulate = accumulate;
         rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, M, N, K, g, 0, num_sms);
-    } else {  // rows that no 16-byte store reaches
+    } else {  // rows that no 16-byte store reaches, or that end inside one
         GemmExt x{};
         g.epi = kEpiLinear;
         x.out_f32 = out_f32;

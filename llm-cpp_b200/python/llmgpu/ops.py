@@ -244,14 +244,14 @@ _err_words = {}
 
 
 def _err_word(device):
-    """The device's error word of these operators (made outside a capture, once per device)."""
+    """Address of the device's error word of these operators (made outside a capture, once)."""
     w = _err_words.get(device.index)
     if w is None:
         if torch.cuda.is_current_stream_capturing():
-            return None  # the first call on this device is being captured: waits stay bounded
+            return 0  # the first call on this device is being captured: waits stay bounded
         w = _err_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()  # any later stream may use it
-    return w
+    return w.data_ptr()
 
 
 def check_device(device="cuda"):
@@ -268,45 +268,88 @@ def check_device(device="cuda"):
             raise KernelError(f"device error code {code}")
 
 
-def _want(ok, what):
-    if not ok:
-        raise KernelError(what)
+def _call(name, device, *args):
+    """The C entry point on the current stream of `device`."""
+    fn = getattr(load(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        raise KernelError(f"{name} failed with status {rc}")
+
+
+def _device_of(*named):
+    """The device of 2-D CUDA tensors given as (tensor, name) pairs."""
+    for t, name in named:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
+            raise KernelError(f"{name}: a 2-D CUDA tensor is needed")
+    return named[0][0].device
 
 
 def _matrix(t, name, dtypes, rows, cols, device, operand=False):
     """Checks a 2-D matrix argument and returns its row stride in elements."""
-    _want(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a CUDA tensor is needed")
-    _want(t.device == device, f"{name}: on {t.device}, not on {device}")
-    _want(t.dtype in dtypes, f"{name}: {t.dtype} is not one of {[str(d) for d in dtypes]}")
-    _want(tuple(t.shape) == (rows, cols), f"{name}: shape {tuple(t.shape)}, not {(rows, cols)}")
-    _want(cols <= 1 or t.stride(1) == 1, f"{name}: neighbouring columns are needed")
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise KernelError(f"{name}: a tensor on {device} is needed, as the first argument")
+    if t.dtype not in dtypes:
+        raise KernelError(f"{name}: {t.dtype} is not one of {[str(d) for d in dtypes]}")
+    if t.shape != (rows, cols):
+        raise KernelError(f"{name}: shape {tuple(t.shape)}, not {(rows, cols)}")
+    sr, sc = t.stride()
+    if sc != 1 and cols > 1:
+        raise KernelError(f"{name}: neighbouring columns are needed")
     if rows <= 1:
-        ld = (cols + 7) // 8 * 8
-    else:
-        ld = t.stride(0)
-        _want(ld >= cols, f"{name}: rows overlap (stride {ld} of {cols} columns)")
-    if operand and t.numel():
-        _want(t.data_ptr() % 16 == 0 and ld % 8 == 0,
-              f"{name}: rows have to start on 16 bytes (address {t.data_ptr():#x}, stride {ld})")
-    return ld
+        sr = (cols + 7) // 8 * 8
+    elif sr < cols:
+        raise KernelError(f"{name}: rows overlap (stride {sr} of {cols} columns)")
+    if operand and (t.data_ptr() % 16 or sr % 8) and rows and cols:
+        raise KernelError(f"{name}: rows have to start on 16 bytes (address {t.data_ptr():#x}, "
+                          f"stride {sr})")
+    return sr
 
 
 def _vector(t, name, dtype, n, device):
-    _want(isinstance(t, torch.Tensor) and t.is_cuda and t.device == device and t.dtype == dtype
-          and tuple(t.shape) == (n,) and t.is_contiguous(),
-          f"{name}: a contiguous {dtype} tensor of {n} on {device} is needed")
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or \
+            t.shape != (n,) or not t.is_contiguous():
+        raise KernelError(f"{name}: a contiguous {dtype} tensor of {n} on {device} is needed")
 
 
 def _rows(rows, cols, dtype, device):
+    """A matrix whose rows start on 16 bytes."""
+    if cols % 8 == 0:
+        return torch.empty(rows, cols, dtype=dtype, device=device)
     return torch.empty(rows, (cols + 7) // 8 * 8, dtype=dtype, device=device)[:, :cols]
 
 
 def _drop(p, rng, device):
-    _want(0.0 <= p <= 1.0, f"p = {p} is not in [0, 1]")
-    if p > 0.0:
-        _want(rng is not None, "dropout needs rng, an int64 tensor (seed, offset) on the device")
+    if not 0.0 <= p <= 1.0:
+        raise KernelError(f"p = {p} is not in [0, 1]")
     if rng is not None:
         _vector(rng, "rng", torch.int64, 2, device)
+        return rng.data_ptr()
+    if p > 0.0:
+        raise KernelError("dropout needs rng, an int64 tensor (seed, offset) on the device")
+    return 0
+
+
+def _act(act):
+    if act not in ACT:
+        raise KernelError(f"act: {act!r} is not one of {sorted(ACT)}")
+    return ACT[act]
+
+
+def _grad_w(dw, w_mn, rows, cols, device, accumulate, name="dw"):
+    """(dw, row stride): the given weight gradient, or a new one in the weight's layout."""
+    shape = (cols, rows) if w_mn else (rows, cols)
+    if dw is None:
+        if accumulate:
+            raise KernelError(f"accumulate: {name} has to be given")
+        dw = _rows(*shape, torch.bfloat16, device)
+    ld = _matrix(dw, name, _FLOATS, *shape, device)
+    if accumulate and dw.dtype != torch.float32:
+        raise KernelError(f"accumulate: {name} has to be f32")
+    return dw, ld
 
 
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -318,24 +361,23 @@ def dropout_fwd(x, p, rng, site=0, resid=None, out=None, out_dtype=None):
     given). `rng`: int64 device tensor (seed, offset); `site` tells the dropouts of a step apart.
     The mask depends on (seed, offset + site, row, column) alone and p counts in steps of
     1 / 65536; see llmgpu_op_dropout. `out` may be x or resid."""
-    _want(isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2, "x: a 2-D CUDA tensor is needed")
+    dev = _device_of((x, "x"))
     rows, cols = x.shape
-    dev = x.device
     ldx = _matrix(x, "x", _FLOATS, rows, cols, dev)
-    _drop(p, rng, dev)
-    _want(rng is not None, "dropout needs rng, an int64 tensor (seed, offset) on the device")
+    prng = _drop(p, rng, dev)
+    if not prng:
+        raise KernelError("dropout needs rng, an int64 tensor (seed, offset) on the device")
     if out is None:
         out = _rows(rows, cols, out_dtype or x.dtype, dev)
-    _want(out_dtype is None or out.dtype == out_dtype, f"out: {out.dtype} is not {out_dtype}")
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise KernelError(f"out: {out.dtype} is not {out_dtype}")
     ldo = _matrix(out, "out", _FLOATS, rows, cols, dev)
-    ldr = 0
+    pr = ldr = 0
     if resid is not None:
         ldr = _matrix(resid, "resid", (out.dtype,), rows, cols, dev)
-    with torch.cuda.device(dev):
-        _check(load().llmgpu_op_dropout(
-            _ptr(x), int(x.dtype == torch.float32), ldx, _ptr(resid), ldr, _ptr(out),
-            int(out.dtype == torch.float32), ldo, rows, cols, p, _ptr(rng), site, _stream()),
-            "llmgpu_op_dropout")
+        pr = resid.data_ptr()
+    _call("llmgpu_op_dropout", dev, x.data_ptr(), x.dtype == torch.float32, ldx, pr, ldr,
+          out.data_ptr(), out.dtype == torch.float32, ldo, rows, cols, p, prng, site)
     return out
 
 
@@ -345,15 +387,14 @@ def dropout_bwd(dy, p, rng, site=0, out=None, out_dtype=None):
 
 
 def _linear_shapes(x, w, w_mn):
-    for t, n in ((x, "x"), (w, "w")):
-        _want(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2,
-              f"{n}: a 2-D CUDA tensor is needed")
+    dev = _device_of((x, "x"), (w, "w"))
     M, K = x.shape
     N = w.shape[1] if w_mn else w.shape[0]
-    _want(N > 0 and K > 0, f"an empty product: x {tuple(x.shape)}, w {tuple(w.shape)}")
-    ldx = _matrix(x, "x", _BF16, M, K, x.device, operand=True)
-    ldw = _matrix(w, "w", _BF16, K if w_mn else N, N if w_mn else K, x.device, operand=True)
-    return M, K, N, ldx, ldw
+    if N <= 0 or K <= 0:
+        raise KernelError(f"an empty product: x {tuple(x.shape)}, w {tuple(w.shape)}")
+    ldx = _matrix(x, "x", _BF16, M, K, dev, operand=True)
+    ldw = _matrix(w, "w", _BF16, K if w_mn else N, N if w_mn else K, dev, operand=True)
+    return dev, M, K, N, ldx, ldw
 
 
 def linear_fwd(x, w, bias=None, act="none", p=0.0, rng=None, site=0, resid=None, w_mn=False,
@@ -362,27 +403,26 @@ def linear_fwd(x, w, bias=None, act="none", p=0.0, rng=None, site=0, resid=None,
     `w_mn`) are bf16 with rows on 16 bytes, bias [N] f32, act one of ACT, (p, rng, site) as in
     dropout_fwd, resid of the result's type. Returns (y, pre): pre = x w^T + bias in bf16 when
     `save_pre` (linear_bwd needs it unless act is "none"), else None."""
-    M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
-    dev = x.device
-    _want(act in ACT, f"act: {act!r} is not one of {sorted(ACT)}")
-    _drop(p, rng, dev)
+    dev, M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
+    a = _act(act)
+    prng = _drop(p, rng, dev)
+    pb = pr = pp = ldr = ldp = 0
     if bias is not None:
         _vector(bias, "bias", torch.float32, N, dev)
+        pb = bias.data_ptr()
     if out is None:
         out = _rows(M, N, out_dtype, dev)
     ldo = _matrix(out, "out", _FLOATS, M, N, dev)
-    ldr = ldp = 0
     if resid is not None:
         ldr = _matrix(resid, "resid", (out.dtype,), M, N, dev)
+        pr = resid.data_ptr()
     pre = None
     if save_pre:
         pre = _rows(M, N, torch.bfloat16, dev)
-        ldp = _matrix(pre, "pre", _BF16, M, N, dev)
-    with torch.cuda.device(dev):
-        _check(load().llmgpu_op_linear_fwd(
-            _ptr(x), ldx, _ptr(w), ldw, int(w_mn), _ptr(bias), ACT[act], p, _ptr(rng), site,
-            _ptr(resid), ldr, _ptr(pre), ldp, _ptr(out), int(out.dtype == torch.float32), ldo, M, N,
-            K, _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_fwd")
+        ldp, pp = (N + 7) // 8 * 8, pre.data_ptr()
+    _call("llmgpu_op_linear_fwd", dev, x.data_ptr(), ldx, w.data_ptr(), ldw, w_mn, pb, a, p, prng,
+          site, pr, ldr, pp, ldp, out.data_ptr(), out.dtype == torch.float32, ldo, M, N, K,
+          _err_word(dev))
     return out, pre
 
 
@@ -393,42 +433,47 @@ def linear_bwd(dy, x, w, pre=None, act="none", p=0.0, rng=None, site=0, w_mn=Fal
     result, with the forward's x, w, pre, act and (p, rng, site); the residual's gradient is dy. dw
     has w's layout, bf16 unless given; `accumulate` adds into the given dw (f32) and dbias. What
     is not needed is None."""
-    M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
-    dev = x.device
-    _want(act in ACT, f"act: {act!r} is not one of {sorted(ACT)}")
-    _drop(p, rng, dev)
+    dev, M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
+    a = _act(act)
+    prng = _drop(p, rng, dev)
     lddy = _matrix(dy, "dy", _FLOATS, M, N, dev)
-    ldp = 0
+    pp = ldp = px = lddx = pw = lddw = pb = 0
     if act != "none":
-        _want(pre is not None, f"act {act!r}: the backward needs pre")
-        ldp = _matrix(pre, "pre", _BF16, M, N, dev)
-    dx = _rows(M, K, dx_dtype, dev) if need_dx else None
-    lddx = _matrix(dx, "dx", _FLOATS, M, K, dev) if need_dx else 0
-    wr, wc = (K, N) if w_mn else (N, K)
-    if not need_dw:
+        if pre is None:
+            raise KernelError(f"act {act!r}: the backward needs pre")
+        ldp, pp = _matrix(pre, "pre", _BF16, M, N, dev), pre.data_ptr()
+    dx = None
+    if need_dx:
+        dx = _rows(M, K, dx_dtype, dev)
+        lddx, px = _matrix(dx, "dx", _FLOATS, M, K, dev), dx.data_ptr()
+    if need_dw:
+        dw, lddw = _grad_w(dw, w_mn, N, K, dev, accumulate)
+        pw = dw.data_ptr()
+    else:
         dw = None
-    elif dw is None:
-        _want(not accumulate, "accumulate: dw has to be given")
-        dw = _rows(wr, wc, torch.bfloat16, dev)
-    lddw = _matrix(dw, "dw", _FLOATS, wr, wc, dev) if need_dw else 0
-    _want(not (accumulate and need_dw) or dw.dtype == torch.float32, "accumulate: dw has to be f32")
-    if not need_dbias:
-        dbias = None
-    elif dbias is None:
-        _want(not accumulate, "accumulate: dbias has to be given")
-        dbias = torch.empty(N, dtype=torch.float32, device=dev)
     if need_dbias:
+        if dbias is None:
+            if accumulate:
+                raise KernelError("accumulate: dbias has to be given")
+            dbias = torch.empty(N, dtype=torch.float32, device=dev)
         _vector(dbias, "dbias", torch.float32, N, dev)
-    lib = load()
-    work = torch.empty(int(lib.llmgpu_op_linear_bwd_work(M, N, K)), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _check(lib.llmgpu_op_linear_bwd(
-            _ptr(dy), int(dy.dtype == torch.float32), lddy, _ptr(x), ldx, _ptr(w), ldw, int(w_mn),
-            _ptr(pre), ldp, ACT[act], p, _ptr(rng), site, _ptr(dx),
-            int(dx_dtype == torch.float32), lddx, _ptr(dw),
-            int(need_dw and dw.dtype == torch.float32), lddw, _ptr(dbias), int(accumulate), M, N,
-            K, _ptr(work), _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_bwd")
+        pb = dbias.data_ptr()
+    else:
+        dbias = None
+    work = torch.empty(load().llmgpu_op_linear_bwd_work(M, N, K), dtype=torch.uint8, device=dev)
+    _call("llmgpu_op_linear_bwd", dev, dy.data_ptr(), dy.dtype == torch.float32, lddy, x.data_ptr(),
+          ldx, w.data_ptr(), ldw, w_mn, pp, ldp, a, p, prng, site, px, dx_dtype == torch.float32,
+          lddx, pw, need_dw and dw.dtype == torch.float32, lddw, pb, accumulate, M, N, K,
+          work.data_ptr(), _err_word(dev))
     return dx, dw, dbias
+
+
+def _head_args(x, w, targets, smoothing, w_mn):
+    dev, rows, C, V, ldx, ldw = _linear_shapes(x, w, w_mn)
+    if not 0.0 <= smoothing < 1.0:
+        raise KernelError(f"smoothing = {smoothing} is not in [0, 1)")
+    _vector(targets, "targets", torch.int32, rows, dev)
+    return dev, rows, C, V, ldx, ldw
 
 
 def linear_cross_entropy_fwd(x, w, targets, smoothing=0.0, w_mn=False):
@@ -436,18 +481,13 @@ def linear_cross_entropy_fwd(x, w, targets, smoothing=0.0, w_mn=False):
     f32 [rows]. x [rows, C] and w [V, C] (or [C, V] with `w_mn`) are bf16 with rows on 16 bytes,
     targets int32 [rows]; a target outside [0, V) leaves its row out (loss 0). `smoothing` s:
     targets of 1 - s and s / (V - 1) elsewhere, in the loss as in the gradient."""
-    rows, C, V, ldx, ldw = _linear_shapes(x, w, w_mn)
-    dev = x.device
-    _want(0.0 <= smoothing < 1.0, f"smoothing = {smoothing} is not in [0, 1)")
-    _vector(targets, "targets", torch.int32, rows, dev)
+    dev, rows, C, V, ldx, ldw = _head_args(x, w, targets, smoothing, w_mn)
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     lse = torch.empty(rows, dtype=torch.float32, device=dev)
-    lib = load()
-    work = torch.empty(int(lib.llmgpu_op_linear_ce_fwd_work(rows, V)), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _check(lib.llmgpu_op_linear_ce_fwd(
-            _ptr(x), ldx, _ptr(w), ldw, int(w_mn), _ptr(targets), rows, C, V, smoothing, _ptr(loss),
-            _ptr(lse), _ptr(work), _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_ce_fwd")
+    work = torch.empty(load().llmgpu_op_linear_ce_fwd_work(rows, V), dtype=torch.uint8, device=dev)
+    _call("llmgpu_op_linear_ce_fwd", dev, x.data_ptr(), ldx, w.data_ptr(), ldw, w_mn,
+          targets.data_ptr(), rows, C, V, smoothing, loss.data_ptr(), lse.data_ptr(),
+          work.data_ptr(), _err_word(dev))
     return loss, lse
 
 
@@ -458,31 +498,27 @@ def linear_cross_entropy_bwd(x, w, targets, lse, dloss=None, scale=1.0, smoothin
     the forward's arguments and its lse. The logits are formed again in pieces of `piece` columns of
     the vocabulary (a multiple of 256; 0: chosen by the library), which bounds the workspace. dw
     has w's layout, bf16 unless given; `accumulate` adds into the given f32 dw."""
-    rows, C, V, ldx, ldw = _linear_shapes(x, w, w_mn)
-    dev = x.device
-    _want(0.0 <= smoothing < 1.0, f"smoothing = {smoothing} is not in [0, 1)")
-    _want(piece >= 0 and piece % 256 == 0, f"piece = {piece} is not a multiple of 256")
-    _vector(targets, "targets", torch.int32, rows, dev)
+    dev, rows, C, V, ldx, ldw = _head_args(x, w, targets, smoothing, w_mn)
+    if piece < 0 or piece % 256:
+        raise KernelError(f"piece = {piece} is not a multiple of 256")
     _vector(lse, "lse", torch.float32, rows, dev)
+    pd = px = lddx = pw = lddw = 0
     if dloss is not None:
         _vector(dloss, "dloss", torch.float32, rows, dev)
-    dx = _rows(rows, C, dx_dtype, dev) if need_dx else None
-    lddx = _matrix(dx, "dx", _FLOATS, rows, C, dev) if need_dx else 0
-    wr, wc = (C, V) if w_mn else (V, C)
-    if not need_dw:
+        pd = dloss.data_ptr()
+    dx = None
+    if need_dx:
+        dx = _rows(rows, C, dx_dtype, dev)
+        lddx, px = _matrix(dx, "dx", _FLOATS, rows, C, dev), dx.data_ptr()
+    if need_dw:
+        dw, lddw = _grad_w(dw, w_mn, V, C, dev, accumulate)
+        pw = dw.data_ptr()
+    else:
         dw = None
-    elif dw is None:
-        _want(not accumulate, "accumulate: dw has to be given")
-        dw = _rows(wr, wc, torch.bfloat16, dev)
-    lddw = _matrix(dw, "dw", _FLOATS, wr, wc, dev) if need_dw else 0
-    _want(not (accumulate and need_dw) or dw.dtype == torch.float32, "accumulate: dw has to be f32")
-    lib = load()
-    work = torch.empty(int(lib.llmgpu_op_linear_ce_bwd_work(rows, C, V, piece)), dtype=torch.uint8,
+    work = torch.empty(load().llmgpu_op_linear_ce_bwd_work(rows, C, V, piece), dtype=torch.uint8,
                        device=dev)
-    with torch.cuda.device(dev):
-        _check(lib.llmgpu_op_linear_ce_bwd(
-            _ptr(x), ldx, _ptr(w), ldw, int(w_mn), _ptr(targets), _ptr(lse), _ptr(dloss), scale,
-            rows, C, V, smoothing, _ptr(dx), int(dx_dtype == torch.float32), lddx, _ptr(dw),
-            int(need_dw and dw.dtype == torch.float32), lddw, int(accumulate), piece, _ptr(work),
-            _ptr(_err_word(dev)), _stream()), "llmgpu_op_linear_ce_bwd")
+    _call("llmgpu_op_linear_ce_bwd", dev, x.data_ptr(), ldx, w.data_ptr(), ldw, w_mn,
+          targets.data_ptr(), lse.data_ptr(), pd, scale, rows, C, V, smoothing, px,
+          dx_dtype == torch.float32, lddx, pw, need_dw and dw.dtype == torch.float32, lddw,
+          accumulate, piece, work.data_ptr(), _err_word(dev))
     return dx, dw

@@ -253,6 +253,10 @@ def test_linear_bwd(cuda, M, K, N, act, p, dyt, w_mn):
         _norm_close(gw, dw, NORM16, "dw")
     # f32 gradients, added to what is there; rows of any stride
     wr, wc = (K, N) if w_mn else (N, K)
+    ow, check = _guard(wr, wc, BF, cuda, -(-wc // 8) * 8 + 8)
+    ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn, dw=ow)
+    assert torch.equal(ow, gw)
+    check()
     aw, check = _guard(wr, wc, F32, cuda, wc + 3, 1)
     aw.fill_(0.5)
     ab = torch.full((N,), 2.0, device=cuda)
@@ -362,6 +366,10 @@ def test_loss_head(cuda, rows, C, V, piece, smoothing, w_mn, ignored):
         _norm_close(gx, dx, NORM16, "dx")
         _norm_close(gw, dw, NORM16, "dw")
     wr, wc = (C, V) if w_mn else (V, C)
+    ow, check = _guard(wr, wc, BF, cuda, -(-wc // 8) * 8 + 8)
+    ops.linear_cross_entropy_bwd(x, w, t, gs, d, 0.5, smoothing, w_mn, dw=ow, piece=piece)
+    assert torch.equal(ow, gw)
+    check()
     aw, check = _guard(wr, wc, F32, cuda, wc + 3, 1)
     aw.fill_(0.25)
     gx32, _ = ops.linear_cross_entropy_bwd(x, w, t, gs, d, 0.5, smoothing, w_mn, dx_dtype=F32, dw=aw,
