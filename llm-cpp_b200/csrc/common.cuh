@@ -255,6 +255,17 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 ra, rb, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\t"
+        "mov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\t"
+        "mov.b64 {%0, %1}, rd;}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 
 // 3-D tiled TMA load into this CTA (c2 the outermost coordinate).
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar,
@@ -441,6 +452,23 @@ __device__ __forceinline__ uint64_t make_sw128_desc(uint32_t smem_addr, uint32_t
     d |= (uint64_t)2 << 61;  // SWIZZLE_128B
     return d;
 }
+// The descriptors of one operand's ring of stages, for the issuing thread: that of k-step kk of
+// stage s is one addition to the low word (addresses count in 16 bytes and stay below 2^14, so
+// nothing carries into the next field). Building them afresh cost that thread, which shares its
+// scheduler with busy epilogue warps, more cycles per k-block than the MMAs take.
+struct OperandDesc {
+    uint32_t lo, hi, step;
+    __device__ __forceinline__ OperandDesc(uint32_t smem_base, int mn_major) {
+        const uint64_t d = mn_major ? make_sw128_desc(smem_base, 8192, 1024)
+                                    : make_sw128_desc(smem_base, 16, 1024);
+        lo = (uint32_t)d;
+        hi = (uint32_t)(d >> 32);
+        step = mn_major ? 2048u >> 4 : 32u >> 4;  // 16 of K
+    }
+    __device__ __forceinline__ uint64_t at(uint32_t stage_off, int kk) const {
+        return ((uint64_t)hi << 32) | (lo + stage_off + (uint32_t)kk * step);
+    }
+};
 // Instruction descriptor for kind::f16 with bf16 A/B and fp32 D.
 __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int a_mn_major,
                                                       int b_mn_major) {

@@ -131,11 +131,10 @@ __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(
 #pragma unroll
         for (int u = 0; u < kDropUnroll; ++u) {
             if (ur[u] >= rows) break;
-            const uint32_t m = drop_keep8(key, uc[u], ur[u], thr);
+            if (thr) drop_apply8(key, uc[u], ur[u], thr, scale, v[u]);
+            if (RES) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[u][j] = ((m >> j) & 1u) ? v[u][j] * scale : 0.0f;
-                if (RES) v[u][j] += r[u][j];
+                for (int j = 0; j < 8; ++j) v[u][j] += r[u][j];
             }
             const int c = (int)(uc[u] * 8);
             if (c + 8 <= cols) {

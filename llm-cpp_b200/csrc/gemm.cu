@@ -551,47 +551,63 @@ struct ExtOf<kFamBase> {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// 1 / (1 + exp(-t)) from the special-function unit's 2^x and reciprocal: a few units in the last
-// place, which an f32 output keeps. t far below 0: exp overflows to inf and the result is 0.
-__device__ __forceinline__ float sigmoid_f32(float t) {
-    return rcp_approx(1.0f + ex2_approx(-t * kLog2e));
+// Activations of a pair of pre-activations, z / (1 + exp(-t)) with t = z (silu) or 2 k (z + 0.044715
+// z^3) (gelu: 0.5 z (1 + tanh u) = z sigmoid(2u)), from the special-function unit's 2^x and
+// reciprocal, a few units in the last place, which an f32 output keeps. Far left, 2^x overflows
+// to inf and the result is -0. Packed pairs: 7 issue slots for two gelus besides the 4
+// special-function ones, since the epilogue's warps, two per scheduler, are what bounds a
+// product of K near 1024.
+__device__ __forceinline__ float2 sigmoid_of_log2(float2 t) {  // 1 / (1 + 2^t)
+    const float2 d = fadd2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.f, 1.f));
+    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
 }
-__device__ __forceinline__ float act_apply(int act, float z) {
-    switch (act) {
-        case kActRelu:
-            return z > 0.0f ? z : (z == z ? 0.0f : z);
-        case kActGelu: {
-            // 0.5 z (1 + tanh u) = z sigmoid(2u)
-            const float u2 = 1.5957691216f * z * fmaf(0.044715f * z, z, 1.0f);
-            return z * sigmoid_f32(u2);
-        }
-        case kActSilu:
-            return z * sigmoid_f32(z);
-        default:
-            return z;
+template <int ACT>
+__device__ __forceinline__ float2 act_pair(float2 z) {
+    if constexpr (ACT == kActRelu) {  // NaN stays NaN
+        return make_float2(z.x <= 0.0f ? 0.0f : z.x, z.y <= 0.0f ? 0.0f : z.y);
+    } else if constexpr (ACT == kActGelu) {
+        constexpr float c = -1.5957691216f * kLog2e;
+        const float2 w = ffma2(fmul2(z, z), make_float2(c * 0.044715f, c * 0.044715f),
+                               make_float2(c, c));
+        return fmul2(z, sigmoid_of_log2(fmul2(w, z)));
+    } else if constexpr (ACT == kActSilu) {
+        return fmul2(z, sigmoid_of_log2(fmul2(z, make_float2(-kLog2e, -kLog2e))));
+    } else {
+        return z;
+    }
+}
+template <int ACT>
+__device__ __forceinline__ void act_all(float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const float2 y = act_pair<ACT>(make_float2(v[j], v[j + 1]));
+        v[j] = y.x;
+        v[j + 1] = y.y;
     }
 }
 
 // One lane's 32 accumulator columns [col0, col0 + 32) plus the bias.
 __device__ __forceinline__ void linear_bias(const GemmArgs& a, const GemmExt& x, int col0, int lane,
                                             const uint32_t (&r)[32], float (&v)[32]) {
-    if (!x.bias) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-    } else if (col0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(x.bias) & 15) == 0) {
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+    if (!x.bias) return;
+    if (col0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(x.bias) & 15) == 0) {
         const float4* b4 = reinterpret_cast<const float4*>(x.bias + col0);  // same for all lanes
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             const float4 b = b4[q];
-            v[4 * q] = __uint_as_float(r[4 * q]) + b.x;
-            v[4 * q + 1] = __uint_as_float(r[4 * q + 1]) + b.y;
-            v[4 * q + 2] = __uint_as_float(r[4 * q + 2]) + b.z;
-            v[4 * q + 3] = __uint_as_float(r[4 * q + 3]) + b.w;
+            const float2 lo = fadd2(make_float2(v[4 * q], v[4 * q + 1]), make_float2(b.x, b.y));
+            const float2 hi = fadd2(make_float2(v[4 * q + 2], v[4 * q + 3]), make_float2(b.z, b.w));
+            v[4 * q] = lo.x;
+            v[4 * q + 1] = lo.y;
+            v[4 * q + 2] = hi.x;
+            v[4 * q + 3] = hi.y;
         }
     } else {
         const float b = col0 + lane < a.N ? x.bias[col0 + lane] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + __shfl_sync(0xffffffffu, b, j);
+        for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
     }
 }
 // act, then dropout, of those columns.
@@ -600,29 +616,22 @@ __device__ __forceinline__ void linear_act_drop(const GemmExt& x, const DropKey&
     // the switch stands outside the loops: one branch for 32 columns
     switch (x.act) {
         case kActRelu:
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_apply(kActRelu, v[j]);
+            act_all<kActRelu>(v);
             break;
         case kActGelu:
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_apply(kActGelu, v[j]);
+            act_all<kActGelu>(v);
             break;
         case kActSilu:
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_apply(kActSilu, v[j]);
+            act_all<kActSilu>(v);
             break;
         default:
             break;
     }
     if (x.rng) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint32_t m =
-                drop_keep8(key, (uint32_t)(col0 >> 3) + q, (uint32_t)row, x.drop_thr);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                v[8 * q + j] = ((m >> j) & 1u) ? v[8 * q + j] * x.drop_scale : 0.0f;
-        }
+        for (int q = 0; q < 4; ++q)
+            drop_apply8(key, (uint32_t)(col0 >> 3) + q, (uint32_t)row, x.drop_thr, x.drop_scale,
+                        v + 8 * q);
     }
 }
 
@@ -850,6 +859,24 @@ __device__ __forceinline__ bool chain_sum(int chains, uint32_t tmem0, int acc_co
     tmem_st_wait();
     return true;
 }
+// k-blocks [kb0, kb1) of tile t, for the MMA role, which needs nothing else of it: ungrouped products
+// of one split skip the divisions of tile_work, which stood between two tiles' MMAs.
+template <int FAM>
+__device__ __forceinline__ bool tile_kblocks(const GemmArgs& a, const int* s_grp, int t, int num_m,
+                                             int num_n, int tiles_mn, int kblocks, int& kb0,
+                                             int& kb1) {
+    if constexpr (FAM != kFamBase) {
+        const int split = a.splits > 1 ? t / tiles_mn : 0;
+        kb0 = a.splits > 1 ? (int)((long long)split * kblocks / a.splits) : 0;
+        kb1 = a.splits > 1 ? (int)((long long)(split + 1) * kblocks / a.splits) : kblocks;
+        return true;
+    } else {
+        int m_blk, n_blk, split, g;
+        return tile_work(a, s_grp, t, num_m, num_n, tiles_mn, kblocks, m_blk, n_blk, split, g, kb0,
+                         kb1);
+    }
+}
+
 // k-blocks of a chain of a tile whose k-blocks are [kb0, kb1).
 template <int FAM>
 __device__ __forceinline__ int chain_blocks(const typename ExtOf<FAM>::type& x, int kb0, int kb1) {
@@ -1180,15 +1207,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (lane == 0) {
             // ---------------- MMA issuer
             const uint32_t idesc = make_idesc_bf16(BM, BN, args.a_mn_major, args.b_mn_major);
+            const OperandDesc da(smem_u32(sA), args.a_mn_major), db(smem_u32(sB), args.b_mn_major);
             int stage = 0;
             uint32_t phase = 0;
             int acc = 0;
             uint32_t acc_phase = 0;
             bool ok = true;
             for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-                int m_blk, n_blk, split, g, kb0, kb1;
-                if (!tile_work(args, s_grp, t, num_m, num_n, tiles_mn, kblocks, m_blk, n_blk,
-                               split, g, kb0, kb1))
+                int kb0, kb1;
+                if (!tile_kblocks<FAM>(args, s_grp, t, num_m, num_n, tiles_mn, kblocks, kb0, kb1))
                     continue;
                 // one accumulator for the tile, or one for each chain of it
                 const int ck = chain_blocks<FAM>(ext, kb0, kb1);
@@ -1208,18 +1235,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t a_addr = smem_u32(sA + stage * Cfg::A_BYTES);
-                        const uint32_t b_addr = smem_u32(sB + stage * Cfg::B_BYTES);
+                        const uint32_t ao = (uint32_t)stage * (Cfg::A_BYTES >> 4);
+                        const uint32_t bo = (uint32_t)stage * (Cfg::B_BYTES >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < BK / 16; ++kk) {
-                            const uint64_t ad =
-                                args.a_mn_major ? make_sw128_desc(a_addr + kk * 2048, 8192, 1024)
-                                                : make_sw128_desc(a_addr + kk * 32, 16, 1024);
-                            const uint64_t bd =
-                                args.b_mn_major ? make_sw128_desc(b_addr + kk * 2048, 8192, 1024)
-                                                : make_sw128_desc(b_addr + kk * 32, 16, 1024);
-                            umma_bf16(d, ad, bd, idesc, (kb > kc || kk > 0) ? 1u : 0u);
-                        }
+                        for (int kk = 0; kk < BK / 16; ++kk)
+                            umma_bf16(d, da.at(ao, kk), db.at(bo, kk), idesc,
+                                      (kb > kc || kk > 0) ? 1u : 0u);
                         umma_commit(&empty[stage]);
                         if (++stage == STAGES) {
                             stage = 0;
@@ -1302,19 +1323,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // commits arrive on the stage / accumulator barriers of both CTAs; both CTAs' loads count
 // their bytes on the leader's stage barrier; the follower's epilogue arrives remotely on
 // the leader's accumulator-free barrier.
-struct PairCfg {
+template <int FAM>
+struct PairCfgOf {
     static constexpr int BMP = 256;
     static constexpr int BN = 256;
     static constexpr int BNH = 128;
     static constexpr int A_BYTES = BM * BK * 2;
     static constexpr int B_BYTES = BNH * BK * 2;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 5;
+    // the softmax statistics write no boxes: their share of shared memory goes to the ring
+    static constexpr int STAGES = FAM == kFamHeadStats ? 7 : 5;
+    static constexpr int EPI_BYTES = FAM == kFamHeadStats ? 0 : kPairEpiStageBytes;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + kPairEpiStageBytes + 256;
-    // the last 256 bytes: stage, accumulator and epilogue barriers, then the TMEM address
-    static_assert((2 * STAGES + 4 + 2 * kPairEpiWarps) * 8 + 4 <= 256, "barrier area");
+    static constexpr int BAR_BYTES = 320;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_BYTES + BAR_BYTES;
+    // the last bytes: stage, accumulator and epilogue barriers, then the TMEM address
+    static_assert((2 * STAGES + 4 + 2 * kPairEpiWarps) * 8 + 4 <= BAR_BYTES, "barrier area");
 };
+using PairCfg = PairCfgOf<kFamBase>;  // the tile's shape, alike in all
 
 // Bytes one CTA of a pair loads per k-block (A rows from am, B rows from bn); boxes wholly
 // past M or N are not loaded (their rows or columns are discarded by the epilogue).
@@ -1481,7 +1507,7 @@ struct PairItems {
 template <int NG, int FAM>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_bf16_pair_kernel(const __grid_constant__ PairParams<NG, FAM> P) {
-    using Cfg = PairCfg;
+    using Cfg = PairCfgOf<FAM>;
     constexpr int STAGES = Cfg::STAGES;
     constexpr int BN = Cfg::BN;
     extern __shared__ uint8_t smem_raw[];
@@ -1490,7 +1516,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint8_t* sA = smem;
     uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
     uint8_t* sEpi = smem + STAGES * Cfg::STAGE_BYTES;  // 2 boxes per epilogue warp
-    uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + kPairEpiStageBytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + Cfg::EPI_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
@@ -1651,9 +1677,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 const PairShape sh = pair_shape(args);
                 const uint32_t idesc =
                     make_idesc_bf16(Cfg::BMP, BN, args.a_mn_major, args.b_mn_major);
-                int m_blk, n_blk, split, gi, kb0, kb1;
-                tile_work(args, s_grp, t, sh.num_m, sh.num_n, sh.tiles_mn, sh.kblocks, m_blk,
-                          n_blk, split, gi, kb0, kb1);
+                const OperandDesc da(smem_u32(sA), args.a_mn_major),
+                    db(smem_u32(sB), args.b_mn_major);
+                int kb0, kb1;
+                tile_kblocks<FAM>(args, s_grp, t, sh.num_m, sh.num_n, sh.tiles_mn, sh.kblocks, kb0,
+                                  kb1);
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 int kc = kb0;
                 do {
@@ -1671,18 +1699,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t a_addr = smem_u32(sA + stage * Cfg::A_BYTES);
-                        const uint32_t b_addr = smem_u32(sB + stage * Cfg::B_BYTES);
+                        const uint32_t ao = (uint32_t)stage * (Cfg::A_BYTES >> 4);
+                        const uint32_t bo = (uint32_t)stage * (Cfg::B_BYTES >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < BK / 16; ++kk) {
-                            const uint64_t ad =
-                                args.a_mn_major ? make_sw128_desc(a_addr + kk * 2048, 8192, 1024)
-                                                : make_sw128_desc(a_addr + kk * 32, 16, 1024);
-                            const uint64_t bd =
-                                args.b_mn_major ? make_sw128_desc(b_addr + kk * 2048, 8192, 1024)
-                                                : make_sw128_desc(b_addr + kk * 32, 16, 1024);
-                            umma_bf16_pair(d, ad, bd, idesc, (kb > kc || kk > 0) ? 1u : 0u);
-                        }
+                        for (int kk = 0; kk < BK / 16; ++kk)
+                            umma_bf16_pair(d, da.at(ao, kk), db.at(bo, kk), idesc,
+                                      (kb > kc || kk > 0) ? 1u : 0u);
                         umma_commit_pair(&empty[stage], 0x3);
                         if (++stage == STAGES) {
                             stage = 0;
@@ -2066,7 +2088,7 @@ int launch_bn(const GemmPlan& p, cudaStream_t stream) {
 template <int NG, int FAM>
 int pair_set_attr() {
     static std::atomic<uint64_t> done{0};
-    return set_smem_limit(gemm_bf16_pair_kernel<NG, FAM>, PairCfg::SMEM, done);
+    return set_smem_limit(gemm_bf16_pair_kernel<NG, FAM>, PairCfgOf<FAM>::SMEM, done);
 }
 
 // Clusters of two that can be resident at once (one CTA per SM).
@@ -2102,7 +2124,7 @@ int launch_pair_params(const PairParams<NG, FAM>& P, int grid, cudaStream_t stre
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3(kPairThreads, 1, 1);
-    cfg.dynamicSmemBytes = PairCfg::SMEM;
+    cfg.dynamicSmemBytes = PairCfgOf<FAM>::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

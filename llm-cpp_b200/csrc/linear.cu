@@ -98,9 +98,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
             load8(dy + row * lddy + col, n, v8, v);
             if (act != kActNone) load8(pre + row * ld_pre + col, n, v8, z);
             if (drop.rng) {
-                const uint32_t m = drop_keep8(key, (uint32_t)col >> 3, (uint32_t)row, drop.thr);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ((m >> i) & 1u) ? v[i] * drop.scale : 0.0f;
+                drop_apply8(key, (uint32_t)col >> 3, (uint32_t)row, drop.thr, drop.scale, v);
             }
             if (act != kActNone) {
 #pragma unroll

@@ -52,7 +52,21 @@ __device__ __forceinline__ uint4 philox_10(uint4 c, uint32_t k0, uint32_t k1) {
     return c;
 }
 
-// Bit j: column 8 * col8 + j of `row` is kept.
+// Columns 8 col8 .. 8 col8 + 7 of `row`: v = kept ? v * scale : 0. thr in [1, 65536]; a lane is at
+// least thr when, moved to a word's upper half, it is above (thr << 16) - 1.
+__device__ __forceinline__ void drop_apply8(const DropKey& k, uint32_t col8, uint32_t row,
+                                            uint32_t thr, float scale, float* v) {
+    const uint4 r = philox_10(make_uint4(col8, row, k.c2, k.c3), k.k0, k.k1);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    const uint32_t below = (thr << 16) - 1u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = (w[i] << 16) > below ? v[2 * i] * scale : 0.0f;
+        v[2 * i + 1] = w[i] > below ? v[2 * i + 1] * scale : 0.0f;
+    }
+}
+
+// Bit j: column 8 * col8 + j of `row` is kept. thr in [0, 65536].
 __device__ __forceinline__ uint32_t drop_keep8(const DropKey& k, uint32_t col8, uint32_t row,
                                                uint32_t thr) {
     const uint4 r = philox_10(make_uint4(col8, row, k.c2, k.c3), k.k0, k.k1);
