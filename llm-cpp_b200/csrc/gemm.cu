@@ -1573,7 +1573,130 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    if (warp == 0) {
+    if (NG == 1 && warp == 0) {
+        // ---------------- TMA producer (both CTAs), single products: the whole warp keeps the
+        // ring, one elected lane issues
+        const GemmArgs& args = P.args[0];
+        const PairShape sh = pair_shape(args);
+        const uint32_t full_leader = mapa_shared(smem_u32(&full[0]), 0);
+        const bool lead = elect_one_sync() != 0;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        int g, t;
+        PairItems<NG> items(P, cid, nclusters);
+        while (ok && items.get(g, t)) {
+            int m_blk, n_blk, split, gi, kb0, kb1;
+            tile_work(args, s_grp, t, sh.num_m, sh.num_n, sh.tiles_mn, sh.kblocks, m_blk, n_blk,
+                      split, gi, kb0, kb1);
+            const int M = args.M, N = args.N;
+            const int m0 = m_blk * Cfg::BMP, n0 = n_blk * BN;
+            const int am = m0 + 128 * (int)rank, bn = n0 + Cfg::BNH * (int)rank;
+            const uint32_t all_bytes = leader ? pair_stage_bytes(args, m0, n0) +
+                                                    pair_stage_bytes(args, m0 + 128, n0 + Cfg::BNH)
+                                              : 0u;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_warp_cluster(&empty[stage], phase ^ 1u, err, kDevTimeoutEmpty)) {
+                    ok = false;
+                    break;
+                }
+                if (lead) {
+                    if (leader) mbar_arrive_expect_tx(&full[stage], all_bytes);
+                    const uint32_t fb = full_leader + 8u * (uint32_t)stage;
+                    const int k0 = kb * BK;
+                    uint8_t* a = sA + stage * Cfg::A_BYTES;
+                    uint8_t* b = sB + stage * Cfg::B_BYTES;
+                    if (!args.a_mn_major) {
+                        if (am < M) tma_load_2d_pair(a, &P.tmA[0], fb, k0, am);
+                    } else {
+                        if (am < M) tma_load_2d_pair(a, &P.tmA[0], fb, am, k0);
+                        if (am + 64 < M) tma_load_2d_pair(a + 8192, &P.tmA[0], fb, am + 64, k0);
+                    }
+                    if (!args.b_mn_major) {
+                        if (bn < N) tma_load_2d_pair(b, &P.tmB[0], fb, k0, bn);
+                    } else {
+                        if (bn < N) tma_load_2d_pair(b, &P.tmB[0], fb, bn, k0);
+                        if (bn + 64 < N) tma_load_2d_pair(b + 8192, &P.tmB[0], fb, bn + 64, k0);
+                    }
+                }
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok) spin_ns(100000);  // error path: let copies in flight land first
+    } else if (NG == 1 && warp == 1) {
+        if (leader) {
+            // ---------------- MMA issuer (leader only), single products
+            const GemmArgs& args = P.args[0];
+            const PairShape sh = pair_shape(args);
+            const uint32_t acc_full_peer = mapa_shared(smem_u32(&acc_full[0]), 1);
+            const uint32_t idesc =
+                make_idesc_bf16(Cfg::BMP, BN, args.a_mn_major, args.b_mn_major);
+            const OperandDesc da(smem_u32(sA), args.a_mn_major), db(smem_u32(sB), args.b_mn_major);
+            const bool lead = elect_one_sync() != 0;
+            int stage = 0;
+            uint32_t phase = 0;
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            bool ok = true;
+            int g, t;
+            PairItems<NG> items(P, cid, nclusters);
+            while (ok && items.get(g, t)) {
+                int kb0, kb1;
+                tile_kblocks<FAM>(args, s_grp, t, sh.num_m, sh.num_n, sh.tiles_mn, sh.kblocks, kb0,
+                                  kb1);
+                const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
+                int kc = kb0;
+                do {
+                    const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
+                    if (!mbar_wait_warp_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
+                                                kDevTimeoutAccFree)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+                    for (int kb = kc; kb < kend; ++kb) {
+                        if (!mbar_wait_warp_cluster(&full[stage], phase, err, kDevTimeoutFull)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        if (lead) {
+                            const uint32_t ao = (uint32_t)stage * (Cfg::A_BYTES >> 4);
+                            const uint32_t bo = (uint32_t)stage * (Cfg::B_BYTES >> 4);
+#pragma unroll
+                            for (int kk = 0; kk < BK / 16; ++kk)
+                                umma_bf16_pair(d, da.at(ao, kk), db.at(bo, kk), idesc,
+                                               (kb > kc || kk > 0) ? 1u : 0u);
+                            umma_commit_pair(&empty[stage], 0x3);
+                        }
+                        __syncwarp();
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                    if (!ok) break;
+                    if (lead) {
+                        if (kb1 > kb0) {
+                            umma_commit_pair(&acc_full[acc], 0x3);
+                        } else {  // empty group: both epilogues write zeros
+                            mbar_arrive(&acc_full[acc]);
+                            mbar_arrive_cluster(acc_full_peer + 8u * (uint32_t)acc);
+                        }
+                    }
+                    __syncwarp();
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1u;
+                    kc = kend;
+                } while (FAM == kFamLinear && kc < kb1);
+            }
+        }
+    } else if (NG == 2 && warp == 0) {
         if (lane == 0) {
             // ---------------- TMA producer (both CTAs)
             const uint32_t full_leader = mapa_shared(smem_u32(&full[0]), 0);
@@ -1652,7 +1775,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
             if (!ok) spin_ns(100000);  // error path: let copies in flight land first
         }
-    } else if (warp == 1) {
+    } else if (NG == 2 && warp == 1) {
         if (lane == 0 && leader) {
             // ---------------- MMA issuer (leader only)
             const uint32_t acc_full_peer = mapa_shared(smem_u32(&acc_full[0]), 1);
