@@ -87,6 +87,24 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     }
 }
 
+// The same for a whole warp: the outcome is a vote, so that what follows stays uniform and the
+// compiler keeps the role's addresses and descriptors in uniform registers, where the bulk copies
+// and MMAs take them from.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err, int code) {
+    constexpr uint32_t all = 0xffffffffu;
+    if (__all_sync(all, mbar_try_wait(bar, parity))) return true;
+    const unsigned long long t0 = globaltimer_ns();
+    uint32_t it = 0;
+    while (true) {
+        if (__all_sync(all, mbar_try_wait(bar, parity))) return true;
+        if ((++it & 255u) == 0) {
+            const bool late = globaltimer_ns() - t0 > kWaitLimitNs;
+            if (late && err) atomicCAS(err, 0, code);
+            if (__any_sync(all, late || (err && *((volatile int*)err) != 0))) return false;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
@@ -386,9 +404,7 @@ __device__ __forceinline__ bool mbar_wait_bounded_cluster(uint64_t* bar, uint32_
         }
     }
 }
-// The same for a whole warp: the outcome is a vote, so that what follows stays uniform and the
-// compiler keeps the role's addresses and descriptors in uniform registers, where the bulk copies
-// and MMAs take them from.
+// The same for a whole warp (see mbar_wait_warp).
 __device__ __forceinline__ bool mbar_wait_warp_cluster(uint64_t* bar, uint32_t parity, int* err,
                                                        int code) {
     constexpr uint32_t all = 0xffffffffu;

@@ -43,40 +43,69 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const TI* x, long
     const int lane = threadIdx.x & 31;
     const int segs = (cols + 255) / 256;
     const long long total = (long long)rows * segs;
-    const DropKey key = drop_key(rng, site);
+    const DropKeys key = drop_keys(rng, site);
     for (long long i = ((long long)blockIdx.x * kDropThreads + threadIdx.x) >> 5; i < total;
          i += ((long long)gridDim.x * kDropThreads) >> 5) {
         const int row = (int)(i / segs);
         const int c0 = (int)(i - (long long)row * segs) * 256;
+        TI xv[8];
+        TO rv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // all loads in flight before the generator's arithmetic
+            const int c = c0 + 32 * j + lane;
+            if (c < cols) {
+                xv[j] = x[row * ldx + c];
+                if (resid) rv[j] = resid[row * ldr + c];
+            }
+        }
         const uint32_t m = drop_keep8(key, (uint32_t)(c0 >> 3) + lane, (uint32_t)row, thr);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t mj = __shfl_sync(0xffffffffu, m, 4 * j + (lane >> 3));
             const int c = c0 + 32 * j + lane;
             if (c >= cols) continue;
-            float v = 0.0f;
-            if ((mj >> (lane & 7)) & 1u) v = to_f32(x[row * ldx + c]) * scale;
-            if (resid) v += to_f32(resid[row * ldr + c]);
+            float v = ((mj >> (lane & 7)) & 1u) ? to_f32(xv[j]) * scale : 0.0f;
+            if (resid) v += to_f32(rv[j]);
             out[row * ldo + c] = from_f32<TO>(v);
         }
     }
 }
 
-// Eight neighbouring elements, 16 bytes at a time.
-__device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight neighbouring elements as they lie in memory: loads stay in flight until raw_f32.
+template <typename T>
+struct Raw8 {
+    uint4 q[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ void load_raw(const T* p, Raw8<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.q[i] = reinterpret_cast<const uint4*>(p)[i];
+}
+// n < 8 of them, the others 0
+template <typename T>
+__device__ __forceinline__ void load_raw_n(const T* p, int n, Raw8<T>& r) {
+    alignas(16) T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = j < n ? p[j] : from_f32<T>(0.0f);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.q[i] = reinterpret_cast<const uint4*>(t)[i];
+}
+__device__ __forceinline__ void raw_f32(const Raw8<bf16>& r, float (&v)[8]) {
+    const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[2 * i] = bf16_lo(w[i]);
         v[2 * i + 1] = bf16_hi(w[i]);
     }
 }
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0];
-    const float4 b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+__device__ __forceinline__ void raw_f32(const Raw8<float>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        v[4 * i] = __uint_as_float(r.q[i].x);
+        v[4 * i + 1] = __uint_as_float(r.q[i].y);
+        v[4 * i + 2] = __uint_as_float(r.q[i].z);
+        v[4 * i + 3] = __uint_as_float(r.q[i].w);
+    }
 }
 __device__ __forceinline__ void store8(bf16* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) =
@@ -88,37 +117,42 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// Rows on 16 bytes: a thread takes 8 columns (one call of the generator) at a time, kDropUnroll of
-// them with all loads in flight before the generator's arithmetic. The positions of a thread lie
+// Rows on 16 bytes: a thread takes 8 columns (one call of the generator) at a time, U of them with
+// all loads in flight, as raw words, before the generator's arithmetic. The positions of a thread lie
 // gridDim * 256 groups of 8 apart; (dr, dc) is that distance in rows and groups, so the loop
 // divides nothing.
-constexpr int kDropUnroll = 4;
+//
+// Bound by memory for f32 (16384 x 4096: bf16 + f32 residual -> f32 106 us, 6.3 TB/s; f32 -> f32 86
+// us) and by the generator's integer arithmetic for bf16 -> bf16 (54 us, 5.0 TB/s). U = 3 keeps
+// the most blocks resident but for f32 -> f32, where 4 moves more at once (86 against 97 us).
+template <typename TI, typename TO, bool RES>
+constexpr int kDropUnroll = (!RES && sizeof(TI) == 4 && sizeof(TO) == 4) ? 4 : 3;
 template <typename TI, typename TO, bool RES>
 __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(
     const TI* x, long long ldx, const TO* resid, long long ldr, TO* out, long long ldo,
     uint32_t rows, int cols, uint32_t n8, uint32_t dr, uint32_t dc, uint32_t thr, float scale,
     const uint64_t* rng, uint64_t site) {
     pdl_enter();
-    const DropKey key = drop_key(rng, site);
+    constexpr int U = kDropUnroll<TI, TO, RES>;
+    const DropKeys key = drop_keys(rng, site);
     const uint32_t first = blockIdx.x * kDropThreads + threadIdx.x;
     uint32_t row = first / n8, c8 = first - row * n8;
     while (row < rows) {
-        float v[kDropUnroll][8], r[kDropUnroll][8];
-        uint32_t ur[kDropUnroll], uc[kDropUnroll];
+        Raw8<TI> xr[U];
+        Raw8<TO> rr[U];
+        uint32_t ur[U], uc[U];
 #pragma unroll
-        for (int u = 0; u < kDropUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             ur[u] = row;
             uc[u] = c8;
             const int c = (int)(c8 * 8);
             if (row < rows) {
                 if (c + 8 <= cols) {
-                    load8(x + row * ldx + c, v[u]);
-                    if (RES) load8(resid + row * ldr + c, r[u]);
+                    load_raw(x + row * ldx + c, xr[u]);
+                    if (RES) load_raw(resid + row * ldr + c, rr[u]);
                 } else {
-                    for (int j = 0; j < 8; ++j) {
-                        v[u][j] = c + j < cols ? to_f32(x[row * ldx + c + j]) : 0.0f;
-                        if (RES) r[u][j] = c + j < cols ? to_f32(resid[row * ldr + c + j]) : 0.0f;
-                    }
+                    load_raw_n(x + row * ldx + c, cols - c, xr[u]);
+                    if (RES) load_raw_n(resid + row * ldr + c, cols - c, rr[u]);
                 }
             }
             row += dr;
@@ -129,19 +163,23 @@ __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(
             }
         }
 #pragma unroll
-        for (int u = 0; u < kDropUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             if (ur[u] >= rows) break;
-            if (thr) drop_apply8(key, uc[u], ur[u], thr, scale, v[u]);
+            float v[8];
+            raw_f32(xr[u], v);
+            if (thr) drop_apply8(key, uc[u], ur[u], thr, scale, v);
             if (RES) {
+                float r[8];
+                raw_f32(rr[u], r);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[u][j] += r[u][j];
+                for (int j = 0; j < 8; ++j) v[j] += r[j];
             }
             const int c = (int)(uc[u] * 8);
             if (c + 8 <= cols) {
-                store8(out + ur[u] * ldo + c, v[u]);
+                store8(out + ur[u] * ldo + c, v);
             } else {
                 for (int j = 0; j < 8; ++j)
-                    if (c + j < cols) out[ur[u] * ldo + c + j] = from_f32<TO>(v[u][j]);
+                    if (c + j < cols) out[ur[u] * ldo + c + j] = from_f32<TO>(v[j]);
             }
         }
     }

@@ -1067,7 +1067,7 @@ __device__ __forceinline__ DropKey family_key(const typename ExtOf<FAM>::type& x
     if constexpr (FAM == kFamLinear) {
         if (x.rng) return drop_key(x.rng, x.site);
     }
-    return DropKey{0u, 0u, 0u, 0u};
+    return DropKey{};
 }
 
 template <int BN, int FAM>
@@ -1132,47 +1132,47 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---------------- TMA producer
-            int stage = 0;
-            uint32_t phase = 0;
-            uint32_t last_phase[STAGES];
-            bool pending[STAGES];
+        // ---------------- TMA producer: the whole warp keeps the ring, one lane issues
+        const bool lead = elect_one_sync() != 0;
+        int stage = 0;
+        uint32_t phase = 0;
+        uint32_t last_phase[STAGES];
+        bool pending[STAGES];
 #pragma unroll
-            for (int s = 0; s < STAGES; ++s) {
-                last_phase[s] = 0;
-                pending[s] = false;
-            }
-            bool ok = true;
-            for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-                int m_blk, n_blk, split, g, kb0, kb1;
-                if (!tile_work(args, s_grp, t, num_m, num_n, tiles_mn, kblocks, m_blk, n_blk,
-                               split, g, kb0, kb1))
-                    continue;
-                const int m0 = m_blk * BM, n0 = n_blk * BN;
-                // row-grouped products read group g of B from row g * b_grp_rows on
-                const int bg = (args.grp_mode == kGroupRows) ? (int)(g * args.b_grp_rows) : 0;
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, args.err,
-                                           kDevTimeoutEmpty)) {
-                        ok = false;
-                        break;
-                    }
-                    const int k0 = kb * BK;
-                    uint8_t* a = sA + stage * Cfg::A_BYTES;
-                    uint8_t* b = sB + stage * Cfg::B_BYTES;
-                    uint32_t bytes = 0;
-                    if (!args.a_mn_major) {
-                        bytes += Cfg::A_BYTES;
-                    } else {
-                        bytes += 8192u * ((m0 + 64 < M) ? 2u : 1u);
-                    }
-                    if (!args.b_mn_major) {
-                        bytes += Cfg::B_BYTES;
-                    } else {
-                        for (int j = 0; j < BN / 64; ++j)
-                            if (n0 + 64 * j < N) bytes += 8192u;
-                    }
+        for (int s = 0; s < STAGES; ++s) {
+            last_phase[s] = 0;
+            pending[s] = false;
+        }
+        bool ok = true;
+        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            int m_blk, n_blk, split, g, kb0, kb1;
+            if (!tile_work(args, s_grp, t, num_m, num_n, tiles_mn, kblocks, m_blk, n_blk,
+                           split, g, kb0, kb1))
+                continue;
+            const int m0 = m_blk * BM, n0 = n_blk * BN;
+            // row-grouped products read group g of B from row g * b_grp_rows on
+            const int bg = (args.grp_mode == kGroupRows) ? (int)(g * args.b_grp_rows) : 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_warp(&empty[stage], phase ^ 1u, args.err, kDevTimeoutEmpty)) {
+                    ok = false;
+                    break;
+                }
+                const int k0 = kb * BK;
+                uint8_t* a = sA + stage * Cfg::A_BYTES;
+                uint8_t* b = sB + stage * Cfg::B_BYTES;
+                uint32_t bytes = 0;
+                if (!args.a_mn_major) {
+                    bytes += Cfg::A_BYTES;
+                } else {
+                    bytes += 8192u * ((m0 + 64 < M) ? 2u : 1u);
+                }
+                if (!args.b_mn_major) {
+                    bytes += Cfg::B_BYTES;
+                } else {
+                    for (int j = 0; j < BN / 64; ++j)
+                        if (n0 + 64 * j < N) bytes += 8192u;
+                }
+                if (lead) {
                     mbar_arrive_expect_tx(&full[stage], bytes);
                     if (!args.a_mn_major) {
                         tma_load_2d(a, &tmA, &full[stage], k0, m0);
@@ -1188,75 +1188,81 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                                 tma_load_2d(b + j * 8192, &tmB, &full[stage], n0 + 64 * j,
                                             k0 + bg);
                     }
-                    last_phase[stage] = phase;
-                    pending[stage] = true;
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                }
+                __syncwarp();
+                last_phase[stage] = phase;
+                pending[stage] = true;
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            if (!ok) {
-                // Error path: let issued copies land before the CTA exits.
+        }
+        if (!ok) {
+            // Error path: let issued copies land before the CTA exits.
 #pragma unroll
-                for (int s = 0; s < STAGES; ++s)
-                    if (pending[s]) mbar_wait_bounded(&full[s], last_phase[s], nullptr, 0);
-            }
+            for (int s = 0; s < STAGES; ++s)
+                if (pending[s]) mbar_wait_warp(&full[s], last_phase[s], nullptr, 0);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // ---------------- MMA issuer
-            const uint32_t idesc = make_idesc_bf16(BM, BN, args.a_mn_major, args.b_mn_major);
-            const OperandDesc da(smem_u32(sA), args.a_mn_major), db(smem_u32(sB), args.b_mn_major);
-            int stage = 0;
-            uint32_t phase = 0;
-            int acc = 0;
-            uint32_t acc_phase = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-                int kb0, kb1;
-                if (!tile_kblocks<FAM>(args, s_grp, t, num_m, num_n, tiles_mn, kblocks, kb0, kb1))
-                    continue;
-                // one accumulator for the tile, or one for each chain of it
-                const int ck = chain_blocks<FAM>(ext, kb0, kb1);
-                int kc = kb0;
-                do {
-                    const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
-                    if (!mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1u, args.err,
-                                           kDevTimeoutAccFree)) {
+        // ---------------- MMA issuer
+        const bool lead = elect_one_sync() != 0;
+        const uint32_t idesc = make_idesc_bf16(BM, BN, args.a_mn_major, args.b_mn_major);
+        const OperandDesc da(smem_u32(sA), args.a_mn_major), db(smem_u32(sB), args.b_mn_major);
+        int stage = 0;
+        uint32_t phase = 0;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            int kb0, kb1;
+            if (!tile_kblocks<FAM>(args, s_grp, t, num_m, num_n, tiles_mn, kblocks, kb0, kb1))
+                continue;
+            // one accumulator for the tile, or one for each chain of it
+            const int ck = chain_blocks<FAM>(ext, kb0, kb1);
+            int kc = kb0;
+            do {
+                const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
+                if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1u, args.err,
+                                    kDevTimeoutAccFree)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+                for (int kb = kc; kb < kend; ++kb) {
+                    if (!mbar_wait_warp(&full[stage], phase, args.err, kDevTimeoutFull)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-                    for (int kb = kc; kb < kend; ++kb) {
-                        if (!mbar_wait_bounded(&full[stage], phase, args.err, kDevTimeoutFull)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t ao = (uint32_t)stage * (Cfg::A_BYTES >> 4);
-                        const uint32_t bo = (uint32_t)stage * (Cfg::B_BYTES >> 4);
+                    const uint32_t ao = (uint32_t)stage * (Cfg::A_BYTES >> 4);
+                    const uint32_t bo = (uint32_t)stage * (Cfg::B_BYTES >> 4);
+                    if (lead) {
 #pragma unroll
                         for (int kk = 0; kk < BK / 16; ++kk)
                             umma_bf16(d, da.at(ao, kk), db.at(bo, kk), idesc,
                                       (kb > kc || kk > 0) ? 1u : 0u);
                         umma_commit(&empty[stage]);
-                        if (++stage == STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
                     }
-                    if (!ok) break;
+                    __syncwarp();
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                if (lead) {
                     if (kb1 > kb0)
                         umma_commit(&acc_full[acc]);
                     else
                         mbar_arrive(&acc_full[acc]);  // empty group: the epilogue writes zeros
-                    acc ^= 1;
-                    if (acc == 0) acc_phase ^= 1u;
-                    kc = kend;
-                } while (FAM == kFamLinear && kc < kb1);
-            }
+                }
+                __syncwarp();
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+                kc = kend;
+            } while (FAM == kFamLinear && kc < kb1);
         }
     } else if (warp >= 4) {
         // ---------------- epilogue warpgroup

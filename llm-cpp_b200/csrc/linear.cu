@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
     for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
     if (n > 0) {
         const bool v8 = vec && n == 8;
-        const DropKey key = drop.rng ? drop_key(drop.rng, drop.site) : DropKey{0u, 0u, 0u, 0u};
+        const DropKeys key = drop.rng ? drop_keys(drop.rng, drop.site) : DropKeys{};
         for (int row = blockIdx.y * kDzRows + wr; row < M; row += gridDim.y * kDzRows) {
             float v[8], z[8];
             load8(dy + row * lddy + col, n, v8, v);

@@ -17,6 +17,13 @@ struct DropKey {
     uint32_t k0, k1;  // seed
     uint32_t c2, c3;  // offset + site
 };
+// The same with the ten rounds' keys formed once: twenty registers for twenty additions a call,
+// which the elementwise kernels can spare (bf16 16384 x 4096: 62 -> 55 us) and the products'
+// epilogue cannot.
+struct DropKeys {
+    uint32_t k0[10], k1[10];
+    uint32_t c2, c3;
+};
 
 // Host side: threshold and scale of a drop probability p in [0, 1]; false for any other p.
 inline bool drop_params(float p, uint32_t* thr, float* scale) {
@@ -38,25 +45,41 @@ __device__ __forceinline__ DropKey drop_key(const uint64_t* rng, uint64_t site) 
     const uint64_t seed = rng[0], off = rng[1] + site;
     return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
 }
+__device__ __forceinline__ DropKeys drop_keys(const uint64_t* rng, uint64_t site) {
+    const DropKey d = drop_key(rng, site);
+    DropKeys k;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        k.k0[r] = d.k0 + r * 0x9E3779B9u;
+        k.k1[r] = d.k1 + r * 0xBB67AE85u;
+    }
+    k.c2 = d.c2;
+    k.c3 = d.c3;
+    return k;
+}
+__device__ __forceinline__ uint32_t round_key0(const DropKey& k, int r) { return k.k0 + r * 0x9E3779B9u; }
+__device__ __forceinline__ uint32_t round_key1(const DropKey& k, int r) { return k.k1 + r * 0xBB67AE85u; }
+__device__ __forceinline__ uint32_t round_key0(const DropKeys& k, int r) { return k.k0[r]; }
+__device__ __forceinline__ uint32_t round_key1(const DropKeys& k, int r) { return k.k1[r]; }
 
-__device__ __forceinline__ uint4 philox_10(uint4 c, uint32_t k0, uint32_t k1) {
+template <typename Key>
+__device__ __forceinline__ uint4 philox_10(uint4 c, const Key& k) {
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t a = (uint64_t)c.x * 0xD2511F53u;
         const uint64_t b = (uint64_t)c.z * 0xCD9E8D57u;
-        c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ k0, (uint32_t)b,
-                       (uint32_t)(a >> 32) ^ c.w ^ k1, (uint32_t)a);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
+        c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ round_key0(k, r), (uint32_t)b,
+                       (uint32_t)(a >> 32) ^ c.w ^ round_key1(k, r), (uint32_t)a);
     }
     return c;
 }
 
 // Columns 8 col8 .. 8 col8 + 7 of `row`: v = kept ? v * scale : 0. thr in [1, 65536]; a lane is at
 // least thr when, moved to a word's upper half, it is above (thr << 16) - 1.
-__device__ __forceinline__ void drop_apply8(const DropKey& k, uint32_t col8, uint32_t row,
+template <typename Key>
+__device__ __forceinline__ void drop_apply8(const Key& k, uint32_t col8, uint32_t row,
                                             uint32_t thr, float scale, float* v) {
-    const uint4 r = philox_10(make_uint4(col8, row, k.c2, k.c3), k.k0, k.k1);
+    const uint4 r = philox_10(make_uint4(col8, row, k.c2, k.c3), k);
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
     const uint32_t below = (thr << 16) - 1u;
 #pragma unroll
@@ -67,9 +90,10 @@ __device__ __forceinline__ void drop_apply8(const DropKey& k, uint32_t col8, uin
 }
 
 // Bit j: column 8 * col8 + j of `row` is kept. thr in [0, 65536].
-__device__ __forceinline__ uint32_t drop_keep8(const DropKey& k, uint32_t col8, uint32_t row,
+template <typename Key>
+__device__ __forceinline__ uint32_t drop_keep8(const Key& k, uint32_t col8, uint32_t row,
                                                uint32_t thr) {
-    const uint4 r = philox_10(make_uint4(col8, row, k.c2, k.c3), k.k0, k.k1);
+    const uint4 r = philox_10(make_uint4(col8, row, k.c2, k.c3), k);
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
     uint32_t m = 0;
 #pragma unroll
