@@ -149,12 +149,193 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict
     }
 }
 
+// ------------------------------------------------------------------------------ a few rows
+// Decoding: out [M <= 8, N] with every weight read once and no tensor map or tile in the way. The
+// products are sums in f32 registers; the epilogue is the linear layer's.
+constexpr int kFewRows = 8;
+
+struct RowsArgs {
+    const bf16* x;
+    long long ldx;
+    const bf16* w;
+    long long ldw;
+    const float* bias;
+    int act;
+    DropArgs drop;
+    const void* resid;
+    long long ldr;
+    bf16* pre;
+    long long ld_pre;
+    void* out;
+    int out_f32;
+    long long ldo;
+    int M, N, K;
+};
+
+__device__ __forceinline__ void rows_store(const RowsArgs& a, int m, int n, float z) {
+    if (a.bias) z += a.bias[n];
+    if (a.pre) a.pre[m * a.ld_pre + n] = __float2bfloat16_rn(z);
+    float y = z;
+    if (a.act == kActRelu) {
+        y = z <= 0.0f ? 0.0f : z;
+    } else if (a.act == kActGelu) {
+        const float t = -1.5957691216f * 1.4426950408889634f * z * fmaf(0.044715f * z, z, 1.0f);
+        y = z * rcp_approx(1.0f + ex2_approx(t));
+    } else if (a.act == kActSilu) {
+        y = z * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * z));
+    }
+    if (a.drop.rng) {
+        const DropKey key = drop_key(a.drop.rng, a.drop.site);
+        const uint32_t keep = drop_keep8(key, (uint32_t)n >> 3, (uint32_t)m, a.drop.thr);
+        y = ((keep >> (n & 7)) & 1u) ? y * a.drop.scale : 0.0f;
+    }
+    if (a.out_f32) {
+        if (a.resid) y += reinterpret_cast<const float*>(a.resid)[m * a.ldr + n];
+        reinterpret_cast<float*>(a.out)[m * a.ldo + n] = y;
+    } else {
+        if (a.resid) y += __bfloat162float(reinterpret_cast<const bf16*>(a.resid)[m * a.ldr + n]);
+        reinterpret_cast<bf16*>(a.out)[m * a.ldo + n] = __float2bfloat16_rn(y);
+    }
+}
+
+// Eight bf16 of a row from k on (16-byte aligned), zeros past K.
+__device__ __forceinline__ uint4 row_chunk(const bf16* p, int k, int K) {
+    if (k + 8 <= K) return *reinterpret_cast<const uint4*>(p + k);
+    uint32_t h[4] = {0u, 0u, 0u, 0u};
+    for (int j = 0; j < 8; ++j)
+        if (k + j < K) h[j >> 1] |= (uint32_t)__bfloat16_as_ushort(p[k + j]) << (16 * (j & 1));
+    return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
+// w [N, K]: a warp takes one output column, its lanes 8 of K at a time, four steps in flight.
+template <int MR>
+__global__ void __launch_bounds__(256) linear_rows_kernel(const RowsArgs a) {
+    pdl_enter();
+    const int lane = threadIdx.x & 31;
+    const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (n >= a.N) return;
+    const bf16* w = a.w + n * a.ldw;
+    float acc[MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[m] = 0.0f;
+    for (int k0 = 8 * lane; k0 < a.K; k0 += 4 * 256) {
+        uint4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            u[i] = k0 + 256 * i < a.K ? row_chunk(w, k0 + 256 * i, a.K) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + 256 * i;
+            if (k >= a.K) break;
+            const uint32_t ww[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                if (m >= a.M) break;
+                const uint4 q = row_chunk(a.x + m * a.ldx, k, a.K);
+                const uint32_t xx[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[m] = fmaf(bf16_lo(ww[j]), bf16_lo(xx[j]), acc[m]);
+                    acc[m] = fmaf(bf16_hi(ww[j]), bf16_hi(xx[j]), acc[m]);
+                }
+            }
+        }
+    }
+    float mine = 0.0f;
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+        float v = acc[m];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == m) mine = v;
+    }
+    if (lane < a.M) rows_store(a, lane, n, mine);
+}
+
+// w [K, N]: a block takes 32 columns, four lanes of 8 side by side; its 128 groups of four lanes
+// stride over K, their sums meet in shared memory.
+constexpr int kRowsThreads = 512;
+template <int MR>
+__global__ void __launch_bounds__(kRowsThreads) linear_rows_mn_kernel(const RowsArgs a) {
+    pdl_enter();
+    __shared__ float part[kRowsThreads / 32][MR][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n0 = blockIdx.x * 32, n = n0 + 8 * (lane & 3);
+    float acc[MR][8];
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[m][j] = 0.0f;
+    if (n < a.N) {
+        constexpr int kStep = kRowsThreads / 4;
+        for (int k0 = threadIdx.x >> 2; k0 < a.K; k0 += 4 * kStep) {
+            uint4 u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = k0 + i * kStep;
+                u[i] = k < a.K ? row_chunk(a.w + k * a.ldw, n, a.N) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = k0 + i * kStep;
+                if (k >= a.K) break;
+                const uint32_t ww[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+                for (int m = 0; m < MR; ++m) {
+                    if (m >= a.M) break;
+                    const float xv = __bfloat162float(a.x[m * a.ldx + k]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        acc[m][2 * j] = fmaf(xv, bf16_lo(ww[j]), acc[m][2 * j]);
+                        acc[m][2 * j + 1] = fmaf(xv, bf16_hi(ww[j]), acc[m][2 * j + 1]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float v = acc[m][j];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane < 4) part[warp][m][8 * lane + j] = v;
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * a.M; i += kRowsThreads) {
+        const int m = i >> 5, c = i & 31;
+        if (n0 + c >= a.N) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kRowsThreads / 32; ++q) v += part[q][m][c];
+        rows_store(a, m, n0 + c, v);
+    }
+}
+
+template <int MR>
+int launch_rows(const RowsArgs& a, int w_mn, cudaStream_t s) {
+    if (w_mn)
+        return launch_kernel(linear_rows_mn_kernel<MR>, (a.N + 31) / 32, kRowsThreads, 0, s, a);
+    return launch_kernel(linear_rows_kernel<MR>, (a.N + 7) / 8, 256, 0, s, a);
+}
+int run_rows(const RowsArgs& a, int w_mn, cudaStream_t s) {
+    if (a.M == 1) return launch_rows<1>(a, w_mn, s);
+    if (a.M == 2) return launch_rows<2>(a, w_mn, s);
+    return a.M <= 4 ? launch_rows<4>(a, w_mn, s) : launch_rows<8>(a, w_mn, s);
+}
+
 }  // namespace
 
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
             int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
             int* err, cudaStream_t s) {
     if (accumulate && !out_f32) return -1;
+    if (M <= kFewRows && !a_mn) {
+        RowsArgs r{A, lda, B, ldb, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo, nullptr, 0,
+                   out, out_f32, ldo, M, N, K};
+        return run_rows(r, b_mn, s);
+    }
     GemmArgs g{};
     g.out = out;
     g.ldo = ldo;
@@ -183,6 +364,12 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
     if (a.M == 0) return 0;
     if (!a.x || !a.w || !a.out) return -1;
     if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw)) return kBadOperand;
+    if (a.M <= kFewRows) {
+        RowsArgs r{a.x, a.ldx, a.w, a.ldw, a.bias, a.act, a.drop, a.resid, a.ldr, a.pre, a.ld_pre,
+                   a.out, a.out_f32, a.ldo, a.M, a.N, a.K};
+        if (r.drop.thr == 0) r.drop.rng = nullptr;
+        return run_rows(r, a.w_mn_major, s);
+    }
     GemmArgs g{};
     g.epi = kEpiLinear;
     g.out = a.out;
