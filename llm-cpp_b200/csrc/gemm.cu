@@ -586,11 +586,20 @@ __device__ __forceinline__ void act_all(float (&v)[32]) {
     }
 }
 
-// One lane's 32 accumulator columns [col0, col0 + 32) plus the bias.
+// One lane's 32 accumulator columns [col0, col0 + 32), scaled, plus the bias.
 __device__ __forceinline__ void linear_bias(const GemmArgs& a, const GemmExt& x, int col0, int lane,
                                             const uint32_t (&r)[32], float (&v)[32]) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+    if (x.alpha) {
+        const float f = *x.alpha;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            const float2 y = fmul2(make_float2(v[j], v[j + 1]), make_float2(f, f));
+            v[j] = y.x;
+            v[j + 1] = y.y;
+        }
+    }
     if (!x.bias) return;
     if (col0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(x.bias) & 15) == 0) {
         const float4* b4 = reinterpret_cast<const float4*>(x.bias + col0);  // same for all lanes
@@ -980,7 +989,12 @@ __device__ __forceinline__ void head_stats_tile(const GemmArgs& a, const GemmExt
     }
 }
 
-// coef * (softmax - y) of the recomputed logits, bf16, through 32 x 64 boxes (two chunks).
+// c * (softmax / on - y) of the recomputed logits, bf16, through 32 x 64 boxes (two chunks). The
+// row's weight relative to the largest one and the target's share 1 (on is divided out, and both
+// factors come back in f32 behind the products) make the target's entry -1 + softmax / on in a
+// batch of equal weights: an untrained or unlikely target's entry is then nearly exact, where
+// -0.9 / rows, say, would round the same way in every row and bias the whole gradient by up to
+// 2^-8.
 template <int NCOLS>
 __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt& x,
                                                const CUtensorMap* tmO, uint32_t tbase, int row0,
@@ -990,8 +1004,8 @@ __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt&
     const int row = row0 + lane;
     const int t = row < a.M ? x.targets[row] : -1;
     const bool counts = t >= 0 && t < x.V;
-    const float coef = counts ? x.scale * (x.dloss ? x.dloss[row] : 1.0f) : 0.0f;
-    const float ll = counts ? x.lse[row] * kLog2e : 0.0f;
+    const float coef = counts && x.dloss ? x.dloss[row] / x.top[0] : 1.0f;
+    const float ll = counts ? fmaf(x.lse[row], kLog2e, log2f(x.on)) : 0.0f;
 #pragma unroll 1
     for (int c = c_begin; c < c_end; c += 2) {
         const int col0 = n0 + c * 32;
@@ -1017,7 +1031,7 @@ __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt&
                         const int j = 8 * ch + 2 * k + i;
                         const float p =
                             ex2_approx(fmaf(__uint_as_float(r[h][j]), kLog2e, -ll));
-                        const float y = (32 * h + j == tj) ? x.on : x.off;
+                        const float y = (32 * h + j == tj) ? 1.0f : x.off_on;
                         g[i] = counts ? coef * (p - y) : 0.0f;
                     }
                     o[k] = pack_bf16x2(g[0], g[1]);

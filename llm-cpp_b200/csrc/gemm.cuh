@@ -34,6 +34,7 @@ enum LinearAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 // Arguments of the epilogues from kEpiLinear on.
 struct GemmExt {
     // kEpiLinear
+    const float* alpha;   // device scalar that multiplies acc, nullable
     const float* bias;    // [N], nullable
     int act;              // LinearAct
     int out_f32;          // out and resid are f32, else bf16
@@ -53,11 +54,12 @@ struct GemmExt {
     float2* part;
     float* zsum;
     float* zt;
-    // kEpiHeadGrad: out = coef * (exp(z - lse) - y), coef = scale * dloss[m] (dloss nullable: 1),
-    // y = on at the target and off elsewhere; 0 in rows left out
+    // kEpiHeadGrad: out = c * (exp(z - lse) / on - y), c = dloss[m] / top[0] (dloss nullable: 1),
+    // y = 1 at the target and off_on elsewhere; 0 in rows left out
     const float* lse;
     const float* dloss;
-    float scale, on, off;
+    const float* top;
+    float on, off_on;
 };
 
 struct GemmArgs {

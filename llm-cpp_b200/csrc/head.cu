@@ -3,6 +3,8 @@
 // again a piece of the vocabulary at a time, writes the gradient by them in bf16 straight from
 // tensor memory (kEpiHeadGrad), and feeds that piece to the products for dx and dw. The method
 // costs one product more than keeping [rows, V] logits and none of their memory.
+#include <cfloat>
+
 #include "common.cuh"
 #include "linear.cuh"
 
@@ -75,15 +77,44 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const float2* __restri
 }
 
 // Copy of x with zeros in the rows left out (0 times what they hold could be NaN in dw), its row
-// stride a multiple of 8 elements.
+// stride a multiple of 8 elements. The last block finds the largest finite |dloss| of the rows
+// that count: top = {that (1 if it is 0 or there is no dloss), factor times it}, what the gradient by
+// the logits is divided by and what the products multiply back.
 __global__ void __launch_bounds__(256) head_rows_kernel(const bf16* __restrict__ x, long long ldx,
                                                         const int32_t* __restrict__ targets,
-                                                        int rows, int C, int V,
-                                                        bf16* __restrict__ out, int ldo) {
+                                                        const float* __restrict__ dloss,
+                                                        float factor, int rows, int C, int V,
+                                                        bf16* __restrict__ out, int ldo,
+                                                        float* __restrict__ top) {
     pdl_enter();
+    if (blockIdx.x == gridDim.x - 1) {
+        float m = 0.0f;
+        if (dloss) {
+#pragma unroll 8
+            for (int r = threadIdx.x; r < rows; r += 256) {
+                const int t = targets[r];
+                const float d = fabsf(dloss[r]);
+                if (t >= 0 && t < V && d <= FLT_MAX) m = fmaxf(m, d);
+            }
+        }
+        __shared__ float red[8];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
+            if (m == 0.0f) m = 1.0f;
+            top[0] = m;
+            top[1] = factor * m;
+        }
+        return;
+    }
     const int n8 = ldo >> 3;
     const long long total = (long long)rows * n8;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long step = (gridDim.x - 1) * 256ll;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += step) {
         const int row = (int)(i / n8), c = (int)(i - (long long)row * n8) * 8;
         const int t = targets[row];
         uint4 u = make_uint4(0u, 0u, 0u, 0u);
@@ -104,12 +135,14 @@ __global__ void __launch_bounds__(256) head_rows_kernel(const bf16* __restrict__
     }
 }
 
-// dx = sum of the planes [n][rows][ldp], in their order.
+// dx = alpha times the sum of the planes [n][rows][ldp], in their order.
 template <typename T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ planes, int n,
-                                                      int rows, int C, int ldp, T* __restrict__ dx,
-                                                      long long lddx) {
+                                                      int rows, int C, int ldp,
+                                                      const float* __restrict__ alpha,
+                                                      T* __restrict__ dx, long long lddx) {
     pdl_enter();
+    const float f = *alpha;
     const long long total = (long long)rows * C, plane = (long long)rows * ldp;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const int row = (int)(i / C), c = (int)(i - (long long)row * C);
@@ -117,9 +150,9 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
         float v = p[0];
         for (int k = 1; k < n; ++k) v += p[k * plane];
         if constexpr (sizeof(T) == 4)
-            dx[row * lddx + c] = v;
+            dx[row * lddx + c] = v * f;
         else
-            dx[row * lddx + c] = __float2bfloat16_rn(v);
+            dx[row * lddx + c] = __float2bfloat16_rn(v * f);
     }
 }
 
@@ -144,7 +177,7 @@ int dx_splits(int rows, int C, int piece) {
 
 struct HeadLayout {
     int piece, splits, ldx, ldg, ldp;
-    size_t x, g, planes, total;  // byte offsets and the whole
+    size_t x, g, planes, top, total;  // byte offsets and the whole
 };
 
 HeadLayout head_layout(int rows, int C, int V, int piece) {
@@ -157,7 +190,8 @@ HeadLayout head_layout(int rows, int C, int V, int piece) {
     l.x = 0;
     l.g = align256((size_t)rows * l.ldx * 2);
     l.planes = l.g + align256((size_t)rows * l.ldg * 2);
-    l.total = l.planes + (size_t)l.splits * rows * l.ldp * 4;
+    l.top = l.planes + align256((size_t)l.splits * rows * l.ldp * 4);
+    l.total = l.top + 8;
     return l;
 }
 
@@ -253,10 +287,12 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
     bf16* xr = reinterpret_cast<bf16*>(wk + l.x);
     bf16* gp = reinterpret_cast<bf16*>(wk + l.g);
     float* planes = reinterpret_cast<float*>(wk + l.planes);
+    float* top = reinterpret_cast<float*>(wk + l.top);
+    const float on = 1.0f - a.smoothing;
     const long long n8 = (long long)a.rows * (l.ldx / 8);
-    const int rb = (int)(n8 < 148ll * 8 * 256 ? (n8 + 255) / 256 : 148 * 8);
-    int rc = launch_kernel(head_rows_kernel, rb, 256, 0, s, a.x, a.ldx, a.targets, a.rows, a.C, a.V,
-                           xr, l.ldx);
+    const int rb = 1 + (int)(n8 < 148ll * 8 * 256 ? (n8 + 255) / 256 : 148 * 8);
+    int rc = launch_kernel(head_rows_kernel, rb, 256, 0, s, a.x, a.ldx, a.targets, dloss, scale * on,
+                           a.rows, a.C, a.V, xr, l.ldx, top);
     if (rc) return rc;
     const bool one = l.piece >= a.V && l.splits == 1;  // dx straight from one product
     for (int v0 = 0; v0 < a.V; v0 += l.piece) {
@@ -274,9 +310,9 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
         x.V = a.V;
         x.lse = lse;
         x.dloss = dloss;
-        x.scale = scale;
-        x.off = a.V > 1 ? a.smoothing / (float)(a.V - 1) : 0.0f;
-        x.on = 1.0f - a.smoothing;
+        x.top = top;
+        x.on = on;
+        x.off_on = a.V > 1 ? a.smoothing / (float)(a.V - 1) / on : 0.0f;
         GemmPlan plan;
         rc = gemm_make_plan(&plan, xr, l.ldx, 0, w, a.ldw, a.w_mn_major, a.rows, pw, a.C, g, 0,
                             num_sms, &x);
@@ -284,7 +320,7 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
         if ((rc = gemm_run(plan, s)) != 0) return rc;
         if (dx && one) {
             rc = product(gp, l.ldg, 0, w, a.ldw, a.w_mn_major ? 0 : 1, a.rows, a.C, pw, dx, dx_f32,
-                         lddx, 0, num_sms, a.err, s);
+                         lddx, 0, num_sms, a.err, s, top + 1);
             if (rc) return rc;
         } else if (dx) {
             GemmArgs h{};
@@ -307,9 +343,9 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
         if (dw) {
             char* to = reinterpret_cast<char*>(dw) + (a.w_mn_major ? (long long)v0 : v0 * lddw) * es;
             rc = a.w_mn_major ? product(xr, l.ldx, 1, gp, l.ldg, 1, a.C, pw, a.rows, to, dw_f32,
-                                        lddw, accumulate, num_sms, a.err, s)
+                                        lddw, accumulate, num_sms, a.err, s, top + 1)
                               : product(gp, l.ldg, 1, xr, l.ldx, 1, pw, a.C, a.rows, to, dw_f32,
-                                        lddw, accumulate, num_sms, a.err, s);
+                                        lddw, accumulate, num_sms, a.err, s, top + 1);
             if (rc) return rc;
         }
     }
@@ -317,9 +353,11 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
         const long long n = (long long)a.rows * a.C;
         const int blocks = (int)(n < 148ll * 16 * 256 ? (n + 255) / 256 : 148 * 16);
         rc = dx_f32 ? launch_kernel(head_dx_kernel<float>, blocks, 256, 0, s, planes, l.splits,
-                                    a.rows, a.C, l.ldp, reinterpret_cast<float*>(dx), lddx)
+                                    a.rows, a.C, l.ldp, top + 1, reinterpret_cast<float*>(dx),
+                                    lddx)
                     : launch_kernel(head_dx_kernel<bf16>, blocks, 256, 0, s, planes, l.splits,
-                                    a.rows, a.C, l.ldp, reinterpret_cast<bf16*>(dx), lddx);
+                                    a.rows, a.C, l.ldp, top + 1, reinterpret_cast<bf16*>(dx),
+                                    lddx);
     }
     return rc;
 }

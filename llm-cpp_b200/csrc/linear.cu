@@ -159,6 +159,7 @@ struct RowsArgs {
     long long ldx;
     const bf16* w;
     long long ldw;
+    const float* alpha;
     const float* bias;
     int act;
     DropArgs drop;
@@ -173,6 +174,7 @@ struct RowsArgs {
 };
 
 __device__ __forceinline__ void rows_store(const RowsArgs& a, int m, int n, float z) {
+    if (a.alpha) z *= *a.alpha;
     if (a.bias) z += a.bias[n];
     if (a.pre) a.pre[m * a.ld_pre + n] = __float2bfloat16_rn(z);
     float y = z;
@@ -329,10 +331,10 @@ int run_rows(const RowsArgs& a, int w_mn, cudaStream_t s) {
 
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
             int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
-            int* err, cudaStream_t s) {
+            int* err, cudaStream_t s, const float* alpha) {
     if (accumulate && !out_f32) return -1;
     if (M <= kFewRows && !a_mn) {
-        RowsArgs r{A, lda, B, ldb, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo, nullptr, 0,
+        RowsArgs r{A, lda, B, ldb, alpha, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo, nullptr, 0,
                    out, out_f32, ldo, M, N, K};
         return run_rows(r, b_mn, s);
     }
@@ -344,12 +346,13 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
     GemmPlan plan;
     int rc;
     const int per16 = out_f32 ? 4 : 8;
-    if (aligned16(out) && (ldo % per16) == 0 && (N % per16) == 0) {
+    if (!alpha && aligned16(out) && (ldo % per16) == 0 && (N % per16) == 0) {
         g.epi = out_f32 ? kEpiStoreF32 : kEpiStoreBF16;
         g.accumulate = accumulate;
         rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, M, N, K, g, 0, num_sms);
-    } else {  // rows that no 16-byte store reaches, or that end inside one
+    } else {  // scaled, or rows that no 16-byte store reaches or that end inside one
         GemmExt x{};
+        x.alpha = alpha;
         g.epi = kEpiLinear;
         x.out_f32 = out_f32;
         x.resid = accumulate ? out : nullptr;
@@ -365,7 +368,7 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
     if (!a.x || !a.w || !a.out) return -1;
     if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw)) return kBadOperand;
     if (a.M <= kFewRows) {
-        RowsArgs r{a.x, a.ldx, a.w, a.ldw, a.bias, a.act, a.drop, a.resid, a.ldr, a.pre, a.ld_pre,
+        RowsArgs r{a.x, a.ldx, a.w, a.ldw, nullptr, a.bias, a.act, a.drop, a.resid, a.ldr, a.pre, a.ld_pre,
                    a.out, a.out_f32, a.ldo, a.M, a.N, a.K};
         if (r.drop.thr == 0) r.drop.rng = nullptr;
         return run_rows(r, a.w_mn_major, s);

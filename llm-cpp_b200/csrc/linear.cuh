@@ -100,10 +100,10 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
                   int dx_f32, long long lddx, void* dw, int dw_f32, long long lddw, int accumulate,
                   int piece, int num_sms, cudaStream_t s);
 
-// D[M,N] (+)= A B^T on the tcgen05 kernels into bf16 or f32 `out`, any row stride (accumulate:
-// f32 only).
+// D[M,N] (+)= alpha A B^T on the tcgen05 kernels into bf16 or f32 `out`, any row stride (accumulate:
+// f32 only; alpha: device scalar, nullable).
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
             int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
-            int* err, cudaStream_t s);
+            int* err, cudaStream_t s, const float* alpha = nullptr);
 
 }  // namespace llmgpu

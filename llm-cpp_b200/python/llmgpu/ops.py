@@ -285,54 +285,61 @@ def _call(name, device, *args):
         raise KernelError(f"{name} failed with status {rc}")
 
 
-def _device_of(*named):
-    """The device of 2-D CUDA tensors given as (tensor, name) pairs."""
-    for t, name in named:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
-            raise KernelError(f"{name}: a 2-D CUDA tensor is needed")
-    return named[0][0].device
+def _device_of(t, name):
+    """The device of a 2-D CUDA tensor."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
+        raise KernelError(f"{name}: a 2-D CUDA tensor is needed")
+    return t.device
 
 
 def _matrix(t, name, dtypes, rows, cols, device, operand=False):
-    """Checks a 2-D matrix argument and returns its row stride in elements."""
-    if not isinstance(t, torch.Tensor) or t.device != device:
+    """Checks a 2-D matrix argument and returns its address and row stride in elements."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device.index:
         raise KernelError(f"{name}: a tensor on {device} is needed, as the first argument")
     if t.dtype not in dtypes:
         raise KernelError(f"{name}: {t.dtype} is not one of {[str(d) for d in dtypes]}")
     if t.shape != (rows, cols):
         raise KernelError(f"{name}: shape {tuple(t.shape)}, not {(rows, cols)}")
-    sr, sc = t.stride()
+    ld, sc = t.stride()
     if sc != 1 and cols > 1:
         raise KernelError(f"{name}: neighbouring columns are needed")
     if rows <= 1:
-        sr = (cols + 7) // 8 * 8
-    elif sr < cols:
-        raise KernelError(f"{name}: rows overlap (stride {sr} of {cols} columns)")
-    if operand and (t.data_ptr() % 16 or sr % 8) and rows and cols:
-        raise KernelError(f"{name}: rows have to start on 16 bytes (address {t.data_ptr():#x}, "
-                          f"stride {sr})")
-    return sr
+        ld = (cols + 7) // 8 * 8
+    elif ld < cols:
+        raise KernelError(f"{name}: rows overlap (stride {ld} of {cols} columns)")
+    p = t.data_ptr()
+    if operand and (p % 16 or ld % 8) and rows and cols:
+        raise KernelError(f"{name}: rows have to start on 16 bytes (address {p:#x}, stride {ld})")
+    return p, ld
 
 
 def _vector(t, name, dtype, n, device):
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or \
+    """Checks a contiguous vector and returns its address."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device.index or t.dtype != dtype or \
             t.shape != (n,) or not t.is_contiguous():
         raise KernelError(f"{name}: a contiguous {dtype} tensor of {n} on {device} is needed")
+    return t.data_ptr()
 
 
-def _rows(rows, cols, dtype, device):
-    """A matrix whose rows start on 16 bytes."""
-    if cols % 8 == 0:
-        return torch.empty(rows, cols, dtype=dtype, device=device)
-    return torch.empty(rows, (cols + 7) // 8 * 8, dtype=dtype, device=device)[:, :cols]
+def _new(rows, cols, dtype, device):
+    """A new matrix whose rows start on 16 bytes, its address and row stride."""
+    if dtype not in _FLOATS:
+        raise KernelError(f"{dtype} is not one of {[str(d) for d in _FLOATS]}")
+    ld = (cols + 7) // 8 * 8
+    t = torch.empty((rows, ld), dtype=dtype, device=device)
+    p = t.data_ptr()
+    return (t if ld == cols else t[:, :cols]), p, ld
+
+
+def _work(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _drop(p, rng, device):
     if not 0.0 <= p <= 1.0:
         raise KernelError(f"p = {p} is not in [0, 1]")
     if rng is not None:
-        _vector(rng, "rng", torch.int64, 2, device)
-        return rng.data_ptr()
+        return _vector(rng, "rng", torch.int64, 2, device)
     if p > 0.0:
         raise KernelError("dropout needs rng, an int64 tensor (seed, offset) on the device")
     return 0
@@ -344,17 +351,17 @@ def _act(act):
     return ACT[act]
 
 
-def _grad_w(dw, w_mn, rows, cols, device, accumulate, name="dw"):
-    """(dw, row stride): the given weight gradient, or a new one in the weight's layout."""
-    shape = (cols, rows) if w_mn else (rows, cols)
+def _grad_w(dw, w_mn, rows, cols, device, accumulate):
+    """(dw, address, row stride): the given weight gradient, or a new one in the weight's layout."""
+    if w_mn:
+        rows, cols = cols, rows
     if dw is None:
         if accumulate:
-            raise KernelError(f"accumulate: {name} has to be given")
-        dw = _rows(*shape, torch.bfloat16, device)
-    ld = _matrix(dw, name, _FLOATS, *shape, device)
+            raise KernelError("accumulate: dw has to be given")
+        return _new(rows, cols, torch.bfloat16, device)
     if accumulate and dw.dtype != torch.float32:
-        raise KernelError(f"accumulate: {name} has to be f32")
-    return dw, ld
+        raise KernelError("accumulate: dw has to be f32")
+    return (dw, *_matrix(dw, "dw", _FLOATS, rows, cols, device))
 
 
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -366,23 +373,23 @@ def dropout_fwd(x, p, rng, site=0, resid=None, out=None, out_dtype=None):
     given). `rng`: int64 device tensor (seed, offset); `site` tells the dropouts of a step apart.
     The mask depends on (seed, offset + site, row, column) alone and p counts in steps of
     1 / 65536; see llmgpu_op_dropout. `out` may be x or resid."""
-    dev = _device_of((x, "x"))
+    dev = _device_of(x, "x")
     rows, cols = x.shape
-    ldx = _matrix(x, "x", _FLOATS, rows, cols, dev)
+    px, ldx = _matrix(x, "x", _FLOATS, rows, cols, dev)
     prng = _drop(p, rng, dev)
     if not prng:
         raise KernelError("dropout needs rng, an int64 tensor (seed, offset) on the device")
     if out is None:
-        out = _rows(rows, cols, out_dtype or x.dtype, dev)
+        out, po, ldo = _new(rows, cols, out_dtype or x.dtype, dev)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise KernelError(f"out: {out.dtype} is not {out_dtype}")
-    ldo = _matrix(out, "out", _FLOATS, rows, cols, dev)
+    else:
+        po, ldo = _matrix(out, "out", _FLOATS, rows, cols, dev)
     pr = ldr = 0
     if resid is not None:
-        ldr = _matrix(resid, "resid", (out.dtype,), rows, cols, dev)
-        pr = resid.data_ptr()
-    _call("llmgpu_op_dropout", dev, x.data_ptr(), x.dtype == torch.float32, ldx, pr, ldr,
-          out.data_ptr(), out.dtype == torch.float32, ldo, rows, cols, p, prng, site)
+        pr, ldr = _matrix(resid, "resid", (out.dtype,), rows, cols, dev)
+    _call("llmgpu_op_dropout", dev, px, x.dtype == torch.float32, ldx, pr, ldr, po,
+          out.dtype == torch.float32, ldo, rows, cols, p, prng, site)
     return out
 
 
@@ -392,14 +399,17 @@ def dropout_bwd(dy, p, rng, site=0, out=None, out_dtype=None):
 
 
 def _linear_shapes(x, w, w_mn):
-    dev = _device_of((x, "x"), (w, "w"))
+    """(device, M, K, N, address and row stride of x, of w)"""
+    dev = _device_of(x, "x")
+    _device_of(w, "w")
     M, K = x.shape
-    N = w.shape[1] if w_mn else w.shape[0]
+    wr, wc = w.shape
+    N = wc if w_mn else wr
     if N <= 0 or K <= 0:
         raise KernelError(f"an empty product: x {tuple(x.shape)}, w {tuple(w.shape)}")
-    ldx = _matrix(x, "x", _BF16, M, K, dev, operand=True)
-    ldw = _matrix(w, "w", _BF16, K if w_mn else N, N if w_mn else K, dev, operand=True)
-    return dev, M, K, N, ldx, ldw
+    px, ldx = _matrix(x, "x", _BF16, M, K, dev, True)
+    pw, ldw = _matrix(w, "w", _BF16, K if w_mn else N, N if w_mn else K, dev, True)
+    return dev, M, K, N, px, ldx, pw, ldw
 
 
 def linear_fwd(x, w, bias=None, act="none", p=0.0, rng=None, site=0, resid=None, w_mn=False,
@@ -408,26 +418,23 @@ def linear_fwd(x, w, bias=None, act="none", p=0.0, rng=None, site=0, resid=None,
     `w_mn`) are bf16 with rows on 16 bytes, bias [N] f32, act one of ACT, (p, rng, site) as in
     dropout_fwd, resid of the result's type. Returns (y, pre): pre = x w^T + bias in bf16 when
     `save_pre` (linear_bwd needs it unless act is "none"), else None."""
-    dev, M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
+    dev, M, K, N, px, ldx, pw, ldw = _linear_shapes(x, w, w_mn)
     a = _act(act)
     prng = _drop(p, rng, dev)
     pb = pr = pp = ldr = ldp = 0
     if bias is not None:
-        _vector(bias, "bias", torch.float32, N, dev)
-        pb = bias.data_ptr()
+        pb = _vector(bias, "bias", torch.float32, N, dev)
     if out is None:
-        out = _rows(M, N, out_dtype, dev)
-    ldo = _matrix(out, "out", _FLOATS, M, N, dev)
+        out, po, ldo = _new(M, N, out_dtype, dev)
+    else:
+        po, ldo = _matrix(out, "out", _FLOATS, M, N, dev)
     if resid is not None:
-        ldr = _matrix(resid, "resid", (out.dtype,), M, N, dev)
-        pr = resid.data_ptr()
+        pr, ldr = _matrix(resid, "resid", (out.dtype,), M, N, dev)
     pre = None
     if save_pre:
-        pre = _rows(M, N, torch.bfloat16, dev)
-        ldp, pp = (N + 7) // 8 * 8, pre.data_ptr()
-    _call("llmgpu_op_linear_fwd", dev, x.data_ptr(), ldx, w.data_ptr(), ldw, w_mn, pb, a, p, prng,
-          site, pr, ldr, pp, ldp, out.data_ptr(), out.dtype == torch.float32, ldo, M, N, K,
-          _err_word(dev))
+        pre, pp, ldp = _new(M, N, torch.bfloat16, dev)
+    _call("llmgpu_op_linear_fwd", dev, px, ldx, pw, ldw, w_mn, pb, a, p, prng, site, pr, ldr, pp, ldp,
+          po, out.dtype == torch.float32, ldo, M, N, K, _err_word(dev))
     return out, pre
 
 
@@ -438,22 +445,20 @@ def linear_bwd(dy, x, w, pre=None, act="none", p=0.0, rng=None, site=0, w_mn=Fal
     result, with the forward's x, w, pre, act and (p, rng, site); the residual's gradient is dy. dw
     has w's layout, bf16 unless given; `accumulate` adds into the given dw (f32) and dbias. What
     is not needed is None."""
-    dev, M, K, N, ldx, ldw = _linear_shapes(x, w, w_mn)
+    dev, M, K, N, px, ldx, pw, ldw = _linear_shapes(x, w, w_mn)
     a = _act(act)
     prng = _drop(p, rng, dev)
-    lddy = _matrix(dy, "dy", _FLOATS, M, N, dev)
-    pp = ldp = px = lddx = pw = lddw = pb = 0
+    pdy, lddy = _matrix(dy, "dy", _FLOATS, M, N, dev)
+    pp = ldp = pdx = lddx = pdw = lddw = pb = 0
     if act != "none":
         if pre is None:
             raise KernelError(f"act {act!r}: the backward needs pre")
-        ldp, pp = _matrix(pre, "pre", _BF16, M, N, dev), pre.data_ptr()
+        pp, ldp = _matrix(pre, "pre", _BF16, M, N, dev)
     dx = None
     if need_dx:
-        dx = _rows(M, K, dx_dtype, dev)
-        lddx, px = _matrix(dx, "dx", _FLOATS, M, K, dev), dx.data_ptr()
+        dx, pdx, lddx = _new(M, K, dx_dtype, dev)
     if need_dw:
-        dw, lddw = _grad_w(dw, w_mn, N, K, dev, accumulate)
-        pw = dw.data_ptr()
+        dw, pdw, lddw = _grad_w(dw, w_mn, N, K, dev, accumulate)
     else:
         dw = None
     if need_dbias:
@@ -461,24 +466,22 @@ def linear_bwd(dy, x, w, pre=None, act="none", p=0.0, rng=None, site=0, w_mn=Fal
             if accumulate:
                 raise KernelError("accumulate: dbias has to be given")
             dbias = torch.empty(N, dtype=torch.float32, device=dev)
-        _vector(dbias, "dbias", torch.float32, N, dev)
-        pb = dbias.data_ptr()
+        pb = _vector(dbias, "dbias", torch.float32, N, dev)
     else:
         dbias = None
-    work = torch.empty(load().llmgpu_op_linear_bwd_work(M, N, K), dtype=torch.uint8, device=dev)
-    _call("llmgpu_op_linear_bwd", dev, dy.data_ptr(), dy.dtype == torch.float32, lddy, x.data_ptr(),
-          ldx, w.data_ptr(), ldw, w_mn, pp, ldp, a, p, prng, site, px, dx_dtype == torch.float32,
-          lddx, pw, need_dw and dw.dtype == torch.float32, lddw, pb, accumulate, M, N, K,
-          work.data_ptr(), _err_word(dev))
+    work = _work(load().llmgpu_op_linear_bwd_work(M, N, K), dev)
+    _call("llmgpu_op_linear_bwd", dev, pdy, dy.dtype == torch.float32, lddy, px, ldx, pw, ldw, w_mn,
+          pp, ldp, a, p, prng, site, pdx, dx_dtype == torch.float32, lddx, pdw,
+          need_dw and dw.dtype == torch.float32, lddw, pb, accumulate, M, N, K, work.data_ptr(),
+          _err_word(dev))
     return dx, dw, dbias
 
 
 def _head_args(x, w, targets, smoothing, w_mn):
-    dev, rows, C, V, ldx, ldw = _linear_shapes(x, w, w_mn)
     if not 0.0 <= smoothing < 1.0:
         raise KernelError(f"smoothing = {smoothing} is not in [0, 1)")
-    _vector(targets, "targets", torch.int32, rows, dev)
-    return dev, rows, C, V, ldx, ldw
+    shapes = _linear_shapes(x, w, w_mn)
+    return shapes, _vector(targets, "targets", torch.int32, shapes[1], shapes[0])
 
 
 def linear_cross_entropy_fwd(x, w, targets, smoothing=0.0, w_mn=False):
@@ -486,13 +489,12 @@ def linear_cross_entropy_fwd(x, w, targets, smoothing=0.0, w_mn=False):
     f32 [rows]. x [rows, C] and w [V, C] (or [C, V] with `w_mn`) are bf16 with rows on 16 bytes,
     targets int32 [rows]; a target outside [0, V) leaves its row out (loss 0). `smoothing` s:
     targets of 1 - s and s / (V - 1) elsewhere, in the loss as in the gradient."""
-    dev, rows, C, V, ldx, ldw = _head_args(x, w, targets, smoothing, w_mn)
+    (dev, rows, C, V, px, ldx, pw, ldw), pt = _head_args(x, w, targets, smoothing, w_mn)
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     lse = torch.empty(rows, dtype=torch.float32, device=dev)
-    work = torch.empty(load().llmgpu_op_linear_ce_fwd_work(rows, V), dtype=torch.uint8, device=dev)
-    _call("llmgpu_op_linear_ce_fwd", dev, x.data_ptr(), ldx, w.data_ptr(), ldw, w_mn,
-          targets.data_ptr(), rows, C, V, smoothing, loss.data_ptr(), lse.data_ptr(),
-          work.data_ptr(), _err_word(dev))
+    work = _work(load().llmgpu_op_linear_ce_fwd_work(rows, V), dev)
+    _call("llmgpu_op_linear_ce_fwd", dev, px, ldx, pw, ldw, w_mn, pt, rows, C, V, smoothing,
+          loss.data_ptr(), lse.data_ptr(), work.data_ptr(), _err_word(dev))
     return loss, lse
 
 
@@ -503,27 +505,23 @@ def linear_cross_entropy_bwd(x, w, targets, lse, dloss=None, scale=1.0, smoothin
     the forward's arguments and its lse. The logits are formed again in pieces of `piece` columns of
     the vocabulary (a multiple of 256; 0: chosen by the library), which bounds the workspace. dw
     has w's layout, bf16 unless given; `accumulate` adds into the given f32 dw."""
-    dev, rows, C, V, ldx, ldw = _head_args(x, w, targets, smoothing, w_mn)
+    (dev, rows, C, V, px, ldx, pw, ldw), pt = _head_args(x, w, targets, smoothing, w_mn)
     if piece < 0 or piece % 256:
         raise KernelError(f"piece = {piece} is not a multiple of 256")
-    _vector(lse, "lse", torch.float32, rows, dev)
-    pd = px = lddx = pw = lddw = 0
+    pl = _vector(lse, "lse", torch.float32, rows, dev)
+    pd = pdx = lddx = pdw = lddw = 0
     if dloss is not None:
-        _vector(dloss, "dloss", torch.float32, rows, dev)
-        pd = dloss.data_ptr()
+        pd = _vector(dloss, "dloss", torch.float32, rows, dev)
     dx = None
     if need_dx:
-        dx = _rows(rows, C, dx_dtype, dev)
-        lddx, px = _matrix(dx, "dx", _FLOATS, rows, C, dev), dx.data_ptr()
+        dx, pdx, lddx = _new(rows, C, dx_dtype, dev)
     if need_dw:
-        dw, lddw = _grad_w(dw, w_mn, V, C, dev, accumulate)
-        pw = dw.data_ptr()
+        dw, pdw, lddw = _grad_w(dw, w_mn, V, C, dev, accumulate)
     else:
         dw = None
-    work = torch.empty(load().llmgpu_op_linear_ce_bwd_work(rows, C, V, piece), dtype=torch.uint8,
-                       device=dev)
-    _call("llmgpu_op_linear_ce_bwd", dev, x.data_ptr(), ldx, w.data_ptr(), ldw, w_mn,
-          targets.data_ptr(), lse.data_ptr(), pd, scale, rows, C, V, smoothing, px,
-          dx_dtype == torch.float32, lddx, pw, need_dw and dw.dtype == torch.float32, lddw,
-          accumulate, piece, work.data_ptr(), _err_word(dev))
+    work = _work(load().llmgpu_op_linear_ce_bwd_work(rows, C, V, piece), dev)
+    _call("llmgpu_op_linear_ce_bwd", dev, px, ldx, pw, ldw, w_mn, pt, pl, pd, scale, rows, C, V,
+          smoothing, pdx, dx_dtype == torch.float32, lddx, pdw,
+          need_dw and dw.dtype == torch.float32, lddw, accumulate, piece, work.data_ptr(),
+          _err_word(dev))
     return dx, dw

@@ -430,6 +430,28 @@ def test_loss_head_extreme_logits(cuda):
     assert bool(torch.isfinite(dx.float()).all())
 
 
+def test_loss_head_row_weights(cuda):
+    """Weights of any kind: all zero; signs and sizes mixed over 60 binades; one that is infinite,
+    which reaches its own row of dx (and dw) alone."""
+    from llmgpu import ops
+    x, w, t, _ = _head_case(cuda, 96, 64, 400, False, False, 8)
+    _, lse = ops.linear_cross_entropy_fwd(x, w, t)
+    dx, dw = ops.linear_cross_entropy_bwd(x, w, t, lse, torch.zeros(96, device=cuda))
+    assert not dx.any() and not dw.any()
+    g = torch.Generator().manual_seed(1)
+    d = (torch.randn(96, generator=g) * torch.exp2(torch.randint(-30, 30, (96,), generator=g))).to(cuda)
+    _, _, _, _, wx, ex, ww, ew = _head_want(x, w, t, d, 2.0, 0.0, False)
+    dx, dw = ops.linear_cross_entropy_bwd(x, w, t, lse, d, 2.0)
+    _close(dx, wx, ex + H16 * (wx.abs() + ex), "dx")
+    _close(dw, ww, ew + H16 * (ww.abs() + ew), "dw")
+    one = torch.ones(96, device=cuda)
+    dx, _ = ops.linear_cross_entropy_bwd(x, w, t, lse, one)
+    one[17] = float("inf")
+    ix, _ = ops.linear_cross_entropy_bwd(x, w, t, lse, one)
+    keep = torch.arange(96, device=cuda) != 17
+    assert torch.equal(ix[keep], dx[keep]) and not bool(torch.isfinite(ix[17].float()).all())
+
+
 def test_loss_head_no_rows(cuda):
     from llmgpu import ops
     x, w = torch.empty(0, 16, dtype=BF, device=cuda), torch.ones(40, 16, dtype=BF, device=cuda)
