@@ -953,12 +953,14 @@ __device__ __forceinline__ void head_stats_tile(const GemmArgs& a, const GemmExt
             tmem_ld_32x32b_x32(tbase + (uint32_t)(c * 32), r);
             tmem_ld_wait();
             const int nv = min(32, a.N - col0);
+            if (nv < 32) {  // the vocabulary's last columns
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (j >= nv) r[j] = 0xff800000u;
+            }
             float mc = ninf;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                if (j >= nv) r[j] = 0xff800000u;
-                mc = fmaxf(mc, __uint_as_float(r[j]));
-            }
+            for (int j = 0; j < 32; ++j) mc = fmaxf(mc, __uint_as_float(r[j]));
             if (x.zsum) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) zs += j < nv ? __uint_as_float(r[j]) : 0.0f;
@@ -976,9 +978,15 @@ __device__ __forceinline__ void head_stats_tile(const GemmArgs& a, const GemmExt
                 s = s == 0.0f ? 0.0f : s * ex2_approx((m - mc) * kLog2e);
                 m = mc;
             }
-            const float ml = m == ninf ? 0.0f : m * kLog2e;
+            const float ml = m == ninf ? 0.0f : -m * kLog2e;
+            float2 s2 = make_float2(s, 0.0f);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s += ex2_approx(fmaf(__uint_as_float(r[j]), kLog2e, -ml));
+            for (int j = 0; j < 32; j += 2) {
+                const float2 e = ffma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                       make_float2(kLog2e, kLog2e), make_float2(ml, ml));
+                s2 = fadd2(s2, make_float2(ex2_approx(e.x), ex2_approx(e.y)));
+            }
+            s = s2.x + s2.y;
         }
         if (row < a.M) {
             const long long at = (long long)((n0 + c4 * 32) >> 7) * a.M + row;
@@ -1004,8 +1012,9 @@ __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt&
     const int row = row0 + lane;
     const int t = row < a.M ? x.targets[row] : -1;
     const bool counts = t >= 0 && t < x.V;
-    const float coef = counts && x.dloss ? x.dloss[row] / x.top[0] : 1.0f;
-    const float ll = counts ? fmaf(x.lse[row], kLog2e, log2f(x.on)) : 0.0f;
+    // rows left out: weight 0 (their rows of the operand are zeros, so the logits are finite)
+    const float coef = !counts ? 0.0f : x.dloss ? x.dloss[row] / x.top[0] : 1.0f;
+    const float ll = counts ? -fmaf(x.lse[row], kLog2e, log2f(x.on)) : 0.0f;
 #pragma unroll 1
     for (int c = c_begin; c < c_end; c += 2) {
         const int col0 = n0 + c * 32;
@@ -1018,6 +1027,7 @@ __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt&
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
         const int tj = t - (x.v0 + col0);
+        const bool here = __any_sync(0xffffffffu, tj >= 0 && tj < 64);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -1025,16 +1035,18 @@ __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt&
                 uint32_t o[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float g[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int j = 8 * ch + 2 * k + i;
-                        const float p =
-                            ex2_approx(fmaf(__uint_as_float(r[h][j]), kLog2e, -ll));
-                        const float y = (32 * h + j == tj) ? 1.0f : x.off_on;
-                        g[i] = counts ? coef * (p - y) : 0.0f;
+                    const int j = 8 * ch + 2 * k;
+                    const float2 e = ffma2(
+                        make_float2(__uint_as_float(r[h][j]), __uint_as_float(r[h][j + 1])),
+                        make_float2(kLog2e, kLog2e), make_float2(ll, ll));
+                    float2 g = fadd2(make_float2(ex2_approx(e.x), ex2_approx(e.y)),
+                                     make_float2(-x.off_on, -x.off_on));
+                    if (here) {  // some row's target lies in these 64 columns
+                        if (32 * h + j == tj) g.x += x.off_on - 1.0f;
+                        if (32 * h + j + 1 == tj) g.y += x.off_on - 1.0f;
                     }
-                    o[k] = pack_bf16x2(g[0], g[1]);
+                    g = fmul2(g, make_float2(coef, coef));
+                    o[k] = pack_bf16x2(g.x, g.y);
                 }
                 *reinterpret_cast<uint4*>(box + box_off_f32(lane, 4 * h + ch)) =
                     make_uint4(o[0], o[1], o[2], o[3]);

@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "linear.cuh"
+#include "rowio.cuh"
 
 namespace llmgpu {
 
@@ -39,15 +40,27 @@ __global__ void __launch_bounds__(1024) head_merge_kernel(const float2* __restri
     const float ninf = __int_as_float(0xff800000);
     float m = ninf, s = 0.0f, z = 0.0f;
     if (row < rows) {
-        for (int p = w; p < slots; p += 32) {
-            const float2 q = part[(long long)p * rows + row];
-            const float mn = fmaxf(m, q.x);
+        constexpr int U = 8;  // slots in flight
+        for (int p0 = w; p0 < slots; p0 += 32 * U) {
+            float2 q[U];
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int p = p0 + 32 * u;
+                q[u] = p < slots ? part[(long long)p * rows + row] : make_float2(ninf, 0.0f);
+            }
+            if (zsum)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (p0 + 32 * u < slots) z += zsum[(long long)(p0 + 32 * u) * rows + row];
+#pragma unroll
+            for (int u = 0; u < U; ++u) mn = fmaxf(mn, q[u].x);
             // a side that holds nothing (sum 0) adds 0; an unordered one passes NaN on
-            const float a = s == 0.0f ? 0.0f : s * ex2_approx((m - mn) * kLog2);
-            const float b = q.y == 0.0f ? 0.0f : q.y * ex2_approx((q.x - mn) * kLog2);
+            s = s == 0.0f ? 0.0f : s * ex2_approx((m - mn) * kLog2);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                s += q[u].y == 0.0f ? 0.0f : q[u].y * ex2_approx((q[u].x - mn) * kLog2);
             m = mn;
-            s = a + b;
-            if (zsum) z += zsum[(long long)p * rows + row];
         }
     }
     sm[w][lane] = m;
@@ -135,25 +148,67 @@ __global__ void __launch_bounds__(256) head_rows_kernel(const bf16* __restrict__
     }
 }
 
-// dx = alpha times the sum of the planes [n][rows][ldp], in their order.
+// dx = alpha times the sum of the planes [n][rows][ldp], in their order; a thread takes 4 columns,
+// with the planes' loads in flight together. The positions of a thread lie (dr, dc) rows and
+// groups of 4 apart. Bound by memory.
 template <typename T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ planes, int n,
-                                                      int rows, int C, int ldp,
+                                                      uint32_t rows, int C, int ldp, uint32_t dr,
+                                                      uint32_t dc, int vec,
                                                       const float* __restrict__ alpha,
                                                       T* __restrict__ dx, long long lddx) {
     pdl_enter();
     const float f = *alpha;
-    const long long total = (long long)rows * C, plane = (long long)rows * ldp;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        const int row = (int)(i / C), c = (int)(i - (long long)row * C);
-        const float* p = planes + (long long)row * ldp + c;
-        float v = p[0];
-        for (int k = 1; k < n; ++k) v += p[k * plane];
-        if constexpr (sizeof(T) == 4)
-            dx[row * lddx + c] = v * f;
-        else
-            dx[row * lddx + c] = __float2bfloat16_rn(v * f);
+    const uint32_t n4 = (uint32_t)ldp >> 2;
+    const long long plane = (long long)rows * ldp;
+    const uint32_t first = blockIdx.x * 256u + threadIdx.x;
+    uint32_t row = first / n4, c4 = first - row * n4;
+    while (row < rows) {
+        const float* p = planes + (long long)row * ldp + 4 * c4;
+        float4 q[kMaxSplits];
+#pragma unroll
+        for (int k = 0; k < kMaxSplits; ++k)
+            if (k < n) q[k] = *reinterpret_cast<const float4*>(p + k * plane);
+        float4 v = q[0];
+#pragma unroll
+        for (int k = 1; k < kMaxSplits; ++k)
+            if (k < n) {
+                v.x += q[k].x;
+                v.y += q[k].y;
+                v.z += q[k].z;
+                v.w += q[k].w;
+            }
+        const float w[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        T* o = dx + row * lddx + 4 * c4;
+        if (vec && 4 * (int)c4 + 4 <= C) {
+            if constexpr (sizeof(T) == 4)
+                *reinterpret_cast<float4*>(o) = make_float4(w[0], w[1], w[2], w[3]);
+            else
+                *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
+        } else {
+            for (int j = 0; j < 4; ++j)
+                if (4 * (int)c4 + j < C) o[j] = from_f32<T>(w[j]);
+        }
+        row += dr;
+        c4 += dc;
+        if (c4 >= n4) {
+            c4 -= n4;
+            ++row;
+        }
     }
+}
+
+template <typename T>
+int launch_dx(const float* planes, int n, int rows, int C, int ldp, const float* alpha, void* dx,
+              long long lddx, cudaStream_t s) {
+    const uint32_t n4 = (uint32_t)ldp / 4;
+    const long long items = (long long)rows * n4;
+    const long long most = 148 * 8;
+    const uint32_t blocks = (uint32_t)((items + 255) / 256 < most ? (items + 255) / 256 : most);
+    const uint32_t step = blocks * 256;
+    const int vec = (reinterpret_cast<uintptr_t>(dx) % (4 * sizeof(T))) == 0 && lddx % 4 == 0;
+    return launch_kernel(head_dx_kernel<T>, (int)blocks, 256, 0, s, planes, n, (uint32_t)rows, C, ldp,
+                         step / n4, step % n4, vec, alpha, (T*)dx, lddx);
 }
 
 long long waves(long long tiles) { return (tiles + kPairSlots - 1) / kPairSlots; }
@@ -350,14 +405,8 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
         }
     }
     if (dx && !one) {
-        const long long n = (long long)a.rows * a.C;
-        const int blocks = (int)(n < 148ll * 16 * 256 ? (n + 255) / 256 : 148 * 16);
-        rc = dx_f32 ? launch_kernel(head_dx_kernel<float>, blocks, 256, 0, s, planes, l.splits,
-                                    a.rows, a.C, l.ldp, top + 1, reinterpret_cast<float*>(dx),
-                                    lddx)
-                    : launch_kernel(head_dx_kernel<bf16>, blocks, 256, 0, s, planes, l.splits,
-                                    a.rows, a.C, l.ldp, top + 1, reinterpret_cast<bf16*>(dx),
-                                    lddx);
+        rc = dx_f32 ? launch_dx<float>(planes, l.splits, a.rows, a.C, l.ldp, top + 1, dx, lddx, s)
+                    : launch_dx<bf16>(planes, l.splits, a.rows, a.C, l.ldp, top + 1, dx, lddx, s);
     }
     return rc;
 }

@@ -5,6 +5,7 @@
 
 #include "common.cuh"
 #include "philox.cuh"
+#include "rowio.cuh"
 
 namespace llmgpu {
 
@@ -26,60 +27,47 @@ int dz_groups(int M, int N) {
     return gy < 1 ? 1 : gy;
 }
 
-__device__ __forceinline__ float act_grad(int act, float z) {
-    switch (act) {
-        case kActRelu:
-            return z > 0.0f ? 1.0f : 0.0f;
-        case kActGelu: {
-            // gelu(z) = z h, h = sigmoid(2u): h + z h (1 - h) 2u'
-            const float z2 = z * z;
-            const float t = 1.5957691216f * z * fmaf(0.044715f, z2, 1.0f);
-            const float h = rcp_approx(1.0f + ex2_approx(-t * 1.4426950408889634f));
-            return h + z * h * (1.0f - h) * 1.5957691216f * fmaf(0.134145f, z2, 1.0f);
+// Derivatives of a pair of activations, from the same sigmoid as the forward's: gelu(z) = z h with
+// h = sigmoid(2u): h + z h (1 - h) 2u'; silu: h (1 + z (1 - h)).
+template <int ACT>
+__device__ __forceinline__ float2 act_grad_pair(float2 z) {
+    constexpr float kLog2 = 1.4426950408889634f;
+    if constexpr (ACT == kActRelu) {
+        return make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
+    } else if constexpr (ACT == kActGelu || ACT == kActSilu) {
+        const float2 one = make_float2(1.0f, 1.0f);
+        const float2 z2 = fmul2(z, z);
+        float2 t;
+        if constexpr (ACT == kActGelu) {
+            constexpr float c = -1.5957691216f * kLog2;
+            t = fmul2(ffma2(z2, make_float2(c * 0.044715f, c * 0.044715f), make_float2(c, c)), z);
+        } else {
+            t = fmul2(z, make_float2(-kLog2, -kLog2));
         }
-        case kActSilu: {
-            const float h = rcp_approx(1.0f + ex2_approx(-z * 1.4426950408889634f));
-            return h * (1.0f + z * (1.0f - h));
+        const float2 d = fadd2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), one);
+        const float2 h = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+        const float2 g = ffma2(h, make_float2(-1.0f, -1.0f), one);  // 1 - h
+        if constexpr (ACT == kActGelu) {
+            constexpr float k = 1.5957691216f;
+            const float2 q =
+                fmul2(ffma2(z2, make_float2(k * 0.134145f, k * 0.134145f), make_float2(k, k)), z);
+            return ffma2(fmul2(h, g), q, h);
+        } else {
+            return fmul2(h, ffma2(z, g, one));
         }
-        default:
-            return 1.0f;
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        if (vec) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = bf16_lo(w[i]);
-                v[2 * i + 1] = bf16_hi(w[i]);
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.0f;
     } else {
-        if (vec) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0];
-            const float4 b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+        return make_float2(1.0f, 1.0f);
     }
 }
 
-// dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable). `vec`:
-// rows of dy and pre start on 16 bytes.
-template <typename T>
+// dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable). `vec`: rows
+// of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a time, their
+// loads in flight together as raw words: bound by memory at 8192 x 4096 bf16 (201 MB).
+constexpr int kDzInFlight = 4;
+template <typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long lddy,
                                                         const bf16* __restrict__ pre,
-                                                        long long ld_pre, int act, DropArgs drop,
+                                                        long long ld_pre, DropArgs drop,
                                                         bf16* __restrict__ dz, long long ldz,
                                                         float* __restrict__ part, int M, int N,
                                                         int vec) {
@@ -87,37 +75,62 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
     const int lane = threadIdx.x & 31, wr = threadIdx.x >> 5;
     const int col = blockIdx.x * kDzCols + lane * 8;
     const int n = min(8, N - col);
-    float sum[8];
+    float2 sum[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+    for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.0f, 0.0f);
     if (n > 0) {
         const bool v8 = vec && n == 8;
-        const DropKeys key = drop.rng ? drop_keys(drop.rng, drop.site) : DropKeys{};
-        for (int row = blockIdx.y * kDzRows + wr; row < M; row += gridDim.y * kDzRows) {
-            float v[8], z[8];
-            load8(dy + row * lddy + col, n, v8, v);
-            if (act != kActNone) load8(pre + row * ld_pre + col, n, v8, z);
-            if (drop.rng) {
-                drop_apply8(key, (uint32_t)col >> 3, (uint32_t)row, drop.thr, drop.scale, v);
-            }
-            if (act != kActNone) {
+        DropKeys key;
+        if constexpr (DROP) key = drop_keys(drop.rng, drop.site);
+        const int step = gridDim.y * kDzRows;
+        for (long long row0 = blockIdx.y * kDzRows + wr; row0 < M; row0 += kDzInFlight * step) {
+            Raw8<T> dr[kDzInFlight];
+            Raw8<bf16> pr[kDzInFlight];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= act_grad(act, z[i]);
+            for (int u = 0; u < kDzInFlight; ++u) {
+                const long long row = row0 + u * step;
+                if (row >= M) break;
+                if (v8) {
+                    load_raw(dy + row * lddy + col, dr[u]);
+                    if (ACT != kActNone) load_raw(pre + row * ld_pre + col, pr[u]);
+                } else {
+                    load_raw_n(dy + row * lddy + col, n, dr[u]);
+                    if (ACT != kActNone) load_raw_n(pre + row * ld_pre + col, n, pr[u]);
+                }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += v[i];
-            if (dz) {
+            for (int u = 0; u < kDzInFlight; ++u) {
+                const long long row = row0 + u * step;
+                if (row >= M) break;
+                float v[8];
+                raw_f32(dr[u], v);
+                if constexpr (DROP)
+                    drop_apply8(key, (uint32_t)col >> 3, (uint32_t)row, drop.thr, drop.scale, v);
+                if constexpr (ACT != kActNone) {
+                    float z[8];
+                    raw_f32(pr[u], z);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 y = fmul2(make_float2(v[2 * i], v[2 * i + 1]),
+                                               act_grad_pair<ACT>(make_float2(z[2 * i], z[2 * i + 1])));
+                        v[2 * i] = y.x;
+                        v[2 * i + 1] = y.y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = fadd2(sum[i], make_float2(v[2 * i], v[2 * i + 1]));
                 // columns past N, up to the padded stride, are written as zeros
-                *reinterpret_cast<uint4*>(dz + row * ldz + col) =
-                    make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                               pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+                if (dz) store8(dz + row * ldz + col, v);
             }
         }
     }
     if (!part) return;
     __shared__ float red[kDzRows][kDzCols];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) red[wr][lane * 8 + i] = sum[i];
+    for (int i = 0; i < 4; ++i) {
+        red[wr][lane * 8 + 2 * i] = sum[i].x;
+        red[wr][lane * 8 + 2 * i + 1] = sum[i].y;
+    }
     __syncthreads();
     const int c = blockIdx.x * kDzCols + threadIdx.x;
     if (c < N) {
@@ -125,6 +138,28 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
 #pragma unroll
         for (int r = 0; r < kDzRows; ++r) t += red[r][threadIdx.x];
         part[(long long)blockIdx.y * N + c] = t;
+    }
+}
+
+template <typename T, int ACT>
+int launch_dz_act(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* sums, int vec,
+                  cudaStream_t s) {
+    return launch_kernel(drop.rng ? linear_dz_kernel<T, ACT, true> : linear_dz_kernel<T, ACT, false>,
+                         grid, 256, 0, s, (const T*)a.dy, a.lddy, a.pre, a.ld_pre, drop, to,
+                         ceil8(a.N), sums, a.M, a.N, vec);
+}
+template <typename T>
+int launch_dz(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* sums, int vec,
+              cudaStream_t s) {
+    switch (a.act) {
+        case kActRelu:
+            return launch_dz_act<T, kActRelu>(a, drop, grid, to, sums, vec, s);
+        case kActGelu:
+            return launch_dz_act<T, kActGelu>(a, drop, grid, to, sums, vec, s);
+        case kActSilu:
+            return launch_dz_act<T, kActSilu>(a, drop, grid, to, sums, vec, s);
+        default:
+            return launch_dz_act<T, kActNone>(a, drop, grid, to, sums, vec, s);
     }
 }
 
@@ -441,13 +476,8 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
         const dim3 grid((a.N + kDzCols - 1) / kDzCols, groups);
         bf16* to = need_dz ? buf : nullptr;
         float* sums = a.dbias ? part : nullptr;
-        int rc;
-        if (a.dy_f32)
-            rc = launch_kernel(linear_dz_kernel<float>, grid, 256, 0, s, (const float*)a.dy, a.lddy,
-                               a.pre, a.ld_pre, a.act, drop, to, ceil8(a.N), sums, a.M, a.N, vec);
-        else
-            rc = launch_kernel(linear_dz_kernel<bf16>, grid, 256, 0, s, (const bf16*)a.dy, a.lddy,
-                               a.pre, a.ld_pre, a.act, drop, to, ceil8(a.N), sums, a.M, a.N, vec);
+        int rc = a.dy_f32 ? launch_dz<float>(a, drop, grid, to, sums, vec, s)
+                          : launch_dz<bf16>(a, drop, grid, to, sums, vec, s);
         if (rc) return rc;
         if (a.dbias) {
             rc = launch_kernel(linear_db_kernel, (a.N + 31) / 32, 1024, 0, s, part, groups, a.N,
