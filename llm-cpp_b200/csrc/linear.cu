@@ -63,7 +63,7 @@ __device__ __forceinline__ float2 act_grad_pair(float2 z) {
 // dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable). `vec`: rows
 // of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a time, their
 // loads in flight together as raw words: bound by memory at 8192 x 4096 bf16 (201 MB).
-constexpr int kDzInFlight = 4;
+constexpr int kDzInFlight = 2;
 template <typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long lddy,
                                                         const bf16* __restrict__ pre,
@@ -353,8 +353,8 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_mn_kernel(const Rows
 template <int MR>
 int launch_rows(const RowsArgs& a, int w_mn, cudaStream_t s) {
     if (w_mn)
-        return launch_kernel(linear_rows_mn_kernel<MR>, (a.N + 31) / 32, kRowsThreads, 0, s, a);
-    return launch_kernel(linear_rows_kernel<MR>, (a.N + 7) / 8, 256, 0, s, a);
+        return launch_kernel_pdl(linear_rows_mn_kernel<MR>, (a.N + 31) / 32, kRowsThreads, 0, s, a);
+    return launch_kernel_pdl(linear_rows_kernel<MR>, (a.N + 7) / 8, 256, 0, s, a);
 }
 int run_rows(const RowsArgs& a, int w_mn, cudaStream_t s) {
     if (a.M == 1) return launch_rows<1>(a, w_mn, s);

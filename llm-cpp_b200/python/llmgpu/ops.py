@@ -268,13 +268,16 @@ def check_device(device="cuda"):
             raise KernelError(f"device error code {code}")
 
 
+_fns = {}
 # the raw handle of a device's current stream, without making a Stream object (3 us a call)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _call(name, device, *args):
     """The C entry point on the current stream of `device`."""
-    fn = getattr(load(), name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
     i = device.index
     if i == torch.cuda.current_device():
         rc = fn(*args, _raw_stream(i))
@@ -326,9 +329,8 @@ def _new(rows, cols, dtype, device):
     if dtype not in _FLOATS:
         raise KernelError(f"{dtype} is not one of {[str(d) for d in _FLOATS]}")
     ld = (cols + 7) // 8 * 8
-    t = torch.empty((rows, ld), dtype=dtype, device=device)
-    p = t.data_ptr()
-    return (t if ld == cols else t[:, :cols]), p, ld
+    t = torch.empty_strided((rows, cols), (ld, 1), dtype=dtype, device=device)
+    return t, t.data_ptr(), ld
 
 
 def _work(nbytes, device):
