@@ -29,7 +29,6 @@ constexpr int BK = 64;
 constexpr int kGemmThreads = 256;
 // CTA-pair kernel: warp 0 TMA, warp 1 MMA, warps 4..11 epilogue (two warps per TMEM lane
 // quarter, each draining half of a tile's columns)
-constexpr int kPairThreads = 384;
 constexpr int kPairEpiWarps = 8;
 constexpr int kChainBlocks = 8;  // k-blocks of an accumulator chain (512 products), see chain_sum
 constexpr int kGroupM = 16;  // tile raster: groups of 16 m-blocks share B tiles in L2
@@ -237,7 +236,6 @@ __device__ __forceinline__ void epi_store(const GemmArgs& a, int row, int col0, 
 // epi_store.
 constexpr int kEpiSlotBytes = 4096;
 constexpr int kEpiStageBytes = 4 * 2 * kEpiSlotBytes;
-constexpr int kPairEpiStageBytes = kPairEpiWarps * 2 * kEpiSlotBytes;
 
 // byte offset of 16-byte chunk `ch` of row r in a box of 128-byte rows (fp32, 128-byte
 // swizzle: chunk ^= row % 8) or 64-byte rows (bf16, 64-byte swizzle: chunk ^= (row / 2) % 4)
@@ -645,8 +643,8 @@ __device__ __forceinline__ void linear_act_drop(const GemmExt& x, const DropKey&
 }
 
 // Outputs (and a residual) of any stride and alignment, and the rare pairs of them that the boxes
-// below do not cover: a lane's 32 columns are turned through the warp's 8 KB of shared memory (32
-// rows of 33 floats), so that every access to global memory is 32 neighbouring columns of a row.
+// below do not cover: a lane's 32 columns are turned through 4 KB of the warp's shared memory (32
+// rows of 32 floats, column j of row i at j ^ i), so that every access to global memory is 32 neighbouring columns of a row.
 __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const GemmExt& x,
                                                    const DropKey& key, uint32_t tbase, int row0,
                                                    int n0, int lane, EpiWarp& w, int c_begin,
@@ -667,24 +665,24 @@ __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const Gemm
         linear_bias(a, x, col0, lane, r, v);
         if (a.aux) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = v[j];
+            for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = v[j];
             __syncwarp();
             __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.aux) + row0 * a.ld_aux + col;
             if (in)
                 for (int i = 0; i < nrows; ++i)
-                    p[i * a.ld_aux] = __float2bfloat16_rn(tile[i * 33 + lane]);
+                    p[i * a.ld_aux] = __float2bfloat16_rn(tile[i * 32 + (lane ^ i)]);
             __syncwarp();
         }
         linear_act_drop(x, key, col0, row0 + lane, v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = v[j];
+        for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = v[j];
         __syncwarp();
         if (in && x.out_f32) {
             float* p = reinterpret_cast<float*>(a.out) + row0 * a.ldo + col;
             const float* q = reinterpret_cast<const float*>(x.resid) + row0 * x.ldr + col;
 #pragma unroll 4
             for (int i = 0; i < nrows; ++i) {
-                float o = tile[i * 33 + lane];
+                float o = tile[i * 32 + (lane ^ i)];
                 if (x.resid) o += q[i * x.ldr];
                 p[i * a.ldo] = o;
             }
@@ -694,7 +692,7 @@ __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const Gemm
                 reinterpret_cast<const __nv_bfloat16*>(x.resid) + row0 * x.ldr + col;
 #pragma unroll 4
             for (int i = 0; i < nrows; ++i) {
-                float o = tile[i * 33 + lane];
+                float o = tile[i * 32 + (lane ^ i)];
                 if (x.resid) o += __bfloat162float(q[i * x.ldr]);
                 p[i * a.ldo] = __float2bfloat16_rn(o);
             }
@@ -716,6 +714,7 @@ __device__ __forceinline__ int linear_box_end(const GemmArgs& a, const GemmExt& 
 
 // The residual's first two units of a tile, loaded before the accumulator is ready (see
 // epilogue_prefetch): f32 units are 32 columns, bf16 units 64, 4 KB each.
+template <int SLOTS>
 __device__ __forceinline__ void linear_prefetch(const GemmArgs& a, const GemmExt& x,
                                                 const CUtensorMap* tmX, int row0, int n0, int lane,
                                                 EpiWarp& w, int c_begin, int c_end) {
@@ -725,14 +724,16 @@ __device__ __forceinline__ void linear_prefetch(const GemmArgs& a, const GemmExt
     if (lane == 0 && ce > c_begin) {
         bulk_wait_group_read<0>();
         epi_load_unit(tmX, w, w.slot, n0 + c_begin * 32, row0);
-        if (c_begin + u < ce) epi_load_unit(tmX, w, w.slot ^ 1, n0 + (c_begin + u) * 32, row0);
+        if (SLOTS > 1 && c_begin + u < ce)
+            epi_load_unit(tmX, w, w.slot ^ 1, n0 + (c_begin + u) * 32, row0);
     }
     __syncwarp();
 }
 
 // resid + drop(act(acc + bias)) through swizzled boxes and bulk stores: f32 outputs 32 columns at a
 // time, bf16 outputs 64 (with `pre` beside them, 32 of each). A residual arrives by bulk loads
-// in the box that it is combined in, one unit ahead.
+// in the box that it is combined in, one unit ahead where a warp has two boxes (SLOTS).
+template <int SLOTS>
 __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt& x,
                                                 const DropKey& key, const CUtensorMap* tmO,
                                                 const CUtensorMap* tmX, uint32_t tbase, int row0,
@@ -745,12 +746,13 @@ __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt
     for (int c = c_begin; c < ce; c += u) {
         if (res) {
             // the next unit's residual goes into the box the previous unit stored from
-            if (c > c_begin && c + u < ce && lane == 0) {
+            const int ahead = SLOTS > 1 ? u : 0;
+            if (c > c_begin && c + ahead < ce && lane == 0) {
                 bulk_wait_group_read<0>();
-                epi_load_unit(tmX, w, w.slot ^ 1, n0 + (c + u) * 32, row0);
+                epi_load_unit(tmX, w, SLOTS > 1 ? w.slot ^ 1 : 0, n0 + (c + ahead) * 32, row0);
             }
         } else if (lane == 0) {
-            bulk_wait_group_read<1>();  // this box's previous store has read it
+            bulk_wait_group_read<SLOTS - 1>();  // this box's previous store has read it
         }
         __syncwarp();
         uint8_t* box = w.stage + w.slot * kEpiSlotBytes;
@@ -816,7 +818,7 @@ __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt
             }
             bulk_commit_group();
         }
-        w.slot ^= 1;
+        w.slot ^= SLOTS - 1;
     }
     if (ce < c_end && n0 + ce * 32 < a.N && row0 < a.M) {
         if (lane == 0) bulk_wait_group_read<0>();  // the boxes are about to be reused
@@ -897,7 +899,7 @@ __device__ __forceinline__ int chain_blocks(const typename ExtOf<FAM>::type& x, 
 
 // out_f32 planes [split][M][ldo]: plane `split` (+)= the partial product of its k-range. One tile
 // owns an element of a plane in a launch, so the sums do not depend on the tiles' order.
-template <int NCOLS>
+template <int NCOLS, int SLOTS>
 __device__ __forceinline__ void plane_epilogue_tile(const GemmArgs& a, const CUtensorMap* tmO,
                                                     uint32_t tbase, int row0, int n0, int split,
                                                     int lane, EpiWarp& w, int c_begin, int c_end) {
@@ -913,7 +915,7 @@ __device__ __forceinline__ void plane_epilogue_tile(const GemmArgs& a, const CUt
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
         uint8_t* box = w.stage + w.slot * kEpiSlotBytes;
-        if (lane == 0) bulk_wait_group_read<1>();
+        if (lane == 0) bulk_wait_group_read<SLOTS - 1>();
         __syncwarp();
         box_put_f32(box, lane, v);
         fence_proxy_async_smem();
@@ -925,7 +927,7 @@ __device__ __forceinline__ void plane_epilogue_tile(const GemmArgs& a, const CUt
                 tma_store_3d(tmO, box, col0, row0, split);
             bulk_commit_group();
         }
-        w.slot ^= 1;
+        w.slot ^= SLOTS - 1;
     }
 }
 
@@ -1003,7 +1005,7 @@ __device__ __forceinline__ void head_stats_tile(const GemmArgs& a, const GemmExt
 // batch of equal weights: an untrained or unlikely target's entry is then nearly exact, where
 // -0.9 / rows, say, would round the same way in every row and bias the whole gradient by up to
 // 2^-8.
-template <int NCOLS>
+template <int NCOLS, int SLOTS>
 __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt& x,
                                                const CUtensorMap* tmO, uint32_t tbase, int row0,
                                                int n0, int lane, EpiWarp& w, int c_begin,
@@ -1024,7 +1026,7 @@ __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt&
         tmem_ld_32x32b_x32(tbase + (uint32_t)((c + 1) * 32), r[1]);
         tmem_ld_wait();
         uint8_t* box = w.stage + w.slot * kEpiSlotBytes;
-        if (lane == 0) bulk_wait_group_read<1>();
+        if (lane == 0) bulk_wait_group_read<SLOTS - 1>();
         __syncwarp();
         const int tj = t - (x.v0 + col0);
         const bool here = __any_sync(0xffffffffu, tj >= 0 && tj < 64);
@@ -1058,12 +1060,12 @@ __device__ __forceinline__ void head_grad_tile(const GemmArgs& a, const GemmExt&
             tma_store_3d(tmO, box, col0, row0, 0);
             bulk_commit_group();
         }
-        w.slot ^= 1;
+        w.slot ^= SLOTS - 1;
     }
 }
 
 // One accumulator tile of one warp, any family.
-template <int FAM, int NCOLS>
+template <int FAM, int NCOLS, int SLOTS>
 __device__ __forceinline__ void family_tile(const GemmArgs& a,
                                             const typename ExtOf<FAM>::type& x,
                                             const DropKey& key, const CUtensorMap* tmO,
@@ -1075,15 +1077,15 @@ __device__ __forceinline__ void family_tile(const GemmArgs& a,
                              c_end);
     } else if constexpr (FAM == kFamLinear) {
         if (a.epi == kEpiPlaneAdd)
-            plane_epilogue_tile<NCOLS>(a, tmO, tbase, row0, n0, split, lane, w, c_begin, c_end);
+            plane_epilogue_tile<NCOLS, SLOTS>(a, tmO, tbase, row0, n0, split, lane, w, c_begin, c_end);
         else if (a.tma_epi)
-            linear_box_tile(a, x, key, tmO, tmX, tbase, row0, n0, lane, w, c_begin, c_end);
+            linear_box_tile<SLOTS>(a, x, key, tmO, tmX, tbase, row0, n0, lane, w, c_begin, c_end);
         else
             linear_turned_tile(a, x, key, tbase, row0, n0, lane, w, c_begin, c_end);
     } else if constexpr (FAM == kFamHeadStats) {
         head_stats_tile<NCOLS>(a, x, tbase, row0, n0, lane, c_begin, c_end);
     } else {
-        head_grad_tile<NCOLS>(a, x, tmO, tbase, row0, n0, lane, w, c_begin, c_end);
+        head_grad_tile<NCOLS, SLOTS>(a, x, tmO, tbase, row0, n0, lane, w, c_begin, c_end);
     }
 }
 
@@ -1310,7 +1312,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             };
             bool ready;
             if constexpr (FAM == kFamLinear && BN <= 128) {
-                linear_prefetch(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
+                linear_prefetch<2>(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
                 const int ck = chain_blocks<FAM>(ext, kb0, kb1);
                 const int chains = (kb1 - kb0 + ck - 1) / ck;
                 ready = chains > 1
@@ -1320,7 +1322,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             : wait_acc(acc, acc_phase);
             } else {
                 if constexpr (FAM == kFamLinear)
-                    linear_prefetch(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
+                    linear_prefetch<2>(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
                 ready = wait_acc(acc, acc_phase);
             }
             if (!ready) {
@@ -1330,7 +1332,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             tc_fence_after();
             const uint32_t tbase =
                 tmem_base + (uint32_t)(acc * BN) + ((uint32_t)(q * 32) << 16);
-            family_tile<FAM, BN>(args, ext, key, &tmO, &tmX, tbase, kb1 <= kb0, m0 + q * 32, n0,
+            family_tile<FAM, BN, 2>(args, ext, key, &tmO, &tmX, tbase, kb1 <= kb0, m0 + q * 32, n0,
                                  split, g, lane, ew, 0, BN / 32);
             tc_fence_before();
             mbar_arrive(&acc_empty[acc]);
@@ -1363,14 +1365,22 @@ struct PairCfgOf {
     static constexpr int A_BYTES = BM * BK * 2;
     static constexpr int B_BYTES = BNH * BK * 2;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    // the softmax statistics write no boxes: their share of shared memory goes to the ring
-    static constexpr int STAGES = FAM == kFamHeadStats ? 7 : 5;
-    static constexpr int EPI_BYTES = FAM == kFamHeadStats ? 0 : kPairEpiStageBytes;
+    // what an epilogue leaves of shared memory goes to the ring: the softmax statistics write no
+    // boxes, the gradient by the logits one a warp
+    static constexpr int STAGES = FAM == kFamHeadStats ? 7 : FAM == kFamHeadGrad ? 6 : 5;
+    // The linear epilogue runs on four warps a scheduler (8192 x 1024 x 4096 gelu: 122k -> 110k
+    // cycles), whose boxes then come to one a warp; the head's are no faster for it.
+    static constexpr int EPI_WARPS = FAM == kFamLinear ? 16 : kPairEpiWarps;
+    static constexpr int EPI_SLOTS = FAM == kFamLinear || FAM == kFamHeadGrad ? 1 : 2;
+    static constexpr int EPI_COLS = BN / (EPI_WARPS / 4);  // columns of a warp
+    static constexpr int THREADS = 128 + 32 * EPI_WARPS;
+    static constexpr int EPI_BYTES =
+        FAM == kFamHeadStats ? 0 : EPI_WARPS * EPI_SLOTS * kEpiSlotBytes;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
-    static constexpr int BAR_BYTES = 320;
+    static constexpr int BAR_BYTES = 384;
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_BYTES + BAR_BYTES;
     // the last bytes: stage, accumulator and epilogue barriers, then the TMEM address
-    static_assert((2 * STAGES + 4 + 2 * kPairEpiWarps) * 8 + 4 <= BAR_BYTES, "barrier area");
+    static_assert((2 * STAGES + 4 + EPI_SLOTS * EPI_WARPS) * 8 + 4 <= BAR_BYTES, "barrier area");
 };
 using PairCfg = PairCfgOf<kFamBase>;  // the tile's shape, alike in all
 
@@ -1537,7 +1547,7 @@ struct PairItems {
 };
 
 template <int NG, int FAM>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
     gemm_bf16_pair_kernel(const __grid_constant__ PairParams<NG, FAM> P) {
     using Cfg = PairCfgOf<FAM>;
     constexpr int STAGES = Cfg::STAGES;
@@ -1553,7 +1563,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
     uint64_t* epi_bar = acc_empty + 2;  // two per epilogue warp
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_bar + 2 * kPairEpiWarps);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_bar + Cfg::EPI_SLOTS * Cfg::EPI_WARPS);
 
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
@@ -1579,9 +1589,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 2 * 32 * kPairEpiWarps);  // epilogue threads, both CTAs
+            mbar_init(&acc_empty[i], 2 * 32 * Cfg::EPI_WARPS);  // epilogue threads, both CTAs
         }
-        for (int i = 0; i < 2 * kPairEpiWarps; ++i) mbar_init(&epi_bar[i], 1);
+        for (int i = 0; i < Cfg::EPI_SLOTS * Cfg::EPI_WARPS; ++i) mbar_init(&epi_bar[i], 1);
         fence_barrier_init();
     }
     if (warp == 0 && lane == 0) {
@@ -1881,11 +1891,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
     } else if (warp >= 4) {
         // ---------------- epilogue warps (both CTAs): warp 4 + e drains TMEM lane quarter
-        // e % 4, columns [half * BN/2, (half + 1) * BN/2) with half = e / 4
+        // e % 4, the (e / 4)-th EPI_COLS of the tile's columns
         const int e = warp - 4;
-        const int q = e & 3, half = e >> 2;
+        const int q = e & 3, part = e >> 2;
         const uint32_t acc_empty_leader = mapa_shared(smem_u32(&acc_empty[0]), 0);
-        EpiWarp ew{sEpi + e * 2 * kEpiSlotBytes, &epi_bar[2 * e], 0u, 0, 0u};
+        EpiWarp ew{sEpi + e * Cfg::EPI_SLOTS * kEpiSlotBytes, &epi_bar[Cfg::EPI_SLOTS * e], 0u, 0, 0u};
+        constexpr int kChunks = Cfg::EPI_COLS / 32;  // of a warp
         const DropKey key = family_key<FAM>(P.ext);
         int acc = 0;
         uint32_t acc_phase = 0;
@@ -1908,15 +1919,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                       split, gi, kb0, kb1);
             const int m0 = m_blk * Cfg::BMP + 128 * (int)rank, n0 = n_blk * BN;
             if constexpr (FAM == kFamBase)
-                epilogue_prefetch(args, &P.tmX[g], m0 + q * 32, n0, lane, ew, half * (BN / 64),
-                                  (half + 1) * (BN / 64));
+                epilogue_prefetch(args, &P.tmX[g], m0 + q * 32, n0, lane, ew, part * kChunks,
+                                  (part + 1) * kChunks);
             auto wait_acc = [&](int i, uint32_t ph) {
                 return mbar_wait_bounded_cluster(&acc_full[i], ph, err, kDevTimeoutAcc);
             };
             bool ready;
             if constexpr (FAM == kFamLinear) {
-                linear_prefetch(args, P.ext, &P.tmX[g], m0 + q * 32, n0, lane, ew,
-                                half * (BN / 64), (half + 1) * (BN / 64));
+                linear_prefetch<Cfg::EPI_SLOTS>(args, P.ext, &P.tmX[g], m0 + q * 32, n0, lane, ew,
+                                part * kChunks, (part + 1) * kChunks);
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 const int chains = (kb1 - kb0 + ck - 1) / ck;
                 auto free_acc = [&](int i) {
@@ -1926,9 +1937,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         mbar_arrive_cluster(acc_empty_leader + 8u * (uint32_t)i);
                 };
                 ready = chains > 1
-                            ? chain_sum<BN / 2>(chains,
+                            ? chain_sum<Cfg::EPI_COLS>(chains,
                                                 tmem_base + ((uint32_t)(q * 32) << 16) +
-                                                    (uint32_t)(half * (BN / 2)),
+                                                    (uint32_t)(part * Cfg::EPI_COLS),
                                                 BN, acc, acc_phase, wait_acc, free_acc)
                             : wait_acc(acc, acc_phase);
             } else {
@@ -1941,9 +1952,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const uint32_t tbase =
                 tmem_base + (uint32_t)(acc * BN) + ((uint32_t)(q * 32) << 16);
-            family_tile<FAM, BN>(args, P.ext, key, &P.tmO[g], &P.tmX[g], tbase, kb1 <= kb0,
-                                 m0 + q * 32, n0, split, gi, lane, ew, half * (BN / 64),
-                                 (half + 1) * (BN / 64));
+            family_tile<FAM, BN, Cfg::EPI_SLOTS>(args, P.ext, key, &P.tmO[g], &P.tmX[g], tbase, kb1 <= kb0,
+                                 m0 + q * 32, n0, split, gi, lane, ew, part * kChunks,
+                                 (part + 1) * kChunks);
             tc_fence_before();
             if (leader)
                 mbar_arrive(&acc_empty[acc]);
@@ -2255,7 +2266,7 @@ int pair_max_clusters(int num_sms) {
         if (pair_set_attr<1, kFamBase>()) return;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * (num_sms / 2), 1, 1);
-        cfg.blockDim = dim3(kPairThreads, 1, 1);
+        cfg.blockDim = dim3(PairCfg::THREADS, 1, 1);
         cfg.dynamicSmemBytes = PairCfg::SMEM;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -2278,7 +2289,7 @@ int launch_pair_params(const PairParams<NG, FAM>& P, int grid, cudaStream_t stre
     if (pair_set_attr<NG, FAM>()) return -10;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.blockDim = dim3(PairCfgOf<FAM>::THREADS, 1, 1);
     cfg.dynamicSmemBytes = PairCfgOf<FAM>::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
