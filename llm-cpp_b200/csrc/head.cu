@@ -18,7 +18,7 @@ long long ceil8(long long n) { return (n + 7) & ~7ll; }
 
 constexpr int kMaxV = 1 << 30;   // piece offsets stay in 32 bits
 constexpr int kSlot = 128;       // vocabulary columns of one (max, sum) slot
-constexpr int kMaxSplits = 4;    // planes of the dx product
+constexpr int kMaxSplits = 32;   // planes of the dx product
 constexpr int kPairSlots = 74;   // CTA pairs of a B200, for the choice of piece and splits only
 constexpr size_t kPieceBytes = (size_t)320 << 20;  // gradient piece at most, where chosen here
 
@@ -165,19 +165,21 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
     uint32_t row = first / n4, c4 = first - row * n4;
     while (row < rows) {
         const float* p = planes + (long long)row * ldp + 4 * c4;
-        float4 q[kMaxSplits];
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k0 = 0; k0 < n; k0 += 4) {
+            float4 q[4];
 #pragma unroll
-        for (int k = 0; k < kMaxSplits; ++k)
-            if (k < n) q[k] = *reinterpret_cast<const float4*>(p + k * plane);
-        float4 v = q[0];
+            for (int k = 0; k < 4; ++k)
+                if (k0 + k < n) q[k] = *reinterpret_cast<const float4*>(p + (k0 + k) * plane);
 #pragma unroll
-        for (int k = 1; k < kMaxSplits; ++k)
-            if (k < n) {
-                v.x += q[k].x;
-                v.y += q[k].y;
-                v.z += q[k].z;
-                v.w += q[k].w;
-            }
+            for (int k = 0; k < 4; ++k)
+                if (k0 + k < n) {
+                    v.x += q[k].x;
+                    v.y += q[k].y;
+                    v.z += q[k].z;
+                    v.w += q[k].w;
+                }
+        }
         const float w[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
         T* o = dx + row * lddx + 4 * c4;
         if (vec && 4 * (int)c4 + 4 <= C) {
@@ -214,14 +216,20 @@ int launch_dx(const float* planes, int n, int rows, int C, int ldp, const float*
 long long waves(long long tiles) { return (tiles + kPairSlots - 1) / kPairSlots; }
 
 // k-splits of the dx product (each into a plane of its own): the count whose last wave of
-// 256 x 256 tiles wastes least, a tile costing its k-blocks and about 4 more.
-int dx_splits(int rows, int C, int piece) {
+// 256 x 256 tiles wastes least, a tile costing its k-blocks and about 4 more. Where one piece is
+// the whole vocabulary (`all`) and one split would do, the planes' summing kernel is not needed:
+// about 12 k-blocks of a pair (4 us).
+int dx_splits(int rows, int C, int piece, bool all) {
     const long long tiles = (long long)((rows + 255) / 256) * ((C + 255) / 256);
     const int kb = (piece + 63) / 64;
+    // a plane is written (added to) once a piece and read once: 8 bytes an element at about
+    // 6 TB/s, against 0.3 us a k-block
+    const double plane = (double)rows * C * 8.0 / 6e6 / 0.3;
     int best = 1;
     double cost = 1e30;
-    for (int n = 1; n <= kMaxSplits && n <= kb; ++n) {
-        const double c = (double)waves(tiles * n) * ((double)kb / n + 4.0);
+    for (int n = 1; n <= kMaxSplits && n <= kb; n += n < 4 ? 1 : n < 16 ? 2 : 8) {
+        const double c = (double)waves(tiles * n) * ((double)kb / n + 4.0) + n * plane +
+                         (all && n > 1 ? 12.0 : 0.0);
         if (c < cost * 0.97) {
             cost = c;
             best = n;
@@ -238,7 +246,7 @@ struct HeadLayout {
 HeadLayout head_layout(int rows, int C, int V, int piece) {
     HeadLayout l;
     l.piece = head_piece(rows, C, V, piece);
-    l.splits = dx_splits(rows, C, l.piece);
+    l.splits = dx_splits(rows, C, l.piece, l.piece >= V);
     l.ldx = (int)ceil8(C);
     l.ldg = (int)ceil8(l.piece);
     l.ldp = (C + 3) & ~3;
@@ -267,7 +275,7 @@ int head_piece(int rows, int C, int V, int piece) {
         double c = 0.0;
         for (int v = 0; v < all; v += p) {
             const int w = all - v < p ? all - v : p;
-            const int n = dx_splits(rows, C, w * 256);
+            const int n = dx_splits(rows, C, w * 256, false);
             c += (double)waves((long long)tr * w) * ((C + 63) / 64 + 4) +
                  (double)waves((long long)w * tc) * ((rows + 63) / 64 + 4) +
                  (double)waves((long long)tr * tc * n) * (4.0 * w / n + 4);
