@@ -60,8 +60,8 @@ __device__ __forceinline__ float2 act_grad_pair(float2 z) {
     }
 }
 
-// dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable). `vec`: rows
-// of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a time, their
+// dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable; with one row of
+// blocks it is dbias itself, added to when `accumulate`). `vec`: rows of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a time, their
 // loads in flight together as raw words: bound by memory at 8192 x 4096 bf16 (201 MB).
 constexpr int kDzInFlight = 2;
 template <typename T, int ACT, bool DROP>
@@ -69,8 +69,8 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
                                                         const bf16* __restrict__ pre,
                                                         long long ld_pre, DropArgs drop,
                                                         bf16* __restrict__ dz, long long ldz,
-                                                        float* __restrict__ part, int M, int N,
-                                                        int vec) {
+                                                        float* __restrict__ part, int accumulate,
+                                                        int M, int N, int vec) {
     pdl_enter();
     const int lane = threadIdx.x & 31, wr = threadIdx.x >> 5;
     const int col = blockIdx.x * kDzCols + lane * 8;
@@ -137,16 +137,18 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
         float t = 0.0f;
 #pragma unroll
         for (int r = 0; r < kDzRows; ++r) t += red[r][threadIdx.x];
-        part[(long long)blockIdx.y * N + c] = t;
+        float* to = part + (long long)blockIdx.y * N + c;
+        *to = accumulate ? *to + t : t;
     }
 }
 
 template <typename T, int ACT>
 int launch_dz_act(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* sums, int vec,
                   cudaStream_t s) {
+    const int accumulate = grid.y == 1 && a.accumulate;
     return launch_kernel(drop.rng ? linear_dz_kernel<T, ACT, true> : linear_dz_kernel<T, ACT, false>,
                          grid, 256, 0, s, (const T*)a.dy, a.lddy, a.pre, a.ld_pre, drop, to,
-                         ceil8(a.N), sums, a.M, a.N, vec);
+                         ceil8(a.N), sums, accumulate, a.M, a.N, vec);
 }
 template <typename T>
 int launch_dz(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* sums, int vec,
@@ -184,184 +186,6 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict
     }
 }
 
-// ------------------------------------------------------------------------------ a few rows
-// Decoding: out [M <= 8, N] with every weight read once and no tensor map or tile in the way. The
-// products are sums in f32 registers; the epilogue is the linear layer's.
-constexpr int kFewRows = 8;
-
-struct RowsArgs {
-    const bf16* x;
-    long long ldx;
-    const bf16* w;
-    long long ldw;
-    const float* alpha;
-    const float* bias;
-    int act;
-    DropArgs drop;
-    const void* resid;
-    long long ldr;
-    bf16* pre;
-    long long ld_pre;
-    void* out;
-    int out_f32;
-    long long ldo;
-    int M, N, K;
-};
-
-__device__ __forceinline__ void rows_store(const RowsArgs& a, int m, int n, float z) {
-    if (a.alpha) z *= *a.alpha;
-    if (a.bias) z += a.bias[n];
-    if (a.pre) a.pre[m * a.ld_pre + n] = __float2bfloat16_rn(z);
-    float y = z;
-    if (a.act == kActRelu) {
-        y = z <= 0.0f ? 0.0f : z;
-    } else if (a.act == kActGelu) {
-        const float t = -1.5957691216f * 1.4426950408889634f * z * fmaf(0.044715f * z, z, 1.0f);
-        y = z * rcp_approx(1.0f + ex2_approx(t));
-    } else if (a.act == kActSilu) {
-        y = z * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * z));
-    }
-    if (a.drop.rng) {
-        const DropKey key = drop_key(a.drop.rng, a.drop.site);
-        const uint32_t keep = drop_keep8(key, (uint32_t)n >> 3, (uint32_t)m, a.drop.thr);
-        y = ((keep >> (n & 7)) & 1u) ? y * a.drop.scale : 0.0f;
-    }
-    if (a.out_f32) {
-        if (a.resid) y += reinterpret_cast<const float*>(a.resid)[m * a.ldr + n];
-        reinterpret_cast<float*>(a.out)[m * a.ldo + n] = y;
-    } else {
-        if (a.resid) y += __bfloat162float(reinterpret_cast<const bf16*>(a.resid)[m * a.ldr + n]);
-        reinterpret_cast<bf16*>(a.out)[m * a.ldo + n] = __float2bfloat16_rn(y);
-    }
-}
-
-// Eight bf16 of a row from k on (16-byte aligned), zeros past K.
-__device__ __forceinline__ uint4 row_chunk(const bf16* p, int k, int K) {
-    if (k + 8 <= K) return *reinterpret_cast<const uint4*>(p + k);
-    uint32_t h[4] = {0u, 0u, 0u, 0u};
-    for (int j = 0; j < 8; ++j)
-        if (k + j < K) h[j >> 1] |= (uint32_t)__bfloat16_as_ushort(p[k + j]) << (16 * (j & 1));
-    return make_uint4(h[0], h[1], h[2], h[3]);
-}
-
-// w [N, K]: a warp takes one output column, its lanes 8 of K at a time, four steps in flight.
-template <int MR>
-__global__ void __launch_bounds__(256) linear_rows_kernel(const RowsArgs a) {
-    pdl_enter();
-    const int lane = threadIdx.x & 31;
-    const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (n >= a.N) return;
-    const bf16* w = a.w + n * a.ldw;
-    float acc[MR];
-#pragma unroll
-    for (int m = 0; m < MR; ++m) acc[m] = 0.0f;
-    for (int k0 = 8 * lane; k0 < a.K; k0 += 4 * 256) {
-        uint4 u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            u[i] = k0 + 256 * i < a.K ? row_chunk(w, k0 + 256 * i, a.K) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = k0 + 256 * i;
-            if (k >= a.K) break;
-            const uint32_t ww[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                if (m >= a.M) break;
-                const uint4 q = row_chunk(a.x + m * a.ldx, k, a.K);
-                const uint32_t xx[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    acc[m] = fmaf(bf16_lo(ww[j]), bf16_lo(xx[j]), acc[m]);
-                    acc[m] = fmaf(bf16_hi(ww[j]), bf16_hi(xx[j]), acc[m]);
-                }
-            }
-        }
-    }
-    float mine = 0.0f;
-#pragma unroll
-    for (int m = 0; m < MR; ++m) {
-        float v = acc[m];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == m) mine = v;
-    }
-    if (lane < a.M) rows_store(a, lane, n, mine);
-}
-
-// w [K, N]: a block takes 32 columns, four lanes of 8 side by side; its 128 groups of four lanes
-// stride over K, their sums meet in shared memory.
-constexpr int kRowsThreads = 512;
-template <int MR>
-__global__ void __launch_bounds__(kRowsThreads) linear_rows_mn_kernel(const RowsArgs a) {
-    pdl_enter();
-    __shared__ float part[kRowsThreads / 32][MR][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n0 = blockIdx.x * 32, n = n0 + 8 * (lane & 3);
-    float acc[MR][8];
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[m][j] = 0.0f;
-    if (n < a.N) {
-        constexpr int kStep = kRowsThreads / 4;
-        for (int k0 = threadIdx.x >> 2; k0 < a.K; k0 += 4 * kStep) {
-            uint4 u[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = k0 + i * kStep;
-                u[i] = k < a.K ? row_chunk(a.w + k * a.ldw, n, a.N) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = k0 + i * kStep;
-                if (k >= a.K) break;
-                const uint32_t ww[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-                for (int m = 0; m < MR; ++m) {
-                    if (m >= a.M) break;
-                    const float xv = __bfloat162float(a.x[m * a.ldx + k]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        acc[m][2 * j] = fmaf(xv, bf16_lo(ww[j]), acc[m][2 * j]);
-                        acc[m][2 * j + 1] = fmaf(xv, bf16_hi(ww[j]), acc[m][2 * j + 1]);
-                    }
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float v = acc[m][j];
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane < 4) part[warp][m][8 * lane + j] = v;
-        }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * a.M; i += kRowsThreads) {
-        const int m = i >> 5, c = i & 31;
-        if (n0 + c >= a.N) continue;
-        float v = 0.0f;
-#pragma unroll
-        for (int q = 0; q < kRowsThreads / 32; ++q) v += part[q][m][c];
-        rows_store(a, m, n0 + c, v);
-    }
-}
-
-template <int MR>
-int launch_rows(const RowsArgs& a, int w_mn, cudaStream_t s) {
-    if (w_mn)
-        return launch_kernel_pdl(linear_rows_mn_kernel<MR>, (a.N + 31) / 32, kRowsThreads, 0, s, a);
-    return launch_kernel_pdl(linear_rows_kernel<MR>, (a.N + 7) / 8, 256, 0, s, a);
-}
-int run_rows(const RowsArgs& a, int w_mn, cudaStream_t s) {
-    if (a.M == 1) return launch_rows<1>(a, w_mn, s);
-    if (a.M == 2) return launch_rows<2>(a, w_mn, s);
-    return a.M <= 4 ? launch_rows<4>(a, w_mn, s) : launch_rows<8>(a, w_mn, s);
-}
-
 }  // namespace
 
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
@@ -371,8 +195,10 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
     if (M <= kFewRows && !a_mn) {
         RowsArgs r{A, lda, B, ldb, alpha, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo, nullptr, 0,
                    out, out_f32, ldo, M, N, K};
-        return run_rows(r, b_mn, s);
+        return rows_product(r, b_mn, s);
     }
+    if (K <= kOuterRows && a_mn && b_mn)
+        return outer_product(A, lda, B, ldb, M, N, K, out, out_f32, ldo, accumulate, alpha, s);
     GemmArgs g{};
     g.out = out;
     g.ldo = ldo;
@@ -406,7 +232,7 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
         RowsArgs r{a.x, a.ldx, a.w, a.ldw, nullptr, a.bias, a.act, a.drop, a.resid, a.ldr, a.pre, a.ld_pre,
                    a.out, a.out_f32, a.ldo, a.M, a.N, a.K};
         if (r.drop.thr == 0) r.drop.rng = nullptr;
-        return run_rows(r, a.w_mn_major, s);
+        return rows_product(r, a.w_mn_major, s);
     }
     GemmArgs g{};
     g.epi = kEpiLinear;
@@ -475,11 +301,11 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
                         (a.act == kActNone || (aligned16(a.pre) && (a.ld_pre & 7) == 0));
         const dim3 grid((a.N + kDzCols - 1) / kDzCols, groups);
         bf16* to = need_dz ? buf : nullptr;
-        float* sums = a.dbias ? part : nullptr;
+        float* sums = !a.dbias ? nullptr : groups == 1 ? a.dbias : part;
         int rc = a.dy_f32 ? launch_dz<float>(a, drop, grid, to, sums, vec, s)
                           : launch_dz<bf16>(a, drop, grid, to, sums, vec, s);
         if (rc) return rc;
-        if (a.dbias) {
+        if (a.dbias && groups > 1) {
             rc = launch_kernel(linear_db_kernel, (a.N + 31) / 32, 1024, 0, s, part, groups, a.N,
                                a.dbias, a.accumulate);
             if (rc) return rc;

@@ -100,6 +100,35 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
                   int dx_f32, long long lddx, void* dw, int dw_f32, long long lddw, int accumulate,
                   int piece, int num_sms, cudaStream_t s);
 
+// Products of a few rows (linear_rows.cu): decoding, where every weight is read once and a 128-row
+// tile would be empty. out [M <= kFewRows, N] = resid + drop(act(alpha x w^T + bias)), w [N, K] or
+// (w_mn) [K, N].
+constexpr int kFewRows = 16;
+struct RowsArgs {
+    const bf16* x;
+    long long ldx;
+    const bf16* w;
+    long long ldw;
+    const float* alpha;
+    const float* bias;
+    int act;
+    DropArgs drop;
+    const void* resid;
+    long long ldr;
+    bf16* pre;
+    long long ld_pre;
+    void* out;
+    int out_f32;
+    long long ldo;
+    int M, N, K;
+};
+int rows_product(const RowsArgs& a, int w_mn, cudaStream_t s);
+// out[M,N] (+)= alpha sum_k A[k,M] B[k,N] over K <= kOuterRows rows: bound by the result's writes.
+constexpr int kOuterRows = 8;
+int outer_product(const bf16* A, long long lda, const bf16* B, long long ldb, int M, int N, int K,
+                  void* out, int out_f32, long long ldo, int accumulate, const float* alpha,
+                  cudaStream_t s);
+
 // D[M,N] (+)= alpha A B^T on the tcgen05 kernels into bf16 or f32 `out`, any row stride (accumulate:
 // f32 only; alpha: device scalar, nullable).
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,

@@ -119,11 +119,12 @@ def test_loss_head_bwd_refusals(bad):
 
 
 def test_workspace_covers_any_piece():
-    """The workspace grows with the piece and never past the whole vocabulary's."""
+    """The workspace holds at least the gradient of one piece and a copy of x; a piece past the
+    vocabulary is the whole of it."""
     f = _lib().llmgpu_op_linear_ce_bwd_work
-    sizes = [f(100, 64, 5000, p) for p in (256, 512, 2048, 4096, 8192, 1 << 20)]
-    assert sizes == sorted(sizes) and sizes[-1] == sizes[-2] and sizes[0] > 0
-    assert f(100, 64, 5000, 0) <= sizes[-1]
+    for p in (256, 512, 2048, 4096, 8192):
+        assert f(100, 64, 5000, p) >= 100 * (min(p, 5000) + 64) * 2
+    assert f(100, 64, 5000, 8192) == f(100, 64, 5000, 1 << 20) == f(100, 64, 5000, 0)
 
 
 def test_wrappers_refuse_cpu_tensors():
