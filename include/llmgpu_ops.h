@@ -167,7 +167,8 @@ int llmgpu_op_dropout(const void* x, int x_f32, long long ldx, const void* resid
 int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long ldw, int w_mn_major,
                          const float* bias, int act, float p, const uint64_t* rng, uint64_t site,
                          const void* resid, long long ldr, void* pre, long long ld_pre, void* out,
-                         int out_f32, long long ldo, int M, int N, int K, int* err, void* stream);
+                         int out_f32, long long ldo, int M, int N, int K, void* work, int* err,
+                         void* stream);
 /* Its backward: dz = drop(dy) * act'(pre), rounded to bf16 for the products; dbias = column sums of
  * dz before that rounding, dx = dz w, dw = dz^T x (in w's layout); the residual's gradient is dy
  * itself. dx, dw, dbias are nullable; dx and dw are bf16 or f32. `accumulate` adds into dw (f32

@@ -16,6 +16,7 @@
 #include <vector>
 #include <algorithm>
 
+#include "act.cuh"
 #include "common.cuh"
 #include "gemm.cuh"
 #include "philox.cuh"
@@ -547,33 +548,6 @@ struct ExtOf<kFamBase> {
     using type = NoExt;
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-// Activations of a pair of pre-activations, z / (1 + exp(-t)) with t = z (silu) or 2 k (z + 0.044715
-// z^3) (gelu: 0.5 z (1 + tanh u) = z sigmoid(2u)), from the special-function unit's 2^x and
-// reciprocal, a few units in the last place, which an f32 output keeps. Far left, 2^x overflows
-// to inf and the result is -0. Packed pairs: 7 issue slots for two gelus besides the 4
-// special-function ones, since the epilogue's warps, two per scheduler, are what bounds a
-// product of K near 1024.
-__device__ __forceinline__ float2 sigmoid_of_log2(float2 t) {  // 1 / (1 + 2^t)
-    const float2 d = fadd2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.f, 1.f));
-    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
-}
-template <int ACT>
-__device__ __forceinline__ float2 act_pair(float2 z) {
-    if constexpr (ACT == kActRelu) {  // NaN stays NaN
-        return make_float2(z.x <= 0.0f ? 0.0f : z.x, z.y <= 0.0f ? 0.0f : z.y);
-    } else if constexpr (ACT == kActGelu) {
-        constexpr float c = -1.5957691216f * kLog2e;
-        const float2 w = ffma2(fmul2(z, z), make_float2(c * 0.044715f, c * 0.044715f),
-                               make_float2(c, c));
-        return fmul2(z, sigmoid_of_log2(fmul2(w, z)));
-    } else if constexpr (ACT == kActSilu) {
-        return fmul2(z, sigmoid_of_log2(fmul2(z, make_float2(-kLog2e, -kLog2e))));
-    } else {
-        return z;
-    }
-}
 template <int ACT>
 __device__ __forceinline__ void act_all(float (&v)[32]) {
 #pragma unroll

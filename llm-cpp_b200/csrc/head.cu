@@ -7,7 +7,6 @@
 
 #include "common.cuh"
 #include "linear.cuh"
-#include "rowio.cuh"
 
 namespace llmgpu {
 
@@ -148,71 +147,6 @@ __global__ void __launch_bounds__(256) head_rows_kernel(const bf16* __restrict__
     }
 }
 
-// dx = alpha times the sum of the planes [n][rows][ldp], in their order; a thread takes 4 columns,
-// with the planes' loads in flight together. The positions of a thread lie (dr, dc) rows and
-// groups of 4 apart. Bound by memory.
-template <typename T>
-__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ planes, int n,
-                                                      uint32_t rows, int C, int ldp, uint32_t dr,
-                                                      uint32_t dc, int vec,
-                                                      const float* __restrict__ alpha,
-                                                      T* __restrict__ dx, long long lddx) {
-    pdl_enter();
-    const float f = *alpha;
-    const uint32_t n4 = (uint32_t)ldp >> 2;
-    const long long plane = (long long)rows * ldp;
-    const uint32_t first = blockIdx.x * 256u + threadIdx.x;
-    uint32_t row = first / n4, c4 = first - row * n4;
-    while (row < rows) {
-        const float* p = planes + (long long)row * ldp + 4 * c4;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k0 = 0; k0 < n; k0 += 4) {
-            float4 q[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k0 + k < n) q[k] = *reinterpret_cast<const float4*>(p + (k0 + k) * plane);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k0 + k < n) {
-                    v.x += q[k].x;
-                    v.y += q[k].y;
-                    v.z += q[k].z;
-                    v.w += q[k].w;
-                }
-        }
-        const float w[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-        T* o = dx + row * lddx + 4 * c4;
-        if (vec && 4 * (int)c4 + 4 <= C) {
-            if constexpr (sizeof(T) == 4)
-                *reinterpret_cast<float4*>(o) = make_float4(w[0], w[1], w[2], w[3]);
-            else
-                *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
-        } else {
-            for (int j = 0; j < 4; ++j)
-                if (4 * (int)c4 + j < C) o[j] = from_f32<T>(w[j]);
-        }
-        row += dr;
-        c4 += dc;
-        if (c4 >= n4) {
-            c4 -= n4;
-            ++row;
-        }
-    }
-}
-
-template <typename T>
-int launch_dx(const float* planes, int n, int rows, int C, int ldp, const float* alpha, void* dx,
-              long long lddx, cudaStream_t s) {
-    const uint32_t n4 = (uint32_t)ldp / 4;
-    const long long items = (long long)rows * n4;
-    const long long most = 148 * 8;
-    const uint32_t blocks = (uint32_t)((items + 255) / 256 < most ? (items + 255) / 256 : most);
-    const uint32_t step = blocks * 256;
-    const int vec = (reinterpret_cast<uintptr_t>(dx) % (4 * sizeof(T))) == 0 && lddx % 4 == 0;
-    return launch_kernel(head_dx_kernel<T>, (int)blocks, 256, 0, s, planes, n, (uint32_t)rows, C, ldp,
-                         step / n4, step % n4, vec, alpha, (T*)dx, lddx);
-}
-
 long long waves(long long tiles) { return (tiles + kPairSlots - 1) / kPairSlots; }
 
 // k-splits of the dx product (each into a plane of its own): the count whose last wave of
@@ -249,7 +183,7 @@ HeadLayout head_layout(int rows, int C, int V, int piece) {
     l.splits = dx_splits(rows, C, l.piece, l.piece >= V);
     l.ldx = (int)ceil8(C);
     l.ldg = (int)ceil8(l.piece);
-    l.ldp = (C + 3) & ~3;
+    l.ldp = (int)ceil8(C);
     l.x = 0;
     l.g = align256((size_t)rows * l.ldx * 2);
     l.planes = l.g + align256((size_t)rows * l.ldg * 2);
@@ -413,8 +347,9 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
         }
     }
     if (dx && !one) {
-        rc = dx_f32 ? launch_dx<float>(planes, l.splits, a.rows, a.C, l.ldp, top + 1, dx, lddx, s)
-                    : launch_dx<bf16>(planes, l.splits, a.rows, a.C, l.ldp, top + 1, dx, lddx, s);
+        RowsArgs r{nullptr, 0, nullptr, 0, top + 1, nullptr, kActNone, {}, nullptr, 0, nullptr, 0, dx,
+                   dx_f32, lddx, a.rows, a.C, 0};
+        rc = finish_planes(r, planes, l.splits, l.ldp, s);
     }
     return rc;
 }

@@ -3,6 +3,7 @@
 // and the bias gradient's partial sums, then two products give dx and dw.
 #include "linear.cuh"
 
+#include "act.cuh"
 #include "common.cuh"
 #include "philox.cuh"
 #include "rowio.cuh"
@@ -25,39 +26,6 @@ int dz_groups(int M, int N) {
     const int most = (M + kDzRows - 1) / kDzRows;
     if (gy > most) gy = most;
     return gy < 1 ? 1 : gy;
-}
-
-// Derivatives of a pair of activations, from the same sigmoid as the forward's: gelu(z) = z h with
-// h = sigmoid(2u): h + z h (1 - h) 2u'; silu: h (1 + z (1 - h)).
-template <int ACT>
-__device__ __forceinline__ float2 act_grad_pair(float2 z) {
-    constexpr float kLog2 = 1.4426950408889634f;
-    if constexpr (ACT == kActRelu) {
-        return make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
-    } else if constexpr (ACT == kActGelu || ACT == kActSilu) {
-        const float2 one = make_float2(1.0f, 1.0f);
-        const float2 z2 = fmul2(z, z);
-        float2 t;
-        if constexpr (ACT == kActGelu) {
-            constexpr float c = -1.5957691216f * kLog2;
-            t = fmul2(ffma2(z2, make_float2(c * 0.044715f, c * 0.044715f), make_float2(c, c)), z);
-        } else {
-            t = fmul2(z, make_float2(-kLog2, -kLog2));
-        }
-        const float2 d = fadd2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), one);
-        const float2 h = make_float2(rcp_approx(d.x), rcp_approx(d.y));
-        const float2 g = ffma2(h, make_float2(-1.0f, -1.0f), one);  // 1 - h
-        if constexpr (ACT == kActGelu) {
-            constexpr float k = 1.5957691216f;
-            const float2 q =
-                fmul2(ffma2(z2, make_float2(k * 0.134145f, k * 0.134145f), make_float2(k, k)), z);
-            return ffma2(fmul2(h, g), q, h);
-        } else {
-            return fmul2(h, ffma2(z, g, one));
-        }
-    } else {
-        return make_float2(1.0f, 1.0f);
-    }
 }
 
 // dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable; with one row of
@@ -186,11 +154,139 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict
     }
 }
 
+// out = resid + drop(act(alpha sum_p planes[p] + bias)) over planes [n][M][ldp] of a product split
+// along K: a thread takes 8 columns, two planes' loads in flight. Bound by memory.
+template <typename TO>
+__global__ void __launch_bounds__(256) linear_finish_kernel(const RowsArgs a,
+                                                            const float* __restrict__ planes, int n,
+                                                            int ldp, uint32_t n8, uint32_t dr,
+                                                            uint32_t dc, int vec) {
+    pdl_enter();
+    const long long plane = (long long)a.M * ldp;
+    const float f = a.alpha ? *a.alpha : 1.0f;
+    DropKey key{};
+    if (a.drop.rng) key = drop_key(a.drop.rng, a.drop.site);
+    const uint32_t first = blockIdx.x * 256u + threadIdx.x;
+    uint32_t row = first / n8, c8 = first - row * n8;
+    const uint32_t rows = (uint32_t)a.M;
+    while (row < rows) {
+        const int col = (int)(c8 * 8), left = min(8, a.N - col);
+        const float* p = planes + (long long)row * ldp + col;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        for (int k0 = 0; k0 < n; k0 += 2) {
+            Raw8<float> q[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (k0 + k < n) load_raw(p + (k0 + k) * plane, q[k]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (k0 + k < n) {
+                    float w[8];
+                    raw_f32(q[k], w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += w[j];
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= f;
+        if (a.bias)
+            for (int j = 0; j < left; ++j) v[j] += a.bias[col + j];
+        if (a.pre)
+            for (int j = 0; j < left; ++j) a.pre[row * a.ld_pre + col + j] = __float2bfloat16_rn(v[j]);
+        with_act(a.act, [&](auto tag) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float2 y = act_pair<decltype(tag)::value>(make_float2(v[j], v[j + 1]));
+                v[j] = y.x;
+                v[j + 1] = y.y;
+            }
+        });
+        if (a.drop.rng) drop_apply8(key, c8, row, a.drop.thr, a.drop.scale, v);
+        TO* o = reinterpret_cast<TO*>(a.out) + row * a.ldo + col;
+        const TO* r = reinterpret_cast<const TO*>(a.resid) + row * a.ldr + col;
+        if (vec && left == 8) {
+            if (a.resid) {
+                Raw8<TO> q;
+                float w[8];
+                load_raw(r, q);
+                raw_f32(q, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += w[j];
+            }
+            store8(o, v);
+        } else {
+            for (int j = 0; j < left; ++j) o[j] = from_f32<TO>(a.resid ? v[j] + to_f32(r[j]) : v[j]);
+        }
+        row += dr;
+        c8 += dc;
+        if (c8 >= n8) {
+            c8 -= n8;
+            ++row;
+        }
+    }
+}
+
+template <typename TO>
+int launch_finish(const RowsArgs& a, const float* planes, int n, int ldp, cudaStream_t s) {
+    const uint32_t n8 = (uint32_t)(a.N + 7) / 8;
+    const long long items = (long long)a.M * n8, most = 148 * 8;
+    const uint32_t blocks = (uint32_t)((items + 255) / 256 < most ? (items + 255) / 256 : most);
+    const uint32_t step = blocks * 256;
+    const int vec = rows_on_16((const TO*)a.out, a.ldo) &&
+                    (!a.resid || rows_on_16((const TO*)a.resid, a.ldr));
+    return launch_kernel(linear_finish_kernel<TO>, (int)blocks, 256, 0, s, a, planes, n, ldp, n8,
+                         step / n8, step % n8, vec);
+}
+
+}  // namespace
+
+// A product whose 128 x 64 tiles fill less than half of the SMs walks its K on few of them, at about
+// 0.27 us a k-block; split along K it fills them, for a second kernel of about 4 us. 256 x 4096 x 512:
+// 18 us in one piece.
+int product_splits(int M, int N, int K) {
+    const long long tiles = (long long)((M + 127) / 128) * ((N + 63) / 64);
+    const int kb = (K + 63) / 64;
+    if (M <= kFewRows || tiles > 74 || kb < 32) return 1;
+    long long n = 148 / tiles;
+    if (n > kb / 8) n = kb / 8;
+    return n > 16 ? 16 : (int)n;
+}
+size_t product_work(int M, int N, int K) {
+    const int n = product_splits(M, N, K);
+    return n > 1 ? align256((size_t)n * M * ceil8(N) * 4) : 0;
+}
+
+int finish_planes(const RowsArgs& a, const float* planes, int n, int ldp, cudaStream_t s) {
+    return a.out_f32 ? launch_finish<float>(a, planes, n, ldp, s)
+                     : launch_finish<bf16>(a, planes, n, ldp, s);
+}
+
+namespace {
+
+// The k-split product of A and B into planes, then the epilogue `a`.
+int split_product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int K,
+                  int n, void* work, const RowsArgs& a, int num_sms, int* err, cudaStream_t s) {
+    GemmArgs g{};
+    g.epi = kEpiPlaneAdd;
+    g.out = work;
+    g.ldo = ceil8(a.N);
+    g.splits = n;
+    g.err = err;
+    const GemmExt x{};
+    GemmPlan plan;
+    int rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, a.M, a.N, K, g, 0, num_sms, &x);
+    if (rc) return rc;
+    if ((rc = gemm_run(plan, s)) != 0) return rc;
+    return finish_planes(a, reinterpret_cast<const float*>(work), n, (int)ceil8(a.N), s);
+}
+
 }  // namespace
 
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
             int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
-            int* err, cudaStream_t s, const float* alpha) {
+            int* err, cudaStream_t s, const float* alpha, void* work) {
     if (accumulate && !out_f32) return -1;
     if (M <= kFewRows && !a_mn) {
         RowsArgs r{A, lda, B, ldb, alpha, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo, nullptr, 0,
@@ -199,6 +295,11 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
     }
     if (K <= kOuterRows && a_mn && b_mn)
         return outer_product(A, lda, B, ldb, M, N, K, out, out_f32, ldo, accumulate, alpha, s);
+    if (const int n = work ? product_splits(M, N, K) : 1; n > 1) {
+        RowsArgs r{nullptr, 0, nullptr, 0, alpha, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo,
+                   nullptr, 0, out, out_f32, ldo, M, N, K};
+        return split_product(A, lda, a_mn, B, ldb, b_mn, K, n, work, r, num_sms, err, s);
+    }
     GemmArgs g{};
     g.out = out;
     g.ldo = ldo;
@@ -227,12 +328,16 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
     if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.act < kActNone || a.act > kActSilu) return -1;
     if (a.M == 0) return 0;
     if (!a.x || !a.w || !a.out) return -1;
-    if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw)) return kBadOperand;
-    if (a.M <= kFewRows) {
+    if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw) || !operand_ok(a.work, 0))
+        return kBadOperand;
+    const int n = a.work ? product_splits(a.M, a.N, a.K) : 1;
+    if (a.M <= kFewRows || n > 1) {
         RowsArgs r{a.x, a.ldx, a.w, a.ldw, nullptr, a.bias, a.act, a.drop, a.resid, a.ldr, a.pre, a.ld_pre,
                    a.out, a.out_f32, a.ldo, a.M, a.N, a.K};
         if (r.drop.thr == 0) r.drop.rng = nullptr;
-        return rows_product(r, a.w_mn_major, s);
+        return n > 1 ? split_product(a.x, a.ldx, 0, a.w, a.ldw, a.w_mn_major, a.K, n, a.work, r,
+                                     num_sms, a.err, s)
+                     : rows_product(r, a.w_mn_major, s);
     }
     GemmArgs g{};
     g.epi = kEpiLinear;
@@ -261,9 +366,13 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
 }
 
 size_t linear_backward_work(int M, int N, int K) {
-    (void)K;
-    if (M <= 0 || N <= 0) return 0;
-    return align256((size_t)M * ceil8(N) * 2) + align256((size_t)dz_groups(M, N) * N * 4);
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    // dw is [N, K] or [K, N]: the larger of the two; its planes follow dx's in the same place
+    size_t planes = product_work(M, K, N);
+    const size_t dw = product_work(N, K, M), dw_mn = product_work(K, N, M);
+    if (dw > planes) planes = dw;
+    if (dw_mn > planes) planes = dw_mn;
+    return align256((size_t)M * ceil8(N) * 2) + align256((size_t)dz_groups(M, N) * N * 4) + planes;
 }
 
 int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
@@ -288,6 +397,9 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
     const bool need_dz = !as_is && (a.dx || a.dw);
     const bf16* dz = reinterpret_cast<const bf16*>(a.dy);
     long long ldz = a.lddy;
+    void* planes = a.work ? reinterpret_cast<char*>(a.work) + align256((size_t)a.M * ceil8(a.N) * 2) +
+                                align256((size_t)dz_groups(a.M, a.N) * a.N * 4)
+                          : nullptr;
     if (need_dz || a.dbias) {
         if (!a.work || !aligned16(a.work)) return -1;
         bf16* buf = reinterpret_cast<bf16*>(a.work);
@@ -317,16 +429,16 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
     }
     if (a.dx) {  // dz [M,N] times w
         const int rc = product(dz, ldz, 0, a.w, a.ldw, a.w_mn_major ? 0 : 1, a.M, a.K, a.N, a.dx,
-                               a.dx_f32, a.lddx, 0, num_sms, a.err, s);
+                               a.dx_f32, a.lddx, 0, num_sms, a.err, s, nullptr, planes);
         if (rc) return rc;
     }
     if (a.dw) {
         const int rc =
             a.w_mn_major
                 ? product(a.x, a.ldx, 1, dz, ldz, 1, a.K, a.N, a.M, a.dw, a.dw_f32, a.lddw,
-                          a.accumulate, num_sms, a.err, s)
+                          a.accumulate, num_sms, a.err, s, nullptr, planes)
                 : product(dz, ldz, 1, a.x, a.ldx, 1, a.N, a.K, a.M, a.dw, a.dw_f32, a.lddw,
-                          a.accumulate, num_sms, a.err, s);
+                          a.accumulate, num_sms, a.err, s, nullptr, planes);
         if (rc) return rc;
     }
     return 0;

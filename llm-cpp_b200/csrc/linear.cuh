@@ -40,6 +40,7 @@ struct LinearFwd {
     int out_f32;
     long long ldo;
     int M, N, K;
+    void* work;  // product_work(M, N, K) bytes, 16-byte aligned; null: K is not split
     int* err;
 };
 int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s);
@@ -129,10 +130,17 @@ int outer_product(const bf16* A, long long lda, const bf16* B, long long ldb, in
                   void* out, int out_f32, long long ldo, int accumulate, const float* alpha,
                   cudaStream_t s);
 
+// Splits along K of a product with too few tiles for the device, and the bytes of their planes.
+int product_splits(int M, int N, int K);
+size_t product_work(int M, int N, int K);
+// out = resid + drop(act(alpha sum of planes [n][M][ldp] + bias)) (x, w of `a` unused); ldp: a
+// multiple of 8.
+int finish_planes(const RowsArgs& a, const float* planes, int n, int ldp, cudaStream_t s);
+
 // D[M,N] (+)= alpha A B^T on the tcgen05 kernels into bf16 or f32 `out`, any row stride (accumulate:
-// f32 only; alpha: device scalar, nullable).
+// f32 only; alpha: device scalar, nullable; work: product_work(M, N, K) bytes, or null).
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
             int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
-            int* err, cudaStream_t s, const float* alpha = nullptr);
+            int* err, cudaStream_t s, const float* alpha = nullptr, void* work = nullptr);
 
 }  // namespace llmgpu

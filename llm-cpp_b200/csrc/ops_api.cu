@@ -219,15 +219,19 @@ static bool linear_drop(float p, const uint64_t* rng, uint64_t site, DropArgs* d
     return true;
 }
 
+extern "C" long long llmgpu_op_linear_fwd_work(int M, int N, int K) {
+    return M > 0 && N > 0 && K > 0 ? (long long)product_work(M, N, K) : 0;
+}
+
 extern "C" int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long ldw,
                                     int w_mn_major, const float* bias, int act, float p,
                                     const uint64_t* rng, uint64_t site, const void* resid,
                                     long long ldr, void* pre, long long ld_pre, void* out,
-                                    int out_f32, long long ldo, int M, int N, int K, int* err,
-                                    void* stream) {
+                                    int out_f32, long long ldo, int M, int N, int K, void* work,
+                                    int* err, void* stream) {
     LinearFwd a{reinterpret_cast<const bf16*>(x), ldx, reinterpret_cast<const bf16*>(w), ldw,
                 w_mn_major != 0, bias, act, {}, resid, ldr, reinterpret_cast<bf16*>(pre), ld_pre,
-                out, out_f32 != 0, ldo, M, N, K, err};
+                out, out_f32 != 0, ldo, M, N, K, work, err};
     if (!linear_drop(p, rng, site, &a.drop)) return -1;
     if (M > 1 && (ldx < K || ldo < N || (resid && ldr < N) || (pre && ld_pre < N))) return -1;
     if (ldw < (w_mn_major ? N : K) && (w_mn_major ? K : N) > 1) return -1;

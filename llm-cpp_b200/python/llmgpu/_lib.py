@@ -57,7 +57,7 @@ def _declare(lib):
                                       c_int, c_float, c_vp, c_u64, c_vp]
     lib.llmgpu_op_linear_fwd.argtypes = [c_vp, c_ll, c_vp, c_ll, c_int, c_vp, c_int, c_float, c_vp,
                                          c_u64, c_vp, c_ll, c_vp, c_ll, c_vp, c_int, c_ll, c_int,
-                                         c_int, c_int, c_vp, c_vp]
+                                         c_int, c_int, c_vp, c_vp, c_vp]
     lib.llmgpu_op_linear_bwd.argtypes = [c_vp, c_int, c_ll, c_vp, c_ll, c_vp, c_ll, c_int, c_vp,
                                          c_ll, c_int, c_float, c_vp, c_u64, c_vp, c_int, c_ll, c_vp,
                                          c_int, c_ll, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp,
@@ -68,7 +68,7 @@ def _declare(lib):
                                             c_float, c_int, c_int, c_int, c_float, c_vp, c_int,
                                             c_ll, c_vp, c_int, c_ll, c_int, c_int, c_vp, c_vp,
                                             c_vp]
-    for n, k in (("llmgpu_op_linear_bwd_work", 3), ("llmgpu_op_linear_ce_fwd_work", 2),
+    for n, k in (("llmgpu_op_linear_fwd_work", 3), ("llmgpu_op_linear_bwd_work", 3), ("llmgpu_op_linear_ce_fwd_work", 2),
                  ("llmgpu_op_linear_ce_bwd_work", 4)):
         getattr(lib, n).argtypes = [c_int] * k
         getattr(lib, n).restype = c_ll

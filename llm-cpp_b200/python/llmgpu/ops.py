@@ -3,6 +3,8 @@
 Arguments are torch CUDA tensors (used only as device allocations); every call
 checks the status code and the device error word and raises on failure.
 """
+import functools
+
 import torch
 
 from ._lib import load
@@ -333,8 +335,19 @@ def _new(rows, cols, dtype, device):
     return t, t.data_ptr(), ld
 
 
-def _work(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(name, *sizes):
+    """A workspace's size, which goes by the call's sizes alone."""
+    return getattr(load(), name)(*sizes)
+
+
+def _work(name, device, *sizes):
+    """(tensor, address) of a new workspace, (None, 0) where none is needed."""
+    n = _work_bytes(name, *sizes)
+    if not n:
+        return None, 0
+    t = torch.empty(n, dtype=torch.uint8, device=device)
+    return t, t.data_ptr()
 
 
 def _drop(p, rng, device):
@@ -435,8 +448,9 @@ def linear_fwd(x, w, bias=None, act="none", p=0.0, rng=None, site=0, resid=None,
     pre = None
     if save_pre:
         pre, pp, ldp = _new(M, N, torch.bfloat16, dev)
+    work, pws = _work("llmgpu_op_linear_fwd_work", dev, M, N, K)
     _call("llmgpu_op_linear_fwd", dev, px, ldx, pw, ldw, w_mn, pb, a, p, prng, site, pr, ldr, pp, ldp,
-          po, out.dtype == torch.float32, ldo, M, N, K, _err_word(dev))
+          po, out.dtype == torch.float32, ldo, M, N, K, pws, _err_word(dev))
     return out, pre
 
 
@@ -471,10 +485,10 @@ def linear_bwd(dy, x, w, pre=None, act="none", p=0.0, rng=None, site=0, w_mn=Fal
         pb = _vector(dbias, "dbias", torch.float32, N, dev)
     else:
         dbias = None
-    work = _work(load().llmgpu_op_linear_bwd_work(M, N, K), dev)
+    work, pws = _work("llmgpu_op_linear_bwd_work", dev, M, N, K)
     _call("llmgpu_op_linear_bwd", dev, pdy, dy.dtype == torch.float32, lddy, px, ldx, pw, ldw, w_mn,
           pp, ldp, a, p, prng, site, pdx, dx_dtype == torch.float32, lddx, pdw,
-          need_dw and dw.dtype == torch.float32, lddw, pb, accumulate, M, N, K, work.data_ptr(),
+          need_dw and dw.dtype == torch.float32, lddw, pb, accumulate, M, N, K, pws,
           _err_word(dev))
     return dx, dw, dbias
 
@@ -494,9 +508,9 @@ def linear_cross_entropy_fwd(x, w, targets, smoothing=0.0, w_mn=False):
     (dev, rows, C, V, px, ldx, pw, ldw), pt = _head_args(x, w, targets, smoothing, w_mn)
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     lse = torch.empty(rows, dtype=torch.float32, device=dev)
-    work = _work(load().llmgpu_op_linear_ce_fwd_work(rows, V), dev)
+    work, pws = _work("llmgpu_op_linear_ce_fwd_work", dev, rows, V)
     _call("llmgpu_op_linear_ce_fwd", dev, px, ldx, pw, ldw, w_mn, pt, rows, C, V, smoothing,
-          loss.data_ptr(), lse.data_ptr(), work.data_ptr(), _err_word(dev))
+          loss.data_ptr(), lse.data_ptr(), pws, _err_word(dev))
     return loss, lse
 
 
@@ -521,9 +535,9 @@ def linear_cross_entropy_bwd(x, w, targets, lse, dloss=None, scale=1.0, smoothin
         dw, pdw, lddw = _grad_w(dw, w_mn, V, C, dev, accumulate)
     else:
         dw = None
-    work = _work(load().llmgpu_op_linear_ce_bwd_work(rows, C, V, piece), dev)
+    work, pws = _work("llmgpu_op_linear_ce_bwd_work", dev, rows, C, V, piece)
     _call("llmgpu_op_linear_ce_bwd", dev, px, ldx, pw, ldw, w_mn, pt, pl, pd, scale, rows, C, V,
           smoothing, pdx, dx_dtype == torch.float32, lddx, pdw,
-          need_dw and dw.dtype == torch.float32, lddw, accumulate, piece, work.data_ptr(),
+          need_dw and dw.dtype == torch.float32, lddw, accumulate, piece, pws,
           _err_word(dev))
     return dx, dw

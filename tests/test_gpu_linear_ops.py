@@ -176,7 +176,9 @@ def _linear_want(x, w, b, r, act, p, w_mn, rng, site):
 
 SHAPES = [(1, 8, 1), (1, 768, 2304), (2, 40, 7), (3, 16, 300), (7, 1024, 257), (8, 264, 64),
           (9, 72, 33), (64, 128, 512), (127, 200, 129), (130, 768, 96), (300, 765, 1021),
-          (513, 64, 640)]
+          (513, 64, 640), (16, 4100, 37), (17, 264, 48),
+          # products split along K: x w^T, dy w, dy^T x
+          (40, 2101, 130), (300, 2048, 64), (33, 72, 2304), (2500, 40, 77)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)

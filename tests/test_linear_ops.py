@@ -53,7 +53,7 @@ def test_empty_calls_do_nothing():
     lib = _lib()
     assert lib.llmgpu_op_dropout(None, 0, 8, None, 0, None, 0, 8, 0, 8, 0.5, None, 0, None) == 0
     assert lib.llmgpu_op_linear_fwd(None, 8, P, 8, 0, None, 0, 0.0, None, 0, None, 0, None, 0, None,
-                                    0, 8, 0, 8, 8, None, None) == 0
+                                    0, 8, 0, 8, 8, None, None, None) == 0
     assert lib.llmgpu_op_linear_ce_fwd(None, 8, P, 8, 0, None, 0, 8, 8, 0.0, None, None, None, None,
                                        None) == 0
     assert lib.llmgpu_op_linear_bwd_work(0, 8, 8) == 0
@@ -65,14 +65,16 @@ def test_empty_calls_do_nothing():
                                  dict(p=2.0), dict(p=0.5), dict(x=None), dict(w=None),
                                  dict(out=None), dict(ldx=8), dict(ldw=8), dict(ldo=8),
                                  dict(resid=P, ldr=8), dict(pre=P, ld_pre=8), dict(x=P + 2),
-                                 dict(ldx=17), dict(w=P + 8), dict(w_mn=1, ldw=8)])
+                                 dict(ldx=17), dict(w=P + 8), dict(w_mn=1, ldw=8),
+                                 dict(work=P + 8)])
 def test_linear_fwd_refusals(bad):
     a = dict(x=P, ldx=16, w=P, ldw=16, w_mn=0, act=0, p=0.0, resid=None, ldr=0, pre=None, ld_pre=0,
-             out=P, ldo=16, M=4, N=16, K=16)
+             out=P, ldo=16, M=4, N=16, K=16, work=P)
     a.update(bad)
     rc = _lib().llmgpu_op_linear_fwd(a["x"], a["ldx"], a["w"], a["ldw"], a["w_mn"], None, a["act"],
                                      a["p"], None, 0, a["resid"], a["ldr"], a["pre"], a["ld_pre"],
-                                     a["out"], 0, a["ldo"], a["M"], a["N"], a["K"], None, None)
+                                     a["out"], 0, a["ldo"], a["M"], a["N"], a["K"], a["work"], None,
+                                     None)
     assert rc in REFUSED
 
 
