@@ -642,33 +642,40 @@ __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const Gemm
             for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = v[j];
             __syncwarp();
             __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.aux) + row0 * a.ld_aux + col;
-            if (in)
-                for (int i = 0; i < nrows; ++i)
-                    p[i * a.ld_aux] = __float2bfloat16_rn(tile[i * 32 + (lane ^ i)]);
+            if (in) {
+#pragma unroll 8
+                for (int i = 0; i < 32; ++i)
+                    if (i < nrows) p[i * a.ld_aux] = __float2bfloat16_rn(tile[i * 32 + (lane ^ i)]);
+            }
             __syncwarp();
         }
         linear_act_drop(x, key, col0, row0 + lane, v);
 #pragma unroll
         for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = v[j];
         __syncwarp();
-        if (in && x.out_f32) {
-            float* p = reinterpret_cast<float*>(a.out) + row0 * a.ldo + col;
-            const float* q = reinterpret_cast<const float*>(x.resid) + row0 * x.ldr + col;
-#pragma unroll 4
-            for (int i = 0; i < nrows; ++i) {
-                float o = tile[i * 32 + (lane ^ i)];
-                if (x.resid) o += q[i * x.ldr];
-                p[i * a.ldo] = o;
+        // eight rows at a time, the residual's loads of all eight in flight
+        const long long o0 = row0 * a.ldo + col, q0 = row0 * x.ldr + col;
+#pragma unroll 1
+        for (int i0 = 0; i0 < nrows; i0 += 8) {
+            float o[8], q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                q[i] = 0.0f;
+                if (x.resid && in && i0 + i < nrows)
+                    q[i] = x.out_f32 ? reinterpret_cast<const float*>(x.resid)[q0 + (i0 + i) * x.ldr]
+                                     : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(
+                                           x.resid)[q0 + (i0 + i) * x.ldr]);
             }
-        } else if (in) {
-            __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + row0 * a.ldo + col;
-            const __nv_bfloat16* q =
-                reinterpret_cast<const __nv_bfloat16*>(x.resid) + row0 * x.ldr + col;
-#pragma unroll 4
-            for (int i = 0; i < nrows; ++i) {
-                float o = tile[i * 32 + (lane ^ i)];
-                if (x.resid) o += __bfloat162float(q[i * x.ldr]);
-                p[i * a.ldo] = __float2bfloat16_rn(o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = tile[(i0 + i) * 32 + (lane ^ (i0 + i))] + q[i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!in || i0 + i >= nrows) continue;
+                if (x.out_f32)
+                    reinterpret_cast<float*>(a.out)[o0 + (i0 + i) * a.ldo] = o[i];
+                else
+                    reinterpret_cast<__nv_bfloat16*>(a.out)[o0 + (i0 + i) * a.ldo] =
+                        __float2bfloat16_rn(o[i]);
             }
         }
         __syncwarp();
@@ -681,7 +688,7 @@ __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const Gemm
 __device__ __forceinline__ int linear_box_end(const GemmArgs& a, const GemmExt& x, int row0, int n0,
                                               int c_begin, int c_end, int u) {
     const int ce = epi_chunk_end(a, row0, n0, c_begin, c_end);
-    if ((a.N & (x.out_f32 ? 3 : 7)) == 0 || n0 + ce * 32 < a.N) return ce;
+    if ((a.N & (x.out_f32 && !a.aux ? 3 : 7)) == 0 || n0 + ce * 32 < a.N) return ce;
     const int whole = (a.N - n0 - c_begin * 32) / (32 * u) * u;  // chunks of whole boxes
     return min(ce, c_begin + max(whole, 0));
 }
@@ -704,16 +711,31 @@ __device__ __forceinline__ void linear_prefetch(const GemmArgs& a, const GemmExt
     __syncwarp();
 }
 
+// `pre` of one lane's 32 columns, 16 bytes at a time (pre's rows are on 16 bytes; N is a multiple of 8
+// where its last columns come here).
+__device__ __forceinline__ void linear_pre_row(const GemmArgs& a, int row, int col0,
+                                               const float (&v)[32]) {
+    uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.aux) + row * a.ld_aux + col0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (col0 + 8 * q < a.N)
+            p[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                              pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
+                              pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+}
+
 // resid + drop(act(acc + bias)) through swizzled boxes and bulk stores: f32 outputs 32 columns at a
-// time, bf16 outputs 64 (with `pre` beside them, 32 of each). A residual arrives by bulk loads
-// in the box that it is combined in, one unit ahead where a warp has two boxes (SLOTS).
+// time, bf16 outputs 64 (with `pre` beside them, 32 of each; beside an f32 output or a residual there
+// is no room, and a lane stores its row's 64 bytes of `pre` itself). A residual arrives by bulk
+// loads in the box that it is combined in, one unit ahead where a warp has two boxes (SLOTS).
 template <int SLOTS>
 __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt& x,
                                                 const DropKey& key, const CUtensorMap* tmO,
                                                 const CUtensorMap* tmX, uint32_t tbase, int row0,
                                                 int n0, int lane, EpiWarp& w, int c_begin,
                                                 int c_end) {
-    const int u = (x.out_f32 || a.aux) ? 1 : 2;
+    const bool pre_box = a.aux && !x.pre_direct;
+    const int u = (x.out_f32 || pre_box) ? 1 : 2;
     const int ce = linear_box_end(a, x, row0, n0, c_begin, c_end, u);
     const bool res = x.resid != nullptr;
 #pragma unroll 1
@@ -743,9 +765,13 @@ __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt
             tmem_ld_32x32b_x32(tbase + (uint32_t)((c + h) * 32), r);
             tmem_ld_wait();
             linear_bias(a, x, col0, lane, r, v);
-            if (a.aux) box_put_bf16(box, lane, v);
+            if (pre_box)
+                box_put_bf16(box, lane, v);
+            else if (a.aux && row0 + lane < a.M)
+                linear_pre_row(a, row0 + lane, col0, v);
+            __syncwarp();
             linear_act_drop(x, key, col0, row0 + lane, v);
-            if (a.aux) {
+            if (pre_box) {
                 box_put_bf16(box + 2048, lane, v);
             } else if (x.out_f32) {
 #pragma unroll
@@ -784,7 +810,7 @@ __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-            if (a.aux) {
+            if (pre_box) {
                 tma_store_3d(tmX, box, n0 + c * 32, row0, 0);
                 tma_store_3d(tmO, box + 2048, n0 + c * 32, row0, 0);
             } else {
@@ -2154,14 +2180,14 @@ bool plan_tma_epilogue(GemmPlan* plan, const GemmArgs& a) {
     return true;
 }
 
-// Tensor maps of the linear epilogue's boxes; false where a stride or address does not allow
-// them, or for the pairs of outputs that one box does not hold (those take linear_turned_tile).
-bool plan_linear_boxes(GemmPlan* plan, const GemmArgs& a, const GemmExt& x) {
-    if ((x.resid || x.out_f32) && a.aux) return false;
+// Tensor maps of the linear epilogue's boxes; false where a stride or address does not allow them
+// (linear_turned_tile then). pre_direct: `pre` has no box.
+bool plan_linear_boxes(GemmPlan* plan, const GemmArgs& a, const GemmExt& x, bool pre_direct) {
+    if (pre_direct && ((reinterpret_cast<uintptr_t>(a.aux) & 15) || (a.ld_aux & 7))) return false;
     auto plane = [&](uint64_t ld_bytes) { return (ld_bytes * (uint64_t)a.M + 15) & ~(uint64_t)15; };
     const uint64_t es = x.out_f32 ? 4 : 2;
     const uint64_t os = (uint64_t)a.ldo * es;
-    const bool wide = !x.out_f32 && !a.aux;
+    const bool wide = !x.out_f32 && (!a.aux || pre_direct);
     if (make_tmap_box(&plan->tmO, a.out, x.out_f32 != 0, (uint64_t)a.N, (uint64_t)a.M, 1, os,
                       plane(os), wide))
         return false;
@@ -2171,7 +2197,7 @@ bool plan_linear_boxes(GemmPlan* plan, const GemmArgs& a, const GemmExt& x) {
         if (make_tmap_box(&plan->tmX, x.resid, x.out_f32 != 0, (uint64_t)a.N, (uint64_t)a.M, 1, rs,
                           plane(rs), wide))
             return false;
-    } else if (a.aux) {
+    } else if (a.aux && !pre_direct) {
         const uint64_t xs = (uint64_t)a.ld_aux * 2;
         if (make_tmap_box(&plan->tmX, a.aux, false, (uint64_t)a.N, (uint64_t)a.M, 1, xs, plane(xs)))
             return false;
@@ -2298,6 +2324,43 @@ int launch_pair(const GemmPlan& p, cudaStream_t stream) {
 
 }  // namespace
 
+// Estimated time in us, with constants fitted to graph replays of some 45 shapes (8192 x 64 x 64 to
+// 8192 x 8192 x 8192) on each tile: the first tile's k-blocks and the last one's epilogue stand
+// alone, the waves between take the longer of the two, and a launch has a fixed part. An epilogue
+// beyond a plain store costs a one-CTA tile, whose four warps drain all its columns, more than a
+// pair's sixteen. Where a pair is within 2% it is taken: it moves a third less through shared
+// memory, which counts under the power cap.
+int gemm_pick_tile(int M, int N, int K, int splits, double epi_weight, bool head, bool wide_256,
+                   int num_sms) {
+    struct Tile {
+        int bn;
+        double kb, store, more, fixed;
+    };
+    // the pair's plain store runs on 8 warps, its linear epilogue on 16
+    const Tile tiles[4] = {{kGemmPairTile, 0.36, epi_weight > 1.0 ? 2.0 : 3.4, 2.5, 3.2},
+                           {256, 0.37, 2.1, 5.5, 2.6},
+                           {128, 0.26, 1.3, 3.0, 2.4},
+                           {64, 0.22, 1.0, 1.65, 2.4}};
+    const double kb = (double)((K + BK - 1) / BK) / splits;
+    double best = 1e30;
+    int bn = 128;
+    for (const Tile& t : tiles) {
+        if (head && (t.bn == 256 || t.bn == 64)) continue;  // the tiles its kernels have
+        if (!wide_256 && t.bn == 256) continue;
+        const bool pair = t.bn == kGemmPairTile;
+        const int bm = pair ? 256 : BM, w = pair ? 256 : t.bn;
+        const long long n = (long long)((M + bm - 1) / bm) * ((N + w - 1) / w) * splits;
+        const int slots = pair ? pair_max_clusters(num_sms) : num_sms;
+        const double epi = t.store + (epi_weight - 1.0) * t.more, mma = kb * t.kb;
+        const double c = (double)((n + slots - 1) / slots - 1) * std::max(mma, epi) + mma + epi + t.fixed;
+        if (c < best * (pair ? 1.0 : 0.98)) {
+            best = c;
+            bn = t.bn;
+        }
+    }
+    return bn;
+}
+
 int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major, const void* B,
                    long long ldb, int b_mn_major, int M, int N, int K, const GemmArgs& epi,
                    int bn_hint, int num_sms, const GemmExt* ext) {
@@ -2353,6 +2416,19 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
     const bool chained = a.epi == kEpiLinear && ext->out_f32 && kblocks > kChainBlocks;
     const bool pair_ok = a.grp_mode != kGroupRows;  // a pair tile spans 256 rows of one group
     int bn = bn_hint;
+    if (bn == 0 && ext) {
+        // what the epilogue does beside storing, in units of a plain bf16 store
+        double weight = a.epi == kEpiHeadStats ? 1.6 : a.epi == kEpiHeadGrad ? 2.0 : 1.0;
+        if (a.epi == kEpiLinear)
+            weight += (ext->act >= kActGelu ? 0.8 : 0.1) + (ext->rng ? 0.8 : 0.0) +
+                      (ext->resid ? 0.6 : 0.0) + (a.aux ? 0.5 : 0.0) + (ext->out_f32 ? 0.5 : 0.0);
+        else if (a.epi == kEpiPlaneAdd)
+            weight = 1.3;
+        bn = gemm_pick_tile(M, N, K, a.splits, weight, head, !chained, num_sms);
+#ifdef TUNE
+        if (const char* e = std::getenv("TUNE_BN")) if (a.epi == kEpiLinear && !(chained && atoi(e) == 256)) bn = atoi(e);
+#endif
+    }
     if (bn == kGemmPairTile && !pair_ok) return -44;
     if (bn == 256 && chained) return -46;
     if (bn != 64 && bn != 128 && bn != 256 && bn != kGemmPairTile) {
@@ -2363,8 +2439,6 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
         const int cands[4] = {kGemmPairTile, 256, 128, 64};
         for (int i = pair_ok ? 0 : 1; i < 4; ++i) {
             const int c = cands[i];
-            if (head && c != kGemmPairTile && c != 128) continue;  // the tiles its kernels have
-            if (chained && c == 256) continue;  // 256 sums a thread do not fit in registers
             double cost;
             if (c == kGemmPairTile) {
                 const long long tiles = (long long)((M + 255) / 256) * ((N + 255) / 256) * a.splits;
@@ -2387,7 +2461,8 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
     if (ext) {
         if (head && bn != kGemmPairTile && bn != 128) return -46;
         if (a.epi == kEpiLinear) {
-            a.tma_epi = plan_linear_boxes(plan, a, *ext) ? 1 : 0;
+            plan->ext.pre_direct = a.aux && (ext->resid || ext->out_f32);
+            a.tma_epi = plan_linear_boxes(plan, a, *ext, plan->ext.pre_direct != 0) ? 1 : 0;
             plan->ext.chain = chained ? kChainBlocks : 0;
         }
         if (a.epi == kEpiHeadGrad || a.epi == kEpiPlaneAdd) {

@@ -45,6 +45,7 @@ struct GemmExt {
     uint32_t drop_thr;
     float drop_scale;
     int chain;            // set by the planner: k-blocks of one accumulator chain, 0: all of them
+    int pre_direct;       // set by the planner: aux is stored by the lanes, not through a box
     // kEpiHeadStats, kEpiHeadGrad: row m's target (left out unless in [0, V)), V = all columns
     // of the vocabulary, this product's column 0 being column v0 of it
     const int32_t* targets;
@@ -132,6 +133,11 @@ struct GemmPlan {
 int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major, const void* B,
                    long long ldb, int b_mn_major, int M, int N, int K, const GemmArgs& epi,
                    int bn_hint, int num_sms, const GemmExt* ext = nullptr);
+// The tile (64, 128, 256 or kGemmPairTile) estimated to run an ungrouped product soonest, for bn_hint.
+// `epi_weight`: the epilogue's work relative to a plain store. wide_256: whether 128 x 256 tiles are
+// open to it.
+int gemm_pick_tile(int M, int N, int K, int splits, double epi_weight, bool head, bool wide_256,
+                   int num_sms);
 // Launches a plan on a stream.
 int gemm_run(const GemmPlan& plan, cudaStream_t stream);
 // CTA pairs of the pair-tile kernel that can be resident at once.

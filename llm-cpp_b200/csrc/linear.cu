@@ -311,7 +311,8 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
     if (!alpha && aligned16(out) && (ldo % per16) == 0 && (N % per16) == 0) {
         g.epi = out_f32 ? kEpiStoreF32 : kEpiStoreBF16;
         g.accumulate = accumulate;
-        rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, M, N, K, g, 0, num_sms);
+        rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, M, N, K, g,
+                            gemm_pick_tile(M, N, K, 1, 1.0, false, true, num_sms), num_sms);
     } else {  // scaled, or rows that no 16-byte store reaches or that end inside one
         GemmExt x{};
         x.alpha = alpha;
