@@ -537,7 +537,14 @@ __device__ __forceinline__ void epilogue_tile(const GemmArgs& a, const CUtensorM
 // ---------------------------------------------------------------------------- epilogue families
 // The epilogues that take a GemmExt are compiled into kernels of their own: family 0 is every
 // epilogue above.
-enum GemmFamily : int { kFamBase = 0, kFamLinear = 1, kFamHeadStats = 2, kFamHeadGrad = 3 };
+enum GemmFamily : int {
+    kFamBase = 0,
+    kFamLinear = 1,
+    kFamHeadStats = 2,
+    kFamHeadGrad = 3,
+    kFamLinearAny = 4  // kFamLinear for outputs that boxes do not reach, wholly or at a row's end
+};
+constexpr bool is_linear(int fam) { return fam == kFamLinear || fam == kFamLinearAny; }
 struct NoExt {};
 template <int FAM>
 struct ExtOf {
@@ -616,9 +623,39 @@ __device__ __forceinline__ void linear_act_drop(const GemmExt& x, const DropKey&
     }
 }
 
-// Outputs (and a residual) of any stride and alignment, and the rare pairs of them that the boxes
-// below do not cover: a lane's 32 columns are turned through 4 KB of the warp's shared memory (32
-// rows of 32 floats, column j of row i at j ^ i), so that every access to global memory is 32 neighbouring columns of a row.
+__device__ __forceinline__ float turned_in(const float* p) { return *p; }
+__device__ __forceinline__ float turned_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void turned_out(float* p, float v) { *p = v; }
+__device__ __forceinline__ void turned_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+// Column `lane` of the turned tile's rows, plus the residual, eight rows' loads in flight.
+template <typename T>
+__device__ __forceinline__ void turned_rows(const float* tile, int lane, bool in, int nrows, T* o,
+                                            long long ldo, const T* resid, long long at,
+                                            long long ldr) {
+    if (!in) return;
+    if (!resid) {
+#pragma unroll 8
+        for (int i = 0; i < nrows; ++i) turned_out(o + i * ldo, tile[i * 32 + (lane ^ i)]);
+        return;
+    }
+    const T* q = resid + at;
+    for (int i0 = 0; i0 < nrows; i0 += 8) {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i < nrows) r[i] = turned_in(q + (i0 + i) * ldr);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i < nrows)
+                turned_out(o + (i0 + i) * ldo, tile[(i0 + i) * 32 + (lane ^ (i0 + i))] + r[i]);
+    }
+}
+
+// Outputs (and a residual) of any stride and alignment, and the last columns of a row that ends
+// inside 16 bytes: a lane's 32 columns are turned through 4 KB of the warp's shared memory (32 rows
+// of 32 floats, column j of row i at j ^ i), so that every access to global memory is 32
+// neighbouring columns of a row. In a kernel of its own (kFamLinearAny): its registers spilled in
+// the tiles that do without it.
 __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const GemmExt& x,
                                                    const DropKey& key, uint32_t tbase, int row0,
                                                    int n0, int lane, EpiWarp& w, int c_begin,
@@ -653,31 +690,13 @@ __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const Gemm
 #pragma unroll
         for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = v[j];
         __syncwarp();
-        // eight rows at a time, the residual's loads of all eight in flight
-        const long long o0 = row0 * a.ldo + col, q0 = row0 * x.ldr + col;
-#pragma unroll 1
-        for (int i0 = 0; i0 < nrows; i0 += 8) {
-            float o[8], q[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[i] = 0.0f;
-                if (x.resid && in && i0 + i < nrows)
-                    q[i] = x.out_f32 ? reinterpret_cast<const float*>(x.resid)[q0 + (i0 + i) * x.ldr]
-                                     : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(
-                                           x.resid)[q0 + (i0 + i) * x.ldr]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = tile[(i0 + i) * 32 + (lane ^ (i0 + i))] + q[i];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!in || i0 + i >= nrows) continue;
-                if (x.out_f32)
-                    reinterpret_cast<float*>(a.out)[o0 + (i0 + i) * a.ldo] = o[i];
-                else
-                    reinterpret_cast<__nv_bfloat16*>(a.out)[o0 + (i0 + i) * a.ldo] =
-                        __float2bfloat16_rn(o[i]);
-            }
-        }
+        if (x.out_f32)
+            turned_rows(tile, lane, in, nrows, reinterpret_cast<float*>(a.out) + row0 * a.ldo + col,
+                        a.ldo, reinterpret_cast<const float*>(x.resid), row0 * x.ldr + col, x.ldr);
+        else
+            turned_rows(tile, lane, in, nrows,
+                        reinterpret_cast<__nv_bfloat16*>(a.out) + row0 * a.ldo + col, a.ldo,
+                        reinterpret_cast<const __nv_bfloat16*>(x.resid), row0 * x.ldr + col, x.ldr);
         __syncwarp();
     }
 }
@@ -728,7 +747,7 @@ __device__ __forceinline__ void linear_pre_row(const GemmArgs& a, int row, int c
 // time, bf16 outputs 64 (with `pre` beside them, 32 of each; beside an f32 output or a residual there
 // is no room, and a lane stores its row's 64 bytes of `pre` itself). A residual arrives by bulk
 // loads in the box that it is combined in, one unit ahead where a warp has two boxes (SLOTS).
-template <int SLOTS>
+template <int SLOTS, bool ANY>
 __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt& x,
                                                 const DropKey& key, const CUtensorMap* tmO,
                                                 const CUtensorMap* tmX, uint32_t tbase, int row0,
@@ -820,7 +839,7 @@ __device__ __forceinline__ void linear_box_tile(const GemmArgs& a, const GemmExt
         }
         w.slot ^= SLOTS - 1;
     }
-    if (ce < c_end && n0 + ce * 32 < a.N && row0 < a.M) {
+    if (ANY && ce < c_end && n0 + ce * 32 < a.N && row0 < a.M) {
         if (lane == 0) bulk_wait_group_read<0>();  // the boxes are about to be reused
         __syncwarp();
         linear_turned_tile(a, x, key, tbase, row0, n0, lane, w, ce, c_end);
@@ -891,7 +910,7 @@ __device__ __forceinline__ bool tile_kblocks(const GemmArgs& a, const int* s_grp
 // k-blocks of a chain of a tile whose k-blocks are [kb0, kb1).
 template <int FAM>
 __device__ __forceinline__ int chain_blocks(const typename ExtOf<FAM>::type& x, int kb0, int kb1) {
-    if constexpr (FAM == kFamLinear) {
+    if constexpr (is_linear(FAM)) {
         if (x.chain > 0) return x.chain;
     }
     return kb1 - kb0;
@@ -1075,11 +1094,12 @@ __device__ __forceinline__ void family_tile(const GemmArgs& a,
     if constexpr (FAM == kFamBase) {
         epilogue_tile<NCOLS>(a, tmO, tmX, tbase, empty, row0, n0, split, g, lane, w, c_begin,
                              c_end);
-    } else if constexpr (FAM == kFamLinear) {
+    } else if constexpr (is_linear(FAM)) {
         if (a.epi == kEpiPlaneAdd)
             plane_epilogue_tile<NCOLS, SLOTS>(a, tmO, tbase, row0, n0, split, lane, w, c_begin, c_end);
-        else if (a.tma_epi)
-            linear_box_tile<SLOTS>(a, x, key, tmO, tmX, tbase, row0, n0, lane, w, c_begin, c_end);
+        else if (FAM == kFamLinear || a.tma_epi)
+            linear_box_tile<SLOTS, FAM == kFamLinearAny>(a, x, key, tmO, tmX, tbase, row0, n0, lane, w,
+                                                         c_begin, c_end);
         else
             linear_turned_tile(a, x, key, tbase, row0, n0, lane, w, c_begin, c_end);
     } else if constexpr (FAM == kFamHeadStats) {
@@ -1092,7 +1112,7 @@ __device__ __forceinline__ void family_tile(const GemmArgs& a,
 // The dropout key of an epilogue warp, read once.
 template <int FAM>
 __device__ __forceinline__ DropKey family_key(const typename ExtOf<FAM>::type& x) {
-    if constexpr (FAM == kFamLinear) {
+    if constexpr (is_linear(FAM)) {
         if (x.rng) return drop_key(x.rng, x.site);
     }
     return DropKey{};
@@ -1250,7 +1270,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const int ck = chain_blocks<FAM>(ext, kb0, kb1);
             int kc = kb0;
             do {
-                const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
+                const int kend = is_linear(FAM) ? min(kc + ck, kb1) : kb1;
                 if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1u, args.err,
                                     kDevTimeoutAccFree)) {
                     ok = false;
@@ -1290,7 +1310,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
                 kc = kend;
-            } while (FAM == kFamLinear && kc < kb1);
+            } while (is_linear(FAM) && kc < kb1);
         }
     } else if (warp >= 4) {
         // ---------------- epilogue warpgroup
@@ -1311,7 +1331,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 return mbar_wait_bounded(&acc_full[i], ph, args.err, kDevTimeoutAcc);
             };
             bool ready;
-            if constexpr (FAM == kFamLinear && BN <= 128) {
+            if constexpr (is_linear(FAM) && BN <= 128) {
                 linear_prefetch<2>(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
                 const int ck = chain_blocks<FAM>(ext, kb0, kb1);
                 const int chains = (kb1 - kb0 + ck - 1) / ck;
@@ -1321,7 +1341,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                                             [&](int i) { mbar_arrive(&acc_empty[i]); })
                             : wait_acc(acc, acc_phase);
             } else {
-                if constexpr (FAM == kFamLinear)
+                if constexpr (is_linear(FAM))
                     linear_prefetch<2>(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
                 ready = wait_acc(acc, acc_phase);
             }
@@ -1370,8 +1390,8 @@ struct PairCfgOf {
     static constexpr int STAGES = FAM == kFamHeadStats ? 7 : FAM == kFamHeadGrad ? 6 : 5;
     // The linear epilogue runs on four warps a scheduler (8192 x 1024 x 4096 gelu: 122k -> 110k
     // cycles), whose boxes then come to one a warp; the head's are no faster for it.
-    static constexpr int EPI_WARPS = FAM == kFamLinear ? 16 : kPairEpiWarps;
-    static constexpr int EPI_SLOTS = FAM == kFamLinear || FAM == kFamHeadGrad ? 1 : 2;
+    static constexpr int EPI_WARPS = is_linear(FAM) ? 16 : kPairEpiWarps;
+    static constexpr int EPI_SLOTS = is_linear(FAM) || FAM == kFamHeadGrad ? 1 : 2;
     static constexpr int EPI_COLS = BN / (EPI_WARPS / 4);  // columns of a warp
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
     static constexpr int EPI_BYTES =
@@ -1693,7 +1713,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 int kc = kb0;
                 do {
-                    const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
+                    const int kend = is_linear(FAM) ? min(kc + ck, kb1) : kb1;
                     if (!mbar_wait_warp_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
                                                 kDevTimeoutAccFree)) {
                         ok = false;
@@ -1735,7 +1755,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1u;
                     kc = kend;
-                } while (FAM == kFamLinear && kc < kb1);
+                } while (is_linear(FAM) && kc < kb1);
             }
         }
     } else if (NG == 2 && warp == 0) {
@@ -1850,7 +1870,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 int kc = kb0;
                 do {
-                    const int kend = FAM == kFamLinear ? min(kc + ck, kb1) : kb1;
+                    const int kend = is_linear(FAM) ? min(kc + ck, kb1) : kb1;
                     if (!mbar_wait_bounded_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
                                                    kDevTimeoutAccFree)) {
                         ok = false;
@@ -1886,7 +1906,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1u;
                     kc = kend;
-                } while (FAM == kFamLinear && kc < kb1);
+                } while (is_linear(FAM) && kc < kb1);
             }
         }
     } else if (warp >= 4) {
@@ -1925,7 +1945,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                 return mbar_wait_bounded_cluster(&acc_full[i], ph, err, kDevTimeoutAcc);
             };
             bool ready;
-            if constexpr (FAM == kFamLinear) {
+            if constexpr (is_linear(FAM)) {
                 linear_prefetch<Cfg::EPI_SLOTS>(args, P.ext, &P.tmX[g], m0 + q * 32, n0, lane, ew,
                                 part * kChunks, (part + 1) * kChunks);
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
@@ -2652,6 +2672,14 @@ int gemm_run(const GemmPlan& p, cudaStream_t stream) {
             return pair ? launch_pair<kFamHeadGrad>(p, stream)
                         : launch_bn<128, kFamHeadGrad>(p, stream);
         case kEpiLinear:
+            // rows that leave in whole boxes, or any
+            if (!p.args.tma_epi || (p.args.N & (p.ext.out_f32 && !p.args.aux ? 3 : 7)) != 0) {
+                if (pair) return launch_pair<kFamLinearAny>(p, stream);
+                if (p.bn == 256) return launch_bn<256, kFamLinearAny>(p, stream);
+                return p.bn == 128 ? launch_bn<128, kFamLinearAny>(p, stream)
+                                   : launch_bn<64, kFamLinearAny>(p, stream);
+            }
+            [[fallthrough]];
         case kEpiPlaneAdd:
             if (pair) return launch_pair<kFamLinear>(p, stream);
             if (p.bn == 256) return launch_bn<256, kFamLinear>(p, stream);
