@@ -154,23 +154,24 @@ def _linear_case(dev, M, K, N, act, p, out, resid, bias, w_mn, seed, pad=0):
 
 
 def _linear_want(x, w, b, r, act, p, w_mn, rng, site):
-    wd = w.double().cpu() if w_mn else w.double().cpu().t()
-    xd = x.double().cpu()
+    wd = w.double() if w_mn else w.double().t()
+    xd = x.double()
     z = xd @ wd
     ez = (x.shape[1] + 4) * ACC * (xd.abs() @ wd.abs())
     if b is not None:
-        z = z + b.double().cpu()
-        ez = ez + H32 * (z.abs() + b.double().cpu().abs())
+        z = z + b.double()
+        ez = ez + H32 * (z.abs() + b.double().abs())
     y = ref.act(z, act)
     # an activation's slope is at most 1.13; its sigmoid is off by a few steps times its argument
     e = 1.13 * ez + (8 + 2 * ref.sigmoid_arg(z, act).abs()) * 2 * H32 * y.abs()
     if p > 0:
         keep, scale = ref.keep_mask(int(rng[0]), int(rng[1]) + site, *z.shape, p)
+        keep = keep.to(z.device)
         y, e = torch.where(keep, y * scale, 0.0), torch.where(keep, e * scale, 0.0)
         e = e + 2 * H32 * y.abs()
     if r is not None:
-        y = y + r.double().cpu()
-        e = e + H32 * (y.abs() + r.double().cpu().abs())
+        y = y + r.double()
+        e = e + H32 * (y.abs() + r.double().abs())
     return z, ez, y, e
 
 
@@ -178,7 +179,9 @@ SHAPES = [(1, 8, 1), (1, 768, 2304), (2, 40, 7), (3, 16, 300), (7, 1024, 257), (
           (9, 72, 33), (64, 128, 512), (127, 200, 129), (130, 768, 96), (300, 765, 1021),
           (513, 64, 640), (16, 4100, 37), (17, 264, 48),
           # products split along K: x w^T, dy w, dy^T x
-          (40, 2101, 130), (300, 2048, 64), (33, 72, 2304), (2500, 40, 77)]
+          (40, 2101, 130), (300, 2048, 64), (33, 72, 2304), (2500, 40, 77),
+          # tiles of 128 and 256 columns and of CTA pairs, whole and ragged
+          (2048, 768, 768), (2100, 1100, 1304), (2100, 1100, 1301), (8192, 128, 512)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
@@ -209,13 +212,14 @@ def test_linear_fwd(cuda, M, K, N, act, p, out, resid, bias, w_mn):
 
 
 def _linear_bwd_want(dy, x, w, pre, act, p, w_mn, rng, site):
-    dz = dy.double().cpu()
+    dz = dy.double()
     if p > 0:
         keep, scale = ref.keep_mask(int(rng[0]), int(rng[1]) + site, *dz.shape, p)
+        keep = keep.to(dz.device)
         dz = torch.where(keep, dz * scale, 0.0)
     e = 4 * H32 * dz.abs()
     if act != "none":
-        zd = pre.double().cpu()
+        zd = pre.double()
         gr = ref.act_grad(zd, act)
         # h + z h (1 - h) c: each sigmoid off by a few steps times its argument
         h = torch.sigmoid(ref.sigmoid_arg(zd, act))
@@ -223,8 +227,8 @@ def _linear_bwd_want(dy, x, w, pre, act, p, w_mn, rng, site):
         eg = (16 + 4 * ref.sigmoid_arg(zd, act).abs()) * 2 * H32 * mag if act != "relu" else 0.0
         e = dz.abs() * eg + e * gr.abs()
         dz = dz * gr
-    xd = x.double().cpu()
-    wd = w.double().cpu().t() if w_mn else w.double().cpu()  # [N, K]
+    xd = x.double()
+    wd = w.double().t() if w_mn else w.double()  # [N, K]
     dx, dw = dz @ wd, dz.t() @ xd
     ex = (H16 * dz.abs() + e) @ wd.abs() + (dz.shape[1] + 4) * ACC * (dz.abs() @ wd.abs())
     ew = (H16 * dz.abs() + e).t() @ xd.abs() + (dz.shape[0] + 4) * ACC * (dz.abs().t() @ xd.abs())
@@ -322,17 +326,17 @@ def _head_case(dev, rows, C, V, w_mn, ignored, seed, sharp=3.0):
 
 
 def _head_want(x, w, t, d, scale, smoothing, w_mn):
-    xd, wd = x.double().cpu(), w.double().cpu()
+    xd, wd = x.double(), w.double()
     if w_mn:
         wd = wd.t()
-    loss, lse, z, y, valid = ref.head(xd, wd, t.cpu(), smoothing)
+    loss, lse, z, y, valid = ref.head(xd, wd, t, smoothing)
     V, C = wd.shape
     ez = (C + 4) * ACC * (xd.abs() @ wd.abs().t())
     el = ez.amax(1) + (4 * H32) * (1 + lse.abs()) + 16 * H32
     # smoothing adds V terms of size smoothing / (V - 1): lse - z, each off by ez + el, summed in f32
     eloss = 2 * el + ez.amax(1) + 4 * H32 * loss.abs() + \
         smoothing * 4 * H32 * (lse.abs() + z.abs().amax(1)) * (1 + math.log2(V))
-    coef = torch.where(valid, d.double().cpu() * scale, 0.0)[:, None]
+    coef = torch.where(valid, d.double() * scale, 0.0)[:, None]
     p = (z - lse[:, None]).exp()
     gr = coef * (p - y)
     eg = coef.abs() * (p * (ez + el[:, None] + (z - lse[:, None]).abs() * 4 * H32 + 8 * H32) +
@@ -346,7 +350,8 @@ def _head_want(x, w, t, d, scale, smoothing, w_mn):
 
 
 HEADS = [(1, 64, 1, 0), (1, 768, 5003, 0), (5, 8, 100, 256), (33, 72, 257, 256), (256, 128, 256, 0),
-         (130, 200, 1000, 512), (300, 765, 3001, 1024), (513, 264, 2048, 2048), (64, 64, 20011, 0)]
+         (130, 200, 1000, 512), (300, 765, 3001, 1024), (513, 264, 2048, 2048), (64, 64, 20011, 0),
+         (1030, 768, 5003, 2560), (2048, 1024, 8192, 0)]
 
 
 @pytest.mark.parametrize("rows,C,V,piece", HEADS)
@@ -542,6 +547,79 @@ def test_gradients_against_differences(cuda):
             reach = float(dy.double().abs().sum()) / 0.75 / (1 if at == 0 else 48) * 4
             tol = reach * (0.6 * h * h / 6 + 8 * H16 + 2 * H16 + 64 * H32 / h)
             assert abs(got - want) <= tol, (at, got, want, tol)
+
+
+# ------------------------------------------------------------------------------ large matrices
+def test_linear_offsets_past_32_bits(cuda):
+    """Results and gradients of more than 2^31 elements: rows on both sides of the border."""
+    from llmgpu import ops
+    M, K, N = 70000, 64, 32768
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.randn(M, K, generator=g, device=cuda).to(BF)
+    w = (torch.randn(N, K, generator=g, device=cuda) * 0.2).to(BF)
+    rng = _rng(cuda, 8, 9)
+    rows = torch.tensor([0, 1, 40000, 65535, 65536, 65537, M - 1])
+    keep, scale = _rows_mask(8, 9, rows, N, 0.25)
+    keep = keep.to(cuda)
+    y, pre = ops.linear_fwd(x, w, None, "gelu", 0.25, rng, save_pre=True)
+    rows = rows.to(cuda)
+    z, ez, _, _ = _linear_want(x[rows], w, None, None, "gelu", 0.0, False, rng, 0)
+    want = torch.where(keep, ref.act(z, "gelu") * scale, 0.0)
+    tol = scale * (1.13 * ez + (8 + 2 * ref.sigmoid_arg(z, "gelu").abs()) * 2 * H32 *
+                   ref.act(z, "gelu").abs()) + (H16 + 2 * H32) * want.abs()
+    _close(y[rows], want, tol, "y")
+    _close(pre[rows], z, ez + H16 * (z.abs() + ez), "pre")
+    dy = y  # any matrix of that size
+    dx, dw, db = ops.linear_bwd(dy, x, w, pre, "gelu", 0.25, rng)
+    dz = torch.where(keep, dy[rows].double() * scale, 0.0) * ref.act_grad(pre[rows].double(), "gelu")
+    _norm_close(dx[rows], dz @ w.double(), NORM16, "dx")
+    # dw and dbias over all rows, in 64 bits on the device
+    n0, n1 = 17, 33
+    keep_n = _rows_mask(8, 9, torch.arange(M), n1, 0.25)[0][:, n0:n1].to(cuda)
+    zc = pre[:, n0:n1].double()
+    dzc = torch.where(keep_n, dy[:, n0:n1].double() * scale, 0.0) * ref.act_grad(zc, "gelu")
+    _norm_close(dw[n0:n1], dzc.t() @ x.double(), NORM16, "dw")
+    _norm_close(db[n0:n1], dzc.sum(0), 1e-5, "dbias")
+    ops.check_device(cuda)
+
+
+def _rows_mask(seed, offset, rows, cols, p):
+    """ref.keep_mask for some rows of a matrix."""
+    import numpy as np
+    n8 = (cols + 7) // 8
+    one = np.ones((len(rows), n8), dtype=np.uint64)
+    words = ref.philox([one * np.arange(n8, dtype=np.uint64), one * rows.numpy().astype(np.uint64)[:, None],
+                        one * np.uint64(offset), one * np.uint64(0)], (seed, 0))
+    lanes = np.stack([(v >> np.uint64(16 * h)) & np.uint64(0xFFFF) for v in words for h in (0, 1)], -1)
+    t = round(p * 65536)
+    keep = lanes.reshape(len(rows), n8 * 8)[:, :cols].astype(np.int64) >= t
+    return torch.from_numpy(keep), 65536 / (65536 - t)
+
+
+def test_loss_head_of_many_rows(cuda):
+    """70000 rows by 33000 classes: 2.3e9 logits, in pieces of the library's choice."""
+    from llmgpu import ops
+    rows, C, V = 70000, 64, 33000
+    g = torch.Generator(device=cuda).manual_seed(2)
+    x = torch.randn(rows, C, generator=g, device=cuda).to(BF)
+    w = (torch.randn(V, C, generator=g, device=cuda) * 0.4).to(BF)
+    t = torch.randint(-1, V, (rows,), generator=g, device=cuda, dtype=torch.int32)
+    d = torch.rand(rows, generator=g, device=cuda) / rows
+    loss, lse = ops.linear_cross_entropy_fwd(x, w, t)
+    dx, dw = ops.linear_cross_entropy_bwd(x, w, t, lse, d)
+    wd = w.double()
+    want_dw = torch.zeros(V, C, dtype=torch.float64, device=cuda)
+    for r in range(0, rows, 2000):
+        s = slice(r, r + 2000)
+        ls, le, z, y, valid = ref.head(x[s].double(), wd, t[s], 0.0)
+        # sums of 33000 exponentials in f32, each slot of 128 merged in turn; logits of 64 products
+        assert float((loss[s].double() - ls).abs().max()) < 2e-5
+        assert float((lse[s].double() - le).abs().max()) < 2e-5
+        gr = torch.where(valid, d[s].double(), 0.0)[:, None] * ((z - le[:, None]).exp() - y)
+        _norm_close(dx[s], gr @ wd, NORM16, "dx")
+        want_dw += gr.t() @ x[s].double()
+    _norm_close(dw, want_dw, NORM16, "dw")
+    ops.check_device(cuda)
 
 
 # ----------------------------------------------------------------------------- used together
