@@ -47,15 +47,28 @@ struct GemmCfg {
 
 __device__ __forceinline__ void decode_tile(int t, int num_m, int num_n, int tiles_mn, int& m_blk,
                                             int& n_blk, int& split) {
-    split = t / tiles_mn;
+    split = t < tiles_mn ? 0 : t / tiles_mn;
     int r = t - split * tiles_mn;
     int per_group = kGroupM * num_n;
     int g = r / per_group;
     int first_m = g * kGroupM;
     int gm = min(kGroupM, num_m - first_m);
     int local = r - g * per_group;
-    m_blk = first_m + local % gm;
-    n_blk = local / gm;
+    n_blk = gm == kGroupM ? local / kGroupM : local / gm;
+    m_blk = first_m + local - n_blk * gm;
+}
+
+// k-blocks [kb0, kb1) of a split. Without splits nothing is divided (50257 x 128 x 768: 42.7k -> 40.2k
+// cycles without the two 64-bit divisions a tile).
+__device__ __forceinline__ void split_range(const GemmArgs& a, int split, int kblocks, int& kb0,
+                                            int& kb1) {
+    if (a.splits <= 1) {
+        kb0 = 0;
+        kb1 = kblocks;
+    } else {
+        kb0 = (int)((long long)split * kblocks / a.splits);
+        kb1 = (int)((long long)(split + 1) * kblocks / a.splits);
+    }
 }
 
 // Resolves tile t into block coordinates, group and k-block range [kb0, kb1). Returns false
@@ -76,8 +89,7 @@ __device__ __forceinline__ bool tile_work(const GemmArgs& a, const int* s_grp, i
         kb0 = min(max(s_grp[g] / BK, 0), kblocks);
         kb1 = min(max(s_grp[g + 1] / BK, kb0), kblocks);
     } else {
-        kb0 = (int)((long long)split * kblocks / a.splits);
-        kb1 = (int)((long long)(split + 1) * kblocks / a.splits);
+        split_range(a, split, kblocks, kb0, kb1);
     }
     return true;
 }
@@ -896,9 +908,7 @@ __device__ __forceinline__ bool tile_kblocks(const GemmArgs& a, const int* s_grp
                                              int num_n, int tiles_mn, int kblocks, int& kb0,
                                              int& kb1) {
     if constexpr (FAM != kFamBase) {
-        const int split = a.splits > 1 ? t / tiles_mn : 0;
-        kb0 = a.splits > 1 ? (int)((long long)split * kblocks / a.splits) : 0;
-        kb1 = a.splits > 1 ? (int)((long long)(split + 1) * kblocks / a.splits) : kblocks;
+        split_range(a, a.splits > 1 ? t / tiles_mn : 0, kblocks, kb0, kb1);
         return true;
     } else {
         int m_blk, n_blk, split, g;
