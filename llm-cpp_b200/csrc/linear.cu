@@ -1,6 +1,9 @@
 // Linear layer with bias, activation, dropout and residual applied where the product's tiles leave
 // tensor memory (gemm.cu, kEpiLinear), and its backward: one elementwise pass forms dz in bf16
-// and the bias gradient's partial sums, then two products give dx and dw.
+// and the bias gradient's partial sums, then two products give dx and dw. dz is rounded to bf16
+// because it is a tensor-core operand; the bias gradient is summed before that rounding.
+// 8192 x 1024 x 4096: forward gelu 64 us (cuBLAS's bare product 57), backward 133 us (34 dz, 4
+// dbias, 95 the products); 8192 x 4096 x 1024 with dropout and f32 residual 69 us.
 #include "linear.cuh"
 
 #include "act.cuh"
@@ -30,7 +33,8 @@ int dz_groups(int M, int N) {
 
 // dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable; with one row of
 // blocks it is dbias itself, added to when `accumulate`). `vec`: rows of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a time, their
-// loads in flight together as raw words: bound by memory at 8192 x 4096 bf16 (201 MB).
+// loads in flight together as raw words. Bound by memory: 8192 x 4096 bf16 gelu, 201 MB, 34 us
+// (5.9 TB/s).
 constexpr int kDzInFlight = 2;
 template <typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long lddy,

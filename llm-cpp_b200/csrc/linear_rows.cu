@@ -1,7 +1,8 @@
 // Linear-layer products of a few rows (decoding, single sequences): the weights are streamed once,
 // 16 bytes a lane straight into mma.sync fragments, with no tile, tensor map or staging between.
 // The legacy matrix instructions carry them because a tcgen05 tile is 128 rows high, and the bound
-// is the weights' bytes: 16 x 4096 x 4096 took 18 us on 64-wide tcgen05 tiles.
+// is the weights' bytes: 4096 x 4096 (33.5 MB) takes 7.4 us for 1 row, 8.9 for 16, where 64-wide tcgen05
+// tiles took 18 us; 1 x 1024 x 4096 3.5 us.
 #include "common.cuh"
 #include "linear.cuh"
 #include "philox.cuh"
