@@ -209,6 +209,19 @@ int llmgpu_op_linear_ce_bwd(const void* x, long long ldx, const void* w, long lo
                             int dw_f32, long long lddw, int accumulate, int piece, void* work,
                             int* err, void* stream);
 
+/* The operators above from a block of arguments, for bindings that pay for each one (ctypes converts
+ * the 23 of llmgpu_op_linear_fwd in 2.3 us, a block in 0.5): `args` holds the integer and pointer
+ * arguments of the call in their order, 8 bytes each, the stream last, then its float arguments as
+ * doubles. An integer that does not fit its argument's type returns -1. */
+enum {
+    LLMGPU_CALL_DROPOUT = 0,
+    LLMGPU_CALL_LINEAR_FWD = 1,
+    LLMGPU_CALL_LINEAR_BWD = 2,
+    LLMGPU_CALL_LINEAR_CE_FWD = 3,
+    LLMGPU_CALL_LINEAR_CE_BWD = 4
+};
+int llmgpu_op_call(int op, const void* args);
+
 /* Number of SMs the library sizes persistent grids for (device 0 of the caller). */
 int llmgpu_op_num_sms(void);
 /* CTA pairs (clusters of two SMs) the 256x256-tile GEMM keeps resident at once. */

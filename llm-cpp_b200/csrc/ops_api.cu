@@ -1,6 +1,7 @@
 // Kernel-level C ABI (include/llmgpu_ops.h): thin wrappers that run one kernel
 // on caller-owned device buffers, used by the per-kernel parity tests.
 #include <cuda_runtime.h>
+#include <string.h>
 
 #include "dropout.cuh"
 #include "gemm.cuh"
@@ -295,4 +296,165 @@ extern "C" int llmgpu_op_linear_ce_bwd(const void* x, long long ldx, const void*
     return head_backward(a, lse, dloss, scale, dx, dx_f32 != 0, lddx, dw, dw_f32 != 0, lddw,
                          accumulate != 0, piece, device_num_sms(),
                          reinterpret_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+// Reads a block of llmgpu_op_call: 8-byte integers and pointers, then doubles.
+struct Block {
+    const char* at;
+    bool fits = true;
+    int64_t word() {
+        int64_t v;
+        memcpy(&v, at, 8);
+        at += 8;
+        return v;
+    }
+    void* ptr() { return reinterpret_cast<void*>((uintptr_t)word()); }
+    template <typename T>
+    T* of() {
+        return reinterpret_cast<T*>((uintptr_t)word());
+    }
+    int i() {
+        const int64_t v = word();
+        if (v != (int64_t)(int)v) fits = false;
+        return (int)v;
+    }
+    float f() {
+        double v;
+        memcpy(&v, at, 8);
+        at += 8;
+        return (float)v;
+    }
+};
+
+}  // namespace
+
+extern "C" int llmgpu_op_call(int op, const void* args) {
+    if (!args) return -1;
+    Block b{reinterpret_cast<const char*>(args)};
+    // the arguments are read one statement each: a call's own argument list has no order
+    switch (op) {
+        case LLMGPU_CALL_DROPOUT: {
+            const void* x = b.ptr();
+            const int x_f32 = b.i();
+            const long long ldx = b.word();
+            const void* resid = b.ptr();
+            const long long ldr = b.word();
+            void* out = b.ptr();
+            const int out_f32 = b.i();
+            const long long ldo = b.word();
+            const int rows = b.i(), cols = b.i();
+            const uint64_t* rng = b.of<const uint64_t>();
+            const uint64_t site = (uint64_t)b.word();
+            void* stream = b.ptr();
+            const float p = b.f();
+            if (!b.fits) return -1;
+            return llmgpu_op_dropout(x, x_f32, ldx, resid, ldr, out, out_f32, ldo, rows, cols, p, rng,
+                                     site, stream);
+        }
+        case LLMGPU_CALL_LINEAR_FWD: {
+            const void* x = b.ptr();
+            const long long ldx = b.word();
+            const void* w = b.ptr();
+            const long long ldw = b.word();
+            const int w_mn = b.i();
+            const float* bias = b.of<const float>();
+            const int act = b.i();
+            const uint64_t* rng = b.of<const uint64_t>();
+            const uint64_t site = (uint64_t)b.word();
+            const void* resid = b.ptr();
+            const long long ldr = b.word();
+            void* pre = b.ptr();
+            const long long ld_pre = b.word();
+            void* out = b.ptr();
+            const int out_f32 = b.i();
+            const long long ldo = b.word();
+            const int M = b.i(), N = b.i(), K = b.i();
+            void* work = b.ptr();
+            int* err = b.of<int>();
+            void* stream = b.ptr();
+            const float p = b.f();
+            if (!b.fits) return -1;
+            return llmgpu_op_linear_fwd(x, ldx, w, ldw, w_mn, bias, act, p, rng, site, resid, ldr, pre,
+                                        ld_pre, out, out_f32, ldo, M, N, K, work, err, stream);
+        }
+        case LLMGPU_CALL_LINEAR_BWD: {
+            const void* dy = b.ptr();
+            const int dy_f32 = b.i();
+            const long long lddy = b.word();
+            const void* x = b.ptr();
+            const long long ldx = b.word();
+            const void* w = b.ptr();
+            const long long ldw = b.word();
+            const int w_mn = b.i();
+            const void* pre = b.ptr();
+            const long long ld_pre = b.word();
+            const int act = b.i();
+            const uint64_t* rng = b.of<const uint64_t>();
+            const uint64_t site = (uint64_t)b.word();
+            void* dx = b.ptr();
+            const int dx_f32 = b.i();
+            const long long lddx = b.word();
+            void* dw = b.ptr();
+            const int dw_f32 = b.i();
+            const long long lddw = b.word();
+            float* dbias = b.of<float>();
+            const int accumulate = b.i(), M = b.i(), N = b.i(), K = b.i();
+            void* work = b.ptr();
+            int* err = b.of<int>();
+            void* stream = b.ptr();
+            const float p = b.f();
+            if (!b.fits) return -1;
+            return llmgpu_op_linear_bwd(dy, dy_f32, lddy, x, ldx, w, ldw, w_mn, pre, ld_pre, act, p, rng,
+                                        site, dx, dx_f32, lddx, dw, dw_f32, lddw, dbias, accumulate, M,
+                                        N, K, work, err, stream);
+        }
+        case LLMGPU_CALL_LINEAR_CE_FWD: {
+            const void* x = b.ptr();
+            const long long ldx = b.word();
+            const void* w = b.ptr();
+            const long long ldw = b.word();
+            const int w_mn = b.i();
+            const int32_t* targets = b.of<const int32_t>();
+            const int rows = b.i(), C = b.i(), V = b.i();
+            float* row_loss = b.of<float>();
+            float* lse = b.of<float>();
+            void* work = b.ptr();
+            int* err = b.of<int>();
+            void* stream = b.ptr();
+            const float smoothing = b.f();
+            if (!b.fits) return -1;
+            return llmgpu_op_linear_ce_fwd(x, ldx, w, ldw, w_mn, targets, rows, C, V, smoothing,
+                                           row_loss, lse, work, err, stream);
+        }
+        case LLMGPU_CALL_LINEAR_CE_BWD: {
+            const void* x = b.ptr();
+            const long long ldx = b.word();
+            const void* w = b.ptr();
+            const long long ldw = b.word();
+            const int w_mn = b.i();
+            const int32_t* targets = b.of<const int32_t>();
+            const float* lse = b.of<const float>();
+            const float* dloss = b.of<const float>();
+            const int rows = b.i(), C = b.i(), V = b.i();
+            void* dx = b.ptr();
+            const int dx_f32 = b.i();
+            const long long lddx = b.word();
+            void* dw = b.ptr();
+            const int dw_f32 = b.i();
+            const long long lddw = b.word();
+            const int accumulate = b.i(), piece = b.i();
+            void* work = b.ptr();
+            int* err = b.of<int>();
+            void* stream = b.ptr();
+            const float scale = b.f(), smoothing = b.f();
+            if (!b.fits) return -1;
+            return llmgpu_op_linear_ce_bwd(x, ldx, w, ldw, w_mn, targets, lse, dloss, scale, rows, C, V,
+                                           smoothing, dx, dx_f32, lddx, dw, dw_f32, lddw, accumulate,
+                                           piece, work, err, stream);
+        }
+        default:
+            return -1;
+    }
 }

@@ -68,6 +68,8 @@ def _declare(lib):
                                             c_float, c_int, c_int, c_int, c_float, c_vp, c_int,
                                             c_ll, c_vp, c_int, c_ll, c_int, c_int, c_vp, c_vp,
                                             c_vp]
+    lib.llmgpu_op_call.argtypes = [c_int, ctypes.c_char_p]
+    lib.llmgpu_op_call.restype = c_int
     for n, k in (("llmgpu_op_linear_fwd_work", 3), ("llmgpu_op_linear_bwd_work", 3), ("llmgpu_op_linear_ce_fwd_work", 2),
                  ("llmgpu_op_linear_ce_bwd_work", 4)):
         getattr(lib, n).argtypes = [c_int] * k

@@ -4,6 +4,7 @@ Arguments are torch CUDA tensors (used only as device allocations); every call
 checks the status code and the device error word and raises on failure.
 """
 import functools
+import struct
 
 import torch
 
@@ -270,22 +271,29 @@ def check_device(device="cuda"):
             raise KernelError(f"device error code {code}")
 
 
-_fns = {}
+# llmgpu_op_call's number and block of each operator: integers and addresses in the order of the C
+# call (the one unsigned word is `site`), the stream last, then the floats
+_BLOCKS = {
+    "llmgpu_op_dropout": (0, struct.Struct("11qQq1d").pack),
+    "llmgpu_op_linear_fwd": (1, struct.Struct("8qQ13q1d").pack),
+    "llmgpu_op_linear_bwd": (2, struct.Struct("12qQ14q1d").pack),
+    "llmgpu_op_linear_ce_fwd": (3, struct.Struct("14q1d").pack),
+    "llmgpu_op_linear_ce_bwd": (4, struct.Struct("22q2d").pack),
+}
 # the raw handle of a device's current stream, without making a Stream object (3 us a call)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _call(name, device, *args):
-    """The C entry point on the current stream of `device`."""
-    fn = _fns.get(name)
-    if fn is None:
-        fn = _fns[name] = getattr(load(), name)
+def _call(name, device, ints, *floats):
+    """The C entry point on the current stream of `device`, its arguments in one block."""
+    op, pack = _BLOCKS[name]
     i = device.index
+    fn = load().llmgpu_op_call
     if i == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(i))
+        rc = fn(op, pack(*ints, _raw_stream(i), *floats))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(i))
+            rc = fn(op, pack(*ints, _raw_stream(i), *floats))
     if rc != 0:
         raise KernelError(f"{name} failed with status {rc}")
 
@@ -380,6 +388,7 @@ def _grad_w(dw, w_mn, rows, cols, device, accumulate):
 
 
 _FLOATS = (torch.float32, torch.bfloat16)
+_U64 = 2 ** 64 - 1
 _BF16 = (torch.bfloat16,)
 
 
@@ -403,8 +412,9 @@ def dropout_fwd(x, p, rng, site=0, resid=None, out=None, out_dtype=None):
     pr = ldr = 0
     if resid is not None:
         pr, ldr = _matrix(resid, "resid", (out.dtype,), rows, cols, dev)
-    _call("llmgpu_op_dropout", dev, px, x.dtype == torch.float32, ldx, pr, ldr, po,
-          out.dtype == torch.float32, ldo, rows, cols, p, prng, site)
+    _call("llmgpu_op_dropout", dev,
+          (px, x.dtype == torch.float32, ldx, pr, ldr, po, out.dtype == torch.float32, ldo, rows, cols,
+           prng, site & _U64), p)
     return out
 
 
@@ -449,8 +459,9 @@ def linear_fwd(x, w, bias=None, act="none", p=0.0, rng=None, site=0, resid=None,
     if save_pre:
         pre, pp, ldp = _new(M, N, torch.bfloat16, dev)
     work, pws = _work("llmgpu_op_linear_fwd_work", dev, M, N, K)
-    _call("llmgpu_op_linear_fwd", dev, px, ldx, pw, ldw, w_mn, pb, a, p, prng, site, pr, ldr, pp, ldp,
-          po, out.dtype == torch.float32, ldo, M, N, K, pws, _err_word(dev))
+    _call("llmgpu_op_linear_fwd", dev,
+          (px, ldx, pw, ldw, w_mn, pb, a, prng, site & _U64, pr, ldr, pp, ldp, po,
+           out.dtype == torch.float32, ldo, M, N, K, pws, _err_word(dev)), p)
     return out, pre
 
 
@@ -486,10 +497,10 @@ def linear_bwd(dy, x, w, pre=None, act="none", p=0.0, rng=None, site=0, w_mn=Fal
     else:
         dbias = None
     work, pws = _work("llmgpu_op_linear_bwd_work", dev, M, N, K)
-    _call("llmgpu_op_linear_bwd", dev, pdy, dy.dtype == torch.float32, lddy, px, ldx, pw, ldw, w_mn,
-          pp, ldp, a, p, prng, site, pdx, dx_dtype == torch.float32, lddx, pdw,
-          need_dw and dw.dtype == torch.float32, lddw, pb, accumulate, M, N, K, pws,
-          _err_word(dev))
+    _call("llmgpu_op_linear_bwd", dev,
+          (pdy, dy.dtype == torch.float32, lddy, px, ldx, pw, ldw, w_mn, pp, ldp, a, prng, site & _U64,
+           pdx, dx_dtype == torch.float32, lddx, pdw, need_dw and dw.dtype == torch.float32, lddw, pb,
+           accumulate, M, N, K, pws, _err_word(dev)), p)
     return dx, dw, dbias
 
 
@@ -509,8 +520,9 @@ def linear_cross_entropy_fwd(x, w, targets, smoothing=0.0, w_mn=False):
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     lse = torch.empty(rows, dtype=torch.float32, device=dev)
     work, pws = _work("llmgpu_op_linear_ce_fwd_work", dev, rows, V)
-    _call("llmgpu_op_linear_ce_fwd", dev, px, ldx, pw, ldw, w_mn, pt, rows, C, V, smoothing,
-          loss.data_ptr(), lse.data_ptr(), pws, _err_word(dev))
+    _call("llmgpu_op_linear_ce_fwd", dev,
+          (px, ldx, pw, ldw, w_mn, pt, rows, C, V, loss.data_ptr(), lse.data_ptr(), pws,
+           _err_word(dev)), smoothing)
     return loss, lse
 
 
@@ -536,8 +548,8 @@ def linear_cross_entropy_bwd(x, w, targets, lse, dloss=None, scale=1.0, smoothin
     else:
         dw = None
     work, pws = _work("llmgpu_op_linear_ce_bwd_work", dev, rows, C, V, piece)
-    _call("llmgpu_op_linear_ce_bwd", dev, px, ldx, pw, ldw, w_mn, pt, pl, pd, scale, rows, C, V,
-          smoothing, pdx, dx_dtype == torch.float32, lddx, pdw,
-          need_dw and dw.dtype == torch.float32, lddw, accumulate, piece, pws,
-          _err_word(dev))
+    _call("llmgpu_op_linear_ce_bwd", dev,
+          (px, ldx, pw, ldw, w_mn, pt, pl, pd, rows, C, V, pdx, dx_dtype == torch.float32, lddx, pdw,
+           need_dw and dw.dtype == torch.float32, lddw, accumulate, piece, pws, _err_word(dev)),
+          scale, smoothing)
     return dx, dw

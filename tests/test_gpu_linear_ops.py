@@ -731,6 +731,49 @@ def test_two_calls_at_once(cuda):
             assert torch.equal(got[i][k], want[i][k]), (i, k)
 
 
+def test_plain_c_calls_equal_the_wrappers(cuda):
+    """Each C entry point called with its own argument list, on a stream of its own."""
+    from llmgpu import load, ops
+    lib = load()
+    g = torch.Generator().manual_seed(5)
+    M, K, N = 70, 96, 136
+    x, w = _mat(g, M, K, BF, cuda)[0], _mat(g, N, K, BF, cuda, 0.1)[0]
+    b = torch.randn(N, generator=g).to(cuda)
+    r = torch.randn(M, N, generator=g).to(cuda)
+    t = torch.randint(-1, N, (M,), generator=g, dtype=torch.int32).to(cuda)
+    d = torch.rand(M, generator=g).to(cuda)
+    rng = _rng(cuda, 3, 1 << 50)
+    want = [ops.dropout_fwd(x, 0.3, rng, 2 ** 63 + 5)]
+    want += ops.linear_fwd(x, w, b, "gelu", 0.2, rng, 7, r, out_dtype=F32, save_pre=True)
+    want += ops.linear_bwd(r, x, w, want[2], "gelu", 0.2, rng, 7)
+    want += ops.linear_cross_entropy_fwd(x, w, t, 0.1)
+    want += ops.linear_cross_entropy_bwd(x, w, t, want[7], d, 3.0, 0.1)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    got = [torch.zeros_like(v) for v in want]
+    work = torch.empty(1 << 24, dtype=torch.uint8, device=cuda)
+    torch.cuda.synchronize()
+    st, ld = s.cuda_stream, x.stride(0)
+
+    def p(v):
+        return v.data_ptr()
+    assert lib.llmgpu_op_dropout(p(x), 0, ld, None, 0, p(got[0]), 0, K, M, K, 0.3, p(rng), 2 ** 63 + 5,
+                                 st) == 0
+    assert lib.llmgpu_op_linear_fwd(p(x), ld, p(w), w.stride(0), 0, p(b), 2, 0.2, p(rng), 7, p(r), N,
+                                    p(got[2]), N, p(got[1]), 1, N, M, N, K, p(work), None, st) == 0
+    assert lib.llmgpu_op_linear_bwd(p(r), 1, N, p(x), ld, p(w), w.stride(0), 0, p(want[2]), N, 2, 0.2,
+                                    p(rng), 7, p(got[3]), 0, K, p(got[4]), 0, K, p(got[5]), 0, M, N, K,
+                                    p(work), None, st) == 0
+    assert lib.llmgpu_op_linear_ce_fwd(p(x), ld, p(w), w.stride(0), 0, p(t), M, K, N, 0.1, p(got[6]),
+                                       p(got[7]), p(work), None, st) == 0
+    assert lib.llmgpu_op_linear_ce_bwd(p(x), ld, p(w), w.stride(0), 0, p(t), p(want[7]), p(d), 3.0, M, K,
+                                       N, 0.1, p(got[8]), 0, K, p(got[9]), 0, K, 0, 0, p(work), None,
+                                       st) == 0
+    torch.cuda.synchronize()
+    for i, (a, c) in enumerate(zip(got, want)):
+        assert torch.equal(a, c), i
+
+
 # ------------------------------------------------------------------------------------ refusals
 def test_wrapper_refusals(cuda):
     from llmgpu import ops

@@ -129,6 +129,35 @@ def test_workspace_covers_any_piece():
     assert f(100, 64, 5000, 8192) == f(100, 64, 5000, 1 << 20) == f(100, 64, 5000, 0)
 
 
+def test_block_call_refusals():
+    """llmgpu_op_call: an unknown operator, no block, an integer past its argument's type, and the
+    refusals of the calls themselves."""
+    from llmgpu import ops
+    lib = _lib()
+
+    def call(name, *args):
+        op, pack = ops._BLOCKS[name]
+        return lib.llmgpu_op_call(op, pack(*args))
+    drop = [P, 0, 8, 0, 0, P, 0, 8, 4, 8, P, 0, 0, 0.5]
+    assert lib.llmgpu_op_call(0, None) == -1 and lib.llmgpu_op_call(99, b"\0" * 256) == -1
+    assert call("llmgpu_op_dropout", *drop[:8], 0, *drop[9:]) == 0  # no rows
+    for i, bad in ((0, 0), (2, 7), (8, 1 << 33), (9, (1 << 30) + 1), (10, 0), (13, 1.5)):
+        assert call("llmgpu_op_dropout", *drop[:i], bad, *drop[i + 1:]) == -1
+    fwd = [P, 16, P, 16, 0, 0, 0, 0, 0, 0, 0, 0, 0, P, 0, 16, 4, 16, 16, 0, 0, 0, 0.0]
+    assert call("llmgpu_op_linear_fwd", *fwd[:16], 0, *fwd[17:]) == 0
+    for i, bad in ((0, 0), (0, P + 2), (1, 8), (6, 4), (16, 1 << 40), (18, 0), (22, 2.0)):
+        assert call("llmgpu_op_linear_fwd", *fwd[:i], bad, *fwd[i + 1:]) in REFUSED
+    bwd = [P, 1, 16, P, 16, P, 16, 0, 0, 16, 0, 0, 0, P, 0, 16, P, 0, 16, P, 0, 4, 16, 16, P, 0, 0, 0.0]
+    for i, bad in ((0, 0), (2, 8), (10, 1), (20, 1), (22, 1 << 32), (24, 0), (27, 0.5)):
+        assert call("llmgpu_op_linear_bwd", *bwd[:i], bad, *bwd[i + 1:]) in REFUSED
+    cef = [P, 16, P, 16, 0, P, 4, 16, 32, P, P, P, 0, 0, 0.0]
+    for i, bad in ((0, 0), (5, 0), (6, -1), (8, 1 << 35), (11, 0), (14, 1.0)):
+        assert call("llmgpu_op_linear_ce_fwd", *cef[:i], bad, *cef[i + 1:]) in REFUSED
+    ceb = [P, 16, P, 16, 0, P, P, 0, 4, 16, 32, P, 0, 16, P, 0, 16, 0, 0, P, 0, 0, 1.0, 0.0]
+    for i, bad in ((0, 0), (6, 0), (17, 1), (18, 100), (19, 0), (23, -0.5)):
+        assert call("llmgpu_op_linear_ce_bwd", *ceb[:i], bad, *ceb[i + 1:]) in REFUSED
+
+
 def test_wrappers_refuse_cpu_tensors():
     from llmgpu import ops
     x, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
