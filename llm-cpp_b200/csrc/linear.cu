@@ -26,7 +26,7 @@ constexpr int kDzRows = 8;    // rows in flight, one per warp
 int dz_groups(int M, int N) {
     const int gx = (N + kDzCols - 1) / kDzCols;
     int gy = (148 * 8 + gx - 1) / gx;
-    const int most = (M + kDzRows - 1) / kDzRows;
+    const int most = (M + 2 * kDzRows - 1) / (2 * kDzRows);  // two rows a warp at least
     if (gy > most) gy = most;
     return gy < 1 ? 1 : gy;
 }
