@@ -2443,7 +2443,8 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
     }
     const int num_m = (M + BM - 1) / BM;
     // f32 results of long sums: see chain_sum
-    const bool chained = a.epi == kEpiLinear && ext->out_f32 && kblocks > kChainBlocks;
+    const bool chained = (a.epi == kEpiLinear || a.epi == kEpiPlaneAdd) && ext->out_f32 &&
+                         (kblocks + a.splits - 1) / a.splits > kChainBlocks;
     const bool pair_ok = a.grp_mode != kGroupRows;  // a pair tile spans 256 rows of one group
     int bn = bn_hint;
     if (bn == 0 && ext) {
@@ -2455,9 +2456,6 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
         else if (a.epi == kEpiPlaneAdd)
             weight = 1.3;
         bn = gemm_pick_tile(M, N, K, a.splits, weight, head, !chained, num_sms);
-#ifdef TUNE
-        if (const char* e = std::getenv("TUNE_BN")) if (a.epi == kEpiLinear && !(chained && atoi(e) == 256)) bn = atoi(e);
-#endif
     }
     if (bn == kGemmPairTile && !pair_ok) return -44;
     if (bn == 256 && chained) return -46;
@@ -2493,8 +2491,8 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
         if (a.epi == kEpiLinear) {
             plan->ext.pre_direct = a.aux && (ext->resid || ext->out_f32);
             a.tma_epi = plan_linear_boxes(plan, a, *ext, plan->ext.pre_direct != 0) ? 1 : 0;
-            plan->ext.chain = chained ? kChainBlocks : 0;
         }
+        plan->ext.chain = chained ? kChainBlocks : 0;
         if (a.epi == kEpiHeadGrad || a.epi == kEpiPlaneAdd) {
             a.tma_epi = plan_tma_epilogue(plan, a) ? 1 : 0;
             if (!a.tma_epi) return -8;

@@ -37,7 +37,7 @@ struct GemmExt {
     const float* alpha;   // device scalar that multiplies acc, nullable
     const float* bias;    // [N], nullable
     int act;              // LinearAct
-    int out_f32;          // out and resid are f32, else bf16
+    int out_f32;          // out and resid are f32, else bf16 (kEpiPlaneAdd: what the planes end in)
     const void* resid;    // nullable; row stride ldr elements
     long long ldr;
     const uint64_t* rng;  // device {seed, offset}; null: no dropout

@@ -278,7 +278,8 @@ int split_product(const bf16* A, long long lda, int a_mn, const bf16* B, long lo
     g.ldo = ceil8(a.N);
     g.splits = n;
     g.err = err;
-    const GemmExt x{};
+    GemmExt x{};
+    x.out_f32 = a.out_f32;
     GemmPlan plan;
     int rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, a.M, a.N, K, g, 0, num_sms, &x);
     if (rc) return rc;
@@ -311,13 +312,11 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
     g.err = err;
     GemmPlan plan;
     int rc;
-    const int per16 = out_f32 ? 4 : 8;
-    if (!alpha && aligned16(out) && (ldo % per16) == 0 && (N % per16) == 0) {
-        g.epi = out_f32 ? kEpiStoreF32 : kEpiStoreBF16;
-        g.accumulate = accumulate;
+    if (!alpha && !out_f32 && aligned16(out) && (ldo & 7) == 0 && (N & 7) == 0) {
+        g.epi = kEpiStoreBF16;
         rc = gemm_make_plan(&plan, A, lda, a_mn, B, ldb, b_mn, M, N, K, g,
                             gemm_pick_tile(M, N, K, 1, 1.0, false, true, num_sms), num_sms);
-    } else {  // scaled, or rows that no 16-byte store reaches or that end inside one
+    } else {  // scaled, f32 (whose long sums go by chains), or rows not on or not ending on 16 bytes
         GemmExt x{};
         x.alpha = alpha;
         g.epi = kEpiLinear;

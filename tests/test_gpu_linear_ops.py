@@ -282,6 +282,26 @@ def test_linear_bwd(cuda, M, K, N, act, p, dyt, w_mn):
     ops.check_device(cuda)
 
 
+@pytest.mark.parametrize("w_mn", [False, True])
+def test_long_sums_in_f32(cuda, w_mn):
+    """f32 results of operands that bf16 holds exactly: a chain is 32 accumulations of 16 products,
+    each off by at most a step (2 H32) of the partial sum, however long the whole sum is."""
+    from llmgpu import ops
+    tol = 32 * 2 * H32
+    for M, K, N in ((300, 16384, 520), (16384, 264, 520)):
+        _, x, w, _, _ = _linear_case(cuda, M, K, N, "none", 0, F32, False, False, w_mn, M, 8)
+        y, _ = ops.linear_fwd(x, w, w_mn=w_mn, out_dtype=F32)
+        wd = w.double() if w_mn else w.double().t()
+        _norm_close(y, x.double() @ wd, tol, "y")
+        dy = torch.randn(M, N, device=cuda).to(BF)
+        dw = torch.zeros(w.shape, device=cuda)
+        dx, _, _ = ops.linear_bwd(dy, x, w, w_mn=w_mn, dx_dtype=F32, dw=dw)
+        want = x.double().t() @ dy.double() if w_mn else dy.double().t() @ x.double()
+        _norm_close(dw, want, tol, "dw")
+        _norm_close(dx, dy.double() @ wd.t(), tol, "dx")
+    ops.check_device(cuda)
+
+
 def test_linear_no_rows(cuda):
     from llmgpu import ops
     x, w = torch.empty(0, 16, dtype=BF, device=cuda), torch.ones(24, 16, dtype=BF, device=cuda)
