@@ -557,6 +557,8 @@ enum GemmFamily : int {
     kFamLinearAny = 4  // kFamLinear for outputs that boxes do not reach, wholly or at a row's end
 };
 constexpr bool is_linear(int fam) { return fam == kFamLinear || fam == kFamLinearAny; }
+// families whose tiles may take several accumulator chains
+constexpr bool has_chains(int fam) { return is_linear(fam) || fam == kFamHeadStats; }
 struct NoExt {};
 template <int FAM>
 struct ExtOf {
@@ -920,7 +922,7 @@ __device__ __forceinline__ bool tile_kblocks(const GemmArgs& a, const int* s_grp
 // k-blocks of a chain of a tile whose k-blocks are [kb0, kb1).
 template <int FAM>
 __device__ __forceinline__ int chain_blocks(const typename ExtOf<FAM>::type& x, int kb0, int kb1) {
-    if constexpr (is_linear(FAM)) {
+    if constexpr (has_chains(FAM)) {
         if (x.chain > 0) return x.chain;
     }
     return kb1 - kb0;
@@ -1280,7 +1282,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const int ck = chain_blocks<FAM>(ext, kb0, kb1);
             int kc = kb0;
             do {
-                const int kend = is_linear(FAM) ? min(kc + ck, kb1) : kb1;
+                const int kend = has_chains(FAM) ? min(kc + ck, kb1) : kb1;
                 if (!mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1u, args.err,
                                     kDevTimeoutAccFree)) {
                     ok = false;
@@ -1320,7 +1322,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
                 kc = kend;
-            } while (is_linear(FAM) && kc < kb1);
+            } while (has_chains(FAM) && kc < kb1);
         }
     } else if (warp >= 4) {
         // ---------------- epilogue warpgroup
@@ -1341,8 +1343,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 return mbar_wait_bounded(&acc_full[i], ph, args.err, kDevTimeoutAcc);
             };
             bool ready;
-            if constexpr (is_linear(FAM) && BN <= 128) {
-                linear_prefetch<2>(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
+            if constexpr (has_chains(FAM) && BN <= 128) {
+                if constexpr (is_linear(FAM))
+                    linear_prefetch<2>(args, ext, &tmX, m0 + q * 32, n0, lane, ew, 0, BN / 32);
                 const int ck = chain_blocks<FAM>(ext, kb0, kb1);
                 const int chains = (kb1 - kb0 + ck - 1) / ck;
                 ready = chains > 1
@@ -1723,7 +1726,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 int kc = kb0;
                 do {
-                    const int kend = is_linear(FAM) ? min(kc + ck, kb1) : kb1;
+                    const int kend = has_chains(FAM) ? min(kc + ck, kb1) : kb1;
                     if (!mbar_wait_warp_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
                                                 kDevTimeoutAccFree)) {
                         ok = false;
@@ -1765,7 +1768,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1u;
                     kc = kend;
-                } while (is_linear(FAM) && kc < kb1);
+                } while (has_chains(FAM) && kc < kb1);
             }
         }
     } else if (NG == 2 && warp == 0) {
@@ -1880,7 +1883,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 int kc = kb0;
                 do {
-                    const int kend = is_linear(FAM) ? min(kc + ck, kb1) : kb1;
+                    const int kend = has_chains(FAM) ? min(kc + ck, kb1) : kb1;
                     if (!mbar_wait_bounded_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
                                                    kDevTimeoutAccFree)) {
                         ok = false;
@@ -1916,7 +1919,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1u;
                     kc = kend;
-                } while (is_linear(FAM) && kc < kb1);
+                } while (has_chains(FAM) && kc < kb1);
             }
         }
     } else if (warp >= 4) {
@@ -1955,9 +1958,10 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                 return mbar_wait_bounded_cluster(&acc_full[i], ph, err, kDevTimeoutAcc);
             };
             bool ready;
-            if constexpr (is_linear(FAM)) {
-                linear_prefetch<Cfg::EPI_SLOTS>(args, P.ext, &P.tmX[g], m0 + q * 32, n0, lane, ew,
-                                part * kChunks, (part + 1) * kChunks);
+            if constexpr (has_chains(FAM)) {
+                if constexpr (is_linear(FAM))
+                    linear_prefetch<Cfg::EPI_SLOTS>(args, P.ext, &P.tmX[g], m0 + q * 32, n0, lane, ew,
+                                                    part * kChunks, (part + 1) * kChunks);
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 const int chains = (kb1 - kb0 + ck - 1) / ck;
                 auto free_acc = [&](int i) {
@@ -2493,6 +2497,9 @@ int gemm_make_plan(GemmPlan* plan, const void* A, long long lda, int a_mn_major,
             a.tma_epi = plan_linear_boxes(plan, a, *ext, plan->ext.pre_direct != 0) ? 1 : 0;
         }
         plan->ext.chain = chained ? kChainBlocks : 0;
+        // the loss is f32: above C = 1024 its logits take chains too, longer ones, since a chain's
+        // end costs the statistics' short tiles more
+        if (a.epi == kEpiHeadStats && kblocks > 2 * kChainBlocks) plan->ext.chain = 2 * kChainBlocks;
         if (a.epi == kEpiHeadGrad || a.epi == kEpiPlaneAdd) {
             a.tma_epi = plan_tma_epilogue(plan, a) ? 1 : 0;
             if (!a.tma_epi) return -8;
