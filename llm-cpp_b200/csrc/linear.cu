@@ -422,7 +422,7 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
                           : launch_dz<bf16>(a, drop, grid, to, sums, vec, s);
         if (rc) return rc;
         if (a.dbias && groups > 1) {
-            rc = launch_kernel(linear_db_kernel, (a.N + 31) / 32, 1024, 0, s, part, groups, a.N,
+            rc = launch_kernel_pdl(linear_db_kernel, (a.N + 31) / 32, 1024, 0, s, part, groups, a.N,
                                a.dbias, a.accumulate);
             if (rc) return rc;
         }

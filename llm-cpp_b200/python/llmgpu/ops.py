@@ -258,8 +258,8 @@ def _err_word(device):
 
 
 def check_device(device="cuda"):
-    """Waits for the device and raises if a wait inside one of these operators' kernels gave up;
-    the word is cleared."""
+    """Waits for the device and raises if a wait inside one of these operators' kernels gave up (its
+    result, and those of the calls after it, are then not to be used); the word is cleared."""
     device = torch.device(device)
     index = torch.cuda.current_device() if device.index is None else device.index
     torch.cuda.synchronize(index)
