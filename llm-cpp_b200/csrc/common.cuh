@@ -50,6 +50,16 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
                      smem_u32(bar))
                  : "memory");
 }
+// Arrivals that release no memory: for a barrier that guards tensor memory alone, whose reads
+// tcgen05.wait::ld has completed. A releasing arrival waits for the thread's shared-memory writes
+// and bulk stores first (1.2k to 2.4k cycles behind a GEMM tile's epilogue).
+__device__ __forceinline__ void mbar_arrive_relaxed(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+                 : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
     asm volatile(
         "{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(

@@ -1169,7 +1169,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 128);
+            mbar_init(&acc_empty[i], 4);  // epilogue warps
         }
         for (int i = 0; i < 8; ++i) mbar_init(&epi_bar[i], 1);
         fence_barrier_init();
@@ -1351,7 +1351,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 ready = chains > 1
                             ? chain_sum<BN>(chains, tmem_base + ((uint32_t)(q * 32) << 16), BN, acc,
                                             acc_phase, wait_acc,
-                                            [&](int i) { mbar_arrive(&acc_empty[i]); })
+                                            [&](int i) {
+                                                __syncwarp();
+                                                if (lane == 0) mbar_arrive_relaxed(&acc_empty[i]);
+                                            })
                             : wait_acc(acc, acc_phase);
             } else {
                 if constexpr (is_linear(FAM))
@@ -1368,7 +1371,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             family_tile<FAM, BN, 2>(args, ext, key, &tmO, &tmX, tbase, kb1 <= kb0, m0 + q * 32, n0,
                                  split, g, lane, ew, 0, BN / 32);
             tc_fence_before();
-            mbar_arrive(&acc_empty[acc]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive_relaxed(&acc_empty[acc]);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1u;
         }
@@ -1622,7 +1626,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 2 * 32 * Cfg::EPI_WARPS);  // epilogue threads, both CTAs
+            mbar_init(&acc_empty[i], 2 * Cfg::EPI_WARPS);  // epilogue warps, both CTAs
         }
         for (int i = 0; i < Cfg::EPI_SLOTS * Cfg::EPI_WARPS; ++i) mbar_init(&epi_bar[i], 1);
         fence_barrier_init();
@@ -1957,6 +1961,15 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
             auto wait_acc = [&](int i, uint32_t ph) {
                 return mbar_wait_bounded_cluster(&acc_full[i], ph, err, kDevTimeoutAcc);
             };
+            auto free_acc = [&](int i) {  // one arrival a warp
+                __syncwarp();
+                if (lane == 0) {
+                    if (leader)
+                        mbar_arrive_relaxed(&acc_empty[i]);
+                    else
+                        mbar_arrive_cluster_relaxed(acc_empty_leader + 8u * (uint32_t)i);
+                }
+            };
             bool ready;
             if constexpr (has_chains(FAM)) {
                 if constexpr (is_linear(FAM))
@@ -1964,12 +1977,6 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                                                     part * kChunks, (part + 1) * kChunks);
                 const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
                 const int chains = (kb1 - kb0 + ck - 1) / ck;
-                auto free_acc = [&](int i) {
-                    if (leader)
-                        mbar_arrive(&acc_empty[i]);
-                    else
-                        mbar_arrive_cluster(acc_empty_leader + 8u * (uint32_t)i);
-                };
                 ready = chains > 1
                             ? chain_sum<Cfg::EPI_COLS>(chains,
                                                 tmem_base + ((uint32_t)(q * 32) << 16) +
@@ -1990,10 +1997,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                                  m0 + q * 32, n0, split, gi, lane, ew, part * kChunks,
                                  (part + 1) * kChunks);
             tc_fence_before();
-            if (leader)
-                mbar_arrive(&acc_empty[acc]);
-            else
-                mbar_arrive_cluster(acc_empty_leader + 8u * (uint32_t)acc);
+            free_acc(acc);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1u;
         }
