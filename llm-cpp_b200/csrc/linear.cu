@@ -394,7 +394,9 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
     }
     if (!a.dy || (a.act != kActNone && !a.pre)) return -1;
     if ((a.dx && !a.w) || (a.dw && !a.x)) return -1;
-    if ((a.dx && !operand_ok(a.w, a.ldw)) || (a.dw && !operand_ok(a.x, a.ldx))) return kBadOperand;
+    if ((a.dx && !operand_ok(a.w, a.ldw)) || (a.dw && !operand_ok(a.x, a.ldx)) ||
+        !operand_ok(a.work, 0))
+        return kBadOperand;
     const bool drops = a.drop.rng && a.drop.thr > 0;
     const bool as_is = !a.dy_f32 && a.act == kActNone && !drops && aligned16(a.dy) &&
                        (a.lddy & 7) == 0;  // dy is the products' operand itself
@@ -405,7 +407,7 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
                                 align256((size_t)dz_groups(a.M, a.N) * a.N * 4)
                           : nullptr;
     if (need_dz || a.dbias) {
-        if (!a.work || !aligned16(a.work)) return -1;
+        if (!a.work) return -1;
         bf16* buf = reinterpret_cast<bf16*>(a.work);
         float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.work) +
                                                align256((size_t)a.M * ceil8(a.N) * 2));

@@ -91,6 +91,13 @@ def test_linear_bwd_refusals(bad):
     assert rc in REFUSED
 
 
+def test_linear_bwd_refuses_a_workspace_off_16_bytes():
+    """Where dy itself is the products' operand (bf16, no activation, dropout or bias gradient), the
+    workspace holds the planes of the products split along K alone."""
+    assert _lib().llmgpu_op_linear_bwd(P, 0, 16, P, 16, P, 16, 0, None, 0, 0, 0.0, None, 0, P, 0, 16,
+                                       P, 0, 16, None, 0, 32, 16, 16, P + 8, None, None) in REFUSED
+
+
 @pytest.mark.parametrize("bad", [dict(smoothing=1.0), dict(smoothing=-0.1), dict(V=0), dict(C=0),
                                  dict(V=(1 << 30) + 1), dict(targets=None), dict(work=None),
                                  dict(lse=None), dict(ldx=8), dict(ldw=8), dict(x=P + 2),
