@@ -33,16 +33,18 @@ __device__ __forceinline__ float2 act_pair(float2 z) {
     }
 }
 // Derivatives of a pair of activations, from the same sigmoid as the forward's: gelu(z) = z h with
-// h = sigmoid(2u): h + z h (1 - h) 2u'; silu: h (1 + z (1 - h)).
+// h = sigmoid(2u): h + z h (1 - h) 2u'; silu: h (1 + z (1 - h)). Past |z| = 12, h is 0 or 1 in f32 and
+// gelu's second term 0; its z^2 stops growing there, since 0 times an overflowed z^3 would be NaN.
 template <int ACT>
 __device__ __forceinline__ float2 act_grad_pair(float2 z) {
     if constexpr (ACT == kActRelu) {
         return make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
     } else if constexpr (ACT == kActGelu || ACT == kActSilu) {
         const float2 one = make_float2(1.0f, 1.0f);
-        const float2 z2 = fmul2(z, z);
+        float2 z2 = fmul2(z, z);
         float2 t;
         if constexpr (ACT == kActGelu) {
+            z2 = make_float2(fminf(z2.x, 144.0f), fminf(z2.y, 144.0f));
             constexpr float c = -1.5957691216f * kLog2e;
             t = fmul2(ffma2(z2, make_float2(c * 0.044715f, c * 0.044715f), make_float2(c, c)), z);
         } else {

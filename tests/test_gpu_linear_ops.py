@@ -332,6 +332,25 @@ def test_linear_activations_at_the_ends(cuda):
         assert bool(nan.isnan().all())
 
 
+def test_linear_gradients_far_out(cuda):
+    """Pre-activations whose square or cube is past f32: the derivatives are 0 on the left and 1 on
+    the right, and NaN stays NaN."""
+    from llmgpu import ops
+    z = torch.tensor([-1e36, -1e20, -1e13, -12.5, 12.5, 1e13, 1e20, 1e36], device=cuda)
+    x, w = torch.zeros(4, 8, dtype=BF, device=cuda), torch.zeros(8, 8, dtype=BF, device=cuda)
+    dy = torch.ones(4, 8, device=cuda)
+    for act in ("relu", "gelu", "silu"):
+        _, _, db = ops.linear_bwd(dy, x, w, z.to(BF).repeat(4, 1), act, need_dx=False, need_dw=False)
+        # silu at +-12.5: e^-12.5 (1 + 12.5) = 5e-5 from its end; four rows are added up
+        want = torch.tensor([0.0] * 4 + [4.0] * 4, dtype=torch.float64)
+        at = torch.tensor([0.0] * 3 + [4 * 5.1e-5] * 2 + [0.0] * 3, dtype=torch.float64)
+        assert bool(((db.double().cpu() - want).abs() <= at * (act == "silu")).all()), (act, db)
+        if act != "relu":
+            nan = torch.full((4, 8), float("nan"), dtype=BF, device=cuda)
+            _, _, db = ops.linear_bwd(dy, x, w, nan, act, need_dx=False, need_dw=False)
+            assert bool(db.isnan().all())
+
+
 # --------------------------------------------------------------------------------------- head
 def _head_case(dev, rows, C, V, w_mn, ignored, seed, sharp=3.0):
     g = torch.Generator().manual_seed(seed)
