@@ -185,7 +185,7 @@ int llmgpu_op_linear_bwd(const void* dy, int dy_f32, long long lddy, const void*
 /* Loss head without logits: softmax cross-entropy of x [rows, C] w^T against targets, w [V, C]
  * (w_mn_major = 0) or [C, V] (1), both bf16 with 16-byte aligned rows. The logits are f32
  * accumulators that are never written. row_loss = sum_v y_v (lse - z_v) with y = 1 - smoothing at the
- * target and smoothing / (V - 1) elsewhere, whose gradient is the backward's below (and that of
+ * target and smoothing / (V - 1) elsewhere (V = 1: loss and gradients are 0), whose gradient is the backward's below (and that of
  * llmgpu_op_cross_entropy, which reports lse - z_target whatever the smoothing); lse [rows]: the
  * rows' log-sum-exp, for the backward. A target outside [0, V) leaves its row out: loss 0. `work`:
  * llmgpu_op_linear_ce_fwd_work(rows, V) bytes, 16-byte aligned. rows = 0 is allowed. */

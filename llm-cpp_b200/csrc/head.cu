@@ -295,7 +295,8 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
     bf16* gp = reinterpret_cast<bf16*>(wk + l.g);
     float* planes = reinterpret_cast<float*>(wk + l.planes);
     float* top = reinterpret_cast<float*>(wk + l.top);
-    const float on = 1.0f - a.smoothing;
+    // a vocabulary of one has nothing to smooth into: the loss is 0, and softmax / on - 1 as well
+    const float on = a.V > 1 ? 1.0f - a.smoothing : 1.0f;
     const long long n8 = (long long)a.rows * (l.ldx / 8);
     const int rb = 1 + (int)(n8 < 148ll * 8 * 256 ? (n8 + 255) / 256 : 148 * 8);
     int rc = launch_kernel(head_rows_kernel, rb, 256, 0, s, a.x, a.ldx, a.targets, dloss, scale * on,

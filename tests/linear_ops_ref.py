@@ -59,6 +59,7 @@ def head(x, w, targets, smoothing):
     valid = (targets >= 0) & (targets < V)
     t = targets.long().clamp(0, V - 1)
     y = torch.full_like(z, smoothing / (V - 1) if V > 1 else 0.0)
-    y.scatter_(1, t[:, None], 1.0 - smoothing)
+    # one class alone: y sums to 1, since a constant loss has no gradient
+    y.scatter_(1, t[:, None], 1.0 - smoothing if V > 1 else 1.0)
     loss = (y * (lse[:, None] - z)).sum(1)
     return torch.where(valid, loss, torch.zeros_like(loss)), lse, z, y, valid

@@ -430,6 +430,21 @@ def test_loss_head(cuda, rows, C, V, piece, smoothing, w_mn, ignored):
     ops.check_device(cuda)
 
 
+def test_loss_head_of_one_class(cuda):
+    """A vocabulary of one: the loss is 0 whatever the logit, smoothed or not, and so are its
+    gradients, up to the rounding of lse (p = 2^(z log2 e - lse log2 e) with each term rounded)."""
+    from llmgpu import ops
+    for rows in (1, 40):
+        x, w, t, d = _head_case(cuda, rows, 64, 1, False, False, 2)
+        for s in (0.0, 0.1, 0.9):
+            loss, lse = ops.linear_cross_entropy_fwd(x, w, t, s)
+            dx, dw = ops.linear_cross_entropy_bwd(x, w, t, lse, d, 1.0, s, dx_dtype=F32)
+            e = 8 * H32 * (1 + lse.double().abs()) * d.double()
+            assert bool((loss.double().abs() <= e).all()), (s, loss)
+            assert bool((dx.double().abs() <= e[:, None] * w.double().abs()).all()), (s, dx)
+            assert bool((dw.double().abs() <= e @ x.double().abs() * (1 + H16)).all()), (s, dw)
+
+
 def test_loss_head_rows_left_out_may_hold_anything(cuda):
     """A padded batch whose padding rows hold NaN and infinities: they reach nothing."""
     from llmgpu import ops
