@@ -162,7 +162,8 @@ int llmgpu_op_dropout(const void* x, int x_f32, long long ldx, const void* resid
  *   nullable; act: 0 none, 1 relu, 2 gelu (tanh form), 3 silu; drop: llmgpu_op_dropout over the
  *   [M, N] result with (p, rng, site), none when p = 0 (rng may then be NULL); resid (nullable) has
  *   out's type, bf16 or f32 (out_f32), and may be out itself. pre (nullable, bf16): z, which the
- *   backward needs when act is not none. out, resid and pre take any row stride. M = 0 is allowed.
+ *   backward needs when act is not none. out, resid and pre take any row stride. M = 0 is allowed;
+ *   M, N, K <= 2^30.
  *   err as in llmgpu_op_gemm. */
 int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long ldw, int w_mn_major,
                          const float* bias, int act, float p, const uint64_t* rng, uint64_t site,
@@ -188,7 +189,8 @@ int llmgpu_op_linear_bwd(const void* dy, int dy_f32, long long lddy, const void*
  * target and smoothing / (V - 1) elsewhere (V = 1: loss and gradients are 0), whose gradient is the backward's below (and that of
  * llmgpu_op_cross_entropy, which reports lse - z_target whatever the smoothing); lse [rows]: the
  * rows' log-sum-exp, for the backward. A target outside [0, V) leaves its row out: loss 0. `work`:
- * llmgpu_op_linear_ce_fwd_work(rows, V) bytes, 16-byte aligned. rows = 0 is allowed. */
+ * llmgpu_op_linear_ce_fwd_work(rows, V) bytes, 16-byte aligned. rows = 0 is allowed;
+ * rows, C, V <= 2^30. */
 long long llmgpu_op_linear_ce_fwd_work(int rows, int V);
 int llmgpu_op_linear_ce_fwd(const void* x, long long ldx, const void* w, long long ldw,
                             int w_mn_major, const int32_t* targets, int rows, int C, int V,

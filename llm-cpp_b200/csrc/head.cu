@@ -23,7 +23,6 @@ namespace {
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 long long ceil8(long long n) { return (n + 7) & ~7ll; }
 
-constexpr int kMaxV = 1 << 30;   // piece offsets stay in 32 bits
 constexpr int kSlot = 128;       // vocabulary columns of one (max, sum) slot
 constexpr int kMaxSplits = 32;   // planes of the dx product
 constexpr int kPairSlots = 74;   // CTA pairs of a B200, for the choice of piece and splits only
@@ -233,13 +232,14 @@ int head_piece(int rows, int C, int V, int piece) {
 }
 
 size_t head_forward_work(int rows, int V) {
-    if (rows <= 0 || V <= 0) return 0;
+    if (rows <= 0 || V <= 0 || rows > kMaxDim || V > kMaxDim) return 0;
     const size_t n = (size_t)slots_of(V) * rows;
     return align256(n * 8) + align256(n * 4) + (size_t)rows * 4;
 }
 
 int head_forward(const HeadArgs& a, float* row_loss, float* lse, int num_sms, cudaStream_t s) {
-    if (a.rows < 0 || a.C <= 0 || a.V <= 0 || a.V > kMaxV || !(a.smoothing >= 0.0f && a.smoothing < 1.0f)) return -1;
+    if (a.rows < 0 || a.C <= 0 || a.V <= 0 || !(a.smoothing >= 0.0f && a.smoothing < 1.0f)) return -1;
+    if (a.rows > kMaxDim || a.C > kMaxDim || a.V > kMaxDim) return -1;
     if (a.rows == 0) return 0;
     if (!a.x || !a.w || !a.targets || !row_loss || !lse || !a.work) return -1;
     if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw) || !operand_ok(a.work, 0))
@@ -269,14 +269,15 @@ int head_forward(const HeadArgs& a, float* row_loss, float* lse, int num_sms, cu
 }
 
 size_t head_backward_work(int rows, int C, int V, int piece) {
-    if (rows <= 0 || C <= 0 || V <= 0) return 0;
+    if (rows <= 0 || C <= 0 || V <= 0 || rows > kMaxDim || C > kMaxDim || V > kMaxDim) return 0;
     return head_layout(rows, C, V, piece).total;
 }
 
 int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float scale, void* dx,
                   int dx_f32, long long lddx, void* dw, int dw_f32, long long lddw, int accumulate,
                   int piece, int num_sms, cudaStream_t s) {
-    if (a.rows < 0 || a.C <= 0 || a.V <= 0 || a.V > kMaxV || !(a.smoothing >= 0.0f && a.smoothing < 1.0f)) return -1;
+    if (a.rows < 0 || a.C <= 0 || a.V <= 0 || !(a.smoothing >= 0.0f && a.smoothing < 1.0f)) return -1;
+    if (a.rows > kMaxDim || a.C > kMaxDim || a.V > kMaxDim) return -1;
     if (piece < 0 || (piece % 256) != 0 || (accumulate && dw && !dw_f32)) return -1;
     const size_t es = dw_f32 ? 4 : 2;
     if (a.rows == 0) {

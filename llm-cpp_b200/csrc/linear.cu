@@ -330,6 +330,7 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
 
 int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
     if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.act < kActNone || a.act > kActSilu) return -1;
+    if (a.M > kMaxDim || a.N > kMaxDim || a.K > kMaxDim) return -1;
     if (a.M == 0) return 0;
     if (!a.x || !a.w || !a.out) return -1;
     if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw) || !operand_ok(a.work, 0))
@@ -370,7 +371,7 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
 }
 
 size_t linear_backward_work(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || M > kMaxDim || N > kMaxDim || K > kMaxDim) return 0;
     // dw is [N, K] or [K, N]: the larger of the two; its planes follow dx's in the same place
     size_t planes = product_work(M, K, N);
     const size_t dw = product_work(N, K, M), dw_mn = product_work(K, N, M);
@@ -381,6 +382,7 @@ size_t linear_backward_work(int M, int N, int K) {
 
 int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
     if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.act < kActNone || a.act > kActSilu) return -1;
+    if (a.M > kMaxDim || a.N > kMaxDim || a.K > kMaxDim) return -1;
     if (a.accumulate && a.dw && !a.dw_f32) return -1;
     if (a.M == 0) {  // no rows: zero gradients, or nothing to add
         if (a.accumulate) return 0;

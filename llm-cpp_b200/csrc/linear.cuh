@@ -13,6 +13,9 @@ inline bool operand_ok(const void* p, long long ld) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0;
 }
 
+// Sizes at most: the index arithmetic of tiles stays in 32 bits.
+constexpr int kMaxDim = 1 << 30;
+
 // Dropout of a linear layer's output; thr 0 keeps everything.
 struct DropArgs {
     const uint64_t* rng;  // device {seed, offset}; null: no dropout

@@ -221,7 +221,8 @@ static bool linear_drop(float p, const uint64_t* rng, uint64_t site, DropArgs* d
 }
 
 extern "C" long long llmgpu_op_linear_fwd_work(int M, int N, int K) {
-    return M > 0 && N > 0 && K > 0 ? (long long)product_work(M, N, K) : 0;
+    if (M <= 0 || N <= 0 || K <= 0 || M > kMaxDim || N > kMaxDim || K > kMaxDim) return 0;
+    return (long long)product_work(M, N, K);
 }
 
 extern "C" int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long ldw,

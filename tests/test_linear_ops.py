@@ -127,6 +127,25 @@ def test_loss_head_bwd_refusals(bad):
         assert lib.llmgpu_op_linear_ce_bwd_work(4, 16, 32, bad["piece"]) < 0
 
 
+@pytest.mark.parametrize("at", ["M", "N", "K"])
+def test_sizes_past_2_30_are_refused(at):
+    """Tile counts and column offsets are 32-bit: nothing is launched, and no workspace named."""
+    big = (1 << 30) + 8
+    d = dict(M=32, N=16, K=16)
+    d[at] = big
+    M, N, K = d["M"], d["N"], d["K"]
+    lib, ld = _lib(), big
+    assert lib.llmgpu_op_linear_fwd(P, ld, P, ld, 0, None, 0, 0.0, None, 0, None, 0, None, 0, P, 0, ld,
+                                    M, N, K, P, None, None) in REFUSED
+    assert lib.llmgpu_op_linear_bwd(P, 1, ld, P, ld, P, ld, 0, None, 0, 0, 0.0, None, 0, P, 0, ld, P, 0,
+                                    ld, P, 0, M, N, K, P, None, None) in REFUSED
+    assert lib.llmgpu_op_linear_ce_fwd(P, ld, P, ld, 0, P, M, K, N, 0.0, P, P, P, None, None) in REFUSED
+    assert lib.llmgpu_op_linear_ce_bwd(P, ld, P, ld, 0, P, P, None, 1.0, M, K, N, 0.0, P, 0, ld, P, 0, ld,
+                                       0, 0, P, None, None) in REFUSED
+    assert lib.llmgpu_op_linear_fwd_work(M, N, K) == lib.llmgpu_op_linear_bwd_work(M, N, K) == 0
+    assert lib.llmgpu_op_linear_ce_bwd_work(M, K, N, 0) == 0
+
+
 def test_workspace_covers_any_piece():
     """The workspace holds at least the gradient of one piece and a copy of x; a piece past the
     vocabulary is the whole of it."""
