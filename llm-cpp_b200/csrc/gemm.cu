@@ -1182,7 +1182,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
         tmem_relinquish();
     }
-    pdl_enter();  // barriers, TMEM and descriptors are set up while the previous kernel ends
+    // barriers, TMEM and descriptors are set up while the previous kernel ends
+    if (!args.early) pdl_wait();
+    pdl_trigger();
     __shared__ int s_grp[kMaxGemmGroups + 1];
     if (args.grp_mode != kGroupNone)
         for (int i = threadIdx.x; i <= args.groups; i += blockDim.x) s_grp[i] = args.grp[i];
@@ -1383,6 +1385,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    if (args.early) pdl_wait();  // whoever waits for this kernel waits for the one in front too
 }
 
 // ---------------------------------------------------------------------------- CTA pairs
@@ -1641,7 +1644,9 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
         tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
         tmem_relinquish_pair();
     }
-    pdl_enter();  // barriers, TMEM and descriptors are set up while the previous kernel ends
+    // barriers, TMEM and descriptors are set up while the previous kernel ends
+    if (!P.args[0].early) pdl_wait();
+    pdl_trigger();
     // row-group table of a grouped product (single products only)
     __shared__ int s_grp[kMaxGemmGroups + 1];
     if (NG == 1 && P.args[0].grp_mode != kGroupNone)
@@ -2009,6 +2014,7 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
     cluster_sync_all();  // neither CTA leaves while the other may still touch its memory
     tc_fence_after();
     if (warp == 1) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+    if (P.args[0].early) pdl_wait();  // whoever waits for this kernel waits for the one in front too
 }
 
 __global__ void splitk_reduce_kernel(const float* __restrict__ part, int splits, int M, int N,

@@ -84,6 +84,11 @@ struct GemmArgs {
     int scalar_store;      // set by the planner when the output is not 16-byte aligned
     int tma_epi;           // set by the planner: outputs (and epilogue inputs) go through TMA
     int* err;              // device error word
+    // Starts beside the kernel in front of it on the stream and ends after it. For a product that
+    // neither reads nor overwrites what that kernel touches, behind a kernel of this library that
+    // waited for its own predecessor or is itself `early` behind such a one: its inputs were then
+    // complete before that kernel's blocks let this one start.
+    int early;
     // Grouped (per-expert) products. `grp` is a device table of groups+1 ascending row
     // offsets, each a multiple of 128 (entry `groups` = rows in use), written by an earlier
     // kernel on the same stream, so the grouping needs no host synchronisation.

@@ -350,11 +350,13 @@ int head_backward(const HeadArgs& a, const float* lse, const float* dloss, float
             if ((rc = gemm_run(plan, s)) != 0) return rc;
         }
         if (dw) {
+            // dw need not wait for dx's product
+            const int early = dx && leaves_room(a.rows, a.C, one ? 1 : l.splits);
             char* to = reinterpret_cast<char*>(dw) + (a.w_mn_major ? (long long)v0 : v0 * lddw) * es;
             rc = a.w_mn_major ? product(xr, l.ldx, 1, gp, l.ldg, 1, a.C, pw, a.rows, to, dw_f32,
-                                        lddw, accumulate, num_sms, a.err, s, top + 1)
+                                        lddw, accumulate, num_sms, a.err, s, top + 1, nullptr, early)
                               : product(gp, l.ldg, 1, xr, l.ldx, 1, pw, a.C, a.rows, to, dw_f32,
-                                        lddw, accumulate, num_sms, a.err, s, top + 1);
+                                        lddw, accumulate, num_sms, a.err, s, top + 1, nullptr, early);
             if (rc) return rc;
         }
     }

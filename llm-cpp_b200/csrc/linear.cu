@@ -271,13 +271,15 @@ namespace {
 
 // The k-split product of A and B into planes, then the epilogue `a`.
 int split_product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int K,
-                  int n, void* work, const RowsArgs& a, int num_sms, int* err, cudaStream_t s) {
+                  int n, void* work, const RowsArgs& a, int num_sms, int* err, int early,
+                  cudaStream_t s) {
     GemmArgs g{};
     g.epi = kEpiPlaneAdd;
     g.out = work;
     g.ldo = ceil8(a.N);
     g.splits = n;
     g.err = err;
+    g.early = early;
     GemmExt x{};
     x.out_f32 = a.out_f32;
     GemmPlan plan;
@@ -291,7 +293,7 @@ int split_product(const bf16* A, long long lda, int a_mn, const bf16* B, long lo
 
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
             int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
-            int* err, cudaStream_t s, const float* alpha, void* work) {
+            int* err, cudaStream_t s, const float* alpha, void* work, int early) {
     if (accumulate && !out_f32) return -1;
     if (M <= kFewRows && !a_mn) {
         RowsArgs r{A, lda, B, ldb, alpha, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo, nullptr, 0,
@@ -303,13 +305,15 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
     if (const int n = work ? product_splits(M, N, K) : 1; n > 1) {
         RowsArgs r{nullptr, 0, nullptr, 0, alpha, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo,
                    nullptr, 0, out, out_f32, ldo, M, N, K};
-        return split_product(A, lda, a_mn, B, ldb, b_mn, K, n, work, r, num_sms, err, s);
+        return split_product(A, lda, a_mn, B, ldb, b_mn, K, n, work, r, num_sms, err,
+                             early, s);
     }
     GemmArgs g{};
     g.out = out;
     g.ldo = ldo;
     g.splits = 1;
     g.err = err;
+    g.early = early;
     GemmPlan plan;
     int rc;
     if (!alpha && !out_f32 && aligned16(out) && (ldo & 7) == 0 && (N & 7) == 0) {
@@ -341,7 +345,7 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
                    a.out, a.out_f32, a.ldo, a.M, a.N, a.K};
         if (r.drop.thr == 0) r.drop.rng = nullptr;
         return n > 1 ? split_product(a.x, a.ldx, 0, a.w, a.ldw, a.w_mn_major, a.K, n, a.work, r,
-                                     num_sms, a.err, s)
+                                     num_sms, a.err, 0, s)
                      : rows_product(r, a.w_mn_major, s);
     }
     GemmArgs g{};
@@ -408,6 +412,9 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
     void* planes = a.work ? reinterpret_cast<char*>(a.work) + align256((size_t)a.M * ceil8(a.N) * 2) +
                                 align256((size_t)dz_groups(a.M, a.N) * a.N * 4)
                           : nullptr;
+    // the products need not wait for what runs in front of them once dz's own kernel has ended: dx
+    // for the second stage of dbias, dw for it and for dx (unless dx's planes lie where dw's go)
+    int early = 0;
     if (need_dz || a.dbias) {
         if (!a.work) return -1;
         bf16* buf = reinterpret_cast<bf16*>(a.work);
@@ -429,6 +436,7 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
             rc = launch_kernel_pdl(linear_db_kernel, (a.N + 31) / 32, 1024, 0, s, part, groups, a.N,
                                a.dbias, a.accumulate);
             if (rc) return rc;
+            early = 1;
         }
         if (need_dz) {
             dz = buf;
@@ -437,16 +445,17 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
     }
     if (a.dx) {  // dz [M,N] times w
         const int rc = product(dz, ldz, 0, a.w, a.ldw, a.w_mn_major ? 0 : 1, a.M, a.K, a.N, a.dx,
-                               a.dx_f32, a.lddx, 0, num_sms, a.err, s, nullptr, planes);
+                               a.dx_f32, a.lddx, 0, num_sms, a.err, s, nullptr, planes, early);
         if (rc) return rc;
+        early = (!planes || product_splits(a.M, a.K, a.N) == 1) && leaves_room(a.M, a.K, 1);
     }
     if (a.dw) {
         const int rc =
             a.w_mn_major
                 ? product(a.x, a.ldx, 1, dz, ldz, 1, a.K, a.N, a.M, a.dw, a.dw_f32, a.lddw,
-                          a.accumulate, num_sms, a.err, s, nullptr, planes)
+                          a.accumulate, num_sms, a.err, s, nullptr, planes, early)
                 : product(dz, ldz, 1, a.x, a.ldx, 1, a.N, a.K, a.M, a.dw, a.dw_f32, a.lddw,
-                          a.accumulate, num_sms, a.err, s, nullptr, planes);
+                          a.accumulate, num_sms, a.err, s, nullptr, planes, early);
         if (rc) return rc;
     }
     return 0;

@@ -136,14 +136,22 @@ int outer_product(const bf16* A, long long lda, const bf16* B, long long ldb, in
 // Splits along K of a product with too few tiles for the device, and the bytes of their planes.
 int product_splits(int M, int N, int K);
 size_t product_work(int M, int N, int K);
+// Whether a product leaves SMs idle for the one behind it to start on: fewer 256 x 256 tiles than the 74
+// pairs. Where it fills them, two products at once only compete (8192 x 768 x 50257 backward: 0.8%
+// slower).
+inline bool leaves_room(int M, int N, int splits) {
+    return (long long)((M + 255) / 256) * ((N + 255) / 256) * splits < 74;
+}
 // out = resid + drop(act(alpha sum of planes [n][M][ldp] + bias)) (x, w of `a` unused); ldp: a
 // multiple of 8.
 int finish_planes(const RowsArgs& a, const float* planes, int n, int ldp, cudaStream_t s);
 
 // D[M,N] (+)= alpha A B^T on the tcgen05 kernels into bf16 or f32 `out`, any row stride (accumulate:
-// f32 only; alpha: device scalar, nullable; work: product_work(M, N, K) bytes, or null).
+// f32 only; alpha: device scalar, nullable; work: product_work(M, N, K) bytes, or null; early: see
+// GemmArgs, of use where the tcgen05 kernels run).
 int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb, int b_mn, int M,
             int N, int K, void* out, int out_f32, long long ldo, int accumulate, int num_sms,
-            int* err, cudaStream_t s, const float* alpha = nullptr, void* work = nullptr);
+            int* err, cudaStream_t s, const float* alpha = nullptr, void* work = nullptr,
+            int early = 0);
 
 }  // namespace llmgpu

@@ -332,6 +332,45 @@ def test_linear_activations_at_the_ends(cuda):
         assert bool(nan.isnan().all())
 
 
+@pytest.mark.parametrize("M,N,K", [(64, 8192, 4800), (200, 1000, 4800), (2000, 64, 700), (40, 24, 64)])
+def test_linear_bwd_products_beside_each_other(cuda, M, N, K):
+    """dw's product may start beside dx's, and dx's beside the bias sum: what reads a gradient right
+    after the call finds it whole, and what the call read may be overwritten. dy doubles from call
+    to call, which doubles every gradient exactly."""
+    from llmgpu import ops
+    g = torch.Generator().manual_seed(M + N)
+    x, _ = _mat(g, M, K, BF, cuda, 1.0, 0, 8)
+    w, _ = _mat(g, N, K, BF, cuda, 1.0, 0, 8)
+    v, _ = _mat(g, 24, K, BF, cuda, 1.0, 0, 8)
+    base = torch.randn(M, N, generator=g).to(cuda)
+    dy = base.clone()
+    xs = torch.empty_strided(x.shape, x.stride(), dtype=BF, device=cuda)  # x's rows on 16 bytes
+
+    def step(dx_dtype):
+        dx, dw, db = ops.linear_bwd(dy, xs, w, dx_dtype=dx_dtype)
+        xs.zero_()
+        dy.zero_()
+        read = [dx.clone(), dw.clone(), db.clone()]
+        if dx_dtype == BF:
+            read.append(ops.linear_fwd(dx, v)[0])
+        return read
+
+    for dtype in (BF, F32):
+        dy.copy_(base), xs.copy_(x)
+        first = step(dtype)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step(dtype)
+        for i in range(1, 9):
+            dy.copy_(base * 2.0 ** i), xs.copy_(x)
+            got = step(dtype)
+            assert all(torch.equal(a, b * 2.0 ** i) for a, b in zip(got, first)), (dtype, i)
+            dy.copy_(base * 2.0 ** -i), xs.copy_(x)
+            graph.replay()
+            assert all(torch.equal(a, b * 2.0 ** -i) for a, b in zip(held, first)), (dtype, -i)
+    ops.check_device(cuda)
+
+
 def test_linear_gradients_far_out(cuda):
     """Pre-activations whose square or cube is past f32: the derivatives are 0 on the left and 1 on
     the right, and NaN stays NaN."""
@@ -427,6 +466,24 @@ def test_loss_head(cuda, rows, C, V, piece, smoothing, w_mn, ignored):
                                                     need_dw=False)[0], gx)
     assert torch.equal(ops.linear_cross_entropy_bwd(x, w, t, gs, d, 0.5, smoothing, w_mn, piece=piece,
                                                     need_dx=False)[1], gw)
+    ops.check_device(cuda)
+
+
+@pytest.mark.parametrize("rows,C,V,piece", [(256, 128, 256, 0), (300, 64, 2000, 512), (64, 4800, 600, 0)])
+def test_loss_head_bwd_products_beside_each_other(cuda, rows, C, V, piece):
+    """As for the linear layer: the weights of the rows double from call to call, and so do the
+    gradients, exactly (the largest weight is divided out before the rounding)."""
+    from llmgpu import ops
+    x, w, t, d = _head_case(cuda, rows, C, V, False, False, 7)
+    _, lse = ops.linear_cross_entropy_fwd(x, w, t)
+    c, first = d.clone(), None
+    for i in range(9):
+        c.copy_(d * 2.0 ** i)
+        dx, dw = ops.linear_cross_entropy_bwd(x, w, t, lse, c, piece=piece)
+        c.zero_()
+        got = [dx.clone(), dw.clone(), ops.linear_fwd(dx, w)[0]]
+        first = first or got
+        assert all(torch.equal(a, b * 2.0 ** i) for a, b in zip(got, first)), i
     ops.check_device(cuda)
 
 
