@@ -7,8 +7,8 @@
 //
 // Bound by the tensor cores (and, over many launches, by the power cap): one product forward,
 // three backward, one more than with [rows, V] logits kept, and none of their memory (824 MB at
-// 8192 x 50257 in bf16, which would also round the loss). 8192 x 768 x 50257: forward 410 us
-// (1.54 PFLOP/s), backward 1440 us (1.32 PFLOP/s counting the recomputed product). Pieces of the
+// 8192 x 50257 in bf16, which would also round the loss). 8192 x 768 x 50257: forward 418 us
+// (1.51 PFLOP/s), backward 1420 us (1.33 PFLOP/s counting the recomputed product). Pieces of the
 // vocabulary rather than blocks of rows: dw, the largest matrix, is then written once instead of
 // summed over row blocks.
 #include <cfloat>

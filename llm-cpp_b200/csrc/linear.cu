@@ -2,8 +2,8 @@
 // tensor memory (gemm.cu, kEpiLinear), and its backward: one elementwise pass forms dz in bf16
 // and the bias gradient's partial sums, then two products give dx and dw. dz is rounded to bf16
 // because it is a tensor-core operand; the bias gradient is summed before that rounding.
-// 8192 x 1024 x 4096: forward gelu 64 us (cuBLAS's bare product 57), backward 133 us (34 dz, 4
-// dbias, 95 the products); 8192 x 4096 x 1024 with dropout and f32 residual 69 us.
+// 8192 x 1024 x 4096: forward gelu 63 us (cuBLAS's bare product 57), backward 132 us (34 dz, 4
+// dbias, 95 the products); 8192 x 4096 x 1024 with dropout and f32 residual 67 us.
 #include "linear.cuh"
 
 #include "act.cuh"
