@@ -18,18 +18,12 @@ _DEV = "cuda"
 _DT = {"bf16": torch.bfloat16, "f32": torch.float32}
 
 
-_loaded = []
-
-
 def _ops():
-    if _loaded:
-        return _loaded[0]
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                         "llm-cpp_b200", "python")
     if path not in sys.path:
         sys.path.insert(0, path)
     from llmgpu import ops
-    _loaded.append(ops)
     return ops
 
 
