@@ -34,17 +34,18 @@ __device__ __forceinline__ float2 act_pair(float2 z) {
 }
 // Derivatives of a pair of activations, from the same sigmoid as the forward's: gelu(z) = z h with
 // h = sigmoid(2u): h + z h (1 - h) 2u'; silu: h (1 + z (1 - h)). Past |z| = 12, h is 0 or 1 in f32 and
-// gelu's second term 0; its z^2 stops growing there, since 0 times an overflowed z^3 would be NaN.
+// gelu's second term 0: z stops growing there in it, since 0 times an overflowed product would be NaN
+// (from 1e13 on for z^3, from 1e37 on for z alone). The sigmoid takes z itself, which keeps a NaN.
 template <int ACT>
 __device__ __forceinline__ float2 act_grad_pair(float2 z) {
     if constexpr (ACT == kActRelu) {
         return make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
     } else if constexpr (ACT == kActGelu || ACT == kActSilu) {
         const float2 one = make_float2(1.0f, 1.0f);
-        float2 z2 = fmul2(z, z);
-        float2 t;
+        float2 zc, z2, t;  // gelu's z within +-12 and its square
         if constexpr (ACT == kActGelu) {
-            z2 = make_float2(fminf(z2.x, 144.0f), fminf(z2.y, 144.0f));
+            zc = make_float2(fminf(fmaxf(z.x, -12.0f), 12.0f), fminf(fmaxf(z.y, -12.0f), 12.0f));
+            z2 = fmul2(zc, zc);
             constexpr float c = -1.5957691216f * kLog2e;
             t = fmul2(ffma2(z2, make_float2(c * 0.044715f, c * 0.044715f), make_float2(c, c)), z);
         } else {
@@ -56,7 +57,7 @@ __device__ __forceinline__ float2 act_grad_pair(float2 z) {
         if constexpr (ACT == kActGelu) {
             constexpr float k = 1.5957691216f;
             const float2 q =
-                fmul2(ffma2(z2, make_float2(k * 0.134145f, k * 0.134145f), make_float2(k, k)), z);
+                fmul2(ffma2(z2, make_float2(k * 0.134145f, k * 0.134145f), make_float2(k, k)), zc);
             return ffma2(fmul2(h, g), q, h);
         } else {
             return fmul2(h, ffma2(z, g, one));

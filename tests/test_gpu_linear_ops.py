@@ -390,6 +390,24 @@ def test_linear_gradients_far_out(cuda):
             assert bool(db.isnan().all())
 
 
+def test_linear_gradients_at_the_types_ends(cuda):
+    """Pre-activations up to bf16's largest values: the derivatives are 0 on the left and 1 on the
+    right (gelu's second term has a factor 2^-205 or less from |z| = 12 on)."""
+    from llmgpu import ops
+    top = torch.finfo(BF).max
+    z = torch.tensor([-top, -3e38, -1.1e37, -1e37, 1e37, 1.1e37, 3e38, top], device=cuda).to(BF)
+    x, w = torch.zeros(4, 8, dtype=BF, device=cuda), torch.zeros(8, 8, dtype=BF, device=cuda)
+    dy = torch.ones(4, 8, device=cuda)
+    want = torch.tensor([0.0] * 4 + [4.0] * 4, device=cuda)
+    for act in ("relu", "gelu", "silu"):
+        _, _, db = ops.linear_bwd(dy, x, w, z.repeat(4, 1), act, need_dx=False, need_dw=False)
+        assert torch.equal(db, want), (act, db)
+    # what overflowed to an infinity has gelu's limits
+    inf = torch.tensor([-math.inf] * 4 + [math.inf] * 4, device=cuda).to(BF)
+    _, _, db = ops.linear_bwd(dy, x, w, inf.repeat(4, 1), "gelu", need_dx=False, need_dw=False)
+    assert torch.equal(db, want), db
+
+
 # --------------------------------------------------------------------------------------- head
 def _head_case(dev, rows, C, V, w_mn, ignored, seed, sharp=3.0):
     g = torch.Generator().manual_seed(seed)
