@@ -76,8 +76,6 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
                 if (row >= M) break;
                 float v[8];
                 raw_f32(dr[u], v);
-                if constexpr (DROP)
-                    drop_apply8(key, (uint32_t)col >> 3, (uint32_t)row, drop.thr, drop.scale, v);
                 if constexpr (ACT != kActNone) {
                     float z[8];
                     raw_f32(pr[u], z);
@@ -89,6 +87,9 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
                         v[2 * i + 1] = y.y;
                     }
                 }
+                // behind act', so that a dropped place is 0 whatever dy and pre hold there
+                if constexpr (DROP)
+                    drop_apply8(key, (uint32_t)col >> 3, (uint32_t)row, drop.thr, drop.scale, v);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = fadd2(sum[i], make_float2(v[2 * i], v[2 * i + 1]));
                 // columns past N, up to the padded stride, are written as zeros

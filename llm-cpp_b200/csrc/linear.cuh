@@ -48,7 +48,7 @@ struct LinearFwd {
 };
 int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s);
 
-// dz = drop'(dy) act'(pre) in bf16, dbias (+)= column sums of dz (before its rounding), dx = dz w,
+// dz = drop(dy act'(pre)) in bf16, dbias (+)= column sums of dz (before its rounding), dx = dz w,
 // dw (+)= dz^T x (laid out as w). dx, dw, dbias nullable.
 struct LinearBwd {
     const void* dy;

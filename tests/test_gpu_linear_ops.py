@@ -282,6 +282,29 @@ def test_linear_bwd(cuda, M, K, N, act, p, dyt, w_mn):
     ops.check_device(cuda)
 
 
+@pytest.mark.parametrize("M", [5, 70])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("dyt,pad", [(BF, 0), (F32, 0), (F32, 3)])
+def test_linear_bwd_dropped_places_count_nothing(cuda, M, act, dyt, pad):
+    """What the forward dropped has no gradient, whatever dy and pre hold there."""
+    from llmgpu import ops
+    g = torch.Generator().manual_seed(M)
+    K, N = 40, 72
+    x, w = _mat(g, M, K, BF, cuda)[0], _mat(g, N, K, BF, cuda)[0]
+    dy, pre = _mat(g, M, N, dyt, cuda, 1.0, 0, pad)[0], _mat(g, M, N, BF, cuda, 1.0, 0, pad)[0]
+    rng = _rng(cuda, 31, 7)
+    keep, _ = ref.keep_mask(31, 7 + 2, M, N, 0.5)
+    gone = ~keep.to(cuda)
+    want = None
+    for dv, zv in ((0.0, 0.0), (math.nan, 1.0), (math.inf, 1.0), (1.0, math.nan), (1.0, math.inf),
+                   (1.0, -math.inf), (torch.finfo(dyt).min, torch.finfo(BF).min)):
+        dy[gone], pre[gone] = dv, zv
+        got = ops.linear_bwd(dy, x, w, pre, act, 0.5, rng, 2)
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (dv, zv)
+    assert all(bool(torch.isfinite(v).all()) for v in want)
+
+
 @pytest.mark.parametrize("w_mn", [False, True])
 def test_long_sums_in_f32(cuda, w_mn):
     """f32 results of operands that bf16 holds exactly: a chain is 32 accumulations of 16 products,
