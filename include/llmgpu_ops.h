@@ -171,9 +171,9 @@ int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long 
                          int out_f32, long long ldo, int M, int N, int K, void* work, int* err,
                          void* stream);
 /* Its backward: dz = drop(dy * act'(pre)), 0 where the forward dropped whatever dy and pre hold
- * there, rounded to bf16 for the products; dbias = column sums of dz before that rounding, dx =
- * dz w, dw = dz^T x (in w's layout); the residual's gradient is dy itself. dx, dw, dbias are
- * nullable; dx and dw are bf16 or f32. `accumulate` adds into dw (f32 only) and dbias. M = 0
+ * there, rounded to bf16 for the products (not for dw where M <= 8); dbias = column sums of dz
+ * before that rounding, dx = dz w, dw = dz^T x (in w's layout); the residual's gradient is dy
+ * itself. dx, dw, dbias are nullable; dx and dw are bf16 or f32. `accumulate` adds into dw (f32 only) and dbias. M = 0
  * writes zero gradients. `work`: llmgpu_op_linear_bwd_work(M, N, K) bytes, 16-byte aligned. dy:
  * bf16 or f32 (dy_f32), any row stride; x, w as in the forward; (p, rng, site) the forward's, with
  * the values that rng held then. */

@@ -1,7 +1,9 @@
 // Linear layer with bias, activation, dropout and residual applied where the product's tiles leave
 // tensor memory (gemm.cu, kEpiLinear), and its backward: one elementwise pass forms dz in bf16
 // and the bias gradient's partial sums, then two products give dx and dw. dz is rounded to bf16
-// because it is a tensor-core operand; the bias gradient is summed before that rounding.
+// because it is a tensor-core operand; the bias gradient is summed before that rounding, and dw of up
+// to 8 rows, whose outer products run on the CUDA cores, takes it in f32. (dx of few rows goes
+// through the tensor cores too: dz in three bf16 terms cost it 1 to 5 us of 4 to 11.)
 // 8192 x 1024 x 4096: forward gelu 63 us (cuBLAS's bare product 57), backward 132 us (34 dz, 4
 // dbias, 95 the products); 8192 x 4096 x 1024 with dropout and f32 residual 67 us.
 #include "linear.cuh"
@@ -31,16 +33,18 @@ int dz_groups(int M, int N) {
     return gy < 1 ? 1 : gy;
 }
 
-// dz [M][ldz] (nullable) and the column sums of a block's rows, part[gy][N] (nullable; with one row of
-// blocks it is dbias itself, added to when `accumulate`). `vec`: rows of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a time, their
-// loads in flight together as raw words. Bound by memory: 8192 x 4096 bf16 gelu, 201 MB, 34 us
-// (5.9 TB/s).
+// dz [M][ldz] in bf16 and in f32 (each nullable) and the column sums of a block's rows,
+// part[gy][N] (nullable; with one row of blocks it is dbias itself, added to when `accumulate`).
+// `vec`: rows of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a
+// time, their loads in flight together as raw words. Bound by memory: 8192 x 4096 bf16 gelu, 201 MB,
+// 34 us (5.9 TB/s).
 constexpr int kDzInFlight = 2;
 template <typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long lddy,
                                                         const bf16* __restrict__ pre,
                                                         long long ld_pre, DropArgs drop,
-                                                        bf16* __restrict__ dz, long long ldz,
+                                                        bf16* __restrict__ dz,
+                                                        float* __restrict__ dz32, long long ldz,
                                                         float* __restrict__ part, int accumulate,
                                                         int M, int N, int vec) {
     pdl_enter();
@@ -94,6 +98,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
                 for (int i = 0; i < 4; ++i) sum[i] = fadd2(sum[i], make_float2(v[2 * i], v[2 * i + 1]));
                 // columns past N, up to the padded stride, are written as zeros
                 if (dz) store8(dz + row * ldz + col, v);
+                if (dz32) store8(dz32 + row * ldz + col, v);
             }
         }
     }
@@ -116,25 +121,25 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
 }
 
 template <typename T, int ACT>
-int launch_dz_act(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* sums, int vec,
-                  cudaStream_t s) {
+int launch_dz_act(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* to32,
+                  float* sums, int vec, cudaStream_t s) {
     const int accumulate = grid.y == 1 && a.accumulate;
     return launch_kernel(drop.rng ? linear_dz_kernel<T, ACT, true> : linear_dz_kernel<T, ACT, false>,
-                         grid, 256, 0, s, (const T*)a.dy, a.lddy, a.pre, a.ld_pre, drop, to,
+                         grid, 256, 0, s, (const T*)a.dy, a.lddy, a.pre, a.ld_pre, drop, to, to32,
                          ceil8(a.N), sums, accumulate, a.M, a.N, vec);
 }
 template <typename T>
-int launch_dz(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* sums, int vec,
-              cudaStream_t s) {
+int launch_dz(const LinearBwd& a, const DropArgs& drop, dim3 grid, bf16* to, float* to32, float* sums,
+              int vec, cudaStream_t s) {
     switch (a.act) {
         case kActRelu:
-            return launch_dz_act<T, kActRelu>(a, drop, grid, to, sums, vec, s);
+            return launch_dz_act<T, kActRelu>(a, drop, grid, to, to32, sums, vec, s);
         case kActGelu:
-            return launch_dz_act<T, kActGelu>(a, drop, grid, to, sums, vec, s);
+            return launch_dz_act<T, kActGelu>(a, drop, grid, to, to32, sums, vec, s);
         case kActSilu:
-            return launch_dz_act<T, kActSilu>(a, drop, grid, to, sums, vec, s);
+            return launch_dz_act<T, kActSilu>(a, drop, grid, to, to32, sums, vec, s);
         default:
-            return launch_dz_act<T, kActNone>(a, drop, grid, to, sums, vec, s);
+            return launch_dz_act<T, kActNone>(a, drop, grid, to, to32, sums, vec, s);
     }
 }
 
@@ -302,7 +307,7 @@ int product(const bf16* A, long long lda, int a_mn, const bf16* B, long long ldb
         return rows_product(r, b_mn, s);
     }
     if (K <= kOuterRows && a_mn && b_mn)
-        return outer_product(A, lda, B, ldb, M, N, K, out, out_f32, ldo, accumulate, alpha, s);
+        return outer_product(A, lda, B, ldb, 0, M, N, K, out, out_f32, ldo, accumulate, alpha, s);
     if (const int n = work ? product_splits(M, N, K) : 1; n > 1) {
         RowsArgs r{nullptr, 0, nullptr, 0, alpha, nullptr, kActNone, {}, accumulate ? out : nullptr, ldo,
                    nullptr, 0, out, out_f32, ldo, M, N, K};
@@ -375,14 +380,32 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
     return rc ? rc : gemm_run(plan, s);
 }
 
-size_t linear_backward_work(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0 || M > kMaxDim || N > kMaxDim || K > kMaxDim) return 0;
-    // dw is [N, K] or [K, N]: the larger of the two; its planes follow dx's in the same place
+namespace {
+
+// The backward's workspace: dz in bf16, the row groups' column sums, the planes of the products (dw's
+// follow dx's in the same place), dz in f32 where rows are few. Byte offsets and the whole.
+struct BackwardLayout {
+    size_t part, planes, dz32, total;
+};
+BackwardLayout backward_layout(int M, int N, int K) {
+    // dw is [N, K] or [K, N]: the larger of the two
     size_t planes = product_work(M, K, N);
     const size_t dw = product_work(N, K, M), dw_mn = product_work(K, N, M);
     if (dw > planes) planes = dw;
     if (dw_mn > planes) planes = dw_mn;
-    return align256((size_t)M * ceil8(N) * 2) + align256((size_t)dz_groups(M, N) * N * 4) + planes;
+    BackwardLayout l;
+    l.part = align256((size_t)M * ceil8(N) * 2);
+    l.planes = l.part + align256((size_t)dz_groups(M, N) * N * 4);
+    l.dz32 = l.planes + planes;
+    l.total = l.dz32 + (M <= kOuterRows ? align256((size_t)M * ceil8(N) * 4) : 0);
+    return l;
+}
+
+}  // namespace
+
+size_t linear_backward_work(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0 || M > kMaxDim || N > kMaxDim || K > kMaxDim) return 0;
+    return backward_layout(M, N, K).total;
 }
 
 int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
@@ -410,17 +433,18 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
     const bool need_dz = !as_is && (a.dx || a.dw);
     const bf16* dz = reinterpret_cast<const bf16*>(a.dy);
     long long ldz = a.lddy;
-    void* planes = a.work ? reinterpret_cast<char*>(a.work) + align256((size_t)a.M * ceil8(a.N) * 2) +
-                                align256((size_t)dz_groups(a.M, a.N) * a.N * 4)
-                          : nullptr;
+    const BackwardLayout l = backward_layout(a.M, a.N, a.K);
+    char* const work = reinterpret_cast<char*>(a.work);
+    void* planes = work ? work + l.planes : nullptr;
+    float* dz32 = nullptr;  // of few rows, for dw
     // the products need not wait for what runs in front of them once dz's own kernel has ended: dx
     // for the second stage of dbias, dw for it and for dx (unless dx's planes lie where dw's go)
     int early = 0;
     if (need_dz || a.dbias) {
         if (!a.work) return -1;
-        bf16* buf = reinterpret_cast<bf16*>(a.work);
-        float* part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.work) +
-                                               align256((size_t)a.M * ceil8(a.N) * 2));
+        bf16* buf = reinterpret_cast<bf16*>(work);
+        float* part = reinterpret_cast<float*>(work + l.part);
+        if (need_dz && a.dw && a.M <= kOuterRows) dz32 = reinterpret_cast<float*>(work + l.dz32);
         const int groups = dz_groups(a.M, a.N);
         DropArgs drop = a.drop;
         if (!drops) drop.rng = nullptr;
@@ -428,10 +452,10 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
         const int vec = aligned16(a.dy) && (a.lddy % per16) == 0 &&
                         (a.act == kActNone || (aligned16(a.pre) && (a.ld_pre & 7) == 0));
         const dim3 grid((a.N + kDzCols - 1) / kDzCols, groups);
-        bf16* to = need_dz ? buf : nullptr;
+        bf16* to = need_dz && (a.dx || !dz32) ? buf : nullptr;
         float* sums = !a.dbias ? nullptr : groups == 1 ? a.dbias : part;
-        int rc = a.dy_f32 ? launch_dz<float>(a, drop, grid, to, sums, vec, s)
-                          : launch_dz<bf16>(a, drop, grid, to, sums, vec, s);
+        int rc = a.dy_f32 ? launch_dz<float>(a, drop, grid, to, dz32, sums, vec, s)
+                          : launch_dz<bf16>(a, drop, grid, to, dz32, sums, vec, s);
         if (rc) return rc;
         if (a.dbias && groups > 1) {
             rc = launch_kernel_pdl(linear_db_kernel, (a.N + 31) / 32, 1024, 0, s, part, groups, a.N,
@@ -450,6 +474,11 @@ int linear_backward(const LinearBwd& a, int num_sms, cudaStream_t s) {
         if (rc) return rc;
         early = (!planes || product_splits(a.M, a.K, a.N) == 1) && leaves_room(a.M, a.K, 1);
     }
+    if (a.dw && dz32)
+        return a.w_mn_major ? outer_product(a.x, a.ldx, dz32, ldz, 2, a.K, a.N, a.M, a.dw, a.dw_f32,
+                                            a.lddw, a.accumulate, nullptr, s)
+                            : outer_product(dz32, ldz, a.x, a.ldx, 1, a.N, a.K, a.M, a.dw, a.dw_f32,
+                                            a.lddw, a.accumulate, nullptr, s);
     if (a.dw) {
         const int rc =
             a.w_mn_major

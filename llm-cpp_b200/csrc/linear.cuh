@@ -48,8 +48,9 @@ struct LinearFwd {
 };
 int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s);
 
-// dz = drop(dy act'(pre)) in bf16, dbias (+)= column sums of dz (before its rounding), dx = dz w,
-// dw (+)= dz^T x (laid out as w). dx, dw, dbias nullable.
+// dz = drop(dy act'(pre)), dbias (+)= column sums of dz, dx = dz w, dw (+)= dz^T x (laid out as w). The
+// tensor cores take dz in bf16; dw of up to kOuterRows rows, which they do not form, takes it in f32.
+// dx, dw, dbias nullable.
 struct LinearBwd {
     const void* dy;
     int dy_f32;
@@ -128,9 +129,10 @@ struct RowsArgs {
 };
 int rows_product(const RowsArgs& a, int w_mn, cudaStream_t s);
 // out[M,N] (+)= alpha sum_k A[k,M] B[k,N] over K <= kOuterRows rows: bound by the result's writes.
+// A and B are bf16, or one of them (f32: 1 A, 2 B) f32 with rows padded to 8 elements, on 16 bytes.
 constexpr int kOuterRows = 8;
-int outer_product(const bf16* A, long long lda, const bf16* B, long long ldb, int M, int N, int K,
-                  void* out, int out_f32, long long ldo, int accumulate, const float* alpha,
+int outer_product(const void* A, long long lda, const void* B, long long ldb, int f32, int M, int N,
+                  int K, void* out, int out_f32, long long ldo, int accumulate, const float* alpha,
                   cudaStream_t s);
 
 // Splits along K of a product with too few tiles for the device, and the bytes of their planes.

@@ -221,10 +221,25 @@ __global__ void __launch_bounds__(32 * kRowsMnWarps) linear_rows_mn_kernel(const
 // --------------------------------------------------------------------------------- outer product
 // A warp writes 256 columns (8 a lane) of 8 rows; the lane keeps its columns of B in registers, the
 // block's 64 rows of A lie in shared memory as f32. KK: K rounded up to a power of two.
+// Everything is f32 but what memory holds in bf16.
 constexpr int kOuterTile = 64;
-template <typename T, int KK>
-__global__ void __launch_bounds__(256) outer_product_kernel(const bf16* __restrict__ A, long long lda,
-                                                            const bf16* __restrict__ B, long long ldb,
+__device__ __forceinline__ void outer_chunk(const bf16* p, int col, int N, float2 (&b)[4]) {
+    uint32_t u[4];
+    row_chunk<8>(p, col, N, u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = make_float2(bf16_lo(u[j]), bf16_hi(u[j]));
+}
+__device__ __forceinline__ void outer_chunk(const float* p, int col, int, float2 (&b)[4]) {
+    Raw8<float> q;
+    float v[8];
+    load_raw(p + col, q);
+    raw_f32(q, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = make_float2(v[2 * j], v[2 * j + 1]);
+}
+template <typename T, int KK, typename TA, typename TB>
+__global__ void __launch_bounds__(256) outer_product_kernel(const TA* __restrict__ A, long long lda,
+                                                            const TB* __restrict__ B, long long ldb,
                                                             int M, int N, int K, int tiles_n,
                                                             T* out, long long ldo, int accumulate,
                                                             int vec,
@@ -237,15 +252,14 @@ __global__ void __launch_bounds__(256) outer_product_kernel(const bf16* __restri
     const float f = alpha ? *alpha : 1.0f;
     for (int i = threadIdx.x; i < KK * kOuterTile; i += 256) {
         const int k = i / kOuterTile, r = i - k * kOuterTile;
-        sa[k][r] = k < K && r0 + r < M ? __bfloat162float(A[k * lda + r0 + r]) : 0.0f;
+        sa[k][r] = k < K && r0 + r < M ? to_f32(A[k * lda + r0 + r]) : 0.0f;
     }
     float2 b[KK][4];
 #pragma unroll
     for (int k = 0; k < KK; ++k) {
-        uint32_t u[4] = {0u, 0u, 0u, 0u};
-        if (k < K && col < N) row_chunk<8>(B + k * ldb, col, N, u);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[k][j] = make_float2(bf16_lo(u[j]), bf16_hi(u[j]));
+        for (int j = 0; j < 4; ++j) b[k][j] = make_float2(0.0f, 0.0f);
+        if (k < K && col < N) outer_chunk(B + k * ldb, col, N, b[k]);
     }
     __syncthreads();
     if (col >= N) return;
@@ -301,31 +315,33 @@ int rows_product(const RowsArgs& a, int w_mn, cudaStream_t s) {
 }
 
 namespace {
-template <typename T, int KK>
-int launch_outer(const bf16* A, long long lda, const bf16* B, long long ldb, int M, int N, int K, void* out,
+template <typename T, int KK, typename TA, typename TB>
+int launch_outer(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, void* out,
                  long long ldo, int accumulate, const float* alpha, cudaStream_t s) {
     const int tiles_n = (N + 255) / 256;
     const int grid = tiles_n * ((M + kOuterTile - 1) / kOuterTile);
     const int vec = rows_on_16((const T*)out, ldo);
-    return launch_kernel(outer_product_kernel<T, KK>, grid, 256, 0, s, A, lda, B, ldb, M, N, K, tiles_n,
-                         (T*)out, ldo, accumulate, vec, alpha);
+    return launch_kernel(outer_product_kernel<T, KK, TA, TB>, grid, 256, 0, s, (const TA*)A, lda,
+                         (const TB*)B, ldb, M, N, K, tiles_n, (T*)out, ldo, accumulate, vec, alpha);
 }
-template <typename T>
-int launch_outer_k(const bf16* A, long long lda, const bf16* B, long long ldb, int M, int N, int K,
+template <typename T, typename TA, typename TB>
+int launch_outer_k(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K,
                    void* out, long long ldo, int accumulate, const float* alpha, cudaStream_t s) {
-    auto* f = K == 1   ? launch_outer<T, 1>
-              : K == 2 ? launch_outer<T, 2>
-              : K <= 4 ? launch_outer<T, 4>
-                       : launch_outer<T, kOuterRows>;
+    auto* f = K == 1   ? launch_outer<T, 1, TA, TB>
+              : K == 2 ? launch_outer<T, 2, TA, TB>
+              : K <= 4 ? launch_outer<T, 4, TA, TB>
+                       : launch_outer<T, kOuterRows, TA, TB>;
     return f(A, lda, B, ldb, M, N, K, out, ldo, accumulate, alpha, s);
 }
 }  // namespace
 
-int outer_product(const bf16* A, long long lda, const bf16* B, long long ldb, int M, int N, int K,
-                  void* out, int out_f32, long long ldo, int accumulate, const float* alpha,
+int outer_product(const void* A, long long lda, const void* B, long long ldb, int f32, int M, int N,
+                  int K, void* out, int out_f32, long long ldo, int accumulate, const float* alpha,
                   cudaStream_t s) {
-    return out_f32 ? launch_outer_k<float>(A, lda, B, ldb, M, N, K, out, ldo, accumulate, alpha, s)
-                   : launch_outer_k<bf16>(A, lda, B, ldb, M, N, K, out, ldo, accumulate, alpha, s);
+    auto* f = f32 == 1   ? (out_f32 ? launch_outer_k<float, float, bf16> : launch_outer_k<bf16, float, bf16>)
+              : f32 == 2 ? (out_f32 ? launch_outer_k<float, bf16, float> : launch_outer_k<bf16, bf16, float>)
+                         : (out_f32 ? launch_outer_k<float, bf16, bf16> : launch_outer_k<bf16, bf16, bf16>);
+    return f(A, lda, B, ldb, M, N, K, out, ldo, accumulate, alpha, s);
 }
 
 }  // namespace llmgpu

@@ -305,6 +305,46 @@ def test_linear_bwd_dropped_places_count_nothing(cuda, M, act, dyt, pad):
     assert all(bool(torch.isfinite(v).all()) for v in want)
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("K,N", [(256, 37), (130, 1021), (768, 640)])
+@pytest.mark.parametrize("act,p,dyt,w_mn", [("none", 0.0, F32, False), ("none", 0.3, BF, True),
+                                            ("gelu", 0.0, BF, False), ("silu", 0.2, F32, True),
+                                            ("relu", 0.5, BF, True)])
+def test_linear_bwd_of_few_rows_keeps_dz(cuda, monkeypatch, M, K, N, act, p, dyt, w_mn):
+    """dw of up to 8 rows comes from dz as it is: no rounding to bf16 stands between."""
+    from llmgpu import ops
+    monkeypatch.setitem(globals(), "H16", 0.0)  # _linear_bwd_want's rounding of dz
+    g, x, w, _, _ = _linear_case(cuda, M, K, N, act, p, dyt, False, False, w_mn, M + K + N, 8)
+    rng, site = _rng(cuda, 5, 99), 8
+    dy = _mat(g, M, N, dyt, cuda, 0.1)[0]
+    pre = _mat(g, M, N, BF, cuda, 2.0)[0] if act != "none" else None
+    _, _, dw, ew, _, _ = _linear_bwd_want(dy, x, w, pre, act, p, w_mn, rng, site)
+    aw = torch.full(tuple(w.shape), 0.5, device=cuda)
+    ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn, dw=aw, dbias=torch.zeros(N, device=cuda),
+                   accumulate=True)
+    _close(aw, dw + 0.5, ew + H32 * (dw.abs() + 0.5 + ew), "accumulated dw")
+    alone = ops.linear_bwd(dy, x, w, pre, act, p, rng, site, w_mn, dw=torch.zeros_like(aw), need_dx=False,
+                           need_dbias=False)[1]
+    _close(alone, dw, ew, "dw alone")
+    ops.check_device(cuda)
+
+
+def test_linear_bwd_of_few_rows_far_out(cuda):
+    """f32's largest values, infinities and NaN in dy of few rows reach dw as they are, each in its own
+    place alone."""
+    from llmgpu import ops
+    x = torch.ones(3, 8, dtype=BF, device=cuda)
+    w = torch.zeros(8, 8, dtype=BF, device=cuda)
+    for w_mn in (False, True):
+        for v in (3.3e38, -3.3e38, torch.finfo(F32).max, 1e-37, math.inf, -math.inf, math.nan):
+            dy = torch.zeros(3, 8, device=cuda)
+            dy[1, 0] = v
+            _, dw, _ = ops.linear_bwd(dy, x, w, w_mn=w_mn, dw=torch.zeros(8, 8, device=cuda))
+            dw = dw if w_mn else dw.t()  # [K, N]
+            assert torch.equal(dw[:, 0], dy[1, 0].expand(8)) or (math.isnan(v) and dw[:, 0].isnan().all())
+            assert not dw[:, 1:].any()
+
+
 @pytest.mark.parametrize("w_mn", [False, True])
 def test_long_sums_in_f32(cuda, w_mn):
     """f32 results of operands that bf16 holds exactly: a chain is 32 accumulations of 16 products,
