@@ -164,7 +164,11 @@ int llmgpu_op_dropout(const void* x, int x_f32, long long ldx, const void* resid
  *   out's type, bf16 or f32 (out_f32), and may be out itself. pre (nullable, bf16): z, which the
  *   backward needs when act is not none. out, resid and pre take any row stride. M = 0 is allowed;
  *   M, N, K <= 2^30.
- *   err as in llmgpu_op_gemm. */
+ *   work: llmgpu_op_linear_fwd_work(M, N, K) bytes (0 where it is not used; the backward's workspace may
+ *   be smaller), 16-byte aligned: a product of few tiles and long K is split along K there. With NULL,
+ *   K stays whole: the same to f32 rounding, but slower.
+ *   err as in llmgpu_op_gemm; NULL: a wait that timed out is not reported. */
+long long llmgpu_op_linear_fwd_work(int M, int N, int K);
 int llmgpu_op_linear_fwd(const void* x, long long ldx, const void* w, long long ldw, int w_mn_major,
                          const float* bias, int act, float p, const uint64_t* rng, uint64_t site,
                          const void* resid, long long ldr, void* pre, long long ld_pre, void* out,

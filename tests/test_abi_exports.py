@@ -36,6 +36,17 @@ def test_library_exports_every_declared_symbol():
     assert not missing, missing
 
 
+def test_headers_declare_every_exported_function():
+    """A caller from C sees whatever the library defines with C linkage."""
+    csrc = os.path.join(ROOT, "llm-cpp_b200", "csrc")
+    defined = set()
+    for f in sorted(os.listdir(csrc)):
+        src = open(os.path.join(csrc, f)).read()
+        defined |= set(re.findall(r'extern "C"[^;{(]*?\b(llmgpu_\w+)\s*\(', src))
+    assert "llmgpu_op_gemm" in defined
+    assert not defined - set(_declared())
+
+
 def test_create_without_device_fails_cleanly():
     torch = pytest.importorskip("torch")
     if torch.cuda.is_available():

@@ -966,6 +966,30 @@ def test_plain_c_calls_equal_the_wrappers(cuda):
         assert torch.equal(a, c), i
 
 
+@pytest.mark.parametrize("M,K,N", [(256, 4096, 512), (40, 2101, 130), (2048, 768, 768)])
+def test_plain_c_linear_forward_stays_in_its_workspace(cuda, M, K, N):
+    """With a workspace of llmgpu_op_linear_fwd_work bytes (products split along K and others), and
+    with none, which leaves K whole: the same to f32 rounding, nothing written behind it."""
+    from llmgpu import load, ops
+    lib = load()
+    g = torch.Generator().manual_seed(K)
+    x, w = _mat(g, M, K, BF, cuda)[0], _mat(g, N, K, BF, cuda, 1 / math.sqrt(K))[0]
+    n = lib.llmgpu_op_linear_fwd_work(M, N, K)
+    buf = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device=cuda)
+    y, z = torch.empty(M, N, device=cuda), torch.empty(M, N, device=cuda)
+    st = torch.cuda.current_stream().cuda_stream
+    for out, work in ((y, buf.data_ptr()), (z, None)):
+        assert lib.llmgpu_op_linear_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), 0, None, 0,
+                                        0.0, None, 0, None, 0, None, 0, out.data_ptr(), 1, N, M, N, K,
+                                        work, None, st) == 0
+    assert torch.equal(y, ops.linear_fwd(x, w, out_dtype=F32)[0])
+    assert bool((buf[n:] == 0xA5).all())
+    xd, wd = x.double(), w.double().t()
+    want, tol = xd @ wd, (K + 4) * ACC * (xd.abs() @ wd.abs())
+    _close(y, want, tol, "with a workspace")
+    _close(z, want, tol, "without")
+
+
 # ------------------------------------------------------------------------------------ refusals
 def test_wrapper_refusals(cuda):
     from llmgpu import ops

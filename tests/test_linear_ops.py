@@ -155,6 +155,17 @@ def test_workspace_covers_any_piece():
     assert f(100, 64, 5000, 8192) == f(100, 64, 5000, 1 << 20) == f(100, 64, 5000, 0)
 
 
+def test_linear_forward_workspace():
+    """Room for two f32 planes of the result at least where K is split, 0 where it is not; the
+    backward's size is another, which may be smaller."""
+    fwd, bwd = _lib().llmgpu_op_linear_fwd_work, _lib().llmgpu_op_linear_bwd_work
+    for M, N, K in ((256, 512, 4096), (40, 130, 2101), (17, 8, 1 << 20)):
+        assert fwd(M, N, K) >= 2 * M * N * 4
+    assert bwd(256, 512, 4096) < fwd(256, 512, 4096)
+    for M, N, K in ((16, 512, 4096), (256, 512, 512), (8192, 4096, 1024)):
+        assert fwd(M, N, K) == 0
+
+
 def test_block_call_refusals():
     """llmgpu_op_call: an unknown operator, no block, an integer past its argument's type, and the
     refusals of the calls themselves."""
