@@ -229,6 +229,12 @@ enum {
 };
 int llmgpu_op_call(int op, const void* args);
 
+/* A device error word (the `err` of these calls) that the library holds for each device, zero at first:
+ * its address on the current device, usable inside a stream capture too. take_error waits for the
+ * current device, stores the word in *code and clears it. */
+int llmgpu_op_error_word(int** word);
+int llmgpu_op_take_error(int* code);
+
 /* Number of SMs the library sizes persistent grids for (device 0 of the caller). */
 int llmgpu_op_num_sms(void);
 /* CTA pairs (clusters of two SMs) the 256x256-tile GEMM keeps resident at once. */

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <string.h>
 
+#include "common.cuh"
 #include "dropout.cuh"
 #include "gemm.cuh"
 #include "kernels.cuh"
@@ -297,6 +298,28 @@ extern "C" int llmgpu_op_linear_ce_bwd(const void* x, long long ldx, const void*
     return head_backward(a, lse, dloss, scale, dx, dx_f32 != 0, lddx, dw, dw_f32 != 0, lddw,
                          accumulate != 0, piece, device_num_sms(),
                          reinterpret_cast<cudaStream_t>(stream));
+}
+
+// Static device memory, so that no call has to allocate it: a first call may be under capture.
+__device__ int g_op_error;
+
+extern "C" int llmgpu_op_error_word(int** word) {
+    if (!word) return -1;
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_op_error) != cudaSuccess) return launch_status();
+    *word = reinterpret_cast<int*>(p);
+    return 0;
+}
+
+extern "C" int llmgpu_op_take_error(int* code) {
+    if (!code) return -1;
+    if (cudaDeviceSynchronize() != cudaSuccess ||
+        cudaMemcpyFromSymbol(code, g_op_error, sizeof(int)) != cudaSuccess)
+        return launch_status();
+    const int zero = 0;
+    if (*code && cudaMemcpyToSymbol(g_op_error, &zero, sizeof(int)) != cudaSuccess)
+        return launch_status();
+    return 0;
 }
 
 namespace {

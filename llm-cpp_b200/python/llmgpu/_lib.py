@@ -70,6 +70,9 @@ def _declare(lib):
                                             c_vp]
     lib.llmgpu_op_call.argtypes = [c_int, ctypes.c_char_p]
     lib.llmgpu_op_call.restype = c_int
+    lib.llmgpu_op_error_word.argtypes = [ctypes.POINTER(c_vp)]
+    lib.llmgpu_op_take_error.argtypes = [ctypes.POINTER(c_int)]
+    lib.llmgpu_op_error_word.restype = lib.llmgpu_op_take_error.restype = c_int
     for n, k in (("llmgpu_op_linear_fwd_work", 3), ("llmgpu_op_linear_bwd_work", 3), ("llmgpu_op_linear_ce_fwd_work", 2),
                  ("llmgpu_op_linear_ce_bwd_work", 4)):
         getattr(lib, n).argtypes = [c_int] * k

@@ -3,6 +3,7 @@
 Arguments are torch CUDA tensors (used only as device allocations); every call
 checks the status code and the device error word and raises on failure.
 """
+import ctypes
 import functools
 import struct
 
@@ -247,28 +248,29 @@ _err_words = {}
 
 
 def _err_word(device):
-    """Address of the device's error word of these operators (made outside a capture, once)."""
+    """Address of the device's error word of these operators, in a capture too."""
     w = _err_words.get(device.index)
     if w is None:
-        if torch.cuda.is_current_stream_capturing():
-            return 0  # the first call on this device is being captured: waits stay bounded
-        w = _err_words[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-        torch.cuda.current_stream(device).synchronize()  # any later stream may use it
-    return w.data_ptr()
+        p = ctypes.c_void_p()
+        with torch.cuda.device(device):
+            rc = load().llmgpu_op_error_word(ctypes.byref(p))
+        if rc != 0:
+            raise KernelError(f"llmgpu_op_error_word failed with status {rc}")
+        w = _err_words[device.index] = p.value
+    return w
 
 
 def check_device(device="cuda"):
     """Waits for the device and raises if a wait inside one of these operators' kernels gave up (its
-    result, and those of the calls after it, are then not to be used); the word is cleared."""
-    device = torch.device(device)
-    index = torch.cuda.current_device() if device.index is None else device.index
-    torch.cuda.synchronize(index)
-    w = _err_words.get(index)
-    if w is not None:
-        code = int(w.item())
-        if code:
-            w.zero_()
-            raise KernelError(f"device error code {code}")
+    result, and those of the calls after it on any stream of the device, are then not to be used);
+    the word is cleared. Nothing else reports it."""
+    code = ctypes.c_int()
+    with torch.cuda.device(torch.device(device)):
+        rc = load().llmgpu_op_take_error(ctypes.byref(code))
+    if rc != 0:
+        raise KernelError(f"llmgpu_op_take_error failed with status {rc}")
+    if code.value:
+        raise KernelError(f"device error code {code.value}")
 
 
 # llmgpu_op_call's number and block of each operator: integers and addresses in the order of the C

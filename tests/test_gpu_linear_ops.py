@@ -4,6 +4,9 @@ step of bf16 and f32 relative to the value; a product of length K accumulated in
 most about K steps of the sum of its terms' magnitudes (ACC per term, two half steps: the tensor
 cores may truncate)."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -12,6 +15,7 @@ import linear_ops_ref as ref
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
+ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 BF, F32 = torch.bfloat16, torch.float32
 H16, H32 = 2.0 ** -8, 2.0 ** -24
 ACC = 2.0 ** -23
@@ -988,6 +992,47 @@ def test_plain_c_linear_forward_stays_in_its_workspace(cuda, M, K, N):
     want, tol = xd @ wd, (K + 4) * ACC * (xd.abs() @ wd.abs())
     _close(y, want, tol, "with a workspace")
     _close(z, want, tol, "without")
+
+
+_CAPTURED_FIRST = """
+import torch
+from llmgpu import ops
+from llmgpu.ops import KernelError
+dev = torch.device("cuda:0")
+x = torch.ones(64, 64, dtype=torch.bfloat16, device=dev)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y, _ = ops.linear_fwd(x, x)
+    word = ops._err_word(dev)
+assert word, "the captured call has no error word"
+g.replay()
+ops.check_device(dev)
+assert bool((y == 64).all()) and ops._err_word(dev) == word
+
+class At:  # the word as a tensor
+    __cuda_array_interface__ = dict(shape=(1,), typestr="<i4", data=(word, False), version=3)
+w = torch.as_tensor(At(), device=dev)
+assert int(w) == 0
+w.fill_(7)
+try:
+    ops.check_device(dev)
+except KernelError as e:
+    assert "7" in str(e)
+else:
+    raise AssertionError("not raised")
+assert int(w) == 0
+ops.check_device(dev)
+print("captured first: ok")
+"""
+
+
+def test_first_call_may_be_captured(cuda):
+    """The first call of a process has its device's error word inside a capture too."""
+    env = dict(os.environ, PYTHONPATH=os.path.join(ROOT, "llm-cpp_b200", "python"))
+    r = subprocess.run([sys.executable, "-c", _CAPTURED_FIRST], env=env, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "captured first: ok" in r.stdout, r.stdout + r.stderr
 
 
 # ------------------------------------------------------------------------------------ refusals

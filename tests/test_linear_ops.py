@@ -195,6 +195,10 @@ def test_block_call_refusals():
         assert call("llmgpu_op_linear_ce_bwd", *ceb[:i], bad, *ceb[i + 1:]) in REFUSED
 
 
+def test_error_word_refusals():
+    assert _lib().llmgpu_op_error_word(None) != 0 and _lib().llmgpu_op_take_error(None) != 0
+
+
 def test_wrappers_refuse_cpu_tensors():
     from llmgpu import ops
     x, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
