@@ -152,7 +152,9 @@ int llmgpu_op_moe_dispatch(const int* idx, int B, int T, int E, int k, int* grp,
  *   everything (out = resid or 0); a dropped element gives 0 whatever x holds.
  *   rng: two uint64 in device memory, {seed, offset}, read when the kernel runs, so that the
  *   replays of a captured step can advance the offset; `site` tells the dropouts of one step
- *   apart. cols <= 2^30. */
+ *   apart. Equal seeds and sums offset + site give equal masks: between steps, and between
+ *   micro-batches, the offset has to move on by more than the largest site, and data-parallel
+ *   ranks need seeds of their own. cols <= 2^30. */
 int llmgpu_op_dropout(const void* x, int x_f32, long long ldx, const void* resid, long long ldr,
                       void* out, int out_f32, long long ldo, int rows, int cols, float p,
                       const uint64_t* rng, uint64_t site, void* stream);

@@ -398,7 +398,9 @@ def dropout_fwd(x, p, rng, site=0, resid=None, out=None, out_dtype=None):
     """resid + (kept ? x / (1 - p) : 0) over a 2-D x (f32 or bf16), in `out_dtype` (x's if not
     given). `rng`: int64 device tensor (seed, offset); `site` tells the dropouts of a step apart.
     The mask depends on (seed, offset + site, row, column) alone and p counts in steps of
-    1 / 65536; see llmgpu_op_dropout. `out` may be x or resid."""
+    1 / 65536; see llmgpu_op_dropout. Between steps or micro-batches the offset has to move on by
+    more than the largest site, or masks come back; data-parallel ranks need seeds of their own.
+    `out` may be x or resid."""
     dev = _device_of(x, "x")
     rows, cols = x.shape
     px, ldx = _matrix(x, "x", _FLOATS, rows, cols, dev)

@@ -1,6 +1,10 @@
 """CPU checks of dropout, the linear layer and the loss head: the generator against its published
 known answers, and the refusals that no kernel has to see (the C ABI's and the wrappers')."""
+import ast
 import ctypes
+import inspect
+import os
+import re
 
 import numpy as np
 import pytest
@@ -8,6 +12,8 @@ import pytest
 import linear_ops_ref as ref
 
 torch = pytest.importorskip("torch")
+
+ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 
 
 @pytest.mark.parametrize("ctr,key,want", [
@@ -28,6 +34,37 @@ def test_mask_frequency():
         keep, scale = ref.keep_mask(5, 11, 512, 1024, p)
         q = 1 / scale
         assert abs(keep.double().mean().item() - q) < 5 * np.sqrt(q * (1 - q) / n)
+
+
+def _written_out_step():
+    """The sites of the training step that INTEGRATION.md writes out, and what it adds to the offset."""
+    from llmgpu import ops
+    md = open(os.path.join(ROOT, "INTEGRATION.md")).read()
+    code, = [c for c in re.findall(r"```python\n(.*?)```", md, re.S) if "dropout_fwd" in c]
+    sites, adds = set(), []
+    for n in ast.walk(ast.parse(code)):
+        if isinstance(n, ast.Call) and ast.unparse(n.func).startswith("ops."):
+            sig = inspect.signature(getattr(ops, n.func.attr))
+            a = sig.bind(*n.args, **{k.arg: k.value for k in n.keywords}).arguments
+            if "rng" in a:
+                sites.add(ast.literal_eval(a["site"]) if "site" in a else 0)
+        elif isinstance(n, ast.AugAssign) and ast.unparse(n.target) == "rng[1]":
+            adds.append(ast.literal_eval(n.value))
+    return sites, adds
+
+
+def test_no_mask_of_the_written_out_step_comes_back():
+    """A mask goes by offset + site: the steps' sums (and so the masks of one shape) are all different."""
+    sites, adds = _written_out_step()
+    assert sites == {0, 1} and len(adds) == 1 and adds[0] > max(sites)
+    masks = [ref.keep_mask(3, step * adds[0] + s, 16, 64, 0.5)[0] for step in range(4) for s in sites]
+    assert not any(torch.equal(a, b) for i, a in enumerate(masks) for b in masks[:i])
+
+
+def test_sites_and_offsets_add_up():
+    """What that rule is for: site 1 of a step has the mask of site 0 at the next offset."""
+    a, b = ref.keep_mask(3, 5 + 1, 16, 64, 0.5)[0], ref.keep_mask(3, 6 + 0, 16, 64, 0.5)[0]
+    assert torch.equal(a, b)
 
 
 def _lib():
