@@ -241,7 +241,8 @@ def moe_dispatch(idx, B, T, E):
 # and allocate what they return (and their workspace) from torch's allocator, so they can be captured
 # into a graph. Matrices are 2-D with neighbouring columns and any row stride; the matrices they
 # return start their rows on 16 bytes (the row stride is rounded up to 8 elements), so that one
-# operator's result can be another's operand.
+# operator's result can be another's operand. They are no autograd functions: what they return
+# requires no gradient, whatever the operands do; the _bwd calls are the backward.
 ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 
 _err_words = {}
