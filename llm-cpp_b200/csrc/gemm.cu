@@ -1589,6 +1589,7 @@ struct PairItems {
 template <int NG, int FAM>
 __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
     gemm_bf16_pair_kernel(const __grid_constant__ PairParams<NG, FAM> P) {
+    static_assert(NG == 1 || FAM == kFamBase, "dual launches take no accumulator chains");
     using Cfg = PairCfgOf<FAM>;
     constexpr int STAGES = Cfg::STAGES;
     constexpr int BN = Cfg::BN;
@@ -1889,46 +1890,38 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
                 int kb0, kb1;
                 tile_kblocks<FAM>(args, s_grp, t, sh.num_m, sh.num_n, sh.tiles_mn, sh.kblocks, kb0,
                                   kb1);
-                const int ck = chain_blocks<FAM>(P.ext, kb0, kb1);
-                int kc = kb0;
-                do {
-                    const int kend = has_chains(FAM) ? min(kc + ck, kb1) : kb1;
-                    if (!mbar_wait_bounded_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
-                                                   kDevTimeoutAccFree)) {
+                if (!mbar_wait_bounded_cluster(&acc_empty[acc], acc_phase ^ 1u, err,
+                                               kDevTimeoutAccFree))
+                    break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait_bounded_cluster(&full[stage], phase, err, kDevTimeoutFull)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-                    for (int kb = kc; kb < kend; ++kb) {
-                        if (!mbar_wait_bounded_cluster(&full[stage], phase, err, kDevTimeoutFull)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t ao = (uint32_t)stage * (Cfg::A_BYTES >> 4);
-                        const uint32_t bo = (uint32_t)stage * (Cfg::B_BYTES >> 4);
+                    const uint32_t ao = (uint32_t)stage * (Cfg::A_BYTES >> 4);
+                    const uint32_t bo = (uint32_t)stage * (Cfg::B_BYTES >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < BK / 16; ++kk)
-                            umma_bf16_pair(d, da.at(ao, kk), db.at(bo, kk), idesc,
-                                      (kb > kc || kk > 0) ? 1u : 0u);
-                        umma_commit_pair(&empty[stage], 0x3);
-                        if (++stage == STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
+                    for (int kk = 0; kk < BK / 16; ++kk)
+                        umma_bf16_pair(d, da.at(ao, kk), db.at(bo, kk), idesc,
+                                       (kb > kb0 || kk > 0) ? 1u : 0u);
+                    umma_commit_pair(&empty[stage], 0x3);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
                     }
-                    if (!ok) break;
-                    if (kb1 > kb0) {
-                        umma_commit_pair(&acc_full[acc], 0x3);
-                    } else {  // empty group: both epilogues write zeros
-                        mbar_arrive(&acc_full[acc]);
-                        mbar_arrive_cluster(acc_full_peer + 8u * (uint32_t)acc);
-                    }
-                    acc ^= 1;
-                    if (acc == 0) acc_phase ^= 1u;
-                    kc = kend;
-                } while (has_chains(FAM) && kc < kb1);
+                }
+                if (!ok) break;
+                if (kb1 > kb0) {
+                    umma_commit_pair(&acc_full[acc], 0x3);
+                } else {  // empty group: both epilogues write zeros
+                    mbar_arrive(&acc_full[acc]);
+                    mbar_arrive_cluster(acc_full_peer + 8u * (uint32_t)acc);
+                }
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
             }
         }
     } else if (warp >= 4) {
