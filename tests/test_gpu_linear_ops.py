@@ -1035,6 +1035,86 @@ def test_first_call_may_be_captured(cuda):
     assert r.returncode == 0 and "captured first: ok" in r.stdout, r.stdout + r.stderr
 
 
+@pytest.mark.parametrize("w_mn", [False, True])
+def test_few_rows_offsets_past_32_bits(cuda, w_mn):
+    """Weights of more than 2^31 elements under 3 rows: columns (and rows of dw) on both sides of it."""
+    from llmgpu import ops
+    M, K, N = 3, 32768, 70000
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.randn(M, K, generator=g, device=cuda).to(BF)
+    w = torch.empty((K, N) if w_mn else (N, K), dtype=BF, device=cuda)
+    w.normal_(0, 0.01, generator=g)
+    at = torch.tensor([0, 1, 40000, 65535, 65536, 65537, N - 1], device=cuda)  # of N
+    wa = (w[:, at].t() if w_mn else w[at]).double()
+    y, _ = ops.linear_fwd(x, w, w_mn=w_mn, out_dtype=F32)
+    xd = x.double()
+    _close(y[:, at], xd @ wa.t(), (K + 4) * ACC * (xd.abs() @ wa.abs().t()), "y")
+    dy = torch.zeros(M, N, device=cuda)
+    dy[:, at] = torch.randn(M, len(at), generator=g, device=cuda)
+    dx, dw, _ = ops.linear_bwd(dy, x, w, w_mn=w_mn, dx_dtype=F32)
+    dz = dy[:, at].double()
+    _close(dx, dz @ wa, (H16 + (N + 4) * ACC) * (dz.abs() @ wa.abs()), "dx")
+    want = dz.t() @ xd
+    got = dw[:, at].t() if w_mn else dw[at]
+    _close(got, want, H16 * want.abs() + (M + 4) * ACC * (dz.abs().t() @ xd.abs()), "dw")
+    assert int(torch.count_nonzero(dw)) == int(torch.count_nonzero(got))
+    ops.check_device(cuda)
+
+
+def test_few_rows_far_apart(cuda):
+    """Two rows whose distance passes 2^31 elements, in every matrix that has them."""
+    from llmgpu import ops
+    M, K, N, ld = 2, 264, 136, 2 ** 31 + 64
+    buf = torch.zeros(M, ld, dtype=BF, device=cuda)
+    g = torch.Generator().manual_seed(4)
+    near = [_mat(g, M, n, BF, cuda)[0] for n in (K, N, N, N)]  # x, resid, dy, pre
+    cut = [0, 512, 1024, 1536, 2048]
+    far = [buf[:, c:c + m.shape[1]] for c, m in zip(cut, near)]
+    for f, m in zip(far, near):
+        f.copy_(m)
+    out = buf[:, 2048:2048 + N]
+    w, rng = _mat(g, N, K, BF, cuda, 0.1)[0], _rng(cuda)
+    ops.linear_fwd(far[0], w, None, "silu", 0.3, rng, 1, far[1], out=out)
+    assert torch.equal(out, ops.linear_fwd(near[0], w, None, "silu", 0.3, rng, 1, near[1])[0])
+    got = ops.linear_bwd(far[2], far[0], w, far[3], "silu", 0.3, rng, 1)
+    want = ops.linear_bwd(near[2], near[0], w, near[3], "silu", 0.3, rng, 1)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for f, m in zip(far, near):
+        assert torch.equal(f, m)
+    ops.check_device(cuda)
+
+
+def test_two_threads_at_once(cuda):
+    """Calls from two threads, each on a stream of its own, give what one thread's give."""
+    import threading
+    from llmgpu import ops
+    s = [_block_state(cuda, 10 + i, rows=300 + 40 * i, C=128, F=512, V=3000) for i in range(2)]
+    rng = _rng(cuda, 1, 1)
+    want = [_block(ops, q, rng) for q in s]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i].append(_block(ops, s[i], rng))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 - shown by the assertion below
+            failed.append(repr(e))
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for i in range(2):
+        assert len(got[i]) == 10
+        for r in got[i]:
+            assert all(torch.equal(r[k], want[i][k]) for k in want[i])
+    ops.check_device(cuda)
+
+
 # ------------------------------------------------------------------------------------ refusals
 def test_wrapper_refusals(cuda):
     from llmgpu import ops
