@@ -37,16 +37,18 @@ int dz_groups(int M, int N) {
 // part[gy][N] (nullable; with one row of blocks it is dbias itself, added to when `accumulate`).
 // `vec`: rows of dy and pre start on 16 bytes. A thread takes 8 columns of kDzInFlight rows at a
 // time, their loads in flight together as raw words. Bound by memory: 8192 x 4096 bf16 gelu, 201 MB,
-// 34 us (5.9 TB/s).
+// 34 us (5.9 TB/s). With an activation alone, the compiler's own choice of registers left a block
+// less on an SM than fits with a few spilled bytes: 4 of bf16 rather than 3 (gelu with its dx product
+// over K = 64 57 -> 53 us, relu 52 -> 48, silu 56 -> 54), 3 of f32 rather than 2 (gelu 68 -> 63, the
+// others as before). With dropout or no activation its choice is as fast or faster.
 constexpr int kDzInFlight = 2;
 template <typename T, int ACT, bool DROP>
-__global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long lddy,
-                                                        const bf16* __restrict__ pre,
-                                                        long long ld_pre, DropArgs drop,
-                                                        bf16* __restrict__ dz,
-                                                        float* __restrict__ dz32, long long ldz,
-                                                        float* __restrict__ part, int accumulate,
-                                                        int M, int N, int vec) {
+constexpr int kDzBlocks = DROP || ACT == kActNone ? 0 : sizeof(T) == 2 ? 4 : 3;  // 0: its choice
+template <typename T, int ACT, bool DROP>
+__global__ void __launch_bounds__(256, kDzBlocks<T, ACT, DROP>) linear_dz_kernel(
+    const T* __restrict__ dy, long long lddy, const bf16* __restrict__ pre, long long ld_pre,
+    DropArgs drop, bf16* __restrict__ dz, float* __restrict__ dz32, long long ldz,
+    float* __restrict__ part, int accumulate, int M, int N, int vec) {
     pdl_enter();
     const int lane = threadIdx.x & 31, wr = threadIdx.x >> 5;
     const int col = blockIdx.x * kDzCols + lane * 8;
