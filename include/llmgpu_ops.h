@@ -144,8 +144,9 @@ int llmgpu_op_moe_dispatch(const int* idx, int B, int T, int E, int k, int* grp,
 
 /* Dropout from a counter-based generator: out = resid + (kept ? x * scale : 0) over [rows, cols],
  * resid nullable. x and out are bf16 or f32 (x_f32, out_f32), resid has out's type; ld*: row
- * strides in elements, any alignment; out may be x or resid itself. Calling it with the gradient
- * in place of x (and no resid) is the backward: the mask is formed again, never stored.
+ * strides in elements, any alignment; out may be x or resid itself, with its type and row stride.
+ * Calling it with the gradient in place of x (and no resid) is the backward: the mask is formed
+ * again, never stored.
  *   Element (row, col) is dropped when its 16-bit lane is below round(p * 65536): lane col % 8 (low
  *   half of word 0 first) of Philox4x32-10 keyed by the seed, at counter (col / 8, row, low and high
  *   half of offset + site). scale = 65536 / (65536 - round(p * 65536)). p in [0, 1]: p = 1 drops
@@ -163,9 +164,9 @@ int llmgpu_op_dropout(const void* x, int x_f32, long long ldx, const void* resid
  *   address and ldx, ldw a multiple of 8 elements: otherwise a negative status); bias [N] f32,
  *   nullable; act: 0 none, 1 relu, 2 gelu (tanh form), 3 silu; drop: llmgpu_op_dropout over the
  *   [M, N] result with (p, rng, site), none when p = 0 (rng may then be NULL); resid (nullable) has
- *   out's type, bf16 or f32 (out_f32), and may be out itself. pre (nullable, bf16): z, which the
- *   backward needs when act is not none. out, resid and pre take any row stride. M = 0 is allowed;
- *   M, N, K <= 2^30.
+ *   out's type, bf16 or f32 (out_f32), and may be out itself, with its row stride. pre (nullable,
+ *   bf16): z, which the backward needs when act is not none. out, resid and pre take any row stride.
+ *   M = 0 is allowed; M, N, K <= 2^30.
  *   work: llmgpu_op_linear_fwd_work(M, N, K) bytes (0 where it is not used; the backward's workspace may
  *   be smaller), 16-byte aligned: a product of few tiles and long K is split along K there. With NULL,
  *   K stays whole: the same to f32 rounding, but slower.

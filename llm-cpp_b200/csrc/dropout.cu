@@ -157,6 +157,10 @@ int dropout_apply(const void* x, int x_f32, long long ldx, const void* resid, lo
     if (rows == 0 || cols == 0) return 0;
     if (!x || !out || !rng || (rows > 1 && (ldx < cols || ldo < cols || (resid && ldr < cols))))
         return -1;
+    // in place, every element keeps its place
+    if ((out == x && ((x_f32 != 0) != (out_f32 != 0) || (rows > 1 && ldo != ldx))) ||
+        (out == resid && rows > 1 && ldo != ldr))
+        return -1;
     if (x_f32)
         return out_f32 ? launch_dropout<float, float>(x, ldx, resid, ldr, out, ldo, rows, cols, thr,
                                                       scale, rng, site, s)

@@ -345,6 +345,7 @@ int linear_forward(const LinearFwd& a, int num_sms, cudaStream_t s) {
     if (a.M > kMaxDim || a.N > kMaxDim || a.K > kMaxDim) return -1;
     if (a.M == 0) return 0;
     if (!a.x || !a.w || !a.out) return -1;
+    if (a.out == a.resid && a.M > 1 && a.ldo != a.ldr) return -1;  // in place, every element keeps its place
     if (!operand_ok(a.x, a.ldx) || !operand_ok(a.w, a.ldw) || !operand_ok(a.work, 0))
         return kBadOperand;
     const int n = a.work ? product_splits(a.M, a.N, a.K) : 1;

@@ -86,6 +86,22 @@ def test_dropout_refusals(bad):
                                     a["rows"], a["cols"], a["p"], a["rng"], 0, None) in REFUSED
 
 
+@pytest.mark.parametrize("bad", [dict(x_f32=1), dict(out_f32=1), dict(ldx=16), dict(ldo=16),
+                                 dict(x=2 * P, resid=P, ldr=16)])
+def test_dropout_over_another_layout_is_refused(bad):
+    """out may be x or resid where every element keeps its place: one type, one row stride."""
+    a = dict(x=P, x_f32=0, ldx=8, resid=None, ldr=0, out_f32=0, ldo=8)
+    a.update(bad)
+    assert _lib().llmgpu_op_dropout(a["x"], a["x_f32"], a["ldx"], a["resid"], a["ldr"], P, a["out_f32"],
+                                    a["ldo"], 4, 8, 0.5, P, 0, None) in REFUSED
+
+
+@pytest.mark.parametrize("M", [4, 40])
+def test_linear_over_a_residual_of_another_stride_is_refused(M):
+    assert _lib().llmgpu_op_linear_fwd(P, 16, P, 16, 0, None, 0, 0.0, None, 0, 2 * P, 24, None, 0, 2 * P, 0,
+                                       16, M, 16, 16, None, None, None) in REFUSED
+
+
 def test_empty_calls_do_nothing():
     lib = _lib()
     assert lib.llmgpu_op_dropout(None, 0, 8, None, 0, None, 0, 8, 0, 8, 0.5, None, 0, None) == 0
