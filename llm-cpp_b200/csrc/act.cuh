@@ -11,8 +11,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // z^3) (gelu: 0.5 z (1 + tanh u) = z sigmoid(2u)), from the special-function unit's 2^x and
 // reciprocal, a few units in the last place, which an f32 output keeps. Far left, 2^x overflows
 // to inf and the result is -0. Packed pairs: 7 issue slots for two gelus besides the 4
-// special-function ones, since the epilogue's warps, two per scheduler, are what bounds a
-// product of K near 1024.
+// special-function ones, since the epilogue's warps (four a scheduler in the pair kernel, one in the
+// others) are what bounds a product of K near 1024.
 __device__ __forceinline__ float2 sigmoid_of_log2(float2 t) {  // 1 / (1 + 2^t)
     const float2 d = fadd2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.f, 1.f));
     return make_float2(rcp_approx(d.x), rcp_approx(d.y));

@@ -570,14 +570,26 @@ __device__ __forceinline__ float gelu_tanh_grad(float v) {
 }
 
 // ---------------------------------------------------------------- programmatic dependent launch
-// The GEMM kernels are launched with programmatic stream serialisation (when enabled): their
-// CTAs may be scheduled while the previous kernel of the stream is still running, set up
-// their barriers, TMEM and descriptors, and wait in pdl_wait() before the first access to
-// global memory until that kernel has completed and its writes are visible. Every kernel of
-// the step calls pdl_enter() first: the trigger in it lets a following GEMM start launching.
-// The other kernels keep plain stream order: their blocks launched early (while the kernel
-// before them finished) made the step slower. In a launch without the attribute both
-// instructions do nothing.
+// Launched with programmatic stream serialisation (when enabled), so that their CTAs may be scheduled
+// while the previous kernel of the stream is still running: the GEMM kernels, which set up their
+// barriers, TMEM and descriptors meanwhile, the few-row products (linear_rows_kernel,
+// linear_rows_mn_kernel) and linear_db_kernel. The other kernels keep plain stream order: their blocks
+// launched early (while the kernel before them finished) made the step slower. In a launch without
+// the attribute both instructions do nothing.
+//
+// What holds them in order:
+// - Every kernel calls pdl_wait() before its first access to global memory (pdl_enter() in all but the
+//   GEMMs): the previous kernel has then completed and its writes are visible. Only behind that
+//   wait comes the trigger that lets a following kernel start.
+// - But for a GEMM with GemmArgs::early: it triggers and runs without that wait and makes it last, so
+//   that whoever waits for it waits for the kernel in front as well. It may read what was complete
+//   before the kernel in front let it start, which is what that kernel's own wait covers. So a kernel
+//   put in front of an early product triggers behind its own wait, or is early behind one that does:
+//   a trigger in front of the wait would be a race that nothing reports.
+// - An early product is not itself a grid that waited for the writes it reads. It relies on a grid that
+//   has completed having its writes in L2, and on reading them from there: operands and residuals by
+//   bulk copies, scalars by a kernel that began after the writes had ended. The wait's guarantee is
+//   worded for the waiting grid only; that it holds for one started by it is what is relied on here.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -603,7 +615,7 @@ inline int launch_kernel(void (*kernel)(Exp...), dim3 grid, dim3 block, size_t s
     return e == cudaSuccess ? 0 : -(1000 + (int)e);
 }
 
-// The same with the programmatic-serialisation attribute when pdl_enabled() (GEMM kernels).
+// The same with the programmatic-serialisation attribute when pdl_enabled() (for which kernels: above).
 template <typename... Exp, typename... Act>
 inline int launch_kernel_pdl(void (*kernel)(Exp...), dim3 grid, dim3 block, size_t smem,
                              cudaStream_t s, Act&&... args) {

@@ -28,8 +28,8 @@ namespace {
 constexpr int BM = 128;
 constexpr int BK = 64;
 constexpr int kGemmThreads = 256;
-// CTA-pair kernel: warp 0 TMA, warp 1 MMA, warps 4..11 epilogue (two warps per TMEM lane
-// quarter, each draining half of a tile's columns)
+// CTA-pair kernel: warp 0 TMA, warp 1 MMA, warps from 4 on epilogue. Eight of them (two per TMEM lane
+// quarter, each draining half of a tile's columns) but for the linear family's sixteen, see PairCfgOf.
 constexpr int kPairEpiWarps = 8;
 constexpr int kChainBlocks = 8;  // k-blocks of an accumulator chain (512 products), see chain_sum
 constexpr int kGroupM = 16;  // tile raster: groups of 16 m-blocks share B tiles in L2
@@ -668,8 +668,8 @@ __device__ __forceinline__ void turned_rows(const float* tile, int lane, bool in
 // Outputs (and a residual) of any stride and alignment, and the last columns of a row that ends
 // inside 16 bytes: a lane's 32 columns are turned through 4 KB of the warp's shared memory (32 rows
 // of 32 floats, column j of row i at j ^ i), so that every access to global memory is 32
-// neighbouring columns of a row. In a kernel of its own (kFamLinearAny): its registers spilled in
-// the tiles that do without it.
+// neighbouring columns of a row. In a kernel of its own (kFamLinearAny): beside the boxes it costs the
+// pair kernel 240 bytes of spilled registers a thread instead of 88, which whole rows need not pay.
 __device__ __forceinline__ void linear_turned_tile(const GemmArgs& a, const GemmExt& x,
                                                    const DropKey& key, uint32_t tbase, int row0,
                                                    int n0, int lane, EpiWarp& w, int c_begin,
@@ -1598,12 +1598,12 @@ __global__ void __launch_bounds__(PairCfgOf<FAM>::THREADS, 1)
     uint8_t* smem = smem_raw + (((raw_u32 + 1023u) & ~1023u) - raw_u32);
     uint8_t* sA = smem;
     uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
-    uint8_t* sEpi = smem + STAGES * Cfg::STAGE_BYTES;  // 2 boxes per epilogue warp
+    uint8_t* sEpi = smem + STAGES * Cfg::STAGE_BYTES;  // EPI_SLOTS boxes per epilogue warp
     uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + Cfg::EPI_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
-    uint64_t* epi_bar = acc_empty + 2;  // two per epilogue warp
+    uint64_t* epi_bar = acc_empty + 2;  // EPI_SLOTS per epilogue warp
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_bar + Cfg::EPI_SLOTS * Cfg::EPI_WARPS);
 
     const uint32_t rank = cluster_ctarank();

@@ -87,7 +87,8 @@ struct GemmArgs {
     // Starts beside the kernel in front of it on the stream and ends after it. For a product that
     // neither reads nor overwrites what that kernel touches, behind a kernel of this library that
     // waited for its own predecessor or is itself `early` behind such a one: its inputs were then
-    // complete before that kernel's blocks let this one start.
+    // complete, and in L2, before that kernel's blocks let this one start. It relies on that, since
+    // it makes no griddepcontrol.wait of its own before it reads them (see pdl_wait in common.cuh).
     int early;
     // Grouped (per-expert) products. `grp` is a device table of groups+1 ascending row
     // offsets, each a multiple of 128 (entry `groups` = rows in use), written by an earlier

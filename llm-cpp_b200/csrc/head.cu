@@ -8,7 +8,7 @@
 // Bound by the tensor cores (and, over many launches, by the power cap): one product forward,
 // three backward, one more than with [rows, V] logits kept, and none of their memory (824 MB at
 // 8192 x 50257 in bf16, which would also round the loss). 8192 x 768 x 50257: forward 418 us
-// (1.51 PFLOP/s), backward 1420 us (1.33 PFLOP/s counting the recomputed product). Pieces of the
+// (1.51 PFLOP/s), backward 1430 us (1.33 PFLOP/s counting the recomputed product). Pieces of the
 // vocabulary rather than blocks of rows: dw, the largest matrix, is then written once instead of
 // summed over row blocks.
 #include <cfloat>
@@ -27,7 +27,7 @@ constexpr int kSlot = 128;       // vocabulary columns of one (max, sum) slot
 constexpr int kMaxSplits = 32;   // planes of the dx product
 constexpr int kPairSlots = 74;   // CTA pairs of a B200, for the choice of piece and splits only
 // Gradient piece at most, where chosen here. 8192 x 768 x 50257, backward by piece: 1024 columns 3509
-// us, 4096 1745, 8192 1684, 18944 1537, the choice below 1438.
+// us, 4096 1745, 8192 1684, 18944 1537, the choice below 1430.
 constexpr size_t kPieceBytes = (size_t)320 << 20;
 
 int slots_of(int V) { return (V + kSlot - 1) / kSlot; }

@@ -4,8 +4,8 @@
 // because it is a tensor-core operand; the bias gradient is summed before that rounding, and dw of up
 // to 8 rows, whose outer products run on the CUDA cores, takes it in f32. (dx of few rows goes
 // through the tensor cores too: dz in three bf16 terms cost it 1 to 5 us of 4 to 11.)
-// 8192 x 1024 x 4096: forward gelu 63 us (cuBLAS's bare product 57), backward 132 us (34 dz, 4
-// dbias, 95 the products); 8192 x 4096 x 1024 with dropout and f32 residual 67 us.
+// 8192 x 1024 x 4096: forward gelu 64 us (cuBLAS's bare product 57), backward 133 us (34 dz, 4
+// dbias, 95 the products); 8192 x 4096 x 1024 with dropout and f32 residual 68 us.
 #include "linear.cuh"
 
 #include "act.cuh"

@@ -73,7 +73,7 @@ struct LinearBwd {
     float* dbias;
     int accumulate;  // into dw (f32 only) and dbias
     int M, N, K;
-    void* work;  // linear_backward_work bytes, 256-byte aligned
+    void* work;  // linear_backward_work bytes, 16-byte aligned
     int* err;
 };
 size_t linear_backward_work(int M, int N, int K);

@@ -1,8 +1,15 @@
 // Linear-layer products of a few rows (decoding, single sequences): the weights are streamed once,
 // 16 bytes a lane straight into mma.sync fragments, with no tile, tensor map or staging between.
-// The legacy matrix instructions carry them because a tcgen05 tile is 128 rows high, and the bound
-// is the weights' bytes: 4096 x 4096 (33.5 MB) takes 7.4 us for 1 row, 8.9 for 16, where 64-wide tcgen05
-// tiles took 18 us; 1 x 1024 x 4096 3.5 us.
+// The legacy matrix instructions carry them because a tcgen05 tile is 128 rows high: 64-wide tcgen05
+// tiles took 18 us for 4096 x 4096.
+// With bias and gelu, in graph replays, weights in L2 and (other weights of 320 MB in between) in HBM:
+//   rows x K x N          w [N, K] L2 / HBM us     w [K, N]          floor (bytes at 6.48 TB/s)
+//    1 x 1024 x 4096          3.4 /  4.1            3.5 /  4.0        1.3
+//    1 x 4096 x 1024          5.5 /  6.9            9.0 / 10.2        1.3
+//    1 x 4096 x 4096          7.2 / 10.4            9.1 / 11.1        5.2
+//   16 x 4096 x 4096          8.4 / 11.4           10.7 / 12.9        5.2
+// From HBM 3.2 TB/s at best: a launch, the wait for the kernel in front and one DRAM latency stand in a
+// row, and w [K, N] has a block to 32 columns only, whatever K is.
 #include "common.cuh"
 #include "linear.cuh"
 #include "philox.cuh"
